@@ -101,8 +101,10 @@ def draw(rng):
 def _quantised(v):
     """Rows of float32 as 8-bit integers in [-127, 127] and one scale each."""
     most = v.abs().amax(-1, keepdim=True)
-    inv = torch.where(most > 0, 127.0 / most, 0.0)
-    return (v * inv).round(), (most / 127.0).squeeze(-1)
+    # a quotient of two tensors is rounded once; one with a number is not
+    top = torch.full_like(most, 127.0)
+    inv = torch.where(most > 0, top / most, 0.0)
+    return (v * inv).round(), (most / top).squeeze(-1)
 
 
 def prepare(case, seed):
@@ -265,9 +267,10 @@ def exact(case, seed):
                 xs = wide["x_scale"][b]
             else:  # what 8 bits hold goes by the 32-bit quotient that places it
                 v = xb.float()
-                top = v.abs().max(-1).values
-                xs = (top / 127.0).double()
-                xb = torch.round(v * torch.nan_to_num(127.0 / top, posinf=0.0)[:, None]).double()
+                top = v.abs().max(-1).values.double()
+                xs = (top / 127.0).float().double()
+                by = torch.nan_to_num(127.0 / top, posinf=0.0).float()
+                xb = torch.round(v * by[:, None]).double()
             out[b] = torch.einsum("nd,kd->nk", xb, c[bc]) * xs[:, None] * wide["c_scale"][bc]
             if "bias" in wide:
                 out[b] += wide["bias"][bc]

@@ -75,6 +75,7 @@ int encode_tmap_3d(CUtensorMap* map, const void* base, int dtype, uint64_t d0, u
   if (!enc) return fail(FK_ERR_TMA, "cuTensorMapEncodeTiled not available from the driver");
   CUtensorMapDataType dt = dtype == FK_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                            : dtype == FK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                           : dtype == FK_I8   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   const cuuint64_t dims[3] = {d0, d1, d2};
   const cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};

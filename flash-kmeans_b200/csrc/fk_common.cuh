@@ -52,7 +52,7 @@ struct Elem<float> {
 };
 
 __host__ __device__ inline int dtype_bytes(int dt) {
-  return dt == FK_F16 || dt == FK_BF16 ? 2 : (dt == FK_F32 || dt == FK_I32 ? 4 : (dt == FK_I64 ? 8 : 0));
+  return dt == FK_I8 ? 1 : dt == FK_F16 || dt == FK_BF16 ? 2 : (dt == FK_F32 || dt == FK_I32 ? 4 : (dt == FK_I64 ? 8 : 0));
 }
 
 // Load one element of a runtime-typed float array as float.

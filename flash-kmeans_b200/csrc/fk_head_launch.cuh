@@ -1,0 +1,144 @@
+// Host side of the cluster head's products: operand maps, tile shapes and
+// launches of head_gemm.
+#pragma once
+#include <atomic>
+#include <mutex>
+
+#include "fk_head_gemm.cuh"
+
+namespace fk {
+namespace head {
+
+// One operand: `parts` x `batches` matrices of `rows` rows of `inner` valid
+// elements, `ld` elements apart, laid out in part-major order `mat` elements
+// apart.  16-bit (FK_F16 / FK_BF16) or FK_I8.
+struct Operand {
+  const void* p;
+  int dtype;
+  int64_t inner, rows, ld, mat;
+  int64_t mats;        // parts * batches
+  int batch_step;      // matrices from one batch to the next (0: shared)
+  int part_step;       // matrices from one part to the next
+  bool mn;             // the contraction runs over rows
+  int64_t off;         // first row / first contraction index
+};
+
+struct ShapeChoice {
+  int cg, bn;
+  int bm() const { return 128 * cg; }
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// 256 x 256 tiles on CTA pairs once they give half of the 74 pairs a tile;
+// below that 128 x 128 tiles, and 128 x 64 ones when even those leave most SMs
+// idle.  Measured in profiles/cluster_head.md.
+inline ShapeChoice choose_shape(int64_t M, int64_t N, int64_t batches, int64_t splittable) {
+  if (M > 128 && ceil_div(M, 256) * ceil_div(N, 256) * batches * splittable >= 37) return {2, 256};
+  if (ceil_div(M, 128) * ceil_div(N, 128) * batches * splittable >= 100) return {1, 128};
+  return {1, 64};
+}
+
+// Number of equal chunks of `units` for which `slots` workers finish `items`
+// items first; every chunk also costs `extra` units.
+inline int choose_chunks(int64_t items, int64_t units, int64_t slots, int64_t most, double extra) {
+  int best = 1;
+  double best_cost = 1e300;
+  if (most > units) most = units;
+  for (int64_t c = 1; c <= most; ++c) {
+    const double cost =
+        static_cast<double>(ceil_div(items * c, slots)) * (ceil_div(units, c) + extra) + (c > 1 ? extra : 0.0);
+    if (cost < best_cost * 0.999) {
+      best_cost = cost;
+      best = static_cast<int>(c);
+    }
+  }
+  return best;
+}
+
+int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows);
+
+template <int CG, int BN, int EPI>
+int launch_shape(Params& prm, cudaStream_t s) {
+  using S = Shape<CG, BN, EPI>;
+  auto kern = head_gemm<CG, BN, EPI>;
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return fail(FK_ERR_CUDA, "bad current device %d", dev);
+  static std::atomic<bool> ready[64];
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  const int sms = sm_count_current();
+  if (sms <= 0) return fail(FK_ERR_CUDA, "no SM count for device %d", dev);
+  const Problem& p = prm.p;
+  const int64_t items = static_cast<int64_t>(p.batches) * p.chunks * p.m_tiles *
+                        (running(EPI) ? 1 : p.n_tiles);
+  const int64_t slots = sms / CG;
+  const unsigned grid = static_cast<unsigned>((items < slots ? items : slots) * CG);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FK_ERR_CUDA, "head_gemm launch failed: %s", cudaGetErrorString(e));
+  }
+  return FK_OK;
+}
+
+// Fills in the product's tiles and maps and launches it.  `kdim` elements are
+// contracted; p.M, p.N, p.batches, p.chunks and the epilogue's fields are set.
+template <int EPI>
+int launch(Params& prm, const Operand& a, const Operand& b, int64_t kdim, ShapeChoice sh,
+           cudaStream_t s) {
+  Problem& p = prm.p;
+  const int step = integer(EPI) ? 128 : 64;
+  p.m_tiles = static_cast<int>(ceil_div(p.M, sh.bm()));
+  p.n_tiles = static_cast<int>(ceil_div(p.N, sh.bn));
+  p.kblocks = static_cast<int>(ceil_div(kdim, step));
+  p.a_mn = a.mn;
+  p.b_mn = b.mn;
+  p.a_batch = a.batch_step;
+  p.b_batch = b.batch_step;
+  p.a_part = a.part_step;
+  p.b_part = b.part_step;
+  p.a_off = static_cast<int>(a.off);
+  p.b_off = static_cast<int>(b.off);
+  // a short A is loaded in a box of its own height: the rows below it hold
+  // what the last stage left, and nothing reads their accumulators
+  p.a_rows = sh.cg == 1 && p.M < 128 ? static_cast<int>(ceil_div(p.M, 8) * 8) : 128;
+  p.group = 8;
+  const int64_t tile_bytes = static_cast<int64_t>(sh.bn) * p.kblocks * kStageRowBytes;
+  p.window = static_cast<int>(std::max<int64_t>(1, (16 << 20) / tile_bytes));
+  if (integer(EPI)) {
+    p.idesc = instr_desc_i8(128 * sh.cg, sh.bn);
+  } else {
+    p.idesc = instr_desc(a.dtype == FK_BF16 ? 1 : 0, 128 * sh.cg, sh.bn) |
+              (a.mn ? 1u << 15 : 0u) | (b.mn ? 1u << 16 : 0u);
+  }
+  int st = encode_operand(&prm.a, a, a.mn ? 64 : p.a_rows);
+  if (st != FK_OK) return st;
+  st = encode_operand(&prm.b, b, b.mn ? 64 : sh.bn / sh.cg);
+  if (st != FK_OK) return st;
+  if (sh.cg == 2) return launch_shape<2, 256, EPI>(prm, s);
+  if (sh.bn == 128) return launch_shape<1, 128, EPI>(prm, s);
+  return launch_shape<1, 64, EPI>(prm, s);
+}
+
+inline int64_t slots_of(ShapeChoice sh) {
+  const int sms = sm_count_current();
+  return (sms > 0 ? sms : 148) / sh.cg;
+}
+
+}  // namespace head
+}  // namespace fk

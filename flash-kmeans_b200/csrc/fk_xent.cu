@@ -1,0 +1,810 @@
+// Softmax cross entropy of points against centroids, and its gradients.
+//
+//   z[n, k] = scale * x[n] . c[k],   d[n, k] = z[n, k] - z[n, y_n]
+//   loss[n] = log sum_k exp(d[n, k]) = log1p(sum_{k != y} exp(d))   (d <= 0)
+//   dz[n, k] = w_n (softmax(z[n])[k] - [k == y_n])
+//   dx = scale * dz . c,   dc = scale * dz^T . x
+//
+// The (N, K) scores never reach memory.  The forward pass is one product whose
+// epilogue keeps each row's running maximum and sum of exponentials over the
+// centroids other than the label; a small kernel joins the column chunks.  The
+// label's term stays out of the sum because a well-fitted row's loss is
+// log1p of what the others add, and 1 + that in 32 bits would round it away.
+//
+// The backward pass goes over the centroids in pieces.  For each it recomputes
+// the scores, writes dz of the piece rounded to 16 bits (the operand type of
+// the tensor cores: one rounding of half a step at most, next to the rounding
+// of the 16-bit gradients themselves) and runs the two products that read it;
+// accumulators are float32 throughout.  That is 8 N K D operations instead of
+// the 6 N K D of a pass that keeps N x K scores.
+//
+// float32 inputs are split exactly into three bf16 parts, and the six products
+// of parts down to 2^-16 of the leading one are accumulated, smallest first:
+// the terms left out are below 2^-24 of |x||c|.  That costs what 3xTF32 costs
+// and keeps one kernel, MN-major operands included.
+#include <algorithm>
+#include <cmath>
+
+#include "fk_head_launch.cuh"
+
+namespace fk {
+namespace head {
+
+// 16-bit P elements of a piece: 256 MB, so that a piece's products have whole
+// waves of tiles, and the float32 sums carried between pieces are few.
+constexpr int64_t kPieceElems = 1ll << 27;
+constexpr int64_t kMaxRowChunk = 16384;
+
+int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows) {
+  const int64_t eb = o.dtype == FK_I8 ? 1 : 2;
+  const uint32_t box0 = o.dtype == FK_I8 ? 128 : 64;
+  return encode_tmap_3d(map, o.p, o.dtype, o.inner, o.rows, o.mats, o.ld * eb,
+                        (o.mats > 1 ? o.mat : o.rows * o.ld) * eb, box0, box_rows);
+}
+
+// ------------------------------------------------------------ operand copies
+// Rows of x as the tensor cores read them: padded to 16 bytes, zeros past D,
+// float32 as three bf16 parts.  With labels, ignored rows become zeros, so that
+// whatever a padded position holds (NaN included) adds nothing to dc.
+__device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
+  uint32_t h = pack_bf16(v, 0.0f) & 0xffffu;
+  if ((h & 0x7f80u) == 0x7f80u && fabsf(v) <= 3.40282347e38f)
+    h = __float_as_uint(v) >> 16;  // would round past the largest bf16: truncate
+  p[0] = static_cast<uint16_t>(h);
+  const float hf = __uint_as_float(h << 16);
+  float r = fabsf(v) <= 3.40282347e38f ? v - hf : 0.0f;  // inf, NaN: all in the first part
+  h = pack_bf16(r, 0.0f) & 0xffffu;
+  p[1] = static_cast<uint16_t>(h);
+  r -= __uint_as_float(h << 16);
+  p[2] = static_cast<uint16_t>(pack_bf16(r, 0.0f) & 0xffffu);
+}
+
+template <typename T>
+__global__ void head_rows_kernel(const T* __restrict__ x, int64_t sb, int64_t sn, int64_t sd, int vec,
+                                 uint16_t* __restrict__ out, int64_t part, int N, int D, int Dp,
+                                 int64_t units, const void* labels, int label_dtype, int64_t lb,
+                                 int64_t ln, int64_t ignore_index) {
+  const int per = Dp / 8;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < units;
+       u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = u / per;
+    const int d0 = static_cast<int>(u - row * per) * 8;
+    const int64_t b = row / N, n = row - b * N;
+    T v[8];
+    const bool zero = labels && load_label(labels, b * lb + n * ln, label_dtype) == ignore_index;
+    const T* src = x + b * sb + n * sn;
+    if (zero) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = Elem<T>::from_f(0.0f);
+    } else if (vec && d0 + 8 <= D) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+        reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src + d0)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = d0 + i < D ? src[(d0 + i) * sd] : Elem<T>::from_f(0.0f);
+    }
+    uint16_t* dst = out + row * Dp + d0;
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
+    } else {
+      uint16_t p[8][3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) split3(v[i], p[i]);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        uint4 w;
+        uint32_t* ww = &w.x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ww[i] = p[2 * i][q] | static_cast<uint32_t>(p[2 * i + 1][q]) << 16;
+        *reinterpret_cast<uint4*>(dst + q * part) = w;
+      }
+    }
+  }
+}
+
+struct Labels {
+  const void* p = nullptr;
+  int dtype = FK_I32;
+  int64_t sb = 0, sn = 0;
+  int64_t ignore = -100;
+};
+
+template <typename T>
+static int rows_copy_typed(const void* x, int64_t B, int64_t N, int64_t D, const int64_t* xs,
+                           uint16_t* out, int64_t Dp, const Labels& y, bool mask, cudaStream_t s) {
+  const int64_t units = B * N * (Dp / 8);
+  const int vec = (xs[2] == 1 || D == 1) && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                  (N == 1 || xs[1] * sizeof(T) % 16 == 0) && (B == 1 || xs[0] * sizeof(T) % 16 == 0);
+  const int sms = sm_count_current();
+  const int64_t cap = (sms > 0 ? sms : 148) * 16ll;
+  const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(units, 256), cap));
+  head_rows_kernel<T><<<blocks, 256, 0, s>>>(static_cast<const T*>(x), xs[0], xs[1], xs[2], vec, out,
+                                             B * N * Dp, static_cast<int>(N), static_cast<int>(D),
+                                             static_cast<int>(Dp), units, mask ? y.p : nullptr,
+                                             y.dtype, y.sb, y.sn, y.ignore);
+  return check_launch("head_rows_kernel");
+}
+
+static int rows_copy(const void* x, int dtype, int64_t B, int64_t N, int64_t D, const int64_t* xs,
+                     uint16_t* out, int64_t Dp, const Labels& y, bool mask, cudaStream_t s) {
+  switch (dtype) {
+    case FK_F16: return rows_copy_typed<__half>(x, B, N, D, xs, out, Dp, y, mask, s);
+    case FK_BF16: return rows_copy_typed<__nv_bfloat16>(x, B, N, D, xs, out, Dp, y, mask, s);
+    default: return rows_copy_typed<float>(x, B, N, D, xs, out, Dp, y, mask, s);
+  }
+}
+
+// ------------------------------------------------------------------ combine
+// One warp column of 16 warps joins the column chunks of 32 rows; block sums
+// of the losses go to `block_part`, and the last block adds them up in block
+// order, so the result does not depend on which block came last.
+constexpr int kCombineWarps = 16;
+
+struct CombineParams {
+  const float2* partial;   // [batch][pieces][N]
+  const float* z_label;    // [batch][N], times log2(e)
+  const void* labels;
+  int label_dtype;
+  int64_t lb, ln, ignore;
+  int64_t K;
+  int N, pieces, batches, row_blocks;
+  int reduction;           // 0 none, 1 mean, 2 sum
+  float* loss;             // rows [batch][N], or one value
+  RowStat* stat;           // optional
+  int32_t* count;          // rows that are not ignored
+  double2* block_part;     // (sum, count) of each block
+  uint32_t* ticket;        // zero before the launch
+  int* status;
+};
+
+__global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const CombineParams p) {
+  __shared__ float2 sm[kCombineWarps][33];
+  __shared__ double2 red[kCombineWarps];
+  __shared__ bool last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.x / p.row_blocks;
+  const int row = (blockIdx.x % p.row_blocks) * 32 + lane;
+  const float2* part = p.partial + static_cast<int64_t>(b) * p.pieces * p.N + row;
+  float m = -INFINITY, s = 0.0f;
+  if (row < p.N) {
+    for (int i = warp; i < p.pieces; i += kCombineWarps) {
+      const float2 v = part[static_cast<int64_t>(i) * p.N];
+      const float mn = fmaxf(m, v.x);
+      const float mu = mn == -INFINITY ? 0.0f : mn;
+      // a piece whose exponents were NaN has a NaN sum, which stays
+      s = s * ex2(m - mu) + v.y * ex2(v.x - mu);
+      m = mn;
+    }
+  }
+  sm[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  double sum = 0.0, cnt = 0.0;
+  if (warp == 0) {
+    for (int w = 1; w < kCombineWarps; ++w) {
+      const float2 v = sm[w][lane];
+      const float mn = fmaxf(m, v.x);
+      const float mu = mn == -INFINITY ? 0.0f : mn;
+      s = s * ex2(m - mu) + v.y * ex2(v.x - mu);
+      m = mn;
+    }
+    if (row < p.N) {
+      const int64_t r = static_cast<int64_t>(b) * p.N + row;
+      const int64_t y = load_label(p.labels, b * p.lb + row * p.ln, p.label_dtype);
+      const bool ignored = y == p.ignore;
+      RowStat st = {0.0f, 0.0f, 0.0f, -1};
+      float loss = 0.0f;
+      if (!ignored && (y < 0 || y >= p.K)) {
+        loss = NAN;
+        st = {0.0f, NAN, NAN, -1};
+        if (p.status) atomicCAS(p.status, 0, FK_DEV_BAD_LABEL);
+      } else if (!ignored) {
+        const float ty = p.z_label[r];
+        const float d = m - ty;  // -inf for K = 1
+        // sum over the others, relative to the larger of the label's term and theirs
+        const float top = fmaxf(m, ty);
+        const float others = s * ex2(m - top);
+        const float own = ex2(ty - top);
+        loss = d > 0.0f ? fmaf(d, 0.69314718056f, logf(others + own)) : log1pf(others);
+        if (!(s == s) || !(ty < INFINITY)) loss = NAN;  // NaN scores, or inf - inf
+        st.m2 = top;
+        st.coef = 1.0f / (others + own);
+        st.at_label = expm1f(-loss);
+        st.label = static_cast<int>(y);
+        if (!(loss == loss)) st.coef = st.at_label = NAN;
+      }
+      if (p.stat) p.stat[r] = st;
+      if (p.reduction == 0) p.loss[r] = loss;
+      sum = loss;
+      cnt = ignored ? 0.0 : 1.0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+    }
+    if (lane == 0) {
+      p.block_part[blockIdx.x] = make_double2(sum, cnt);
+      __threadfence();
+      last = atomicAdd(p.ticket, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  sum = cnt = 0.0;
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kCombineWarps * 32) {
+    const double2 v = __ldcg(p.block_part + i);
+    sum += v.x;
+    cnt += v.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    cnt += __shfl_xor_sync(0xffffffffu, cnt, o);
+  }
+  if (lane == 0) red[warp] = make_double2(sum, cnt);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = cnt = 0.0;
+    for (int w = 0; w < kCombineWarps; ++w) {
+      sum += red[w].x;
+      cnt += red[w].y;
+    }
+    if (p.reduction == 1) *p.loss = static_cast<float>(sum / cnt);  // no row left: 0 / 0
+    if (p.reduction == 2) *p.loss = static_cast<float>(sum);
+    *p.count = static_cast<int32_t>(cnt);
+  }
+}
+
+// --------------------------------------------------------- row weights (none)
+// Losses that stay per row arrive with one upstream gradient each, which goes
+// into the row's weight.  For float16 the weights are taken relative to the
+// largest finite one, so that P stays within float16; it comes back as a factor
+// of the outputs.  The maximum of non-negative floats is the maximum of their
+// bits, whose order of arrival does not matter.
+__global__ void xent_gmax_kernel(const float* __restrict__ g, const RowStat* __restrict__ stat,
+                                 int64_t rows, uint32_t* out) {
+  uint32_t m = 0;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const uint32_t u = __float_as_uint(g[i]) & 0x7fffffffu;
+    if (u < 0x7f800000u && (stat[i].coef != 0.0f || stat[i].at_label != 0.0f)) m = max(m, u);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
+}
+
+__global__ void xent_weight_kernel(const float* __restrict__ g, const RowStat* __restrict__ stat,
+                                   int64_t rows, const float* __restrict__ gmax, RowStat* out,
+                                   float* factor) {
+  // a power of two, so that the division is exact
+  float inv = 1.0f, f = 1.0f;
+  if (gmax && *gmax > 0.0f) {
+    int e;
+    frexpf(*gmax, &e);
+    e = min(max(e, -120), 120);
+    f = ldexpf(1.0f, e);
+    inv = ldexpf(1.0f, -e);
+  }
+  if (factor && blockIdx.x == 0 && threadIdx.x == 0) *factor = f;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    RowStat st = stat[i];
+    const bool ignored = st.label < 0 && st.coef == 0.0f;
+    if (!ignored) {
+      const float w = g[i] * inv;
+      st.coef *= w;
+      st.at_label *= w;
+    }
+    out[i] = st;
+  }
+}
+
+// ---------------------------------------------------- split sums to the output
+__global__ void head_join_kernel(const float* __restrict__ acc, int splits, int64_t split_stride,
+                                 int64_t acc_batch, int64_t acc_ld, void* out, int dtype, int64_t ob,
+                                 int64_t orow, int rows, int cols, int64_t total) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = i / cols;
+    const int c = static_cast<int>(i - r * cols);
+    const int64_t b = r / rows, n = r - b * rows;
+    const float* a = acc + b * acc_batch + n * acc_ld + c;
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v += a[s * split_stride];
+    store_f(out, b * ob + n * orow + c, dtype, v);
+  }
+}
+
+// -------------------------------------------------------------------- plans
+struct Bump {  // workspace layout: the same walk sizes it and hands it out
+  uint8_t* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(int64_t n) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += align_up(static_cast<size_t>(n) * sizeof(T), 256);
+    return p;
+  }
+};
+
+struct Xent {
+  const void *x, *c;
+  int dtype;
+  int64_t B, N, K, D;
+  int64_t xs[3], cs[3];
+  Labels y;
+  float scale;
+  int reduction;
+
+  int parts() const { return dtype == FK_F32 ? 3 : 1; }
+  int mma_dtype() const { return dtype == FK_F16 ? FK_F16 : FK_BF16; }
+  int64_t Dp() const { return ceil_div(D, 8) * 8; }
+  int64_t Bc() const { return cs[0] == 0 ? 1 : B; }  // batches with centroids of their own
+};
+
+// Operand over a caller's tensor (used in place) or its copy in the workspace.
+static bool in_place(const void* p, int dtype, int64_t B, int64_t M, int64_t D, const int64_t* st) {
+  if (dtype == FK_F32 || (B > 1 && st[0] == 0)) return false;
+  int64_t s[3] = {st[0], st[1], D == 1 ? 1 : st[2]};
+  if (M == 1) s[1] = ceil_div(D, 8) * 8;
+  if (B == 1) s[0] = M * s[1];
+  return fk_tma_compatible(p, dtype, D, s) != 0;
+}
+
+static Operand operand(const Xent& q, const void* p, const uint16_t* copy, int64_t B, int64_t M,
+                       const int64_t* st, bool mn, int64_t off) {
+  Operand o;
+  o.dtype = q.mma_dtype();
+  o.inner = q.D;
+  o.rows = M;
+  o.mn = mn;
+  o.off = off;
+  if (copy) {
+    o.p = copy;
+    o.ld = q.Dp();
+    o.mat = M * q.Dp();
+    o.mats = B * q.parts();
+    o.part_step = static_cast<int>(B);
+  } else {
+    o.p = p;
+    o.ld = M == 1 ? q.Dp() : st[1];
+    o.mat = st[0];
+    o.mats = B;
+    o.part_step = 0;
+  }
+  o.batch_step = B > 1 ? 1 : 0;
+  return o;
+}
+
+static void set_pairs(Problem& p, int parts) {
+  // (A part, B part), smallest products first
+  static const int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
+  p.npairs = parts == 3 ? 6 : 1;
+  for (int i = 0; i < kMaxPairs; ++i) {
+    p.pa[i] = parts == 3 ? pa[i] : 0;
+    p.pb[i] = parts == 3 ? pb[i] : 0;
+  }
+}
+
+static int check_args(const Xent& q, const char* who) {
+  if (q.B < 0 || q.N < 0 || q.K <= 0 || q.D <= 0) return fail(FK_ERR_INVALID_ARG, "%s: bad sizes", who);
+  if (q.dtype != FK_F16 && q.dtype != FK_BF16 && q.dtype != FK_F32)
+    return fail(FK_ERR_INVALID_ARG, "%s: unsupported dtype %d", who, q.dtype);
+  if (q.y.dtype != FK_I32 && q.y.dtype != FK_I64)
+    return fail(FK_ERR_INVALID_ARG, "%s: labels must be int32 or int64", who);
+  if (q.reduction < 0 || q.reduction > 2) return fail(FK_ERR_INVALID_ARG, "%s: bad reduction", who);
+  if (!(q.scale > 0.0f) || !std::isfinite(q.scale) || !std::isfinite(q.scale * 1.44269504f))
+    return fail(FK_ERR_INVALID_ARG, "%s: scale must be positive and finite", who);
+  if (q.N >= (1ll << 30) || q.K >= (1ll << 30) || q.D >= (1ll << 30) || q.B * 3 >= (1ll << 30) ||
+      q.B * q.N >= (1ll << 31))
+    return fail(FK_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit", who);
+  return FK_OK;
+}
+
+struct ForwardPlan {
+  ShapeChoice sh;
+  int chunks;
+  int64_t row_blocks;
+  uint16_t *xc, *cc;
+  float2* partial;
+  float* z_label;
+  double2* block_part;
+  uint32_t* ticket;
+  size_t bytes;
+};
+
+static ForwardPlan plan_forward(const Xent& q, void* ws) {
+  ForwardPlan f;
+  Bump b{static_cast<uint8_t*>(ws)};
+  f.sh = choose_shape(q.N, q.K, q.B, 1);
+  f.chunks = choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
+                           2 * slots_of(f.sh), 0.25);
+  f.row_blocks = ceil_div(q.N, 32);
+  f.xc = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
+             ? nullptr
+             : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+  f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
+             ? nullptr
+             : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  f.partial = b.take<float2>(q.B * f.chunks * 2 * q.N);
+  f.z_label = b.take<float>(q.B * q.N);
+  f.block_part = b.take<double2>(q.B * f.row_blocks);
+  f.ticket = b.take<uint32_t>(1);
+  f.bytes = b.used;
+  return f;
+}
+
+static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, void* ws, int* status,
+                   cudaStream_t s) {
+  const ForwardPlan f = plan_forward(q, ws);
+  int st;
+  if (f.xc && (st = rows_copy(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), q.y, false, s)) != FK_OK)
+    return st;
+  if (f.cc && (st = rows_copy(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), q.y, false, s)) != FK_OK)
+    return st;
+  Params prm = {};
+  Problem& p = prm.p;
+  p.M = static_cast<int>(q.N);
+  p.N = static_cast<int>(q.K);
+  p.batches = static_cast<int>(q.B);
+  p.chunks = f.chunks;
+  set_pairs(p, q.parts());
+  p.scale2 = q.scale * 1.44269504f;
+  p.labels = q.y.p;
+  p.label_dtype = q.y.dtype;
+  p.label_sb = q.y.sb;
+  p.label_sn = q.y.sn;
+  p.ignore_index = q.y.ignore;
+  p.partial = f.partial;
+  p.z_label = f.z_label;
+  p.zero = f.ticket;
+  p.zero_n = 1;
+  p.status = status;
+  st = launch<kEpiLse>(prm, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, 0),
+                       operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, 0), q.D, f.sh, s);
+  if (st != FK_OK) return st;
+  CombineParams cp = {};
+  cp.partial = f.partial;
+  cp.z_label = f.z_label;
+  cp.labels = q.y.p;
+  cp.label_dtype = q.y.dtype;
+  cp.lb = q.y.sb;
+  cp.ln = q.y.sn;
+  cp.ignore = q.y.ignore;
+  cp.K = q.K;
+  cp.N = static_cast<int>(q.N);
+  cp.pieces = f.chunks * 2;
+  cp.batches = static_cast<int>(q.B);
+  cp.row_blocks = static_cast<int>(f.row_blocks);
+  cp.reduction = q.reduction;
+  cp.loss = loss;
+  cp.stat = stat;
+  cp.count = count;
+  cp.block_part = f.block_part;
+  cp.ticket = f.ticket;
+  cp.status = status;
+  xent_combine_kernel<<<static_cast<unsigned>(q.B * f.row_blocks), kCombineWarps * 32, 0, s>>>(cp);
+  return check_launch("xent_combine_kernel");
+}
+
+struct BackwardPlan {
+  int64_t R, Kp;               // rows and centroids of a piece
+  int64_t n_chunks, n_pieces;
+  ShapeChoice sh_p, sh_x, sh_c;
+  int split_x, split_c;
+  int64_t ld;                  // of the float32 accumulators
+  uint16_t *xc, *cc, *P;
+  float *acc_x, *acc_c;        // null: the product writes the output itself
+  RowStat* weighted;
+  float* gmax;                 // (largest |g|, the factor it gives)
+  size_t bytes;
+};
+
+static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void* ws) {
+  BackwardPlan f;
+  Bump b{static_cast<uint8_t*>(ws)};
+  const int64_t budget = std::max<int64_t>(kPieceElems / q.parts() / q.B, 256 * 128);
+  const int64_t kall = ceil_div(q.K, 256) * 256;
+  f.R = std::min(q.N, kMaxRowChunk);
+  f.Kp = std::min(kall, std::max<int64_t>(256, budget / std::max<int64_t>(f.R, 128) / 256 * 256));
+  f.R = std::min(q.N, std::max<int64_t>(128, budget / f.Kp / 128 * 128));
+  f.n_pieces = ceil_div(q.K, f.Kp);
+  f.Kp = ceil_div(ceil_div(q.K, f.n_pieces), 256) * 256;
+  f.n_pieces = ceil_div(q.K, f.Kp);
+  f.n_chunks = ceil_div(q.N, f.R);
+  f.R = std::min(q.N, ceil_div(ceil_div(q.N, f.n_chunks), 128) * 128);
+  f.n_chunks = ceil_div(q.N, f.R);
+  const int64_t kw = std::min(f.Kp, q.K);
+  const int pairs = q.parts() == 3 ? 6 : 1;
+  f.sh_p = choose_shape(f.R, kw, q.B, 1);
+  const int64_t steps_x = pairs * ceil_div(kw, 64), steps_c = pairs * ceil_div(f.R, 64);
+  auto pick = [&](int64_t M, int64_t steps, ShapeChoice* sh) {
+    *sh = choose_shape(M, q.D, q.B, std::max<int64_t>(1, steps / 16));
+    const int64_t items = q.B * ceil_div(M, sh->bm()) * ceil_div(q.D, sh->bn);
+    return items >= 4 * slots_of(*sh) ? 1 : choose_chunks(items, steps, slots_of(*sh), 16, 3.0);
+  };
+  f.split_x = pick(f.R, steps_x, &f.sh_x);
+  f.split_c = pick(kw, steps_c, &f.sh_c);
+  f.ld = ceil_div(q.D, 4) * 4;
+  f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+  f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
+             ? nullptr
+             : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  f.P = b.take<uint16_t>(q.parts() * q.B * f.R * f.Kp);
+  f.acc_x = f.acc_c = nullptr;
+  if (want_x && (f.n_pieces > 1 || f.split_x > 1)) f.acc_x = b.take<float>(f.split_x * q.B * q.N * f.ld);
+  if (want_c && (f.n_chunks > 1 || f.split_c > 1)) f.acc_c = b.take<float>(f.split_c * q.B * f.Kp * f.ld);
+  f.weighted = q.reduction == 0 ? b.take<RowStat>(q.B * q.N) : nullptr;
+  f.gmax = q.reduction == 0 ? b.take<float>(2) : nullptr;
+  f.bytes = b.used;
+  return f;
+}
+
+struct Grad {
+  void* p;
+  int64_t sb, sr;
+};
+
+// One gradient product over a piece, into the accumulator or the output.
+static int grad_product(const Xent& q, Problem base, const Operand& a, const Operand& b, int64_t M,
+                        int64_t kdim, ShapeChoice sh, int splits, float* acc, int64_t acc_rows,
+                        int64_t acc_row0, int64_t ld, bool first, bool last, const Grad& g,
+                        int64_t out_row0, cudaStream_t s) {
+  Params prm = {};
+  Problem& p = prm.p;
+  p = base;
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(q.D);
+  const int64_t steps = p.npairs * ceil_div(kdim, 64);
+  p.chunks = static_cast<int>(std::min<int64_t>(splits, steps));
+  const int eb = dtype_bytes(q.dtype);
+  p.out = static_cast<uint8_t*>(g.p) + out_row0 * g.sr * eb;
+  p.out_dtype = q.dtype;
+  p.out_sb = g.sb;
+  p.out_sr = g.sr;
+  p.out_vec = reinterpret_cast<uintptr_t>(p.out) % (4 * eb) == 0 && g.sr % 4 == 0 && g.sb % 4 == 0;
+  if (acc) {
+    p.acc = acc + acc_row0 * ld;
+    p.acc_ld = ld;
+    p.acc_batch = acc_rows * ld;
+    p.acc_split = q.B * acc_rows * ld;
+    p.acc_read = !first;
+    p.acc_write = splits > 1 || !last;
+  }
+  int st = launch<kEpiOut>(prm, a, b, kdim, sh, s);
+  if (st != FK_OK) return st;
+  if (splits > 1 && last) {
+    const int64_t total = q.B * M * q.D;
+    const int sms = sm_count_current();
+    const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(total, 256), (sms > 0 ? sms : 148) * 16ll));
+    // a short last piece may have fewer steps than splits: the others hold
+    // earlier pieces' sums, or were never written if this is the only piece
+    head_join_kernel<<<blocks, 256, 0, s>>>(p.acc, first ? p.chunks : splits, p.acc_split, p.acc_batch,
+                                            ld, p.out, q.dtype, g.sb, g.sr, static_cast<int>(M),
+                                            static_cast<int>(q.D), total);
+    st = check_launch("head_join_kernel");
+  }
+  return st;
+}
+
+static int backward(const Xent& q, const RowStat* stat, const int32_t* count, const float* g,
+                    const Grad& gx, const Grad& gc, void* ws, int* status, cudaStream_t s) {
+  const BackwardPlan f = plan_backward(q, gx.p != nullptr, gc.p != nullptr, ws);
+  const int64_t rows = q.B * q.N;
+  const bool f16 = q.dtype == FK_F16;
+  // float16 P is kept times 2^14: a softmax over 2^20 centroids then still has
+  // ten bits above float16's smallest subnormal, and 1 * 2^14 is in range
+  const float p_scale = f16 ? 16384.0f : 1.0f;
+  int st;
+  if ((st = rows_copy(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), q.y, true, s)) != FK_OK) return st;
+  if (f.cc && (st = rows_copy(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), q.y, false, s)) != FK_OK)
+    return st;
+  const float* factor = q.reduction == 0 ? nullptr : g;
+  if (q.reduction == 0) {
+    const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(rows, 256), 1024));
+    if (f16) {
+      const cudaError_t e = cudaMemsetAsync(f.gmax, 0, 2 * sizeof(float), s);
+      if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+      xent_gmax_kernel<<<blocks, 256, 0, s>>>(g, stat, rows, reinterpret_cast<uint32_t*>(f.gmax));
+      if ((st = check_launch("xent_gmax_kernel")) != FK_OK) return st;
+      factor = f.gmax + 1;
+    }
+    xent_weight_kernel<<<blocks, 256, 0, s>>>(g, stat, rows, f16 ? f.gmax : nullptr, f.weighted,
+                                              f16 ? f.gmax + 1 : nullptr);
+    if ((st = check_launch("xent_weight_kernel")) != FK_OK) return st;
+    stat = f.weighted;
+  }
+
+  for (int64_t piece = 0; piece < f.n_pieces; ++piece) {
+    const int64_t k0 = piece * f.Kp, kw = std::min(f.Kp, q.K - k0);
+    for (int64_t chunk = 0; chunk < f.n_chunks; ++chunk) {
+      const int64_t r0 = chunk * f.R, rw = std::min(f.R, q.N - r0);
+      // dz of the piece
+      Params prm = {};
+      Problem& p = prm.p;
+      p.M = static_cast<int>(rw);
+      p.N = static_cast<int>(kw);
+      p.batches = static_cast<int>(q.B);
+      p.chunks = 1;
+      set_pairs(p, q.parts());
+      p.status = status;
+      p.scale2 = q.scale * 1.44269504f;
+      p.stat = stat;
+      p.stat_rows = q.N;
+      p.stat_off = r0;
+      p.p_scale = p_scale;
+      p.p_out = f.P;
+      p.p_ld = f.Kp;
+      p.p_batch = f.R * f.Kp;
+      p.p_part = q.B * f.R * f.Kp;
+      p.p_parts = q.parts();
+      p.p_bf16 = !f16;
+      st = launch<kEpiGrad>(prm, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, r0),
+                            operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, k0), q.D, f.sh_p, s);
+      if (st != FK_OK) return st;
+
+      Operand po;  // P by rows (for dx); its valid width and height bound the products
+      po.p = f.P;
+      po.dtype = q.mma_dtype();
+      po.inner = kw;
+      po.rows = rw;
+      po.ld = f.Kp;
+      po.mat = f.R * f.Kp;
+      po.mats = q.parts() * q.B;
+      po.batch_step = 1;
+      po.part_step = static_cast<int>(q.B);
+      po.mn = false;
+      po.off = 0;
+      Problem base = {};
+      base.batches = static_cast<int>(q.B);
+      base.status = status;
+      set_pairs(base, q.parts());
+      base.fscale = q.scale / p_scale;
+      base.f_num = factor;
+      base.f_den = q.reduction == 1 ? count : nullptr;
+      if (gx.p) {
+        Operand co = operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, true, k0);
+        st = grad_product(q, base, po, co, rw, kw, f.sh_x, f.split_x, f.acc_x, q.N, r0, f.ld, piece == 0,
+                          piece + 1 == f.n_pieces, gx, r0, s);
+        if (st != FK_OK) return st;
+      }
+      if (gc.p) {
+        Operand pt = po;
+        pt.mn = true;
+        Operand xo = operand(q, q.x, f.xc, q.B, q.N, q.xs, true, r0);
+        st = grad_product(q, base, pt, xo, kw, rw, f.sh_c, f.split_c, f.acc_c, f.Kp, 0, f.ld, chunk == 0,
+                          chunk + 1 == f.n_chunks, gc, k0, s);
+        if (st != FK_OK) return st;
+      }
+    }
+  }
+  return FK_OK;
+}
+
+static int make(Xent& q, const void* x, const void* c, const void* labels, int dtype, int labels_dtype,
+                int64_t B, int64_t N, int64_t K, int64_t D, const int64_t* xs, const int64_t* cs,
+                const int64_t* ls, float scale, int64_t ignore_index, int reduction, const char* who) {
+  q.x = x;
+  q.c = c;
+  q.dtype = dtype;
+  q.B = B;
+  q.N = N;
+  q.K = K;
+  q.D = D;
+  q.y.p = labels;
+  q.y.dtype = labels_dtype;
+  q.y.ignore = ignore_index;
+  q.scale = scale;
+  q.reduction = reduction;
+  if (!xs || !cs || !ls) return fail(FK_ERR_INVALID_ARG, "%s: null strides", who);
+  for (int i = 0; i < 3; ++i) {
+    q.xs[i] = xs[i];
+    q.cs[i] = cs[i];
+  }
+  q.y.sb = ls[0];
+  q.y.sn = ls[1];
+  return check_args(q, who);
+}
+
+static int check_workspace(const void* ws, size_t have, size_t need, const char* who) {
+  if (need == 0) return FK_OK;
+  if (!ws || have < need || reinterpret_cast<uintptr_t>(ws) % 256)
+    return fail(FK_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who,
+                need, have);
+  return FK_OK;
+}
+
+}  // namespace head
+}  // namespace fk
+
+using namespace fk;
+using namespace fk::head;
+
+extern "C" size_t fk_xent_workspace_size(const void* x, const void* centroids, int dtype, int64_t B,
+                                         int64_t N, int64_t K, int64_t D, const int64_t* x_strides3,
+                                         const int64_t* c_strides3, int reduction, int backward_x,
+                                         int backward_c) {
+  Xent q;
+  const int64_t ls[2] = {0, 0};
+  if (make(q, x, centroids, nullptr, dtype, FK_I32, B, N, K, D, x_strides3, c_strides3, ls, 1.0f, 0,
+           reduction, "fk_xent_workspace_size") != FK_OK ||
+      B == 0 || N == 0)
+    return 0;
+  return backward_x || backward_c ? plan_backward(q, backward_x != 0, backward_c != 0, nullptr).bytes
+                                  : plan_forward(q, nullptr).bytes;
+}
+
+extern "C" int fk_xent_forward(const void* x, const void* centroids, const void* labels, int dtype,
+                               int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
+                               const int64_t* x_strides3, const int64_t* c_strides3,
+                               const int64_t* l_strides2, float scale, int64_t ignore_index,
+                               int reduction, float* loss, float* row_stats, int32_t* count,
+                               void* workspace, size_t workspace_bytes, int32_t* dev_status,
+                               void* stream) {
+  Xent q;
+  int st = make(q, x, centroids, labels, dtype, labels_dtype, B, N, K, D, x_strides3, c_strides3,
+                l_strides2, scale, ignore_index, reduction, "fk_xent_forward");
+  if (st != FK_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!count || (!loss && (B * N > 0 || reduction != 0)))
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: null pointer");
+  if (B == 0 || N == 0) {
+    // no rows: a sum of 0, a mean of 0 / 0 (all bits set is a NaN)
+    cudaError_t e = cudaMemsetAsync(count, 0, sizeof(int32_t), s);
+    if (e == cudaSuccess && reduction != 0)
+      e = cudaMemsetAsync(loss, reduction == 1 ? 0xff : 0, sizeof(float), s);
+    return e == cudaSuccess ? FK_OK : fail(FK_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+  }
+  if (!x || !centroids || !labels) return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: null pointer");
+  if (reinterpret_cast<uintptr_t>(row_stats) % 16)
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: row_stats must be 16-byte aligned");
+  st = check_workspace(workspace, workspace_bytes, plan_forward(q, nullptr).bytes, "fk_xent_forward");
+  if (st != FK_OK) return st;
+  return forward(q, loss, reinterpret_cast<RowStat*>(row_stats), count, workspace, dev_status, s);
+}
+
+extern "C" int fk_xent_backward(const void* x, const void* centroids, const void* labels, int dtype,
+                                int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
+                                const int64_t* x_strides3, const int64_t* c_strides3,
+                                const int64_t* l_strides2, float scale, int64_t ignore_index,
+                                int reduction, const float* row_stats, const int32_t* count,
+                                const float* grad_loss, void* grad_x, void* grad_centroids,
+                                const int64_t* gx_strides3, const int64_t* gc_strides3,
+                                void* workspace, size_t workspace_bytes, int32_t* dev_status,
+                                void* stream) {
+  Xent q;
+  int st = make(q, x, centroids, labels, dtype, labels_dtype, B, N, K, D, x_strides3, c_strides3,
+                l_strides2, scale, ignore_index, reduction, "fk_xent_backward");
+  if (st != FK_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if ((grad_x && !gx_strides3) || (grad_centroids && !gc_strides3))
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: null strides");
+  if ((grad_x && D > 1 && gx_strides3[2] != 1) || (grad_centroids && D > 1 && gc_strides3[2] != 1))
+    return fail(FK_ERR_UNSUPPORTED, "fk_xent_backward: gradient rows must have unit stride");
+  if (!grad_x && !grad_centroids) return FK_OK;
+  if (B == 0 || N == 0) {
+    if (!grad_centroids || B == 0) return FK_OK;
+    const int64_t eb = dtype_bytes(dtype);
+    for (int64_t b = 0; b < B; ++b) {
+      const cudaError_t e = cudaMemset2DAsync(static_cast<uint8_t*>(grad_centroids) + b * gc_strides3[0] * eb,
+                                              static_cast<size_t>(std::max(gc_strides3[1], D) * eb), 0,
+                                              static_cast<size_t>(D * eb), static_cast<size_t>(K), s);
+      if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaMemset2DAsync: %s", cudaGetErrorString(e));
+    }
+    return FK_OK;
+  }
+  if (!x || !centroids || !labels || !row_stats || !count || (reduction == 0 && !grad_loss))
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: null pointer");
+  if (reinterpret_cast<uintptr_t>(row_stats) % 16)
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: row_stats must be 16-byte aligned");
+  st = check_workspace(workspace, workspace_bytes,
+                       plan_backward(q, grad_x != nullptr, grad_centroids != nullptr, nullptr).bytes,
+                       "fk_xent_backward");
+  if (st != FK_OK) return st;
+  Grad gx{grad_x, grad_x ? gx_strides3[0] : 0, grad_x ? gx_strides3[1] : 0};
+  Grad gc{grad_centroids, grad_centroids ? gc_strides3[0] : 0, grad_centroids ? gc_strides3[1] : 0};
+  return backward(q, reinterpret_cast<const RowStat*>(row_stats), count, grad_loss, gx, gc, workspace,
+                  dev_status, s);
+}

@@ -14,6 +14,16 @@ from .centroid_update_triton import (
     triton_centroid_update_sorted_euclid,
 )
 from .kmeans_large import kmeans_largeN, kmeans_largeN_assign
+from .cluster_head import (
+    cluster_cross_entropy,
+    cluster_cross_entropy_grad,
+    int8_assign,
+    int8_scores,
+    quantize_rows,
+)
+
+# `__all__` is the reference's list; the cluster head's operators above, which
+# the reference lacks, are public too
 
 __all__ = [
     "batch_kmeans_Euclid",

@@ -16,6 +16,7 @@ LIB_NAME = "libflashkmeans_b200.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", LIB_NAME)
 
 FK_F16, FK_BF16, FK_F32, FK_I32, FK_I64 = 0, 1, 2, 3, 4
+FK_I8 = 6
 FK_F32_XSPLIT = 5   # float32 x split once into tf32 halves (the *_accumulate entry points)
 # Widest rows for which the drivers use FK_F32_XSPLIT: measured 11 % faster at
 # D = 128 and 256, 4 % at 512, no faster at 2048 (there the stages are fed from
@@ -47,6 +48,7 @@ _DTYPE_CODE = {
     torch.float32: FK_F32,
     torch.int32: FK_I32,
     torch.int64: FK_I64,
+    torch.int8: FK_I8,
 }
 
 _P = ctypes.c_void_p
@@ -54,6 +56,7 @@ _I = ctypes.c_int
 _L = ctypes.c_int64
 _S = ctypes.c_size_t
 _PL = ctypes.POINTER(ctypes.c_int64)
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/flash_kmeans_b200.h
 SIGNATURES = {
@@ -82,6 +85,17 @@ SIGNATURES = {
     "fk_centroid_accumulate": (_I, [_P, _I, _L, _L, _L, _L, _PL, _P, _I, _PL, _P, _P, _P, _P,
                                     _S, _P, _P]),
     "fk_centroid_finalize": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _PL, _PL, _P, _P, _I, _P]),
+    "fk_xent_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I, _I, _I]),
+    "fk_xent_forward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P, _P,
+                             _P, _P, _S, _P, _P]),
+    "fk_xent_backward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P,
+                              _P, _P, _P, _P, _PL, _PL, _P, _S, _P, _P]),
+    "fk_quantize_rows": (_I, [_P, _I, _L, _L, _L, _PL, _P, _PL, _P, _PL, _P]),
+    "fk_int8_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I]),
+    "fk_int8_scores": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _PL,
+                            _PL, _PL, _P, _S, _P, _P]),
+    "fk_int8_assign": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _PL, _PL, _PL, _PL, _PL,
+                            _PL, _P, _S, _P, _P]),
     "fk_centroid_finalize_normalized": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _PL, _PL, _P, _I,
                                              _P]),
 }

@@ -63,7 +63,10 @@ extern "C" {
 /* element types.  FK_F32_XSPLIT is accepted by the *_accumulate entry points
  * only: float32 x whose tf32 hi halves and exact rests the workspace holds,
  * split once by fk_assign_accumulate_split_x (see there). */
-enum fk_dtype { FK_F16 = 0, FK_BF16 = 1, FK_F32 = 2, FK_I32 = 3, FK_I64 = 4, FK_F32_XSPLIT = 5 };
+enum fk_dtype {
+  FK_F16 = 0, FK_BF16 = 1, FK_F32 = 2, FK_I32 = 3, FK_I64 = 4, FK_F32_XSPLIT = 5,
+  FK_I8 = 6 /* the fk_int8_* entry points only */
+};
 
 /* host-side status codes */
 enum fk_status {
@@ -254,6 +257,88 @@ int fk_centroid_finalize_normalized(float* sums, int32_t* counts, const void* ol
                                     int64_t D, const int64_t* old_strides3,
                                     const int64_t* new_strides3, float* shift_out,
                                     int reset_accumulators, void* stream);
+
+/* ------------------------------------------------------------ cluster head
+ * A head that is trained on cluster ids and answers with scores: no
+ * counterpart in the reference, whose assignments are these scores' argmax.
+ * Arguments follow the conventions above, but x and centroids may have any
+ * element strides: rows that TMA cannot address, and float32 ones, are copied
+ * into the workspace (256-byte aligned; its size depends on that, hence on the
+ * pointers and strides).  centroids with batch stride 0 are shared by all
+ * batches and read once.  Requires B*N < 2^31, and N, K, D < 2^30. */
+
+/* Softmax cross entropy of scale * x.c^T (scale positive and finite) against
+ * cluster ids, without keeping the scores:
+ *   loss[b,n] = log sum_k exp(scale x.c_k) - scale x.c_label
+ * dtype FK_F16 / FK_BF16 (float32 sums) or FK_F32 (three-part bf16 products,
+ * float32 accuracy).  labels (B,N) FK_I32 / FK_I64.  A label equal to
+ * ignore_index leaves its row out: loss 0, not counted in a mean, whatever x
+ * holds there.  Any other label outside [0, K) makes its row's loss NaN (and
+ * the gradients that it reaches) and sets FK_DEV_BAD_LABEL.
+ *   reduction  0: loss (B,N) contiguous; 1: mean over the rows that are not
+ *              ignored (NaN if there are none); 2: sum
+ *   row_stats  optional (B,N,4) float32, 16-byte aligned: what
+ *              fk_xent_backward needs of this call
+ *   count      one int32: rows that are not ignored */
+size_t fk_xent_workspace_size(const void* x, const void* centroids, int dtype, int64_t B, int64_t N,
+                              int64_t K, int64_t D, const int64_t* x_strides3,
+                              const int64_t* c_strides3, int reduction, int backward_x,
+                              int backward_c);
+int fk_xent_forward(const void* x, const void* centroids, const void* labels, int dtype,
+                    int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
+                    const int64_t* x_strides3, const int64_t* c_strides3,
+                    const int64_t* l_strides2, float scale, int64_t ignore_index, int reduction,
+                    float* loss, float* row_stats, int32_t* count, void* workspace,
+                    size_t workspace_bytes, int32_t* dev_status, void* stream);
+
+/* Gradients of fk_xent_forward's loss by x and by the centroids, in dtype;
+ * either may be NULL.  x, centroids, labels, scale, ignore_index and reduction
+ * as given to it, row_stats and count from it.  grad_loss: float32 device
+ * memory, one value (reduction 1, 2; NULL for 1.0) or (B,N) contiguous
+ * (reduction 0).  Gradient rows have unit stride.  The centroids are gone
+ * through in pieces; a piece's softmax is kept in 16 bits in the workspace
+ * (at most 256 MB, or 64 KiB * B if that is more). */
+int fk_xent_backward(const void* x, const void* centroids, const void* labels, int dtype,
+                     int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
+                     const int64_t* x_strides3, const int64_t* c_strides3,
+                     const int64_t* l_strides2, float scale, int64_t ignore_index, int reduction,
+                     const float* row_stats, const int32_t* count, const float* grad_loss,
+                     void* grad_x, void* grad_centroids, const int64_t* gx_strides3,
+                     const int64_t* gc_strides3, void* workspace, size_t workspace_bytes,
+                     int32_t* dev_status, void* stream);
+
+/* Rows of x as 8-bit integers with one scale each: scale = most / 127 and
+ * q = rint(x * (127 / most)) for the row's largest magnitude `most`, in
+ * float32.  A row with most < 1e-36 becomes zeros with scale 0; one that holds
+ * a NaN or an infinity becomes zeros with scale NaN.  q rows have unit stride. */
+int fk_quantize_rows(const void* x, int dtype, int64_t B, int64_t N, int64_t D,
+                     const int64_t* x_strides3, int8_t* q, const int64_t* q_strides3, float* scale,
+                     const int64_t* scale_strides2, void* stream);
+
+/* z[b,n,k] = ((sum_d x[b,n,d] centroids[b,k,d]) * x_scale[b,n]) * c_scale[b,k]
+ * (+ bias[b,k]): an exact int32 sum, then float32 in this order.
+ * fk_int8_scores stores z rounded to out_dtype (rows of unit stride);
+ * fk_int8_assign stores argmax_k z, as argmax counts it: the lowest index
+ * among equals, NaN before any number.  x_dtype FK_I8, or a float type whose
+ * rows are quantised within the call as by fk_quantize_rows (x_scale NULL
+ * then).  Requires D <= 65536. */
+size_t fk_int8_workspace_size(const void* x, const int8_t* centroids, int x_dtype, int64_t B,
+                              int64_t N, int64_t K, int64_t D, const int64_t* x_strides3,
+                              const int64_t* c_strides3, int argmax);
+int fk_int8_scores(const void* x, const int8_t* centroids, const float* x_scale,
+                   const float* c_scale, const float* bias, void* out, int x_dtype, int out_dtype,
+                   int64_t B, int64_t N, int64_t K, int64_t D, const int64_t* x_strides3,
+                   const int64_t* c_strides3, const int64_t* xs_strides2,
+                   const int64_t* cs_strides2, const int64_t* bias_strides2,
+                   const int64_t* out_strides3, void* workspace, size_t workspace_bytes,
+                   int32_t* dev_status, void* stream);
+int fk_int8_assign(const void* x, const int8_t* centroids, const float* x_scale,
+                   const float* c_scale, const float* bias, int32_t* out, int x_dtype, int64_t B,
+                   int64_t N, int64_t K, int64_t D, const int64_t* x_strides3,
+                   const int64_t* c_strides3, const int64_t* xs_strides2,
+                   const int64_t* cs_strides2, const int64_t* bias_strides2,
+                   const int64_t* out_strides2, void* workspace, size_t workspace_bytes,
+                   int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,175 @@
+"""Cluster head: what is refused, and the host-only entry points (CPU only)."""
+import ctypes
+
+import pytest
+import torch
+
+import flash_kmeans as fk
+
+X = torch.randn(6, 8)
+C = torch.randn(4, 8)
+Y = torch.zeros(6, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("fn", [fk.cluster_cross_entropy, fk.cluster_cross_entropy_grad])
+def test_cross_entropy_refusals(fn):
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fn(X, C, Y)
+    with pytest.raises(ValueError, match="features"):
+        fn(X, torch.randn(4, 7), Y)
+    with pytest.raises(ValueError, match="batches"):
+        fn(torch.randn(2, 6, 8), torch.randn(3, 4, 8), torch.zeros(2, 6, dtype=torch.int32))
+    with pytest.raises(ValueError, match="at least one"):
+        fn(X, torch.randn(0, 8), Y)
+    with pytest.raises(ValueError, match=r"x \(N, D\)"):
+        fn(X[0], C, Y)
+    with pytest.raises(ValueError, match=r"x \(N, D\)"):
+        fn(X, torch.randn(1, 4, 8), Y)      # centroids of more dimensions than x
+    with pytest.raises(TypeError, match="tensors"):
+        fn([1.0], C, Y)
+
+
+class _OnCuda(torch.Tensor):
+    """A CPU tensor that says it is on a GPU: the checks after the device's."""
+    is_cuda = property(lambda self: True)
+
+
+def _cuda(t):
+    return t.as_subclass(_OnCuda)
+
+
+@pytest.mark.parametrize("kw,err,match", [
+    (dict(x=X.double()), TypeError, "dtype"),
+    (dict(c=C.half()), TypeError, "centroids are"),
+    (dict(y=Y.float()), TypeError, "int32 or int64"),
+    (dict(y=Y[:5]), ValueError, "labels have shape"),
+    (dict(scale=0.0), ValueError, "positive and finite"),
+    (dict(scale=-1.0), ValueError, "positive and finite"),
+    (dict(scale=float("nan")), ValueError, "positive and finite"),
+    (dict(scale=float("inf")), ValueError, "positive and finite"),
+    (dict(reduction="max"), ValueError, "reduction"),
+])
+def test_cross_entropy_argument_checks(kw, err, match):
+    a = dict(x=X, c=C, y=Y, scale=1.0, reduction="mean") | kw
+    with pytest.raises(err, match=match):
+        fk.cluster_cross_entropy_grad(_cuda(a["x"]), _cuda(a["c"]), a["y"], scale=a["scale"],
+                                      reduction=a["reduction"])
+
+
+@pytest.mark.parametrize("g,err", [(torch.ones(6), ValueError), (torch.ones((), dtype=torch.float16), TypeError),
+                                   (2.0, TypeError)])
+def test_grad_loss_checks(g, err):
+    with pytest.raises(err, match="grad_loss"):
+        fk.cluster_cross_entropy_grad(_cuda(X), _cuda(C), Y, grad_loss=g)
+
+
+XQ, CQ = torch.zeros(6, 8, dtype=torch.int8), torch.zeros(4, 8, dtype=torch.int8)
+XS, CS = torch.ones(6), torch.ones(4)
+
+
+@pytest.mark.parametrize("fn", [fk.int8_scores, fk.int8_assign])
+@pytest.mark.parametrize("kw,err,match", [
+    (dict(x=XQ), ValueError, "x_scale goes with int8"),
+    (dict(x_scale=XS), ValueError, "x_scale goes with int8"),
+    (dict(c=C), TypeError, "must be int8"),
+    (dict(x=X.double()), TypeError, "dtype"),
+    (dict(c_scale=CS.double()), TypeError, "c_scale"),
+    (dict(c_scale=torch.ones(5)), ValueError, "c_scale has shape"),
+    (dict(bias=torch.ones(6)), ValueError, "bias has shape"),
+    (dict(x=XQ, x_scale=torch.ones(4)), ValueError, "x_scale has shape"),
+    (dict(out=torch.zeros(3)), ValueError, "out must be"),
+])
+def test_int8_argument_checks(fn, kw, err, match):
+    a = dict(x=X, c=CQ, c_scale=CS) | kw
+    x, c, cs = _cuda(a.pop("x")), _cuda(a.pop("c")), a.pop("c_scale")
+    with pytest.raises(err, match=match):
+        fn(x, c, cs, **a)
+
+
+def test_int8_output_checks():
+    with pytest.raises(TypeError, match="out_dtype"):
+        fk.int8_scores(_cuda(X), _cuda(CQ), CS, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="unit stride"):
+        fk.int8_scores(_cuda(X), _cuda(CQ), CS, out=torch.zeros(4, 6).t())
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fk.int8_scores(X, CQ, CS)
+
+
+def test_quantize_rows_refusals():
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        fk.quantize_rows(X)
+    with pytest.raises(TypeError, match="dtype"):
+        fk.quantize_rows(XQ)
+    with pytest.raises(ValueError, match=r"\(N, D\)"):
+        fk.quantize_rows(X[0])
+    with pytest.raises(ValueError, match="at least one"):
+        fk.quantize_rows(torch.zeros(3, 0))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from flash_kmeans import _native
+    return _native.load()
+
+
+P = ctypes.c_void_p(1 << 20)
+L3 = ctypes.c_int64 * 3
+L2 = ctypes.c_int64 * 2
+
+
+def _fwd(lib, x=P, c=P, y=P, dtype=1, ydtype=3, B=1, N=4, K=3, D=8, scale=1.0, reduction=1, loss=P,
+         stats=None, count=P, ws=None, nbytes=0):
+    return lib.fk_xent_forward(x, c, y, dtype, ydtype, B, N, K, D, L3(32, 8, 1), L3(24, 8, 1),
+                               L2(4, 1), scale, -100, reduction, loss, stats, count, ws, nbytes,
+                               None, None)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(K=0), 1), (dict(D=0), 1), (dict(N=-1), 1), (dict(dtype=3), 1), (dict(dtype=6), 1),
+    (dict(ydtype=2), 1), (dict(scale=0.0), 1), (dict(scale=float("inf")), 1), (dict(scale=3e38), 1),
+    (dict(reduction=3), 1), (dict(x=None), 1), (dict(loss=None), 1), (dict(count=None), 1),
+    (dict(stats=ctypes.c_void_p(8)), 1), (dict(N=1 << 30), 2), (dict(B=2, N=(1 << 30) - 1, K=1 << 30), 2),
+    (dict(), 3),                                     # no workspace
+    (dict(ws=ctypes.c_void_p((1 << 20) + 16), nbytes=1 << 30), 3),
+])
+def test_xent_entry_point_checks(lib, kw, code):
+    assert _fwd(lib, **kw) == code
+    assert lib.fk_last_error()
+
+
+def test_xent_workspace_covers_copies_and_the_piece(lib):
+    def size(dtype, D, bx, bc, N=1000, K=5000, p=P):
+        return lib.fk_xent_workspace_size(p, p, dtype, 1, N, K, D, L3(N * D, D, 1), L3(K * D, D, 1),
+                                          1, bx, bc)
+    plain = size(1, 128, 0, 0)
+    assert 0 < plain < 8 << 20
+    # rows of 200 bytes are copied, padded
+    assert size(1, 100, 0, 0) >= plain + 6000 * 104 * 2
+    # float32: three bf16 parts of x and c
+    assert size(2, 128, 0, 0) >= plain + 3 * 6000 * 128 * 2
+    # backward: a copy of x and a piece of the softmax
+    assert size(1, 128, 1, 1) >= 1000 * 128 * 2 + 1000 * 5000 * 2
+    # and never more than a piece of a long vocabulary
+    assert size(1, 128, 1, 1, N=1 << 16, K=1 << 20) < (1 << 28) + (1 << 16) * 128 * 8 + (1 << 27)
+    assert lib.fk_xent_workspace_size(P, P, 1, 0, 4, 3, 8, L3(0, 8, 1), L3(24, 8, 1), 1, 0, 0) == 0
+
+
+def test_int8_entry_point_checks(lib):
+    def scores(x=P, c=P, sx=P, sc=P, out=P, xdt=6, odt=2, B=1, N=4, K=3, D=16, ostr=(12, 3, 1), n=0):
+        return lib.fk_int8_scores(x, c, sx, sc, None, out, xdt, odt, B, N, K, D, L3(64, 16, 1),
+                                  L3(48, 16, 1), L2(4, 1), L2(3, 1), None, L3(*ostr), None, n, None,
+                                  None)
+    assert scores(K=0) == 1 and scores(D=0) == 1 and scores(xdt=3) == 1 and scores(odt=6) == 1
+    assert scores(sx=None) == 1 and scores(xdt=1) == 1 and scores(sc=None) == 1 and scores(out=None) == 1
+    assert scores(D=65537) == 2 and b"overflow" in lib.fk_last_error()
+    assert scores(N=1 << 30) == 2
+    assert scores(ostr=(12, 1, 4)) == 2
+    assert scores(xdt=1, sx=None) == 3              # float x needs room for its integers
+    assert scores(N=0) == 0
+    assert lib.fk_quantize_rows(P, 6, 1, 4, 8, L3(32, 8, 1), P, L3(32, 8, 1), P, L2(4, 1), None) == 1
+    assert lib.fk_quantize_rows(P, 1, 1, 4, 8, L3(32, 8, 1), P, L3(32, 1, 4), P, L2(4, 1), None) == 2
+    assert lib.fk_quantize_rows(P, 1, 1, 0, 8, L3(32, 8, 1), P, L3(32, 8, 1), P, L2(4, 1), None) == 0
+    # 8-bit rows in place need no workspace, others a padded copy
+    ok = lib.fk_int8_workspace_size(P, P, 6, 1, 300, 300, 128, L3(0, 128, 1), L3(0, 128, 1), 0)
+    odd = lib.fk_int8_workspace_size(P, P, 6, 1, 300, 300, 100, L3(0, 100, 1), L3(0, 100, 1), 0)
+    assert ok == 0 and odd >= 600 * 112

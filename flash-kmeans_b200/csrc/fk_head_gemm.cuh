@@ -48,11 +48,11 @@ enum Epilogue {
 __host__ __device__ constexpr bool running(int epi) { return epi == kEpiLse || epi == kEpiArgmax; }
 __host__ __device__ constexpr bool integer(int epi) { return epi == kEpiScores || epi == kEpiArgmax; }
 
-// What the backward pass needs of a row: P = exp2(z * scale2 - m2) * coef at
+// What the backward pass needs of a row: P = exp2((z - top) * scale2) * coef at
 // other columns, `at_label` at the label's.  An ignored row has coef = at_label = 0.
 struct RowStat {
-  float m2;        // row maximum of z * scale2, the label's column included
-  float coef;      // weight / sum_k exp2(z_k * scale2 - m2)
+  float top;       // largest x.c of the row, the label's included
+  float coef;      // weight / sum_k exp2((z_k - top) * scale2)
   float at_label;  // weight * (softmax - 1) at the label
   int label;       // the label's column, -1 for none
 };
@@ -81,10 +81,10 @@ struct Problem {
   int64_t label_sb, label_sn;
   int64_t ignore_index;
   float2* partial;          // kEpiLse / kEpiArgmax: [batch][chunk * 2 + half][row]
-  float* z_label;           // kEpiLse: z * scale2 of the label, [batch][row]
   const RowStat* stat;      // kEpiGrad: [batch][stat_rows], the row block starts at stat_off
   int64_t stat_rows;
   int64_t stat_off;
+  int col_off;              // first column of the piece
   float p_scale;            // kEpiGrad: power of two that keeps float16 P out of its subnormals
   void* p_out;              // kEpiGrad: [part][batch][M][p_ld] 16-bit
   int64_t p_ld, p_part, p_batch;
@@ -146,11 +146,6 @@ __device__ __forceinline__ uint64_t pack2(float a, float b) {
 }
 __device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
@@ -279,7 +274,15 @@ __device__ __forceinline__ void epilogue_sync() {
 }
 
 // ------------------------------------------------------------------- kernel
-template <int CG, int BN, int EPI>
+// EXACT: the tensor core adds to its float32 accumulator with truncation, a
+// bias of up to 2^-24 of the partial sum for every 16 elements.  16-bit inputs
+// leave it at that (the label's score, which the loss hangs on most, is summed
+// in ordinary float32 by the combine kernel); float32 inputs move the
+// accumulator to registers every kSegment steps and add there, rounded.  Their
+// tiles are 128 columns wide: 64 sums a thread leave the epilogue its registers.
+constexpr int kSegment = 4;       // of 64 elements: 16 truncated additions
+
+template <int CG, int BN, int EPI, bool EXACT>
 __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__ Params prm) {
   using S = Shape<CG, BN, EPI>;
   const Problem& p = prm.p;
@@ -392,13 +395,17 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
       Walk<EPI> walk(p, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
-        if (!mbar_wait_cluster(&acc_empty[buf], aphase ^ 1, abort_flag, p.status,
-                               FK_DEV_WAIT_TIMEOUT))
-          break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * BN;
         uint32_t accumulate = 0;
         for (int it = t.it0; it < t.it1; ++it) {
+          if (accumulate == 0) {
+            if (!mbar_wait_cluster(&acc_empty[buf], aphase ^ 1, abort_flag, p.status,
+                                   FK_DEV_WAIT_TIMEOUT)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          const uint32_t d = tmem + buf * BN;
           if (!mbar_wait(&full[stage], phase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT)) {
             ok = false;
             break;
@@ -421,11 +428,13 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             stage = 0;
             phase ^= 1;
           }
+          if (it + 1 == t.it1 || (EXACT && (it + 1 - t.it0) % kSegment == 0)) {
+            mma_commit_cg<CG>(&acc_full[buf]);
+            buf ^= 1;
+            if (buf == 0) aphase ^= 1;
+            accumulate = 0;
+          }
         }
-        if (!ok) break;
-        mma_commit_cg<CG>(&acc_full[buf]);
-        buf ^= 1;
-        if (buf == 0) aphase ^= 1;
       }
     }
   } else if (warp >= kCtlWarps) {
@@ -499,34 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
         epilogue_sync();
       }
 
-      const bool got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
-      if (!__all_sync(0xffffffffu, got)) {
-        if constexpr (EPI == kEpiArgmax) {
-          // the other warps meet at the barrier of every tile: keep to it
-          if (t.last && p.chunks == 1) epilogue_sync();
-          buf ^= 1;
-          if (buf == 0) aphase ^= 1;
-          continue;
-        } else {
-          break;
-        }
-      }
-      tc_fence_after();
-      const uint32_t taddr = tmem + buf * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
-
-      uint32_t r[2][32];
-      tmem_ld32(taddr, r[0]);
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        uint32_t (&v)[32] = r[c & 1];
-        tmem_ld_wait(v);
-        if (c + 1 < kChunks) tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-        else {
-          // the accumulator is in registers: hand it back
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
-        }
+      // one chunk of 32 columns, accumulators in v
+      auto chunk = [&](const int c, uint32_t (&v)[32]) {
         const int cc = col0 + c * 32;
 
         if constexpr (EPI == kEpiLse) {
@@ -538,15 +521,10 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           }
           const int64_t rel = label - cc;
           if (rel >= 0 && rel < 32 && rel < left) {
-            // the label's own term stays out of the sum and is kept aside
-            float zy = 0.0f;
+            // the label's own term stays out of the sum
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (rel == i) {
-                zy = __uint_as_float(v[i]);
-                v[i] = 0xff800000u;
-              }
-            if (row_ok) p.z_label[static_cast<int64_t>(t.b) * p.M + row] = zy * p.scale2;
+              if (rel == i) v[i] = 0xff800000u;
           }
           float mx[4];
 #pragma unroll
@@ -557,28 +535,30 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             for (int q = 0; q < 4; ++q)
               mx[q] = i + 4 + q < 32 ? fmax3(mx[q], __uint_as_float(v[i + q]), __uint_as_float(v[i + 4 + q]))
                                      : fmaxf(mx[q], __uint_as_float(v[i + q]));
-          const float m_new = fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2);
+          // differences of scores first, then the scale: exact near the maximum,
+          // and never above 0, however large the scores are
+          const float m_new = fmaxf(run_m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           const float m_use = m_new == -INFINITY ? 0.0f : m_new;
           const uint64_t s2 = pack2(p.scale2, p.scale2), nm = pack2(-m_use, -m_use);
           uint64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float e0, e1;
-            unpack2(fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), s2, nm), e0, e1);
+            unpack2(mul2(add2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), nm), s2), e0, e1);
             sum[(i >> 1) & 3] = add2(sum[(i >> 1) & 3], pack2(ex2(e0), ex2(e1)));
           }
           float s0, s1;
           unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
-          run_s = run_s * ex2(run_m - m_use) + (s0 + s1);
+          run_s = run_s * ex2((run_m - m_use) * p.scale2) + (s0 + s1);
           run_m = m_new;
         } else if constexpr (EPI == kEpiGrad) {
           // softmax minus one-hot, times the row's weight
-          const int rel = st.label - cc;
-          const uint64_t s2 = pack2(p.scale2, p.scale2), nm = pack2(-st.m2, -st.m2);
+          const int rel = st.label - p.col_off - cc;
+          const uint64_t s2 = pack2(p.scale2, p.scale2), nm = pack2(-st.top, -st.top);
           float e[32];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            unpack2(fma2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), s2, nm), e[i], e[i + 1]);
+            unpack2(mul2(add2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), nm), s2), e[i], e[i + 1]);
             e[i] = ex2(e[i]) * st.coef;
             e[i + 1] = ex2(e[i + 1]) * st.coef;
           }
@@ -725,6 +705,81 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
                   make_float4(z[q * 4], z[q * 4 + 1], z[q * 4 + 2], z[q * 4 + 3]);
           }
         }
+      };
+
+      bool got = true;
+      if constexpr (EXACT) {
+        float sum[kChunks][32];
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
+        for (int it = t.it0; it < t.it1; it += kSegment) {
+          got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p.status,
+                                                  FK_DEV_WAIT_TIMEOUT));
+          if (!got) break;
+          tc_fence_after();
+          const uint32_t taddr =
+              tmem + buf * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t v[32];
+            tmem_ld32(taddr + c * 32, v);
+            tmem_ld_wait(v);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              unpack2(add2(pack2(sum[c][i], sum[c][i + 1]),
+                           pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1]))),
+                      sum[c][i], sum[c][i + 1]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
+          buf ^= 1;
+          if (buf == 0) aphase ^= 1;
+        }
+        if (!got) break;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          uint32_t v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(sum[c][i]);
+          chunk(c, v);
+        }
+      } else {
+        got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p.status,
+                                                FK_DEV_WAIT_TIMEOUT));
+        if (!got) {
+          if constexpr (EPI == kEpiArgmax) {
+            // the other warps meet at the barriers of every tile: keep to them
+            if (t.last && p.chunks == 1) epilogue_sync();
+            buf ^= 1;
+            if (buf == 0) aphase ^= 1;
+            continue;
+          } else {
+            break;
+          }
+        }
+        tc_fence_after();
+        const uint32_t taddr =
+            tmem + buf * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+        uint32_t r[2][32];
+        tmem_ld32(taddr, r[0]);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          tmem_ld_wait(r[c & 1]);
+          if (c + 1 < kChunks) {
+            tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
+          } else {
+            // the accumulator is in registers: hand it back
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
+          }
+          chunk(c, r[c & 1]);
+        }
+        buf ^= 1;
+        if (buf == 0) aphase ^= 1;
       }
 
       if constexpr (EPI == kEpiLse) {
@@ -763,8 +818,6 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           }
         }
       }
-      buf ^= 1;
-      if (buf == 0) aphase ^= 1;
     }
   }
 

@@ -33,8 +33,9 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // 256 x 256 tiles on CTA pairs once they give half of the 74 pairs a tile;
 // below that 128 x 128 tiles, and 128 x 64 ones when even those leave most SMs
 // idle.  Measured in profiles/cluster_head.md.
-inline ShapeChoice choose_shape(int64_t M, int64_t N, int64_t batches, int64_t splittable) {
-  if (M > 128 && ceil_div(M, 256) * ceil_div(N, 256) * batches * splittable >= 37) return {2, 256};
+inline ShapeChoice choose_shape(int64_t M, int64_t N, int64_t batches, int64_t splittable, bool exact) {
+  const int wide = exact ? 128 : 256;
+  if (M > 128 && ceil_div(M, 256) * ceil_div(N, wide) * batches * splittable >= 37) return {2, wide};
   if (ceil_div(M, 128) * ceil_div(N, 128) * batches * splittable >= 100) return {1, 128};
   return {1, 64};
 }
@@ -58,10 +59,10 @@ inline int choose_chunks(int64_t items, int64_t units, int64_t slots, int64_t mo
 
 int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows);
 
-template <int CG, int BN, int EPI>
+template <int CG, int BN, int EPI, bool EXACT>
 int launch_shape(Params& prm, cudaStream_t s) {
   using S = Shape<CG, BN, EPI>;
-  auto kern = head_gemm<CG, BN, EPI>;
+  auto kern = head_gemm<CG, BN, EPI, EXACT>;
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return fail(FK_ERR_CUDA, "bad current device %d", dev);
   static std::atomic<bool> ready[64];
@@ -130,9 +131,16 @@ int launch(Params& prm, const Operand& a, const Operand& b, int64_t kdim, ShapeC
   if (st != FK_OK) return st;
   st = encode_operand(&prm.b, b, b.mn ? 64 : sh.bn / sh.cg);
   if (st != FK_OK) return st;
-  if (sh.cg == 2) return launch_shape<2, 256, EPI>(prm, s);
-  if (sh.bn == 128) return launch_shape<1, 128, EPI>(prm, s);
-  return launch_shape<1, 64, EPI>(prm, s);
+  if constexpr (!integer(EPI)) {
+    if (p.npairs > 1) {
+      if (sh.cg == 2) return launch_shape<2, 128, EPI, true>(prm, s);
+      if (sh.bn == 128) return launch_shape<1, 128, EPI, true>(prm, s);
+      return launch_shape<1, 64, EPI, true>(prm, s);
+    }
+  }
+  if (sh.cg == 2) return launch_shape<2, 256, EPI, false>(prm, s);
+  if (sh.bn == 128) return launch_shape<1, 128, EPI, false>(prm, s);
+  return launch_shape<1, 64, EPI, false>(prm, s);
 }
 
 inline int64_t slots_of(ShapeChoice sh) {

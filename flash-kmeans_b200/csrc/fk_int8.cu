@@ -229,7 +229,7 @@ static ScoresPlan plan_scores(const Scores& q, bool argmax, void* ws) {
     used += align_up(static_cast<size_t>(bytes), 256);
     return p;
   };
-  f.sh = choose_shape(q.N, q.K, q.B, 1);
+  f.sh = choose_shape(q.N, q.K, q.B, 1, false);
   f.chunks = argmax ? choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                                     2 * slots_of(f.sh), 0.25)
                     : 1;

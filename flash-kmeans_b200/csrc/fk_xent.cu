@@ -143,7 +143,10 @@ constexpr int kCombineWarps = 16;
 
 struct CombineParams {
   const float2* partial;   // [batch][pieces][N]
-  const float* z_label;    // [batch][N], times log2(e)
+  const void *x, *c;       // for the label's score
+  int dtype, D, vec;       // vec: rows of both can be read 16 bytes at a time
+  int64_t xs[3], cs[3];
+  float scale, scale2;     // scale2: times log2(e)
   const void* labels;
   int label_dtype;
   int64_t lb, ln, ignore;
@@ -158,8 +161,29 @@ struct CombineParams {
   int* status;
 };
 
+// x[n] . c[y] by one warp, in float32 (each lane's partial sum, then a tree).
+template <typename T>
+__device__ __forceinline__ float row_dot(const T* x, int64_t xd, const T* c, int64_t cd, int D, bool vec,
+                                         int lane) {
+  constexpr int E = 16 / sizeof(T);
+  float s = 0.0f;
+  int d = 0;
+  if (vec) {
+    for (d = lane * E; d + E <= D; d += 32 * E) {
+      const uint4 a = *reinterpret_cast<const uint4*>(x + d), b = *reinterpret_cast<const uint4*>(c + d);
+      const T *pa = reinterpret_cast<const T*>(&a), *pb = reinterpret_cast<const T*>(&b);
+#pragma unroll
+      for (int i = 0; i < E; ++i) s = fmaf(Elem<T>::to_f(pa[i]), Elem<T>::to_f(pb[i]), s);
+    }
+    d = D / E * E;
+  }
+  for (d += lane; d < D; d += 32) s = fmaf(Elem<T>::to_f(x[d * xd]), Elem<T>::to_f(c[d * cd]), s);
+  return warp_sum(s);
+}
+
 __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const CombineParams p) {
   __shared__ float2 sm[kCombineWarps][33];
+  __shared__ float z_label[32];
   __shared__ double2 red[kCombineWarps];
   __shared__ bool last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -173,11 +197,30 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
       const float mn = fmaxf(m, v.x);
       const float mu = mn == -INFINITY ? 0.0f : mn;
       // a piece whose exponents were NaN has a NaN sum, which stays
-      s = s * ex2(m - mu) + v.y * ex2(v.x - mu);
+      s = s * ex2((m - mu) * p.scale2) + v.y * ex2((v.x - mu) * p.scale2);
       m = mn;
     }
   }
   sm[warp][lane] = make_float2(m, s);
+  for (int i = warp; i < 32; i += kCombineWarps) {
+    const int64_t n = (blockIdx.x % p.row_blocks) * 32 + i;
+    if (n >= p.N) break;
+    const int64_t y = load_label(p.labels, b * p.lb + n * p.ln, p.label_dtype);
+    float z = 0.0f;
+    if (y != p.ignore && y >= 0 && y < p.K) {
+      const int64_t xo = b * p.xs[0] + n * p.xs[1], co = b * p.cs[0] + y * p.cs[1];
+      if (p.dtype == FK_F32)
+        z = row_dot(static_cast<const float*>(p.x) + xo, p.xs[2], static_cast<const float*>(p.c) + co,
+                    p.cs[2], p.D, p.vec, lane);
+      else if (p.dtype == FK_F16)
+        z = row_dot(static_cast<const __half*>(p.x) + xo, p.xs[2], static_cast<const __half*>(p.c) + co,
+                    p.cs[2], p.D, p.vec, lane);
+      else
+        z = row_dot(static_cast<const __nv_bfloat16*>(p.x) + xo, p.xs[2],
+                    static_cast<const __nv_bfloat16*>(p.c) + co, p.cs[2], p.D, p.vec, lane);
+    }
+    if (lane == 0) z_label[i] = z;
+  }
   __syncthreads();
   double sum = 0.0, cnt = 0.0;
   if (warp == 0) {
@@ -185,7 +228,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
       const float2 v = sm[w][lane];
       const float mn = fmaxf(m, v.x);
       const float mu = mn == -INFINITY ? 0.0f : mn;
-      s = s * ex2(m - mu) + v.y * ex2(v.x - mu);
+      s = s * ex2((m - mu) * p.scale2) + v.y * ex2((v.x - mu) * p.scale2);
       m = mn;
     }
     if (row < p.N) {
@@ -199,15 +242,15 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
         st = {0.0f, NAN, NAN, -1};
         if (p.status) atomicCAS(p.status, 0, FK_DEV_BAD_LABEL);
       } else if (!ignored) {
-        const float ty = p.z_label[r];
+        const float ty = z_label[lane];
         const float d = m - ty;  // -inf for K = 1
         // sum over the others, relative to the larger of the label's term and theirs
         const float top = fmaxf(m, ty);
-        const float others = s * ex2(m - top);
-        const float own = ex2(ty - top);
-        loss = d > 0.0f ? fmaf(d, 0.69314718056f, logf(others + own)) : log1pf(others);
+        const float others = s * ex2((m - top) * p.scale2);
+        const float own = ex2((ty - top) * p.scale2);
+        loss = d > 0.0f ? fmaf(d, p.scale, logf(others + own)) : log1pf(others);
         if (!(s == s) || !(ty < INFINITY)) loss = NAN;  // NaN scores, or inf - inf
-        st.m2 = top;
+        st.top = top;
         st.coef = 1.0f / (others + own);
         st.at_label = expm1f(-loss);
         st.label = static_cast<int>(y);
@@ -409,7 +452,6 @@ struct ForwardPlan {
   int64_t row_blocks;
   uint16_t *xc, *cc;
   float2* partial;
-  float* z_label;
   double2* block_part;
   uint32_t* ticket;
   size_t bytes;
@@ -418,7 +460,7 @@ struct ForwardPlan {
 static ForwardPlan plan_forward(const Xent& q, void* ws) {
   ForwardPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
-  f.sh = choose_shape(q.N, q.K, q.B, 1);
+  f.sh = choose_shape(q.N, q.K, q.B, 1, q.parts() > 1);
   f.chunks = choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                            2 * slots_of(f.sh), 0.25);
   f.row_blocks = ceil_div(q.N, 32);
@@ -429,7 +471,6 @@ static ForwardPlan plan_forward(const Xent& q, void* ws) {
              ? nullptr
              : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
   f.partial = b.take<float2>(q.B * f.chunks * 2 * q.N);
-  f.z_label = b.take<float>(q.B * q.N);
   f.block_part = b.take<double2>(q.B * f.row_blocks);
   f.ticket = b.take<uint32_t>(1);
   f.bytes = b.used;
@@ -458,7 +499,6 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   p.label_sn = q.y.sn;
   p.ignore_index = q.y.ignore;
   p.partial = f.partial;
-  p.z_label = f.z_label;
   p.zero = f.ticket;
   p.zero_n = 1;
   p.status = status;
@@ -467,7 +507,22 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   if (st != FK_OK) return st;
   CombineParams cp = {};
   cp.partial = f.partial;
-  cp.z_label = f.z_label;
+  cp.x = q.x;
+  cp.c = q.c;
+  cp.dtype = q.dtype;
+  for (int i = 0; i < 3; ++i) {
+    cp.xs[i] = q.xs[i];
+    cp.cs[i] = q.cs[i];
+  }
+  cp.D = static_cast<int>(q.D);
+  cp.scale = q.scale;
+  cp.scale2 = q.scale * 1.44269504f;
+  const int64_t eb = dtype_bytes(q.dtype);
+  auto aligned = [&](const void* t, int64_t B, int64_t M, const int64_t* st) {
+    return (st[2] == 1 || q.D == 1) && reinterpret_cast<uintptr_t>(t) % 16 == 0 &&
+           (M == 1 || st[1] * eb % 16 == 0) && (B == 1 || st[0] * eb % 16 == 0);
+  };
+  cp.vec = aligned(q.x, q.B, q.N, q.xs) && aligned(q.c, q.B, q.K, q.cs);
   cp.labels = q.y.p;
   cp.label_dtype = q.y.dtype;
   cp.lb = q.y.sb;
@@ -518,10 +573,10 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   f.n_chunks = ceil_div(q.N, f.R);
   const int64_t kw = std::min(f.Kp, q.K);
   const int pairs = q.parts() == 3 ? 6 : 1;
-  f.sh_p = choose_shape(f.R, kw, q.B, 1);
+  f.sh_p = choose_shape(f.R, kw, q.B, 1, q.parts() > 1);
   const int64_t steps_x = pairs * ceil_div(kw, 64), steps_c = pairs * ceil_div(f.R, 64);
   auto pick = [&](int64_t M, int64_t steps, ShapeChoice* sh) {
-    *sh = choose_shape(M, q.D, q.B, std::max<int64_t>(1, steps / 16));
+    *sh = choose_shape(M, q.D, q.B, std::max<int64_t>(1, steps / 16), q.parts() > 1);
     const int64_t items = q.B * ceil_div(M, sh->bm()) * ceil_div(q.D, sh->bn);
     return items >= 4 * slots_of(*sh) ? 1 : choose_chunks(items, steps, slots_of(*sh), 16, 3.0);
   };
@@ -634,6 +689,7 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       p.stat = stat;
       p.stat_rows = q.N;
       p.stat_off = r0;
+      p.col_off = static_cast<int>(k0);
       p.p_scale = p_scale;
       p.p_out = f.P;
       p.p_ld = f.Kp;

@@ -9,8 +9,8 @@
 // for 16-bit types, MN-major (the contraction axis is the row axis in memory),
 // so x.c^T, P.c and P^T.x all run without a transposed copy.
 //
-// Warp roles: warp 0 TMA producer, warp 1 MMA issuer (one thread), warps 4-11
-// epilogue (four TMEM lane quarters x two column halves).  With CG = 2 two
+// Warp roles: warp 0 TMA producer, warp 1 MMA issuer (one thread), warps 4 and
+// up epilogue (four TMEM lane quarters x two or four column parts).  With CG = 2 two
 // CTAs of a cluster form one 256 x 256 tile (cta_group::2): each loads its own
 // 128 rows of A and its own half of B, so a CTA moves 32 KB per 64 columns of
 // the contraction instead of the 48 KB of a 128 x 256 tile, which is what
@@ -30,13 +30,9 @@ namespace head {
 
 constexpr int kMaxPairs = 6;
 constexpr int kCtlWarps = 4;
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kCtlWarps + kEpiWarps) * 32;
 constexpr int kStageRowBytes = 128;            // one swizzle row: 64 16-bit or 128 8-bit elements
-constexpr int kStagingBytes = kEpiWarps * 4096;  // 32 rows x 128 bytes for each epilogue warp
-
-constexpr int kTableBytes = 2 * 2 * 256 * 4;     // two tables of 256 column scales and biases
-constexpr int kSlotBytes = 128 * 8;              // one (value, index) for each row of the tile
+constexpr int kTableBytes = 2 * 2 * 256 * 4;   // two tables of 256 column scales and biases
+constexpr int kSlotBytes = 3 * 128 * 8;        // (value, index) of a row from the other column parts
 
 enum Epilogue {
   kEpiLse = 0,     // running maximum and sum of exp2 over the columns
@@ -80,7 +76,7 @@ struct Problem {
   int label_dtype;
   int64_t label_sb, label_sn;
   int64_t ignore_index;
-  float2* partial;          // kEpiLse / kEpiArgmax: [batch][chunk * 2 + half][row]
+  float2* partial;          // kEpiLse / kEpiArgmax: [batch][chunk][part][row]
   const RowStat* stat;      // kEpiGrad: [batch][stat_rows], the row block starts at stat_off
   int64_t stat_rows;
   int64_t stat_off;
@@ -123,13 +119,29 @@ struct Shape {
   static constexpr int kABytes = kARows * kStageRowBytes;
   static constexpr int kBBytes = kBRows * kStageRowBytes;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  // the argmax keeps column tables and the best chunk of every row besides
-  static constexpr int kStages = (EPI == kEpiArgmax ? 160 : 192) * 1024 / kStageBytes;
+  // Epilogue warps: four TMEM lane quarters x column parts.  Four parts give
+  // each scheduler four warps, which is what hides the exponentials' and the
+  // accumulator loads' latency (two left 70 % of the issue slots empty).
+  static constexpr int kParts = BN >= 128 ? 4 : 2;
+  static constexpr int kEpiWarps = 4 * kParts;
+  static constexpr int kThreads = (kCtlWarps + kEpiWarps) * 32;
+  // shared memory of an epilogue warp: 32 rows of 128 bytes (64 for P)
+  static constexpr int kStaging = (EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : 4096);
+  static constexpr int kStagingBytes = kEpiWarps * kStaging;
   static constexpr int kExtra = EPI == kEpiArgmax ? kTableBytes + kSlotBytes : 0;
-  static constexpr int kTmemCols = 2 * BN;
+  static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes - kExtra;
+  static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
+  // accumulators in turn: the more, the less a tile waits for the one before
+  static constexpr int kBufs = BN >= 256 ? 2 : 4;
+  static constexpr int kTmemCols = kBufs * BN;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kStagingBytes + kExtra + 512;
-  static_assert(kSmem <= 232448, "shared memory");
+  static_assert(kStages >= 4 && kSmem <= 232448, "shared memory");
 };
+
+template <int CG, int BN, int EPI>
+constexpr int threads_of() { return Shape<CG, BN, EPI>::kThreads; }
+// column parts that write partial results of a row
+inline int parts_of(int bn) { return bn >= 128 ? 4 : 2; }
 
 // ------------------------------------------------------------------ helpers
 __device__ __forceinline__ float ex2(float v) {
@@ -178,86 +190,125 @@ struct Tile {
   bool first, last;    // of the item
 };
 
+// Every role walks the tiles by itself, in one thread: the decoding is kept to
+// 32-bit divisions, once per item (64-bit ones at every tile took 2000 cycles,
+// more than a short tile's products).
 template <int EPI>
 struct Walk {
   const Problem& p;
-  int64_t item, total;
-  int step;
-  int j, j_begin, j_end;
+  uint32_t item, total;
+  const uint32_t step;
+  Tile t;
+  int j_begin, j_end, w_end, wl, w0;
 
-  __device__ Walk(const Problem& q, int64_t first, int stride) : p(q), item(first), step(stride) {
-    total = static_cast<int64_t>(p.batches) * p.chunks * p.m_tiles * (running(EPI) ? 1 : p.n_tiles);
-    begin();
+  __device__ Walk(const Problem& q, int first, int stride) : p(q), item(first), step(stride) {
+    total = static_cast<uint32_t>(p.batches) * p.chunks * p.m_tiles * (running(EPI) ? 1 : p.n_tiles);
+    decode();
   }
-  __device__ void begin() {
-    if (running(EPI) && item < total) {
-      const int c = static_cast<int>(item % p.chunks);
-      j_begin = static_cast<int>(static_cast<int64_t>(p.n_tiles) * c / p.chunks);
-      j_end = static_cast<int>(static_cast<int64_t>(p.n_tiles) * (c + 1) / p.chunks);
-      j = j_begin;
-    }
+  // Row blocks start at different tiles of a window, so that they do not all
+  // read the same centroids from the same L2 slices at once.
+  __device__ void window(int from) {
+    w0 = from;
+    wl = min(p.window, j_end - from);
+    w_end = from + wl;
+    t.n = w0 + static_cast<int>(static_cast<uint32_t>(t.m) % static_cast<uint32_t>(wl));
   }
-  __device__ bool get(Tile& t) const {
-    if (item >= total) return false;
+  __device__ void decode() {
+    if (item >= total) return;
     const int steps = p.npairs * p.kblocks;
     if constexpr (running(EPI)) {
-      t.chunk = static_cast<int>(item % p.chunks);
-      const int64_t r = item / p.chunks;
-      t.m = static_cast<int>(r % p.m_tiles);
-      t.b = static_cast<int>(r / p.m_tiles);
-      // row blocks start at different tiles of a window, so that they do not
-      // all read the same centroids from the same L2 slices at once
-      const int rel = j - j_begin;
-      const int w0 = rel / p.window * p.window;
-      const int wl = min(p.window, j_end - j_begin - w0);
-      t.n = j_begin + w0 + (rel - w0 + t.m) % wl;
+      uint32_t r = item;
+      uint32_t c = 0;
+      if (p.chunks > 1) {
+        r = item / static_cast<uint32_t>(p.chunks);
+        c = item - r * p.chunks;
+      }
+      t.chunk = c;
+      t.b = r / static_cast<uint32_t>(p.m_tiles);
+      t.m = r - t.b * p.m_tiles;
+      j_begin = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * c / static_cast<uint32_t>(p.chunks));
+      j_end = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * (c + 1) / static_cast<uint32_t>(p.chunks));
       t.it0 = 0;
       t.it1 = steps;
-      t.first = j == j_begin;
-      t.last = j + 1 == j_end;
+      t.first = true;
+      t.last = j_begin + 1 == j_end;
+      window(j_begin);
+      j = j_begin;
     } else {
-      const int per = p.m_tiles * p.n_tiles;
-      const int64_t r = item / per;
-      int i = static_cast<int>(item % per);
-      t.chunk = static_cast<int>(r % p.chunks);
-      t.b = static_cast<int>(r / p.chunks);
-      const int band = p.group * p.n_tiles;
-      const int g0 = i / band * p.group;
-      const int gl = min(p.group, p.m_tiles - g0);
-      i -= g0 * p.n_tiles;
-      t.m = g0 + i % gl;
+      const uint32_t per = static_cast<uint32_t>(p.m_tiles) * p.n_tiles;
+      const uint32_t r = item / per;
+      uint32_t i = item - r * per;
+      t.b = r;
+      t.chunk = 0;
+      t.it0 = 0;
+      t.it1 = steps;
+      if (p.chunks > 1) {
+        t.b = r / static_cast<uint32_t>(p.chunks);
+        t.chunk = r - t.b * p.chunks;
+        t.it0 = static_cast<int>(static_cast<uint32_t>(steps) * t.chunk / static_cast<uint32_t>(p.chunks));
+        t.it1 = static_cast<int>(static_cast<uint32_t>(steps) * (t.chunk + 1) / static_cast<uint32_t>(p.chunks));
+      }
+      const uint32_t g = i / static_cast<uint32_t>(p.group * p.n_tiles);
+      const int g0 = g * p.group;
+      const uint32_t gl = min(p.group, p.m_tiles - g0);
+      i -= static_cast<uint32_t>(g0) * p.n_tiles;
       t.n = i / gl;
-      t.it0 = static_cast<int>(static_cast<int64_t>(steps) * t.chunk / p.chunks);
-      t.it1 = static_cast<int>(static_cast<int64_t>(steps) * (t.chunk + 1) / p.chunks);
+      t.m = g0 + i - t.n * gl;
       t.first = t.last = true;
     }
-    return true;
+  }
+  __device__ bool get(Tile& out) const {
+    out = t;
+    return item < total;
   }
   __device__ void next() {
     if constexpr (running(EPI)) {
-      if (++j < j_end) return;
+      if (++j < j_end) {
+        t.first = false;
+        t.last = j + 1 == j_end;
+        if (j == w_end) window(j);
+        else if (++t.n == w_end) t.n = w0;
+        return;
+      }
     }
     item += step;
-    begin();
+    decode();
   }
+  int j;
 };
 
 __device__ __forceinline__ int64_t load_label(const void* p, int64_t i, int dt) {
   return dt == FK_I64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
-// acc (int32) as float: exact for |acc| < 2^22 by placing it in the mantissa of
-// 1.5 * 2^23 (an add on the integer pipe, an add on the float pipe; the
-// conversion instruction runs at an eighth of their rate), else converted.
-__device__ __forceinline__ float acc_to_f(uint32_t v, bool small) {
-  return small ? __uint_as_float(v + 0x4B400000u) - 12582912.0f
-               : static_cast<float>(static_cast<int32_t>(v));
+// 32 int32 accumulators as floats, in place.  |acc| < 2^22 (`small`): an integer
+// add places it in the mantissa of 1.5 * 2^23 and a float add takes that off
+// again, exact, at an eighth of what the conversion instruction costs.
+__device__ __forceinline__ void acc_to_f(uint32_t (&v)[32], bool small) {
+  if (small) {
+    const uint64_t off = pack2(-12582912.0f, -12582912.0f);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float a, b;
+      unpack2(add2(pack2(__uint_as_float(v[i] + 0x4B400000u), __uint_as_float(v[i + 1] + 0x4B400000u)), off), a, b);
+      v[i] = __float_as_uint(a);
+      v[i + 1] = __float_as_uint(b);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[i])));
+  }
 }
 
 // Maximum that a NaN wins, as argmax counts it.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // Whether (v, i) comes before (m, j): NaN first, then the larger value, then the lower index.
@@ -268,9 +319,15 @@ __device__ __forceinline__ bool argmax_better(float v, int i, float m, int j) {
   return v != v && (m == m || i < j);
 }
 
+// Put into a branch that is seldom taken: the compiler would otherwise turn its
+// 32 conditional moves into selects that every chunk pays for (they were more
+// than half of the epilogues' instructions).
+__device__ __forceinline__ void keep_branch() { asm volatile(""); }
+
 // Barrier of the epilogue warps alone.
+template <int THREADS>
 __device__ __forceinline__ void epilogue_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
 
 // ------------------------------------------------------------------- kernel
@@ -283,18 +340,18 @@ __device__ __forceinline__ void epilogue_sync() {
 constexpr int kSegment = 4;       // of 64 elements: 16 truncated additions
 
 template <int CG, int BN, int EPI, bool EXACT>
-__global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__ Params prm) {
+__global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const __grid_constant__ Params prm) {
   using S = Shape<CG, BN, EPI>;
   const Problem& p = prm.p;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   uint8_t* staging = smem + S::kStages * S::kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kStagingBytes + S::kExtra);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes + S::kExtra);
   uint64_t* empty = full + S::kStages;
   uint64_t* acc_full = empty + S::kStages;
-  uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* acc_empty = acc_full + S::kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kBufs);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -311,9 +368,9 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kBufs; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kEpiWarps * CG);
+      mbar_init(&acc_empty[i], S::kEpiWarps * CG);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -384,6 +441,15 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           }
         }
       }
+      // The last products' commits still arrive on this CTA's barriers, from
+      // the pair's other CTA too: stay until they have.
+      for (int i = 0; ok && i < S::kStages; ++i) {
+        ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
@@ -430,21 +496,31 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           }
           if (it + 1 == t.it1 || (EXACT && (it + 1 - t.it0) % kSegment == 0)) {
             mma_commit_cg<CG>(&acc_full[buf]);
-            buf ^= 1;
-            if (buf == 0) aphase ^= 1;
+            if (++buf == S::kBufs) {
+              buf = 0;
+              aphase ^= 1;
+            }
             accumulate = 0;
           }
+        }
+      }
+      // and so do the epilogues' arrivals on the accumulators' barriers
+      for (int i = 0; ok && i < S::kBufs; ++i) {
+        ok = mbar_wait_cluster(&acc_empty[buf], aphase ^ 1, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
+        if (++buf == S::kBufs) {
+          buf = 0;
+          aphase ^= 1;
         }
       }
     }
   } else if (warp >= kCtlWarps) {
     // ------------------------------------------------------------ epilogue
     const int ew = warp - kCtlWarps;
-    const int half = ew >> 2;
+    const int part = ew >> 2;
     const int quarter = warp & 3;
-    constexpr int kCols = BN / 2;          // columns of this warp
+    constexpr int kCols = BN / S::kParts;  // columns of this warp
     constexpr int kChunks = kCols / 32;
-    uint8_t* stg = staging + ew * 4096;
+    uint8_t* stg = staging + ew * S::kStaging;
     int buf = 0;
     uint32_t aphase = 0;
     Walk<EPI> walk(p, first, stride);
@@ -452,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
     // running state of a row
     float run_m = -INFINITY, run_s = 0.0f;
     int run_i = 0;
-    int64_t label = -1;
+    int label = -1;
     float xs = 0.0f;
     float fac = 0.0f;
     if constexpr (EPI == kEpiOut) {
@@ -461,11 +537,38 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
       if (p.f_den) fac /= static_cast<float>(max(*p.f_den, 1));
     }
 
-    for (Tile t; walk.get(t); walk.next()) {
+    // What the epilogue needs from memory besides the accumulator is fetched a
+    // tile ahead: its latency would stand between the accumulator and its use.
+    Tile t, nt;
+    bool more = walk.get(nt);
+    RowStat st_next = {0.0f, 0.0f, 0.0f, -1};
+    float xs_next = 0.0f, sc_next = 0.0f, bi_next = 0.0f;
+    auto fetch = [&]() {
+      const int64_t row = nt.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+      if constexpr (EPI == kEpiGrad) {
+        st_next = {0.0f, 0.0f, 0.0f, -1};
+        if (row < p.M) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + p.stat_off + row));
+          st_next = {f.x, f.y, f.z, __float_as_int(f.w)};
+        }
+      }
+      if constexpr (integer(EPI)) xs_next = row < p.M ? p.a_scale[nt.b * p.as_sb + row * p.as_sn] : 0.0f;
+      if constexpr (EPI == kEpiArgmax) {
+        const int64_t col = nt.n * BN + ew * 32 + lane;
+        const bool ok = ew * 32 < BN && col < p.N;
+        sc_next = ok ? p.b_scale[nt.b * p.bs_sb + col * p.bs_sn] : 0.0f;
+        bi_next = ok && p.bias ? p.bias[nt.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+      }
+    };
+    if (more) fetch();
+    while (more) {
+      t = nt;
+      walk.next();
+      more = walk.get(nt);
       const int row = t.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       const int row0 = row - lane;
       const bool row_ok = row < p.M;
-      const int col0 = t.n * BN + half * kCols;
+      const int col0 = t.n * BN + part * kCols;
 
       if constexpr (EPI == kEpiLse) {
         if (t.first) {
@@ -474,22 +577,15 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           label = -1;
           if (row_ok) {
             const int64_t y = load_label(p.labels, t.b * p.label_sb + row * p.label_sn, p.label_dtype);
-            label = y == p.ignore_index ? -1 : y;
+            label = y == p.ignore_index || y < 0 || y >= p.N ? -1 : static_cast<int>(y);
           }
         }
       }
-      RowStat st = {0.0f, 0.0f, 0.0f, -1};
-      if constexpr (EPI == kEpiGrad) {
-        if (row_ok) {
-          st = p.stat[t.b * p.stat_rows + p.stat_off + row];
-          st.coef *= p.p_scale;
-          st.at_label *= p.p_scale;
-        }
-      }
-      if constexpr (integer(EPI)) {
-        if (t.first) xs = row_ok ? p.a_scale[t.b * p.as_sb + row * p.as_sn] : 0.0f;
-      }
-      float* table = reinterpret_cast<float*>(staging + kStagingBytes);
+      RowStat st = st_next;
+      st.coef *= p.p_scale;
+      st.at_label *= p.p_scale;
+      xs = xs_next;
+      float* table = reinterpret_cast<float*>(staging + S::kStagingBytes);
       if constexpr (EPI == kEpiArgmax) {
         if (t.first) {
           run_m = -INFINITY;
@@ -497,15 +593,25 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
         }
         // this tile's column scales and biases, two tables in turn; the
         // barrier also keeps the tile before last's readers ahead of the writes
-        table += buf * (2 * 256);
-        const int c = (warp - kCtlWarps) * 32 + lane;
-        if (c < BN) {
-          const int col = t.n * BN + c;
-          const bool ok = col < p.N;
-          table[c] = ok ? p.b_scale[t.b * p.bs_sb + col * p.bs_sn] : 0.0f;
-          table[256 + c] = ok && p.bias ? p.bias[t.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+        table += (buf & 1) * (2 * 256);
+        if (ew * 32 < BN) {
+          table[ew * 32 + lane] = sc_next;
+          table[256 + ew * 32 + lane] = bi_next;
         }
-        epilogue_sync();
+        epilogue_sync<S::kEpiWarps * 32>();
+      }
+      if (more) fetch();
+      // this lane's columns of every chunk
+      float sc[kChunks][4], bi[kChunks][4];
+      if constexpr (EPI == kEpiScores) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int64_t col = col0 + c * 32 + (lane & 7) * 4 + i;
+            sc[c][i] = col < p.N ? p.b_scale[t.b * p.bs_sb + col * p.bs_sn] : 0.0f;
+            bi[c][i] = col < p.N && p.bias ? p.bias[t.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+          }
       }
 
       // one chunk of 32 columns, accumulators in v
@@ -515,12 +621,14 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
         if constexpr (EPI == kEpiLse) {
           const int left = p.N - cc;
           if (left < 32) {
+            keep_branch();
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (i >= left) v[i] = 0xff800000u;  // -inf past the last centroid
           }
-          const int64_t rel = label - cc;
-          if (rel >= 0 && rel < 32 && rel < left) {
+          const int rel = label - cc;
+          if (rel >= 0 && rel < 32) {
+            keep_branch();
             // the label's own term stays out of the sum
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -555,19 +663,20 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           // softmax minus one-hot, times the row's weight
           const int rel = st.label - p.col_off - cc;
           const uint64_t s2 = pack2(p.scale2, p.scale2), nm = pack2(-st.top, -st.top);
+          const uint64_t co = pack2(st.coef, st.coef);
           float e[32];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             unpack2(mul2(add2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), nm), s2), e[i], e[i + 1]);
-            e[i] = ex2(e[i]) * st.coef;
-            e[i + 1] = ex2(e[i + 1]) * st.coef;
+            unpack2(mul2(pack2(ex2(e[i]), ex2(e[i + 1])), co), e[i], e[i + 1]);
           }
           if (rel >= 0 && rel < 32) {
+            keep_branch();
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (rel == i) e[i] = st.at_label;
           }
-          for (int part = 0; part < p.p_parts; ++part) {
+          for (int pp = 0; pp < p.p_parts; ++pp) {
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -586,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             }
             __syncwarp();
             uint8_t* dst = static_cast<uint8_t*>(p.p_out) +
-                           2 * (part * p.p_part + t.b * p.p_batch);
+                           2 * (pp * p.p_part + t.b * p.p_batch);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int rr = i * 8 + (lane >> 2), q = lane & 3;
@@ -596,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             }
           }
         } else if constexpr (EPI == kEpiOut || EPI == kEpiScores) {
-          const bool small = p.small_acc != 0;
+          if constexpr (EPI == kEpiScores) acc_to_f(v, p.small_acc != 0);
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -604,21 +713,12 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             float* ff = &f.x;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              ff[i] = EPI == kEpiScores ? acc_to_f(v[q * 4 + i], small) * xs
-                                        : __uint_as_float(v[q * 4 + i]) * fac;
+              ff[i] = __uint_as_float(v[q * 4 + i]) * (EPI == kEpiScores ? xs : fac);
             *reinterpret_cast<float4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16)) = f;
           }
           __syncwarp();
           const int q = lane & 7;
           const int col = cc + q * 4;
-          float sc[4], bi[4];
-          if constexpr (EPI == kEpiScores) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              sc[i] = col + i < p.N ? p.b_scale[t.b * p.bs_sb + (col + i) * p.bs_sn] : 0.0f;
-              bi[i] = col + i < p.N && p.bias ? p.bias[t.b * p.bias_sb + (col + i) * p.bias_sn] : 0.0f;
-            }
-          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int rr = i * 4 + (lane >> 3);
@@ -629,8 +729,8 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
               float* ff = &f.x;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                ff[k] = __fmul_rn(ff[k], sc[k]);
-                if (p.bias) ff[k] = __fadd_rn(ff[k], bi[k]);
+                ff[k] = __fmul_rn(ff[k], sc[c][k]);
+                if (p.bias) ff[k] = __fadd_rn(ff[k], bi[c][k]);
               }
             } else if (p.acc) {
               float* a = p.acc + t.chunk * p.acc_split + t.b * p.acc_batch + grow * p.acc_ld + col;
@@ -664,20 +764,18 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             }
           }
         } else {  // kEpiArgmax
-          const float* sc = table + half * kCols + c * 32;
-          const float* bi = sc + 256;
-          const bool small = p.small_acc != 0;
+          const float* tsc = table + part * kCols + c * 32;
+          const float* tbi = tsc + 256;
+          acc_to_f(v, p.small_acc != 0);
           const uint64_t x2 = pack2(xs, xs);
           float z[32];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 s4 = *reinterpret_cast<const float4*>(sc + i);
-            uint64_t z0 = mul2(mul2(pack2(acc_to_f(v[i], small), acc_to_f(v[i + 1], small)), x2),
-                               pack2(s4.x, s4.y));
-            uint64_t z1 = mul2(mul2(pack2(acc_to_f(v[i + 2], small), acc_to_f(v[i + 3], small)), x2),
-                               pack2(s4.z, s4.w));
+            const float4 s4 = *reinterpret_cast<const float4*>(tsc + i);
+            uint64_t z0 = mul2(mul2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), x2), pack2(s4.x, s4.y));
+            uint64_t z1 = mul2(mul2(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), x2), pack2(s4.z, s4.w));
             if (p.bias) {
-              const float4 b4 = *reinterpret_cast<const float4*>(bi + i);
+              const float4 b4 = *reinterpret_cast<const float4*>(tbi + i);
               z0 = add2(z0, pack2(b4.x, b4.y));
               z1 = add2(z1, pack2(b4.z, b4.w));
             }
@@ -686,14 +784,19 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           }
           const int left = p.N - cc;
           if (left < 32) {
+            keep_branch();
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (i >= left) z[i] = -INFINITY;
           }
-          float mx[4] = {z[0], z[1], z[2], z[3]};
+          float mx[4];
 #pragma unroll
-          for (int i = 4; i < 32; ++i) mx[i & 3] = max_nan(mx[i & 3], z[i]);
-          const float m = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3]));
+          for (int q = 0; q < 4; ++q) {
+            mx[q] = max_nan3(z[q], z[q + 4], z[q + 8]);
+            mx[q] = max_nan3(mx[q], z[q + 12], z[q + 16]);
+            mx[q] = max_nan(max_nan3(mx[q], z[q + 20], z[q + 24]), z[q + 28]);
+          }
+          const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
           if (left > 0 && argmax_better(m, cc, run_m, run_i)) {
             // keep the chunk: which of its columns won is looked up once, at
             // the end of the row, instead of at every improvement
@@ -720,7 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           if (!got) break;
           tc_fence_after();
           const uint32_t taddr =
-              tmem + buf * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+              tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             uint32_t v[32];
@@ -735,8 +838,10 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
-          buf ^= 1;
-          if (buf == 0) aphase ^= 1;
+          if (++buf == S::kBufs) {
+            buf = 0;
+            aphase ^= 1;
+          }
         }
         if (!got) break;
 #pragma unroll
@@ -752,9 +857,11 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
         if (!got) {
           if constexpr (EPI == kEpiArgmax) {
             // the other warps meet at the barriers of every tile: keep to them
-            if (t.last && p.chunks == 1) epilogue_sync();
-            buf ^= 1;
-            if (buf == 0) aphase ^= 1;
+            if (t.last && p.chunks == 1) epilogue_sync<S::kEpiWarps * 32>();
+            if (++buf == S::kBufs) {
+              buf = 0;
+              aphase ^= 1;
+            }
             continue;
           } else {
             break;
@@ -762,29 +869,29 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
         }
         tc_fence_after();
         const uint32_t taddr =
-            tmem + buf * BN + half * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
-        uint32_t r[2][32];
-        tmem_ld32(taddr, r[0]);
+            tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          tmem_ld_wait(r[c & 1]);
-          if (c + 1 < kChunks) {
-            tmem_ld32(taddr + (c + 1) * 32, r[(c + 1) & 1]);
-          } else {
+          uint32_t v[32];
+          tmem_ld32(taddr + c * 32, v);
+          tmem_ld_wait(v);
+          if (c + 1 == kChunks) {
             // the accumulator is in registers: hand it back
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
           }
-          chunk(c, r[c & 1]);
+          chunk(c, v);
         }
-        buf ^= 1;
-        if (buf == 0) aphase ^= 1;
+        if (++buf == S::kBufs) {
+          buf = 0;
+          aphase ^= 1;
+        }
       }
 
       if constexpr (EPI == kEpiLse) {
         if (t.last && row_ok)
-          p.partial[(static_cast<int64_t>(t.b) * p.chunks * 2 + t.chunk * 2 + half) * p.M + row] =
+          p.partial[((static_cast<int64_t>(t.b) * p.chunks + t.chunk) * S::kParts + part) * p.M + row] =
               make_float2(run_m, run_s);
       }
       if constexpr (EPI == kEpiArgmax) {
@@ -802,18 +909,24 @@ __global__ void __launch_bounds__(kThreads, 1) head_gemm(const __grid_constant__
             run_i += at;
           }
           if (p.chunks == 1) {
-            // the two column halves of a row meet in shared memory
-            float2* slot = reinterpret_cast<float2*>(staging + kStagingBytes + kTableBytes) +
+            // the column parts of a row meet in shared memory
+            float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + kTableBytes) +
                            (quarter * 32 + lane);
-            if (half == 1) *slot = make_float2(run_m, __int_as_float(run_i));
-            epilogue_sync();
-            if (half == 0 && row_ok) {
-              const float2 o = *slot;
-              if (argmax_better(o.x, __float_as_int(o.y), run_m, run_i)) run_i = __float_as_int(o.y);
+            if (part > 0) slot[(part - 1) * 128] = make_float2(run_m, __int_as_float(run_i));
+            epilogue_sync<S::kEpiWarps * 32>();
+            if (part == 0 && row_ok) {
+#pragma unroll
+              for (int o = 0; o < S::kParts - 1; ++o) {
+                const float2 v = slot[o * 128];
+                if (argmax_better(v.x, __float_as_int(v.y), run_m, run_i)) {
+                  run_m = v.x;
+                  run_i = __float_as_int(v.y);
+                }
+              }
               p.label_out[t.b * p.lo_sb + row * p.lo_sn] = run_i;
             }
           } else if (row_ok) {
-            p.partial[(static_cast<int64_t>(t.b) * p.chunks * 2 + t.chunk * 2 + half) * p.M + row] =
+            p.partial[((static_cast<int64_t>(t.b) * p.chunks + t.chunk) * S::kParts + part) * p.M + row] =
                 make_float2(run_m, __int_as_float(run_i));
           }
         }

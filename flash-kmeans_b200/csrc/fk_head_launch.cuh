@@ -76,11 +76,14 @@ int launch_shape(Params& prm, cudaStream_t s) {
   const Problem& p = prm.p;
   const int64_t items = static_cast<int64_t>(p.batches) * p.chunks * p.m_tiles *
                         (running(EPI) ? 1 : p.n_tiles);
+  if (items >= (1ll << 31) || static_cast<int64_t>(p.n_tiles) * p.chunks >= (1ll << 31) ||
+      static_cast<int64_t>(p.npairs) * p.kblocks * p.chunks >= (1ll << 31))
+    return fail(FK_ERR_UNSUPPORTED, "head_gemm: %lld tiles exceed 32-bit", static_cast<long long>(items));
   const int64_t slots = sms / CG;
   const unsigned grid = static_cast<unsigned>((items < slots ? items : slots) * CG);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];

@@ -25,37 +25,51 @@ constexpr int64_t kMaxD8 = 65536;   // 127^2 * D stays below 2^30
 // second pass finds the row in the caches.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-template <typename T>
-__global__ void quantize_rows_kernel(const T* __restrict__ x, int64_t sb, int64_t sn, int64_t sd,
-                                     int vec, int8_t* __restrict__ q, int64_t qb, int64_t qn, int Dp, int qvec,
-                                     float* __restrict__ scale, int64_t scb, int64_t scn, int N, int D,
-                                     int64_t rows, int lanes) {
+// STEPS: 16-byte loads of a thread that hold its whole share of the row in
+// registers, all in flight at once; 0 for longer rows, which are read twice.
+template <typename T, int STEPS>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(
+    const T* __restrict__ x, int64_t sb, int64_t sn, int64_t sd, int vec, int8_t* __restrict__ q,
+    int64_t qb, int64_t qn, int Dq, int qvec, float* __restrict__ scale, int64_t scb, int64_t scn, int N,
+    int D, int64_t rows, int lanes) {
   // `lanes` threads per row: a power of two up to a block
-  __shared__ uint32_t sm[32];
+  __shared__ uint32_t sm[8];
+  constexpr int E = 16 / sizeof(T);
+  constexpr int kHeld = STEPS > 0 ? STEPS : 1;
   const int sub = threadIdx.x & (lanes - 1);
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
   const bool ok = row < rows;
   const int64_t b = ok ? row / N : 0, n = ok ? row - b * N : 0;
   const T* src = x + b * sb + n * sn;
-  constexpr int E = 16;  // elements of a step: one 16-byte store of integers
-  uint32_t most = 0;
-  T v[E];
-  auto load = [&](int d) {
+  auto load = [&](int d) -> uint4 {
+    uint4 u = make_uint4(0, 0, 0, 0);
     if (vec && d + E <= D) {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T)); ++i)
-        reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src + d)[i];
+      u = __ldg(reinterpret_cast<const uint4*>(src + d));
     } else {
+      T* v = reinterpret_cast<T*>(&u);
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = d + i < D ? src[(d + i) * sd] : Elem<T>::from_f(0.0f);
+      for (int i = 0; i < E; ++i)
+        if (d + i < D) v[i] = src[(d + i) * sd];
     }
+    return u;
   };
-  if (ok)
-    for (int d = sub * E; d < D; d += lanes * E) {
-      load(d);
+  auto most_of = [&](uint4 u) {
+    const T* v = reinterpret_cast<const T*>(&u);
+    uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < E; ++i) most = max(most, abs_bits(Elem<T>::to_f(v[i])));
-    }
+    for (int i = 0; i < E; ++i) m = max(m, abs_bits(Elem<T>::to_f(v[i])));
+    return m;
+  };
+  uint32_t most = 0;
+  uint4 held[kHeld];
+  if constexpr (STEPS > 0) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) held[s] = ok ? load((s * lanes + sub) * E) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) most = max(most, most_of(held[s]));
+  } else if (ok) {
+    for (int d = sub * E; d < D; d += lanes * E) most = max(most, most_of(load(d)));
+  }
   for (int o = min(lanes, 32) >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
   if (lanes > 32) {
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = most;
@@ -71,41 +85,64 @@ __global__ void quantize_rows_kernel(const T* __restrict__ x, int64_t sb, int64_
   const float inv = bad || zero ? 0.0f : __fdiv_rn(127.0f, m);
   if (sub == 0) scale[b * scb + n * scn] = bad ? __uint_as_float(0x7fc00000u) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
   int8_t* dst = q + b * qb + n * qn;
-  for (int d = sub * E; d < Dp; d += lanes * E) {
-    load(d);
-    int8_t w[E];
+  auto store = [&](int d, uint4 u) {
+    if (d >= Dq) return;
+    const T* v = reinterpret_cast<const T*>(&u);
+    uint32_t w[E / 4];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int r = bad ? 0 : __float2int_rn(__fmul_rn(Elem<T>::to_f(v[i]), inv));
-      w[i] = static_cast<int8_t>(max(-127, min(127, r)));
+    for (int j = 0; j < E / 4; ++j) {
+      w[j] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // |x * inv| is at most 127 and a rounding
+        const int r = bad ? 0 : __float2int_rn(__fmul_rn(Elem<T>::to_f(v[j * 4 + i]), inv));
+        w[j] |= (static_cast<uint32_t>(r) & 0xffu) << (8 * i);
+      }
     }
-    if (qvec) {
-      *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(w);
+    if (qvec && d + E <= Dq) {
+      if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + d) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(dst + d) = w[0];
     } else {
-      for (int i = 0; i < E && d + i < Dp; ++i) dst[d + i] = w[i];
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (d + i < Dq) dst[d + i] = static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)));
     }
+  };
+  if constexpr (STEPS > 0) {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) store((s * lanes + sub) * E, held[s]);
+  } else {
+    for (int d = sub * E; d < Dq; d += lanes * E) store(d, load(d));
   }
 }
 
+// q's first Dq elements of a row are written (zeros from D on).
 template <typename T>
 static int quantize_typed(const void* x, int64_t B, int64_t N, int64_t D, const int64_t* xs, int8_t* q,
-                          int64_t qb, int64_t qn, int64_t Dp, float* scale, int64_t scb, int64_t scn,
+                          int64_t qb, int64_t qn, int64_t Dq, float* scale, int64_t scb, int64_t scn,
                           cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T);
   const int vec = (xs[2] == 1 || D == 1) && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
                   (N == 1 || xs[1] * sizeof(T) % 16 == 0) && (B == 1 || xs[0] * sizeof(T) % 16 == 0);
-  // enough threads that each holds one or two steps of its row; whole blocks
-  // for the few long rows of a token's call
-  int lanes = 1;
-  const int most = B * N < 2048 ? 256 : 32;
-  while (lanes < most && lanes * 16 < D) lanes *= 2;
+  const int qvec = reinterpret_cast<uintptr_t>(q) % E == 0 && (N == 1 || qn % E == 0) && (B == 1 || qb % E == 0);
+  // a warp's lanes first, then up to eight loads each, then more warps; few
+  // long rows (a token's call) take whole blocks at once
   const int64_t rows = B * N;
-  const int qvec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && Dp % 16 == 0 && (N == 1 || qn % 16 == 0) &&
-                   (B == 1 || qb % 16 == 0);
+  int lanes = 1;
+  while (lanes < 32 && static_cast<int64_t>(lanes) * E < Dq) lanes *= 2;
+  const int held = rows < 1024 ? 2 : 8;
+  while (lanes < 256 && static_cast<int64_t>(lanes) * E * held < Dq) lanes *= 2;
+  const int64_t steps = ceil_div(Dq, static_cast<int64_t>(lanes) * E);
   const int64_t blocks = ceil_div(rows * lanes, 256);
   if (blocks >= (1ll << 31)) return fail(FK_ERR_UNSUPPORTED, "fk_quantize_rows: too many rows");
-  quantize_rows_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, s>>>(
-      static_cast<const T*>(x), xs[0], xs[1], xs[2], vec, q, qb, qn, static_cast<int>(Dp), qvec, scale, scb, scn,
-      static_cast<int>(N), static_cast<int>(D), rows, lanes);
+  auto kern = steps <= 1   ? quantize_rows_kernel<T, 1>
+              : steps <= 2 ? quantize_rows_kernel<T, 2>
+              : steps <= 4 ? quantize_rows_kernel<T, 4>
+              : steps <= 8 ? quantize_rows_kernel<T, 8>
+                           : quantize_rows_kernel<T, 0>;
+  kern<<<static_cast<unsigned>(blocks), 256, 0, s>>>(
+      static_cast<const T*>(x), xs[0], xs[1], xs[2], vec, q, qb, qn, static_cast<int>(Dq), qvec, scale, scb,
+      scn, static_cast<int>(N), static_cast<int>(D), rows, lanes);
   return check_launch("quantize_rows_kernel");
 }
 
@@ -237,7 +274,7 @@ static ScoresPlan plan_scores(const Scores& q, bool argmax, void* ws) {
     f.xq = static_cast<int8_t*>(take(q.B * q.N * q.Dp()));
   if (q.x_dtype != FK_I8) f.sx = static_cast<float*>(take(q.B * q.N * 4));
   if (!in_place8(q.c, q.Bc(), q.K, q.D, q.cs)) f.cq = static_cast<int8_t*>(take(q.Bc() * q.K * q.Dp()));
-  if (f.chunks > 1) f.partial = static_cast<float2*>(take(q.B * f.chunks * 2 * q.N * 8));
+  if (f.chunks > 1) f.partial = static_cast<float2*>(take(q.B * f.chunks * parts_of(f.sh.bn) * q.N * 8));
   f.bytes = used;
   return f;
 }
@@ -316,7 +353,7 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   if (st != FK_OK || !f.partial) return st;
   const int64_t row_blocks = ceil_div(q.N, 32);
   argmax_join_kernel<<<static_cast<unsigned>(q.B * row_blocks), kJoinWarps * 32, 0, s>>>(
-      f.partial, f.chunks * 2, static_cast<int>(q.N), static_cast<int>(row_blocks), label_out, ls[0], ls[1]);
+      f.partial, f.chunks * parts_of(f.sh.bn), static_cast<int>(q.N), static_cast<int>(row_blocks), label_out, ls[0], ls[1]);
   return check_launch("argmax_join_kernel");
 }
 

@@ -288,7 +288,7 @@ __device__ __forceinline__ void mbar_arrive_cg(uint64_t* bar) {
   if constexpr (CG == 1) {
     mbar_arrive(bar);
   } else {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
                      map_to_rank(bar, 0))
                  : "memory");
   }

@@ -32,17 +32,60 @@ _FLOATS = (torch.float16, torch.bfloat16, torch.float32)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _status_word(device):
-    """The device's error word; None while capturing, if it is not there yet
-    (it would belong to the graph's memory)."""
-    key = torch.device(device).index
-    if key not in _ops.DeviceStatus._words and torch.cuda.is_current_stream_capturing():
-        return None
-    return _ops.DeviceStatus.word(device)
+class _Device:
+    """What a call needs of a device: its index and its error word."""
+
+    def __init__(self, device):
+        self.index = device.index
+        self.status = None
+
+    def status_ptr(self):
+        """The device's error word; None while capturing, if it is not there yet
+        (it would belong to the graph's memory)."""
+        if self.status is None:
+            if self.index not in _ops.DeviceStatus._words and torch.cuda.is_current_stream_capturing():
+                return None
+            self.status = _ops.DeviceStatus.word(torch.device("cuda", self.index)).data_ptr()
+        return self.status
 
 
-def _batched(x, centroids, name):
-    """(x, centroids) as (B, N, D) and (B, K, D), with how x was folded."""
+_devices: dict = {}
+# Checked arguments and sizes by everything that they depend on (shapes, strides,
+# types, devices, alignment, options): a call with the same layout skips the
+# checks.  Bounded, because lengths may differ from call to call.
+_layouts: dict = {}
+_MOST_LAYOUTS = 4096
+
+
+def _device(device) -> _Device:
+    d = _devices.get(device)
+    if d is None:
+        d = _devices[device] = _Device(device)
+    return d
+
+
+def _layout(key, make):
+    found = _layouts.get(key)
+    if found is None:
+        found = make()
+        if len(_layouts) >= _MOST_LAYOUTS:
+            _layouts.clear()
+        _layouts[key] = found
+    return found
+
+
+def _call(fn, what, dev: _Device, *args):
+    """fn(*args, status word, current stream) on device dev."""
+    if torch.cuda.current_device() == dev.index:
+        st = fn(*args, dev.status_ptr(), torch.cuda.current_stream(dev.index).cuda_stream)
+    else:
+        with torch.cuda.device(dev.index):
+            st = fn(*args, dev.status_ptr(), torch.cuda.current_stream(dev.index).cuda_stream)
+    if st:
+        nat.check(st, what)
+
+
+def _check_pair(x, centroids, name):
     if not isinstance(x, torch.Tensor) or not isinstance(centroids, torch.Tensor):
         raise TypeError(f"{name}: x and centroids must be tensors")
     if x.dim() not in (2, 3) or centroids.dim() not in (2, 3) or centroids.dim() > x.dim():
@@ -57,94 +100,121 @@ def _batched(x, centroids, name):
     _ops._require_cuda(x, centroids)
     if x.device != centroids.device:
         raise ValueError(f"{name}: x is on {x.device}, centroids on {centroids.device}")
-    x, centroids = x.detach(), centroids.detach()
-    if centroids.dim() == 2:
-        # one codebook: all rows of x are one batch
-        rows = x.reshape(1, -1, x.shape[-1]) if x.dim() == 3 else x.unsqueeze(0)
-        return rows, centroids.unsqueeze(0)
-    return x, centroids
 
 
-def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _three(t):
+    """Shape and strides of (M, D) or (B, M, D) as three."""
+    sh, st = t.shape, t.stride()
+    return (sh, st) if len(sh) == 3 else ((1, *sh), (sh[0] * st[0], *st))
+
+
+def _two(t):
+    sh, st = t.shape, t.stride()
+    return st if len(sh) == 2 else (0, *st)
+
+
+def _c(strides):
+    return (nat.ctypes.c_int64 * len(strides))(*strides)
 
 
 # ------------------------------------------------------------- cross entropy
-class _Xent:
-    """Checked arguments of one cross entropy call."""
+class _XentLayout:
+    """Checked layout of a cross entropy call (x already folded)."""
 
-    def __init__(self, x, centroids, labels, scale, ignore_index, reduction, name):
-        self.x, self.c = _batched(x, centroids, name)
-        if x.dtype not in _FLOATS:
-            raise TypeError(f"{name}: unsupported dtype {x.dtype}")
-        if centroids.dtype != x.dtype:
-            raise TypeError(f"{name}: centroids are {centroids.dtype}, x is {x.dtype}")
-        if not isinstance(labels, torch.Tensor) or labels.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"{name}: labels must be an int32 or int64 tensor")
-        if labels.shape != x.shape[:-1]:
-            raise ValueError(f"{name}: labels have shape {tuple(labels.shape)}, "
-                             f"x {tuple(x.shape)}")
-        if labels.device != x.device:
-            raise ValueError(f"{name}: x is on {x.device}, labels on {labels.device}")
-        scale = float(scale)
-        if not (scale > 0.0 and math.isfinite(scale)):
-            raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
-        if reduction not in _REDUCTIONS:
-            raise ValueError(f"{name}: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-        self.labels = labels.reshape(self.x.shape[:2])
-        self.scale = scale
-        self.ignore = int(ignore_index)
-        self.reduction = reduction
-        self.rows_shape = x.shape[:-1]
+    def __init__(self, x, centroids, labels, scale, ignore_index, reduction):
+        (B, N, D), xs = _three(x)
+        (_, K, _), cs = _three(centroids)
+        self.lib = nat.load()
+        code = _REDUCTIONS[reduction]
+        dtype = nat.dtype_code(x.dtype)
+        sizes = (B, N, K, D)
+        self.rows = B * N
+        xs, cs = _c(xs), _c(cs)
+        self.middle = (dtype, nat.dtype_code(labels.dtype), *sizes, xs, cs, _c(_two(labels)), scale,
+                       ignore_index, code)
+        self.grad_strides = _c((N * D, D, 1)), _c((K * D, D, 1))
+        # by which gradients are wanted; (0, 0) is the forward pass
+        self.bytes = {w: self.lib.fk_xent_workspace_size(x.data_ptr(), centroids.data_ptr(), dtype,
+                                                         *sizes, xs, cs, code, *w)
+                      for w in ((0, 0), (0, 1), (1, 0), (1, 1))}
         self.device = x.device
 
-    def _sizes(self):
-        B, N, D = self.x.shape
-        return B, N, self.c.shape[1], D
 
-    def _head(self):
-        return (nat.ptr(self.x), nat.ptr(self.c), nat.ptr(self.labels),
-                nat.dtype_code(self.x.dtype), nat.dtype_code(self.labels.dtype), *self._sizes(),
-                nat.strides(self.x, 3), nat.strides(self.c, 3), nat.strides(self.labels, 2),
-                self.scale, self.ignore, _REDUCTIONS[self.reduction])
+def _check_xent(x, centroids, labels, scale, ignore_index, reduction, name):
+    _check_pair(x, centroids, name)
+    if x.dtype not in _FLOATS:
+        raise TypeError(f"{name}: unsupported dtype {x.dtype}")
+    if centroids.dtype != x.dtype:
+        raise TypeError(f"{name}: centroids are {centroids.dtype}, x is {x.dtype}")
+    if not isinstance(labels, torch.Tensor) or labels.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name}: labels must be an int32 or int64 tensor")
+    if labels.shape != x.shape[:-1]:
+        raise ValueError(f"{name}: labels have shape {tuple(labels.shape)}, x {tuple(x.shape)}")
+    if labels.device != x.device:
+        raise ValueError(f"{name}: x is on {x.device}, labels on {labels.device}")
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"{name}: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
 
-    def _ws(self, lib, want_x, want_c):
-        nbytes = lib.fk_xent_workspace_size(
-            nat.ptr(self.x), nat.ptr(self.c), nat.dtype_code(self.x.dtype), *self._sizes(),
-            nat.strides(self.x, 3), nat.strides(self.c, 3), _REDUCTIONS[self.reduction],
-            int(want_x), int(want_c))
-        return _workspace(nbytes, self.device), nbytes
 
-    def forward(self, keep_stats: bool):
-        """(loss, row statistics or None, count)"""
-        lib = nat.load()
-        B, N, _, _ = self._sizes()
-        f32 = dict(dtype=torch.float32, device=self.device)
-        loss = torch.empty(self.rows_shape if self.reduction == "none" else (), **f32)
-        stats = torch.empty((B, N, 4), **f32) if keep_stats else None
-        count = torch.empty((), dtype=torch.int32, device=self.device)
-        with torch.cuda.device(self.device):
-            ws, nbytes = self._ws(lib, False, False)
-            nat.check(lib.fk_xent_forward(*self._head(), nat.ptr(loss), nat.ptr(stats),
-                                          nat.ptr(count), nat.ptr(ws), nbytes,
-                                          nat.ptr(_status_word(self.device)),
-                                          nat.stream_handle(self.device)), "fk_xent_forward")
-        return loss, stats, count
+class _Xent:
+    """One cross entropy call: x and labels folded, its layout."""
 
-    def backward(self, stats, count, grad_loss, want_x, want_c):
-        """(gradient by the folded x or None, by the centroids or None)"""
-        lib = nat.load()
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        gx = new(self.x) if want_x else None
-        gc = new(self.c) if want_c else None
-        with torch.cuda.device(self.device):
-            ws, nbytes = self._ws(lib, want_x, want_c)
-            nat.check(lib.fk_xent_backward(
-                *self._head(), nat.ptr(stats), nat.ptr(count), nat.ptr(grad_loss), nat.ptr(gx),
-                nat.ptr(gc), nat.strides(gx, 3) if want_x else None,
-                nat.strides(gc, 3) if want_c else None, nat.ptr(ws), nbytes,
-                nat.ptr(_status_word(self.device)), nat.stream_handle(self.device)),
-                "fk_xent_backward")
+    __slots__ = ("x", "c", "labels", "shapes", "none", "at", "dev")
+
+    def __init__(self, x, centroids, labels, scale, ignore_index, reduction, name):
+        scale, ignore_index = float(scale), int(ignore_index)
+        tensors = isinstance(x, torch.Tensor) and isinstance(centroids, torch.Tensor) and isinstance(
+            labels, torch.Tensor)
+        if not tensors or not x.is_cuda:
+            _check_xent(x, centroids, labels, scale, ignore_index, reduction, name)
+        self.shapes = x.shape, centroids.shape
+        self.none = reduction == "none"
+        if x.dim() == 3 and centroids.dim() == 2:
+            _check_xent(x, centroids, labels, scale, ignore_index, reduction, name)
+            x, labels = x.reshape(-1, x.shape[-1]), labels.reshape(-1)
+        self.x, self.c, self.labels = x, centroids, labels
+        key = (x.shape, x.stride(), x.dtype, x.device, x.data_ptr() & 15, centroids.shape,
+               centroids.stride(), centroids.dtype, centroids.device, centroids.data_ptr() & 15,
+               labels.shape, labels.stride(), labels.dtype, labels.device, scale, ignore_index, reduction)
+
+        def make():
+            _check_xent(x, centroids, labels, scale, ignore_index, reduction, name)
+            return _XentLayout(x, centroids, labels, scale, ignore_index, reduction)
+
+        self.at = _layout(key, make)
+        self.dev = _device(x.device)
+
+    def forward(self, keep: bool):
+        """(loss, row statistics and count for the backward pass, or None)"""
+        at = self.at
+        device = at.device
+        nbytes = at.bytes[0, 0]
+        loss = torch.empty(self.shapes[0][:-1] if self.none else (), dtype=torch.float32, device=device)
+        # the count of rows behind the statistics, or behind the workspace
+        ws = torch.empty(nbytes + 16, dtype=torch.uint8, device=device)
+        kept = torch.empty(4 * at.rows + 4, dtype=torch.float32, device=device) if keep else None
+        stats = kept.data_ptr() if keep else None
+        count = stats + 16 * at.rows if keep else ws.data_ptr() + nbytes
+        _call(at.lib.fk_xent_forward, "fk_xent_forward", self.dev, self.x.data_ptr(), self.c.data_ptr(),
+              self.labels.data_ptr(), *at.middle, loss.data_ptr(), stats, count, ws.data_ptr(), nbytes)
+        return loss, kept
+
+    def backward(self, kept, grad_loss, want_x, want_c):
+        """(gradient by x or None, by the centroids or None)"""
+        at = self.at
+        device = at.device
+        nbytes = at.bytes[int(want_x), int(want_c)]
+        xshape, cshape = self.shapes
+        gx = torch.empty(xshape, dtype=self.x.dtype, device=device) if want_x else None
+        gc = torch.empty(cshape, dtype=self.x.dtype, device=device) if want_c else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        stats = kept.data_ptr()
+        _call(at.lib.fk_xent_backward, "fk_xent_backward", self.dev, self.x.data_ptr(), self.c.data_ptr(),
+              self.labels.data_ptr(), *at.middle, stats, stats + 16 * at.rows,
+              None if grad_loss is None else grad_loss.data_ptr(), gx.data_ptr() if want_x else None,
+              gc.data_ptr() if want_c else None, *at.grad_strides, ws.data_ptr(), nbytes)
         return gx, gc
 
 
@@ -152,20 +222,20 @@ class _ClusterCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, centroids, labels, scale, ignore_index, reduction):
         call = _Xent(x, centroids, labels, scale, ignore_index, reduction, "cluster_cross_entropy")
-        loss, stats, count = call.forward(keep_stats=any(ctx.needs_input_grad[:2]))
-        ctx.save_for_backward(x, centroids, labels, stats, count)
+        loss, kept = call.forward(True)
+        ctx.save_for_backward(x, centroids, labels, kept)
         ctx.args = (scale, ignore_index, reduction)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        x, centroids, labels, stats, count = ctx.saved_tensors
+        x, centroids, labels, kept = ctx.saved_tensors
         call = _Xent(x, centroids, labels, *ctx.args, "cluster_cross_entropy")
-        grad_loss = grad_loss.to(torch.float32).contiguous()
-        gx, gc = call.backward(stats, count, grad_loss, *ctx.needs_input_grad[:2])
-        return (gx.view(x.shape) if gx is not None else None,
-                gc.view(centroids.shape) if gc is not None else None, None, None, None, None)
+        if not grad_loss.is_contiguous():
+            grad_loss = grad_loss.contiguous()
+        gx, gc = call.backward(kept, grad_loss, *ctx.needs_input_grad[:2])
+        return gx, gc, None, None, None, None
 
 
 def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torch.Tensor, *,
@@ -191,7 +261,11 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
     bits once, piece by piece, as the tensor cores take it.  A label outside
     [0, K) other than ``ignore_index`` makes the loss NaN.
     """
-    return _ClusterCrossEntropy.apply(x, centroids, labels, scale, ignore_index, reduction)
+    if torch.is_grad_enabled() and (getattr(x, "requires_grad", False)
+                                    or getattr(centroids, "requires_grad", False)):
+        return _ClusterCrossEntropy.apply(x, centroids, labels, scale, ignore_index, reduction)
+    return _Xent(x, centroids, labels, scale, ignore_index, reduction,
+                 "cluster_cross_entropy").forward(False)[0]
 
 
 def cluster_cross_entropy_grad(x: torch.Tensor, centroids: torch.Tensor, labels: torch.Tensor, *,
@@ -206,22 +280,22 @@ def cluster_cross_entropy_grad(x: torch.Tensor, centroids: torch.Tensor, labels:
     inputs a factor such as a loss scale goes in here).
     """
     name = "cluster_cross_entropy_grad"
-    call = _Xent(x, centroids, labels, scale, ignore_index, reduction, name)
-    shape = call.rows_shape if reduction == "none" else ()
-    if grad_loss is not None:
-        if not isinstance(grad_loss, torch.Tensor) or grad_loss.dtype != torch.float32:
-            raise TypeError(f"{name}: grad_loss must be a float32 tensor")
-        if grad_loss.shape != shape:
-            raise ValueError(f"{name}: grad_loss has shape {tuple(grad_loss.shape)}, "
-                             f"the loss {tuple(shape)}")
-        if grad_loss.device != x.device:
-            raise ValueError(f"{name}: x is on {x.device}, grad_loss on {grad_loss.device}")
-        grad_loss = grad_loss.detach().contiguous()
-    elif reduction == "none":
-        grad_loss = torch.ones(shape, dtype=torch.float32, device=x.device)
-    loss, stats, count = call.forward(keep_stats=True)
-    gx, gc = call.backward(stats, count, grad_loss, True, True)
-    return loss, gx.view(x.shape), gc.view(centroids.shape)
+    with torch.no_grad():
+        call = _Xent(x, centroids, labels, scale, ignore_index, reduction, name)
+        shape = x.shape[:-1] if call.none else ()
+        if grad_loss is not None:
+            if not isinstance(grad_loss, torch.Tensor) or grad_loss.dtype != torch.float32:
+                raise TypeError(f"{name}: grad_loss must be a float32 tensor")
+            if grad_loss.shape != shape:
+                raise ValueError(f"{name}: grad_loss has shape {tuple(grad_loss.shape)}, "
+                                 f"the loss {tuple(shape)}")
+            if grad_loss.device != x.device:
+                raise ValueError(f"{name}: x is on {x.device}, grad_loss on {grad_loss.device}")
+            grad_loss = grad_loss.contiguous()
+        elif call.none:
+            grad_loss = torch.ones(shape, dtype=torch.float32, device=x.device)
+        loss, kept = call.forward(True)
+        return loss, *call.backward(kept, grad_loss, True, True)
 
 
 # ------------------------------------------------------------- 8-bit scores
@@ -257,56 +331,85 @@ def quantize_rows(x: torch.Tensor):
     return (q, scale) if x.dim() == 3 else (q[0], scale[0])
 
 
+def _check_scale(t, shape, device, what, name):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
+        raise TypeError(f"{name}: {what} must be a float32 tensor")
+    if t.shape != shape:
+        raise ValueError(f"{name}: {what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{name}: x is on {device}, {what} on {t.device}")
+
+
+def _check_int8(x, centroids, c_scale, x_scale, bias, name):
+    _check_pair(x, centroids, name)
+    if centroids.dtype != torch.int8:
+        raise TypeError(f"{name}: centroids must be int8 (see quantize_rows), got {centroids.dtype}")
+    if x.dtype != torch.int8 and x.dtype not in _FLOATS:
+        raise TypeError(f"{name}: unsupported dtype {x.dtype}")
+    if (x_scale is None) == (x.dtype == torch.int8):
+        raise ValueError(f"{name}: x_scale goes with int8 x, and only with it")
+    _check_scale(c_scale, centroids.shape[:-1], x.device, "c_scale", name)
+    if bias is not None:
+        _check_scale(bias, centroids.shape[:-1], x.device, "bias", name)
+    if x_scale is not None:
+        _check_scale(x_scale, x.shape[:-1], x.device, "x_scale", name)
+
+
+class _ScoresLayout:
+    """Checked layout of an 8-bit call (x already folded)."""
+
+    def __init__(self, x, centroids, c_scale, x_scale, bias, argmax):
+        (B, N, D), xs = _three(x)
+        (_, K, _), cs = _three(centroids)
+        self.lib = nat.load()
+        self.x_code = nat.dtype_code(x.dtype)
+        self.sizes = (B, N, K, D)
+        xs, cs = _c(xs), _c(cs)
+        two = lambda t: None if t is None else _c(_two(t))  # noqa: E731
+        self.strides = (xs, cs, two(x_scale), two(c_scale), two(bias))
+        self.bytes = self.lib.fk_int8_workspace_size(x.data_ptr(), centroids.data_ptr(), self.x_code,
+                                                     *self.sizes, xs, cs, argmax)
+
+
 class _Scores:
-    """Checked arguments of one 8-bit call."""
+    """One 8-bit call: x folded, its layout."""
 
-    def __init__(self, x, centroids, c_scale, x_scale, bias, name):
-        self.x, self.c = _batched(x, centroids, name)
-        self.lead = x.shape[:-1]
-        self.device = x.device
-        if centroids.dtype != torch.int8:
-            raise TypeError(f"{name}: centroids must be int8 (see quantize_rows), got "
-                            f"{centroids.dtype}")
-        if x.dtype != torch.int8 and x.dtype not in _FLOATS:
-            raise TypeError(f"{name}: unsupported dtype {x.dtype}")
-        if (x_scale is None) == (x.dtype == torch.int8):
-            raise ValueError(f"{name}: x_scale goes with int8 x, and only with it")
-        self.c_scale = self._scale(c_scale, centroids.shape[:-1], "c_scale", name)
-        self.bias = None if bias is None else self._scale(bias, centroids.shape[:-1], "bias", name)
-        self.x_scale = None
-        if x_scale is not None:
-            self.x_scale = self._scale(x_scale, x.shape[:-1], "x_scale", name)
-            if centroids.dim() == 2 and x.dim() == 3:
-                self.x_scale = self.x_scale.reshape(1, -1)
+    __slots__ = ("lead", "device", "at", "dev", "operands")
 
-    def _scale(self, t, shape, what, name):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
-            raise TypeError(f"{name}: {what} must be a float32 tensor")
-        if t.shape != shape:
-            raise ValueError(f"{name}: {what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-        if t.device != self.device:
-            raise ValueError(f"{name}: x is on {self.device}, {what} on {t.device}")
-        t = t.detach()
-        return t if t.dim() == 2 else t.unsqueeze(0)
+    def __init__(self, x, centroids, c_scale, x_scale, bias, argmax, name):
+        if not (isinstance(x, torch.Tensor) and x.is_cuda and isinstance(centroids, torch.Tensor)
+                and isinstance(c_scale, torch.Tensor)
+                and (x_scale is None or isinstance(x_scale, torch.Tensor))
+                and (bias is None or isinstance(bias, torch.Tensor))):
+            _check_int8(x, centroids, c_scale, x_scale, bias, name)
+        self.lead, self.device = x.shape[:-1], x.device
+        if x.dim() == 3 and centroids.dim() == 2:
+            _check_int8(x, centroids, c_scale, x_scale, bias, name)
+            x = x.reshape(-1, x.shape[-1])
+            x_scale = None if x_scale is None else x_scale.reshape(-1)
+        sig = lambda t: None if t is None else (t.shape, t.stride(), t.dtype, t.device)  # noqa: E731
+        key = (x.shape, x.stride(), x.dtype, x.device, x.data_ptr() & 15, centroids.shape,
+               centroids.stride(), centroids.dtype, centroids.device, centroids.data_ptr() & 15,
+               sig(c_scale), sig(x_scale), sig(bias), argmax)
 
-    def sizes(self):
-        B, N, D = self.x.shape
-        return B, N, self.c.shape[1], D
+        def make():
+            _check_int8(x, centroids, c_scale, x_scale, bias, name)
+            return _ScoresLayout(x, centroids, c_scale, x_scale, bias, argmax)
 
-    def operands(self):
-        return (nat.ptr(self.x), nat.ptr(self.c), nat.ptr(self.x_scale), nat.ptr(self.c_scale),
-                nat.ptr(self.bias))
+        self.at = _layout(key, make)
+        self.dev = _device(self.device)
+        # the folded tensors stay referenced until the call is queued
+        self.operands = (x, centroids, x_scale, c_scale, bias)
 
-    def strides(self):
-        two = lambda t: None if t is None else nat.strides(t, 2)  # noqa: E731
-        return (nat.strides(self.x, 3), nat.strides(self.c, 3), two(self.x_scale),
-                two(self.c_scale), two(self.bias))
+    def pointers(self):
+        return [None if t is None else t.data_ptr() for t in self.operands]
 
-    def workspace(self, lib, argmax):
-        nbytes = lib.fk_int8_workspace_size(
-            nat.ptr(self.x), nat.ptr(self.c), nat.dtype_code(self.x.dtype), *self.sizes(),
-            nat.strides(self.x, 3), nat.strides(self.c, 3), int(argmax))
-        return _workspace(nbytes, self.device), nbytes
+    def workspace(self):
+        n = self.at.bytes
+        if not n:
+            return None, None, 0
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        return ws, ws.data_ptr(), n
 
 
 def _check_out(out, shape, dtype, device, name):
@@ -314,6 +417,15 @@ def _check_out(out, shape, dtype, device, name):
         raise ValueError(f"{name}: out must be a {dtype} tensor of shape {tuple(shape)}")
     if out.device != device:
         raise ValueError(f"{name}: x is on {device}, out on {out.device}")
+
+
+def _fold_strides(out, name):
+    """Strides of out with its first two dimensions as one batch of rows."""
+    (B, N), st = out.shape[:2], out.stride()
+    if B > 1 and N > 1 and st[0] != N * st[1]:
+        raise ValueError(f"{name}: with shared centroids, out's batches must follow each other at the "
+                         "distance of its rows")
+    return (0, st[1] if N > 1 else st[0], *st[2:])
 
 
 def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor, *,
@@ -338,7 +450,7 @@ def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
         above, rounded once to ``out_dtype``.
     """
     name = "int8_scores"
-    q = _Scores(x, centroids, c_scale, x_scale, bias, name)
+    q = _Scores(x, centroids, c_scale, x_scale, bias, False, name)
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else x.dtype if x.dtype in _FLOATS else torch.float32
     if out_dtype not in _FLOATS:
@@ -350,15 +462,15 @@ def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
         _check_out(out, shape, out_dtype, q.device, name)
         if shape[-1] > 1 and out.stride(-1) != 1:
             raise ValueError(f"{name}: rows of out must have unit stride")
-    B, N, K, _ = q.sizes()
-    folded = out.view(B, N, K)
-    lib = nat.load()
-    with torch.cuda.device(q.device):
-        ws, nbytes = q.workspace(lib, False)
-        nat.check(lib.fk_int8_scores(
-            *q.operands(), nat.ptr(folded), nat.dtype_code(q.x.dtype), nat.dtype_code(out_dtype),
-            *q.sizes(), *q.strides(), nat.strides(folded, 3), nat.ptr(ws), nbytes,
-            nat.ptr(_status_word(q.device)), nat.stream_handle(q.device)), "fk_int8_scores")
+    B, N, K, _ = q.at.sizes
+    if out.dim() == 3:
+        # (not .view(): a fold over batches needs rows at one distance)
+        strides = out.stride() if B == out.shape[0] else _fold_strides(out, name)
+    else:
+        strides = (N * out.stride(0), *out.stride())
+    ws, ws_ptr, nbytes = q.workspace()
+    _call(q.at.lib.fk_int8_scores, "fk_int8_scores", q.dev, *q.pointers(), out.data_ptr(), q.at.x_code,
+          nat.dtype_code(out_dtype), *q.at.sizes, *q.at.strides, _c(strides), ws_ptr, nbytes)
     return out
 
 
@@ -373,18 +485,17 @@ def int8_assign(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
     to the lowest index, a NaN score counts as the largest.
     """
     name = "int8_assign"
-    q = _Scores(x, centroids, c_scale, x_scale, bias, name)
+    q = _Scores(x, centroids, c_scale, x_scale, bias, True, name)
     if out is None:
         out = torch.empty(q.lead, dtype=torch.int32, device=q.device)
     else:
         _check_out(out, q.lead, torch.int32, q.device, name)
-    B, N, _, _ = q.sizes()
-    folded = out.view(B, N)
-    lib = nat.load()
-    with torch.cuda.device(q.device):
-        ws, nbytes = q.workspace(lib, True)
-        nat.check(lib.fk_int8_assign(
-            *q.operands(), nat.ptr(folded), nat.dtype_code(q.x.dtype), *q.sizes(), *q.strides(),
-            nat.strides(folded, 2), nat.ptr(ws), nbytes, nat.ptr(_status_word(q.device)),
-            nat.stream_handle(q.device)), "fk_int8_assign")
+    B = q.at.sizes[0]
+    if out.dim() == 2:
+        strides = out.stride() if B == out.shape[0] else _fold_strides(out, name)
+    else:
+        strides = (0, *out.stride())
+    ws, ws_ptr, nbytes = q.workspace()
+    _call(q.at.lib.fk_int8_assign, "fk_int8_assign", q.dev, *q.pointers(), out.data_ptr(), q.at.x_code,
+          *q.at.sizes, *q.at.strides, _c(strides), ws_ptr, nbytes)
     return out

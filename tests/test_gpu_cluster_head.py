@@ -199,6 +199,7 @@ INT_SIZES = [
     (0, 1, 1, 1, False), (0, 1, 1000, 128, False), (0, 7, 33, 100, False), (2, 65, 130, 97, False),
     (3, 50, 300, 256, True), (0, 400, 700, 255, False), (0, 1200, 2100, 160, False),
     (4, 300, 257, 1025, False), (0, 3, 4096, 4096, False),
+    (3, 9000, 700, 64, False),    # several row blocks of CTA pairs in turn, one column chunk
 ]
 
 

@@ -21,6 +21,7 @@
 // products of the next.  Every wait is bounded (fk_ptx.cuh).
 #pragma once
 #include <climits>
+#include <type_traits>
 
 #include "fk_common.cuh"
 #include "fk_ptx.cuh"
@@ -31,7 +32,7 @@ namespace head {
 constexpr int kMaxPairs = 6;
 constexpr int kCtlWarps = 4;
 constexpr int kStageRowBytes = 128;            // one swizzle row: 64 16-bit or 128 8-bit elements
-constexpr int kTableBytes = 2 * 2 * 256 * 4;   // two tables of 256 column scales and biases
+constexpr int kTableFloats = 2 * 64;           // column scales and biases of an epilogue warp
 constexpr int kSlotBytes = 3 * 128 * 8;        // (value, index) of a row from the other column parts
 
 enum Epilogue {
@@ -84,7 +85,7 @@ struct Problem {
   float p_scale;            // kEpiGrad: power of two that keeps float16 P out of its subnormals
   void* p_out;              // kEpiGrad: [part][batch][M][p_ld] 16-bit
   int64_t p_ld, p_part, p_batch;
-  int p_parts, p_bf16;
+  int p_bf16;
   float fscale;             // kEpiOut: factor, times *f_num, over max(*f_den, 1)
   const float* f_num;
   const int32_t* f_den;
@@ -128,7 +129,7 @@ struct Shape {
   // shared memory of an epilogue warp: 32 rows of 128 bytes (64 for P)
   static constexpr int kStaging = (EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : 4096);
   static constexpr int kStagingBytes = kEpiWarps * kStaging;
-  static constexpr int kExtra = EPI == kEpiArgmax ? kTableBytes + kSlotBytes : 0;
+  static constexpr int kExtra = EPI == kEpiArgmax ? kEpiWarps * 2 * kTableFloats * 4 + kSlotBytes : 0;
   static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes - kExtra;
   static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
   // accumulators in turn: the more, the less a tile waits for the one before
@@ -150,6 +151,15 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 __device__ __forceinline__ float fmax3(float a, float b, float c) { return fmaxf(a, fmaxf(b, c)); }
+
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 u;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
+  return u;
+}
 
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t r;
@@ -324,10 +334,10 @@ __device__ __forceinline__ bool argmax_better(float v, int i, float m, int j) {
 // than half of the epilogues' instructions).
 __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 
-// Barrier of the epilogue warps alone.
+// Barrier of the epilogue warps that share a lane quarter, hence rows.
 template <int THREADS>
-__device__ __forceinline__ void epilogue_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+__device__ __forceinline__ void quarter_sync(int quarter) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(THREADS) : "memory");
 }
 
 // ------------------------------------------------------------------- kernel
@@ -521,7 +531,9 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
     constexpr int kCols = BN / S::kParts;  // columns of this warp
     constexpr int kChunks = kCols / 32;
     uint8_t* stg = staging + ew * S::kStaging;
-    int buf = 0;
+    // kEpiArgmax: this lane's 128 bytes, 16-byte groups in swizzled order
+    const uint32_t save = smem_u32(stg) + lane * 128 + (lane & 7) * 16;
+    int buf = 0, tab = 0;
     uint32_t aphase = 0;
     Walk<EPI> walk(p, first, stride);
 
@@ -542,7 +554,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
     Tile t, nt;
     bool more = walk.get(nt);
     RowStat st_next = {0.0f, 0.0f, 0.0f, -1};
-    float xs_next = 0.0f, sc_next = 0.0f, bi_next = 0.0f;
+    float xs_next = 0.0f, sc_next[kChunks] = {}, bi_next[kChunks] = {};
     auto fetch = [&]() {
       const int64_t row = nt.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       if constexpr (EPI == kEpiGrad) {
@@ -554,10 +566,12 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
       }
       if constexpr (integer(EPI)) xs_next = row < p.M ? p.a_scale[nt.b * p.as_sb + row * p.as_sn] : 0.0f;
       if constexpr (EPI == kEpiArgmax) {
-        const int64_t col = nt.n * BN + ew * 32 + lane;
-        const bool ok = ew * 32 < BN && col < p.N;
-        sc_next = ok ? p.b_scale[nt.b * p.bs_sb + col * p.bs_sn] : 0.0f;
-        bi_next = ok && p.bias ? p.bias[nt.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          const int64_t col = nt.n * BN + part * kCols + c * 32 + lane;
+          sc_next[c] = col < p.N ? p.b_scale[nt.b * p.bs_sb + col * p.bs_sn] : 0.0f;
+          bi_next[c] = col < p.N && p.bias ? p.bias[nt.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+        }
       }
     };
     if (more) fetch();
@@ -585,20 +599,21 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
       st.coef *= p.p_scale;
       st.at_label *= p.p_scale;
       xs = xs_next;
-      float* table = reinterpret_cast<float*>(staging + S::kStagingBytes);
+      float* table = reinterpret_cast<float*>(staging + S::kStagingBytes) + ew * 2 * kTableFloats;
       if constexpr (EPI == kEpiArgmax) {
         if (t.first) {
           run_m = -INFINITY;
           run_i = INT_MAX;
         }
-        // this tile's column scales and biases, two tables in turn; the
-        // barrier also keeps the tile before last's readers ahead of the writes
-        table += (buf & 1) * (2 * 256);
-        if (ew * 32 < BN) {
-          table[ew * 32 + lane] = sc_next;
-          table[256 + ew * 32 + lane] = bi_next;
+        // this tile's column scales and biases, two tables of the warp in turn
+        table += tab * kTableFloats;
+        tab ^= 1;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          table[c * 32 + lane] = sc_next[c];
+          table[64 + c * 32 + lane] = bi_next[c];
         }
-        epilogue_sync<S::kEpiWarps * 32>();
+        __syncwarp();
       }
       if (more) fetch();
       // this lane's columns of every chunk
@@ -676,7 +691,14 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             for (int i = 0; i < 32; ++i)
               if (rel == i) e[i] = st.at_label;
           }
-          for (int pp = 0; pp < p.p_parts; ++pp) {
+          // rows of this warp in P, four lanes to a row of 64 bytes
+          uint8_t* dst = static_cast<uint8_t*>(p.p_out) +
+                         2 * (t.b * p.p_batch + (row0 + (lane >> 2)) * p.p_ld + cc + (lane & 3) * 8);
+          const int64_t step8 = 16 * p.p_ld;
+          const uint32_t wr = smem_u32(stg) + lane * 64, wx = (lane >> 1) & 3;
+          const uint32_t rd = smem_u32(stg) + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16);
+          const bool in = cc < p.p_ld;
+          auto put = [&](auto bf16, const int pp) {
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -684,25 +706,30 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int k = q * 8 + i * 2;
-                w[i] = p.p_bf16 ? pack_bf16(e[k], e[k + 1]) : pack_f16(e[k], e[k + 1]);
-                if (p.p_parts > 1) {  // what this part leaves for the next
+                w[i] = decltype(bf16)::value ? pack_bf16(e[k], e[k + 1]) : pack_f16(e[k], e[k + 1]);
+                if constexpr (EXACT) {  // what this part leaves for the next
                   e[k] -= __uint_as_float(w[i] << 16);
                   e[k + 1] -= __uint_as_float(w[i] & 0xffff0000u);
                 }
               }
-              *reinterpret_cast<uint4*>(stg + lane * 64 + ((q ^ ((lane >> 1) & 3)) * 16)) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
+              sts128(wr + ((q ^ wx) * 16), w[0], w[1], w[2], w[3]);
             }
             __syncwarp();
-            uint8_t* dst = static_cast<uint8_t*>(p.p_out) +
-                           2 * (pp * p.p_part + t.b * p.p_batch);
+            uint8_t* d = dst + 2 * pp * p.p_part;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int rr = i * 8 + (lane >> 2), q = lane & 3;
-              if (row0 + rr < p.M && cc < p.p_ld)
-                *reinterpret_cast<uint4*>(dst + 2 * ((row0 + rr) * p.p_ld + cc + q * 8)) =
-                    *reinterpret_cast<const uint4*>(stg + rr * 64 + ((q ^ ((rr >> 1) & 3)) * 16));
+              const uint4 u = lds128(rd + i * 512);
+              if (in && row0 + i * 8 + (lane >> 2) < p.M) *reinterpret_cast<uint4*>(d + i * step8) = u;
             }
+          };
+          if constexpr (EXACT) {
+            for (int pp = 0; pp < 3; ++pp) put(std::true_type{}, pp);
+          } else if (p.p_bf16) {
+            keep_branch();
+            put(std::true_type{}, 0);
+          } else {
+            keep_branch();
+            put(std::false_type{}, 0);
           }
         } else if constexpr (EPI == kEpiOut || EPI == kEpiScores) {
           if constexpr (EPI == kEpiScores) acc_to_f(v, p.small_acc != 0);
@@ -728,10 +755,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             if constexpr (EPI == kEpiScores) {
               float* ff = &f.x;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                ff[k] = __fmul_rn(ff[k], sc[c][k]);
-                if (p.bias) ff[k] = __fadd_rn(ff[k], bi[c][k]);
-              }
+              for (int k = 0; k < 4; ++k) ff[k] = __fadd_rn(__fmul_rn(ff[k], sc[c][k]), bi[c][k]);
             } else if (p.acc) {
               float* a = p.acc + t.chunk * p.acc_split + t.b * p.acc_batch + grow * p.acc_ld + col;
               if (p.acc_read) {
@@ -764,8 +788,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             }
           }
         } else {  // kEpiArgmax
-          const float* tsc = table + part * kCols + c * 32;
-          const float* tbi = tsc + 256;
+          const float* tsc = table + c * 32;
+          const float* tbi = tsc + 64;
           acc_to_f(v, p.small_acc != 0);
           const uint64_t x2 = pack2(xs, xs);
           float z[32];
@@ -774,11 +798,10 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             const float4 s4 = *reinterpret_cast<const float4*>(tsc + i);
             uint64_t z0 = mul2(mul2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), x2), pack2(s4.x, s4.y));
             uint64_t z1 = mul2(mul2(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), x2), pack2(s4.z, s4.w));
-            if (p.bias) {
-              const float4 b4 = *reinterpret_cast<const float4*>(tbi + i);
-              z0 = add2(z0, pack2(b4.x, b4.y));
-              z1 = add2(z1, pack2(b4.z, b4.w));
-            }
+            // without a bias the table holds zeros: no branch for every column
+            const float4 b4 = *reinterpret_cast<const float4*>(tbi + i);
+            z0 = add2(z0, pack2(b4.x, b4.y));
+            z1 = add2(z1, pack2(b4.z, b4.w));
             unpack2(z0, z[i], z[i + 1]);
             unpack2(z1, z[i + 2], z[i + 3]);
           }
@@ -804,8 +827,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             run_i = cc;
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-              *reinterpret_cast<float4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16)) =
-                  make_float4(z[q * 4], z[q * 4 + 1], z[q * 4 + 2], z[q * 4 + 3]);
+              sts128(save ^ (q * 16), __float_as_uint(z[q * 4]), __float_as_uint(z[q * 4 + 1]),
+                     __float_as_uint(z[q * 4 + 2]), __float_as_uint(z[q * 4 + 3]));
           }
         }
       };
@@ -856,8 +879,11 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
                                                 FK_DEV_WAIT_TIMEOUT));
         if (!got) {
           if constexpr (EPI == kEpiArgmax) {
-            // the other warps meet at the barriers of every tile: keep to them
-            if (t.last && p.chunks == 1) epilogue_sync<S::kEpiWarps * 32>();
+            // the warps of a row meet at its end: keep to that
+            if (t.last && p.chunks == 1) {
+              quarter_sync<S::kParts * 32>(quarter);
+              quarter_sync<S::kParts * 32>(quarter);
+            }
             if (++buf == S::kBufs) {
               buf = 0;
               aphase ^= 1;
@@ -900,20 +926,23 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             int at = 0;
 #pragma unroll
             for (int q = 7; q >= 0; --q) {
-              const float4 f = *reinterpret_cast<const float4*>(stg + lane * 128 + ((q ^ (lane & 7)) * 16));
-              const float* ff = &f.x;
+              const uint4 f = lds128(save ^ (q * 16));
+              const uint32_t* fu = &f.x;
 #pragma unroll
-              for (int i = 3; i >= 0; --i)
-                if (ff[i] == run_m || ff[i] != ff[i]) at = q * 4 + i;
+              for (int i = 3; i >= 0; --i) {
+                const float g = __uint_as_float(fu[i]);
+                if (g == run_m || g != g) at = q * 4 + i;
+              }
             }
             run_i += at;
           }
           if (p.chunks == 1) {
             // the column parts of a row meet in shared memory
-            float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + kTableBytes) +
+            float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes +
+                                                      S::kEpiWarps * 2 * kTableFloats * 4) +
                            (quarter * 32 + lane);
             if (part > 0) slot[(part - 1) * 128] = make_float2(run_m, __int_as_float(run_i));
-            epilogue_sync<S::kEpiWarps * 32>();
+            quarter_sync<S::kParts * 32>(quarter);
             if (part == 0 && row_ok) {
 #pragma unroll
               for (int o = 0; o < S::kParts - 1; ++o) {
@@ -925,6 +954,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
               }
               p.label_out[t.b * p.lo_sb + row * p.lo_sn] = run_i;
             }
+            // the slots are read before the next row block writes them
+            quarter_sync<S::kParts * 32>(quarter);
           } else if (row_ok) {
             p.partial[((static_cast<int64_t>(t.b) * p.chunks + t.chunk) * S::kParts + part) * p.M + row] =
                 make_float2(run_m, __int_as_float(run_i));

@@ -695,7 +695,6 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       p.p_ld = f.Kp;
       p.p_batch = f.R * f.Kp;
       p.p_part = q.B * f.R * f.Kp;
-      p.p_parts = q.parts();
       p.p_bf16 = !f16;
       st = launch<kEpiGrad>(prm, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, r0),
                             operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, k0), q.D, f.sh_p, s);

@@ -107,9 +107,19 @@ struct Problem {
   int* status;
 };
 
+// kEpiOut runs the two gradient products of a piece in one launch, the one with
+// the longer tiles first; its workers then take the other's tiles so that all
+// finish together.  In the second product every worker has `all` tiles, the
+// workers from `short_from` on (one tile of the first product behind) `more`
+// others, and the last `rest` workers one more.
+constexpr int problems_of(int epi) { return epi == kEpiOut ? 2 : 1; }
+
+template <int NP>
 struct Params {
-  CUtensorMap a, b;
-  Problem p;
+  CUtensorMap a[NP], b[NP];
+  Problem p[NP];
+  int count;
+  int all, short_from, more, rest;
 };
 
 template <int CG, int BN, int EPI>
@@ -195,6 +205,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // Where a tile sits.  Running epilogues visit the column tiles of a
 // (batch, row block, chunk) item in turn; the others one tile per item.
 struct Tile {
+  int q;               // which problem
   int b, m, n, chunk;
   int it0, it1;        // steps of the flattened (pair, kblock) contraction
   bool first, last;    // of the item
@@ -205,26 +216,52 @@ struct Tile {
 // more than a short tile's products).
 template <int EPI>
 struct Walk {
-  const Problem& p;
+  static constexpr int NP = problems_of(EPI);
+  const Params<NP>& prm;
   uint32_t item, total;
-  const uint32_t step;
+  const uint32_t slot, slots;
   Tile t;
-  int j_begin, j_end, w_end, wl, w0;
+  int j_begin, j_end, w_end, wl, w0, j;
 
-  __device__ Walk(const Problem& q, int first, int stride) : p(q), item(first), step(stride) {
-    total = static_cast<uint32_t>(p.batches) * p.chunks * p.m_tiles * (running(EPI) ? 1 : p.n_tiles);
+  __device__ Walk(const Params<NP>& q, int first, int stride) : prm(q), slot(first), slots(stride) {
+    t.q = 0;
+    item = slot;
+    total = items_of(prm.p[0]);
+    j = -1;
+    if (NP > 1 && item >= total) second();
     decode();
+  }
+  __device__ static uint32_t items_of(const Problem& p) {
+    return static_cast<uint32_t>(p.batches) * p.chunks * p.m_tiles * (running(EPI) ? 1 : p.n_tiles);
+  }
+  // this worker's next tile of the second problem
+  __device__ void second() {
+    t.q = NP - 1;
+    total = prm.count > 1 ? items_of(prm.p[NP - 1]) : 0;
+    ++j;
+    const uint32_t behind = prm.short_from, tail = slots - prm.rest;
+    if (j < prm.all) {
+      item = j * slots + slot;
+      return;
+    }
+    const int k = j - prm.all;
+    const int mine = slot >= behind ? prm.more : 0;
+    item = prm.all * slots;
+    if (k < mine) item += k * (slots - behind) + slot - behind;
+    else if (k == mine && slot >= tail) item += prm.more * (slots - behind) + slot - tail;
+    else item = total;
   }
   // Row blocks start at different tiles of a window, so that they do not all
   // read the same centroids from the same L2 slices at once.
   __device__ void window(int from) {
     w0 = from;
-    wl = min(p.window, j_end - from);
+    wl = min(prm.p[0].window, j_end - from);
     w_end = from + wl;
     t.n = w0 + static_cast<int>(static_cast<uint32_t>(t.m) % static_cast<uint32_t>(wl));
   }
   __device__ void decode() {
     if (item >= total) return;
+    const Problem& p = prm.p[NP > 1 ? t.q : 0];
     const int steps = p.npairs * p.kblocks;
     if constexpr (running(EPI)) {
       uint32_t r = item;
@@ -281,10 +318,14 @@ struct Walk {
         return;
       }
     }
-    item += step;
+    if (NP > 1 && t.q > 0) {
+      second();
+    } else {
+      item += slots;
+      if (NP > 1 && item >= total) second();
+    }
     decode();
   }
-  int j;
 };
 
 __device__ __forceinline__ int64_t load_label(const void* p, int64_t i, int dt) {
@@ -350,9 +391,10 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
 constexpr int kSegment = 4;       // of 64 elements: 16 truncated additions
 
 template <int CG, int BN, int EPI, bool EXACT>
-__global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const __grid_constant__ Params prm) {
+__global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const __grid_constant__ Params<problems_of(EPI)> prm) {
+  constexpr int NP = problems_of(EPI);
   using S = Shape<CG, BN, EPI>;
-  const Problem& p = prm.p;
+  const Problem& p0 = prm.p[0];
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -372,8 +414,10 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
   const int stride = gridDim.x / CG;
 
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&prm.a);
-    tma_prefetch_desc(&prm.b);
+    for (int i = 0; i < NP; ++i) {
+      tma_prefetch_desc(&prm.a[i]);
+      tma_prefetch_desc(&prm.b[i]);
+    }
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -395,7 +439,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
     }
   }
   if (warp == 3 && blockIdx.x == 0)
-    for (int i = lane; i < p.zero_n; i += 32) p.zero[i] = 0;
+    for (int i = lane; i < p0.zero_n; i += 32) p0.zero[i] = 0;
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
@@ -404,57 +448,86 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    // One thread issues every load of the CTA, one step of the contraction
+    // after another: what it executes per step bounds the kernel, so all that
+    // does not change from step to step is computed outside.
     if (lane == 0) {
-      const uint32_t tx = static_cast<uint32_t>(
-          (p.a_mn ? S::kABytes : p.a_rows * kStageRowBytes) + S::kBBytes) * CG;
-      const int kstep = integer(EPI) ? 128 : 64;
+      constexpr int kstep = integer(EPI) ? 128 : 64;
+      const uint32_t smem0 = smem_u32(smem), empty0 = smem_u32(empty);
+      const uint32_t full0 = smem_u32(full);                               // of this CTA
+      const uint32_t bar0 = CG == 2 ? map_to_rank(full, 0) : full0;        // of the pair's first
       int stage = 0;
       uint32_t phase = 0;
-      Walk<EPI> walk(p, first, stride);
+      Walk<EPI> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
-        int pair = t.it0 / p.kblocks, kb = t.it0 % p.kblocks;
-        for (int it = t.it0; it < t.it1; ++it) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT)) {
-            ok = false;
-            break;
-          }
-          uint8_t* sa = smem + stage * S::kStageBytes;
-          uint8_t* sb = sa + S::kABytes;
-          if (leader) mbar_arrive_expect_tx(&full[stage], tx);
-          const uint32_t bar = CG == 2 ? map_to_rank(&full[stage], 0) : smem_u32(&full[stage]);
-          const int az = t.b * p.a_batch + p.pa[pair] * p.a_part;
-          const int bz = t.b * p.b_batch + p.pb[pair] * p.b_part;
-          const int am = t.m * S::kBM + static_cast<int>(rank) * S::kARows;
-          const int bn = t.n * BN + static_cast<int>(rank) * S::kBRows;
-          if (p.a_mn) {
+        const Problem& p = prm.p[NP > 1 ? t.q : 0];
+        const CUtensorMap *ma = &prm.a[NP > 1 ? t.q : 0], *mb = &prm.b[NP > 1 ? t.q : 0];
+        const int kblocks = p.kblocks;
+        int pair = 0, kb = t.it0;
+        if (kb >= kblocks) {
+          pair = kb / kblocks;
+          kb -= pair * kblocks;
+        }
+        const int am = t.m * S::kBM + static_cast<int>(rank) * S::kARows;
+        const int bn = t.n * BN + static_cast<int>(rank) * S::kBRows;
+        int left = t.it1 - t.it0;
+        auto load = [&](auto a_mn, auto b_mn) {
+          constexpr bool kA = decltype(a_mn)::value, kB = decltype(b_mn)::value;
+          const uint32_t tx =
+              static_cast<uint32_t>((kA ? S::kABytes : p.a_rows * kStageRowBytes) + S::kBBytes) * CG;
+          const int a_at = kA ? am : p.a_off + am, b_at = kB ? bn : p.b_off + bn;
+          const int a_k = kA ? p.a_off : 0, b_k = kB ? p.b_off : 0;
+          while (left > 0) {
+            const int az = t.b * p.a_batch + p.pa[pair] * p.a_part;
+            const int bz = t.b * p.b_batch + p.pb[pair] * p.b_part;
+            const int n = min(left, kblocks - kb);
+            int c = kb * kstep;
+            for (int i = 0; i < n; ++i, c += kstep) {
+              if (!mbar_wait_at<false>(empty0 + stage * 8, phase ^ 1, abort_flag, p0.status,
+                                       FK_DEV_WAIT_TIMEOUT)) {
+                ok = false;
+                return;
+              }
+              const uint32_t sa = smem0 + stage * S::kStageBytes, sb = sa + S::kABytes;
+              if (leader) mbar_expect_at(full0 + stage * 8, tx);
+              const uint32_t bar = bar0 + stage * 8;
+              if constexpr (kA) {
 #pragma unroll
-            for (int g = 0; g < S::kARows / 64; ++g)
-              tma_load_3d_cg<CG>(sa + g * 8192, &prm.a, bar, am + g * 64, p.a_off + kb * 64, az);
-          } else {
-            tma_load_3d_cg<CG>(sa, &prm.a, bar, kb * kstep, p.a_off + am, az);
-          }
-          if (p.b_mn) {
+                for (int g = 0; g < S::kARows / 64; ++g)
+                  tma_load_3d_cg<CG>(sa + g * 8192, ma, bar, a_at + g * 64, a_k + c, az);
+              } else {
+                tma_load_3d_cg<CG>(sa, ma, bar, c, a_at, az);
+              }
+              if constexpr (kB) {
 #pragma unroll
-            for (int g = 0; g < S::kBRows / 64; ++g)
-              tma_load_3d_cg<CG>(sb + g * 8192, &prm.b, bar, bn + g * 64, p.b_off + kb * 64, bz);
-          } else {
-            tma_load_3d_cg<CG>(sb, &prm.b, bar, kb * kstep, p.b_off + bn, bz);
-          }
-          if (++stage == S::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-          if (++kb == p.kblocks) {
+                for (int g = 0; g < S::kBRows / 64; ++g)
+                  tma_load_3d_cg<CG>(sb + g * 8192, mb, bar, b_at + g * 64, b_k + c, bz);
+              } else {
+                tma_load_3d_cg<CG>(sb, mb, bar, c, b_at, bz);
+              }
+              if (++stage == S::kStages) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
+            left -= n;
             kb = 0;
             ++pair;
           }
+        };
+        if constexpr (EPI == kEpiOut) {
+          // dx: P by rows, centroids by columns; dc: both by columns
+          if (p.a_mn) load(std::true_type{}, std::true_type{});
+          else load(std::false_type{}, std::true_type{});
+        } else {
+          load(std::false_type{}, std::false_type{});
         }
       }
       // The last products' commits still arrive on this CTA's barriers, from
       // the pair's other CTA too: stay until they have.
       for (int i = 0; ok && i < S::kStages; ++i) {
-        ok = mbar_wait(&empty[stage], phase ^ 1, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
+        ok = mbar_wait_at<false>(empty0 + stage * 8, phase ^ 1, abort_flag, p0.status, FK_DEV_WAIT_TIMEOUT);
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1;
@@ -464,59 +537,69 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
     if (lane == 0 && leader) {
-      const uint32_t idesc = p.idesc;
-      const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+      const uint32_t full0 = smem_u32(full), empty0 = smem_u32(empty);
+      const uint32_t acc_full0 = smem_u32(acc_full), acc_empty0 = smem_u32(acc_empty);
+      const uint32_t smem0 = smem_u32(smem);
       int stage = 0, buf = 0;
       uint32_t phase = 0, aphase = 0;
-      Walk<EPI> walk(p, first, stride);
+      Walk<EPI> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
-        uint32_t accumulate = 0;
-        for (int it = t.it0; it < t.it1; ++it) {
-          if (accumulate == 0) {
-            if (!mbar_wait_cluster(&acc_empty[buf], aphase ^ 1, abort_flag, p.status,
-                                   FK_DEV_WAIT_TIMEOUT)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-          }
-          const uint32_t d = tmem + buf * BN;
-          if (!mbar_wait(&full[stage], phase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT)) {
+        const Problem& p = prm.p[NP > 1 ? t.q : 0];
+        const uint32_t idesc = p.idesc;
+        const bool a_mn = EPI == kEpiOut && p.a_mn;
+        constexpr bool b_mn = EPI == kEpiOut;
+        const uint64_t ad0 = a_mn ? smem_desc_sw128_mn(smem0, 8192, 1024) : smem_desc_sw128(smem0);
+        const uint64_t bd0 = b_mn ? smem_desc_sw128_mn(smem0 + S::kABytes, 8192, 1024)
+                                  : smem_desc_sw128(smem0 + S::kABytes);
+        const uint32_t a_step = (a_mn ? 2048 : 32) >> 4;
+        constexpr uint32_t b_step = (b_mn ? 2048 : 32) >> 4;
+        int left = t.it1 - t.it0;
+        while (ok && left > 0) {
+          // one accumulator: a segment (EXACT) or the whole tile
+          const int n = EXACT ? min(left, kSegment) : left;
+          left -= n;
+          if (!mbar_wait_at<true>(acc_empty0 + buf * 8, aphase ^ 1, abort_flag, p0.status,
+                                  FK_DEV_WAIT_TIMEOUT)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * S::kStageBytes);
-          const uint32_t b0 = a0 + S::kABytes;
-          uint64_t ad = p.a_mn ? smem_desc_sw128_mn(a0, 8192, 1024) : smem_desc_sw128(a0);
-          uint64_t bd = p.b_mn ? smem_desc_sw128_mn(b0, 8192, 1024) : smem_desc_sw128(b0);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if constexpr (integer(EPI)) mma_i8_cg<CG>(d, ad, bd, idesc, accumulate);
-            else mma_f16_cg<CG>(d, ad, bd, idesc, accumulate);
-            accumulate = 1;
-            ad += a_step >> 4;
-            bd += b_step >> 4;
-          }
-          mma_commit_cg<CG>(&empty[stage]);
-          if (++stage == S::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
-          if (it + 1 == t.it1 || (EXACT && (it + 1 - t.it0) % kSegment == 0)) {
-            mma_commit_cg<CG>(&acc_full[buf]);
-            if (++buf == S::kBufs) {
-              buf = 0;
-              aphase ^= 1;
+          const uint32_t d = tmem + buf * BN;
+          for (int i = 0; i < n; ++i) {
+            if (!mbar_wait_at<false>(full0 + stage * 8, phase, abort_flag, p0.status,
+                                     FK_DEV_WAIT_TIMEOUT)) {
+              ok = false;
+              break;
             }
-            accumulate = 0;
+            tc_fence_after();
+            const uint32_t at = stage * (S::kStageBytes >> 4);
+            uint64_t ad = ad0 + at, bd = bd0 + at;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t accumulate = k > 0 || i > 0;
+              if constexpr (integer(EPI)) mma_i8_cg<CG>(d, ad, bd, idesc, accumulate);
+              else mma_f16_cg<CG>(d, ad, bd, idesc, accumulate);
+              ad += a_step;
+              bd += b_step;
+            }
+            mma_commit_cg<CG>(empty0 + stage * 8);
+            if (++stage == S::kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          if (!ok) break;
+          mma_commit_cg<CG>(acc_full0 + buf * 8);
+          if (++buf == S::kBufs) {
+            buf = 0;
+            aphase ^= 1;
           }
         }
       }
       // and so do the epilogues' arrivals on the accumulators' barriers
       for (int i = 0; ok && i < S::kBufs; ++i) {
-        ok = mbar_wait_cluster(&acc_empty[buf], aphase ^ 1, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
+        ok = mbar_wait_at<true>(acc_empty0 + buf * 8, aphase ^ 1, abort_flag, p0.status, FK_DEV_WAIT_TIMEOUT);
         if (++buf == S::kBufs) {
           buf = 0;
           aphase ^= 1;
@@ -535,7 +618,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
     const uint32_t save = smem_u32(stg) + lane * 128 + (lane & 7) * 16;
     int buf = 0, tab = 0;
     uint32_t aphase = 0;
-    Walk<EPI> walk(p, first, stride);
+    Walk<EPI> walk(prm, first, stride);
 
     // running state of a row
     float run_m = -INFINITY, run_s = 0.0f;
@@ -544,9 +627,9 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
     float xs = 0.0f;
     float fac = 0.0f;
     if constexpr (EPI == kEpiOut) {
-      fac = p.fscale;
-      if (p.f_num) fac *= *p.f_num;
-      if (p.f_den) fac /= static_cast<float>(max(*p.f_den, 1));
+      fac = p0.fscale;
+      if (p0.f_num) fac *= *p0.f_num;
+      if (p0.f_den) fac /= static_cast<float>(max(*p0.f_den, 1));
     }
 
     // What the epilogue needs from memory besides the accumulator is fetched a
@@ -556,6 +639,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
     RowStat st_next = {0.0f, 0.0f, 0.0f, -1};
     float xs_next = 0.0f, sc_next[kChunks] = {}, bi_next[kChunks] = {};
     auto fetch = [&]() {
+      const Problem& p = p0;
       const int64_t row = nt.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       if constexpr (EPI == kEpiGrad) {
         st_next = {0.0f, 0.0f, 0.0f, -1};
@@ -579,6 +663,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
       t = nt;
       walk.next();
       more = walk.get(nt);
+      const Problem& p = prm.p[NP > 1 ? t.q : 0];
       const int row = t.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       const int row0 = row - lane;
       const bool row_ok = row < p.M;
@@ -841,7 +926,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
         for (int it = t.it0; it < t.it1; it += kSegment) {
-          got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p.status,
+          got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
                                                   FK_DEV_WAIT_TIMEOUT));
           if (!got) break;
           tc_fence_after();
@@ -875,7 +960,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
           chunk(c, v);
         }
       } else {
-        got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p.status,
+        got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
                                                 FK_DEV_WAIT_TIMEOUT));
         if (!got) {
           if constexpr (EPI == kEpiArgmax) {

@@ -1,6 +1,7 @@
 // Host side of the cluster head's products: operand maps, tile shapes and
 // launches of head_gemm.
 #pragma once
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -57,10 +58,39 @@ inline int choose_chunks(int64_t items, int64_t units, int64_t slots, int64_t mo
   return best;
 }
 
+// How `workers` share the tiles of two problems, those of the first (n0 of cost
+// c0 >= c1) dealt out in turn: see Params.
+struct Fill {
+  int all, short_from, more, rest;
+  double span;   // cost of the longest worker
+};
+inline double tile_cost(int64_t steps) { return static_cast<double>(steps) + 3.0; }
+inline double tile_cost(const Problem& p) {
+  return tile_cost(ceil_div(static_cast<int64_t>(p.npairs) * p.kblocks, p.chunks));
+}
+inline Fill fill(int64_t n0, double c0, int64_t n1, double c1, int64_t workers) {
+  Fill f = {};
+  const int64_t ahead = n0 % workers;            // workers with one tile more
+  const int64_t behind = workers - ahead;
+  int64_t more = ahead ? static_cast<int64_t>(c0 / c1) : 0;
+  if (more * behind > n1) more = n1 / behind;
+  const int64_t left = n1 - more * behind;
+  const int64_t all = more < (ahead ? static_cast<int64_t>(c0 / c1) : 0) ? 0 : left / workers;
+  const int64_t rest = left - all * workers;
+  f.all = static_cast<int>(all);
+  f.short_from = static_cast<int>(ahead);
+  f.more = static_cast<int>(more);
+  f.rest = static_cast<int>(rest);
+  const double base = static_cast<double>(n0 / workers) * c0 + static_cast<double>(all) * c1;
+  const double low = base + static_cast<double>(more) * c1;
+  f.span = std::max(ahead ? base + c0 + (rest > behind ? c1 : 0.0) : 0.0, low + (rest > 0 ? c1 : 0.0));
+  return f;
+}
+
 int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows);
 
 template <int CG, int BN, int EPI, bool EXACT>
-int launch_shape(Params& prm, cudaStream_t s) {
+int launch_shape(Params<problems_of(EPI)>& prm, cudaStream_t s) {
   using S = Shape<CG, BN, EPI>;
   auto kern = head_gemm<CG, BN, EPI, EXACT>;
   const int dev = current_device();
@@ -73,14 +103,26 @@ int launch_shape(Params& prm, cudaStream_t s) {
   }
   const int sms = sm_count_current();
   if (sms <= 0) return fail(FK_ERR_CUDA, "no SM count for device %d", dev);
-  const Problem& p = prm.p;
-  const int64_t items = static_cast<int64_t>(p.batches) * p.chunks * p.m_tiles *
-                        (running(EPI) ? 1 : p.n_tiles);
-  if (items >= (1ll << 31) || static_cast<int64_t>(p.n_tiles) * p.chunks >= (1ll << 31) ||
-      static_cast<int64_t>(p.npairs) * p.kblocks * p.chunks >= (1ll << 31))
-    return fail(FK_ERR_UNSUPPORTED, "head_gemm: %lld tiles exceed 32-bit", static_cast<long long>(items));
   const int64_t slots = sms / CG;
-  const unsigned grid = static_cast<unsigned>((items < slots ? items : slots) * CG);
+  int64_t items = 0, first = 0;
+  for (int i = 0; i < prm.count; ++i) {
+    const Problem& p = prm.p[i];
+    const int64_t n = static_cast<int64_t>(p.batches) * p.chunks * p.m_tiles * (running(EPI) ? 1 : p.n_tiles);
+    items += n;
+    if (i == 0) first = n;
+    if (items >= (1ll << 31) || static_cast<int64_t>(p.n_tiles) * p.chunks >= (1ll << 31) ||
+        static_cast<int64_t>(p.npairs) * p.kblocks * p.chunks >= (1ll << 31))
+      return fail(FK_ERR_UNSUPPORTED, "head_gemm: %lld tiles exceed 32-bit", static_cast<long long>(items));
+  }
+  const int64_t workers = items < slots ? items : slots;
+  const unsigned grid = static_cast<unsigned>(workers * CG);
+  if (prm.count > 1) {
+    const Fill f = fill(first, tile_cost(prm.p[0]), items - first, tile_cost(prm.p[1]), workers);
+    prm.all = f.all;
+    prm.short_from = f.short_from;
+    prm.more = f.more;
+    prm.rest = f.rest;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(S::kThreads);
@@ -100,12 +142,12 @@ int launch_shape(Params& prm, cudaStream_t s) {
   return FK_OK;
 }
 
-// Fills in the product's tiles and maps and launches it.  `kdim` elements are
-// contracted; p.M, p.N, p.batches, p.chunks and the epilogue's fields are set.
+// The tiles and maps of prm's problem i.  `kdim` elements are contracted; p.M,
+// p.N, p.batches, p.chunks and the epilogue's fields are set.
 template <int EPI>
-int launch(Params& prm, const Operand& a, const Operand& b, int64_t kdim, ShapeChoice sh,
-           cudaStream_t s) {
-  Problem& p = prm.p;
+int set_problem(Params<problems_of(EPI)>& prm, int i, const Operand& a, const Operand& b, int64_t kdim,
+                ShapeChoice sh) {
+  Problem& p = prm.p[i];
   const int step = integer(EPI) ? 128 : 64;
   p.m_tiles = static_cast<int>(ceil_div(p.M, sh.bm()));
   p.n_tiles = static_cast<int>(ceil_div(p.N, sh.bn));
@@ -130,16 +172,22 @@ int launch(Params& prm, const Operand& a, const Operand& b, int64_t kdim, ShapeC
     p.idesc = instr_desc(a.dtype == FK_BF16 ? 1 : 0, 128 * sh.cg, sh.bn) |
               (a.mn ? 1u << 15 : 0u) | (b.mn ? 1u << 16 : 0u);
   }
-  int st = encode_operand(&prm.a, a, a.mn ? 64 : p.a_rows);
+  const int st = encode_operand(&prm.a[i], a, a.mn ? 64 : p.a_rows);
   if (st != FK_OK) return st;
-  st = encode_operand(&prm.b, b, b.mn ? 64 : sh.bn / sh.cg);
-  if (st != FK_OK) return st;
+  return encode_operand(&prm.b[i], b, b.mn ? 64 : sh.bn / sh.cg);
+}
+
+template <int EPI>
+int launch(Params<problems_of(EPI)>& prm, ShapeChoice sh, cudaStream_t s) {
   if constexpr (!integer(EPI)) {
-    if (p.npairs > 1) {
+    if (prm.p[0].npairs > 1) {
       if (sh.cg == 2) return launch_shape<2, 128, EPI, true>(prm, s);
       if (sh.bn == 128) return launch_shape<1, 128, EPI, true>(prm, s);
       return launch_shape<1, 64, EPI, true>(prm, s);
     }
+  }
+  if constexpr (EPI == kEpiOut) {
+    if (sh.cg == 2 && sh.bn == 128) return launch_shape<2, 128, EPI, false>(prm, s);
   }
   if (sh.cg == 2) return launch_shape<2, 256, EPI, false>(prm, s);
   if (sh.bn == 128) return launch_shape<1, 128, EPI, false>(prm, s);

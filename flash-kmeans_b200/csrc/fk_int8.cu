@@ -325,8 +325,9 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
     st = f.xq ? pack8(q.x, q.B, q.N, q.D, q.xs, f.xq, q.Dp(), s) : FK_OK;
   if (st != FK_OK) return st;
   if (f.cq && (st = pack8(q.c, q.Bc(), q.K, q.D, q.cs, f.cq, q.Dp(), s)) != FK_OK) return st;
-  Params prm = {};
-  Problem& p = prm.p;
+  Params<1> prm = {};
+  prm.count = 1;
+  Problem& p = prm.p[0];
   p = base;
   p.M = static_cast<int>(q.N);
   p.N = static_cast<int>(q.K);
@@ -348,8 +349,9 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   p.lo_sb = ls ? ls[0] : 0;
   p.lo_sn = ls ? ls[1] : 0;
   p.status = status;
-  st = launch<EPI>(prm, operand8(q, q.x, f.xq, q.B, q.N, q.xs), operand8(q, q.c, f.cq, q.Bc(), q.K, q.cs),
-                   q.D, f.sh, s);
+  st = set_problem<EPI>(prm, 0, operand8(q, q.x, f.xq, q.B, q.N, q.xs),
+                        operand8(q, q.c, f.cq, q.Bc(), q.K, q.cs), q.D, f.sh);
+  if (st == FK_OK) st = launch<EPI>(prm, f.sh, s);
   if (st != FK_OK || !f.partial) return st;
   const int64_t row_blocks = ceil_div(q.N, 32);
   argmax_join_kernel<<<static_cast<unsigned>(q.B * row_blocks), kJoinWarps * 32, 0, s>>>(

@@ -254,25 +254,36 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
                : "memory");
 }
 
-// mbar_wait for a barrier that the other CTA of the pair arrives on too.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred P;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2, %3;\n\t"
-      "selp.b32 %0, 1, 0, P;\n\t}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(kSuspendHintNs)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
-                                                  volatile int* abort_flag, int* dev_status,
-                                                  int code) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
+// mbar_wait on a shared-space address, with CLUSTER for a barrier that the other
+// CTA of the pair arrives on too: what a single thread that paces the kernel
+// executes per step is kept short.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_wait_at(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                             int* dev_status, int code) {
+  auto poll = [&]() {
+    uint32_t ok;
+    if constexpr (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred P;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2, %3;\n\t"
+          "selp.b32 %0, 1, 0, P;\n\t}\n"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(kSuspendHintNs)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred P;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+          "selp.b32 %0, 1, 0, P;\n\t}\n"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity), "r"(kSuspendHintNs)
+          : "memory");
+    return ok != 0;
+  };
+  if (poll()) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (poll()) return true;
     if (*abort_flag) return false;
     if (globaltimer_ns() - t0 > FK_WAIT_LIMIT_NS) {
       *abort_flag = code;
@@ -280,6 +291,10 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       return false;
     }
   }
+}
+
+__device__ __forceinline__ void mbar_expect_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
 // One arrival on a barrier of this CTA (CG = 1) or of the pair's first CTA (CG = 2).
@@ -297,18 +312,18 @@ __device__ __forceinline__ void mbar_arrive_cg(uint64_t* bar) {
 // 3-D tiled load into this CTA's shared memory; `bar` is a shared::cluster
 // address, with CG = 2 that of the pair's first CTA.
 template <int CG>
-__device__ __forceinline__ void tma_load_3d_cg(void* smem_dst, const void* tmap, uint32_t bar,
+__device__ __forceinline__ void tma_load_3d_cg(uint32_t smem_dst, const void* tmap, uint32_t bar,
                                                int32_t c0, int32_t c1, int32_t c2) {
   if constexpr (CG == 1) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
   } else {
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_dst),
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
         : "memory");
   }
@@ -352,13 +367,15 @@ __device__ __forceinline__ void mma_i8_cg(uint32_t d_tmem, uint64_t a_desc, uint
 
 // mma_commit; with CG = 2 the barrier's counterparts in both CTAs get the arrival.
 template <int CG>
-__device__ __forceinline__ void mma_commit_cg(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit_cg(uint32_t bar) {
   if constexpr (CG == 1) {
-    mma_commit(bar);
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
   } else {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-        " [%0], %1;" ::"r"(smem_u32(bar)),
+        " [%0], %1;" ::"r"(bar),
         "h"(static_cast<uint16_t>(3))
         : "memory");
   }

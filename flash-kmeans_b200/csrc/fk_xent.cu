@@ -59,32 +59,52 @@ __device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
   p[2] = static_cast<uint16_t>(pack_bf16(r, 0.0f) & 0xffffu);
 }
 
+struct Labels {
+  const void* p = nullptr;
+  int dtype = FK_I32;
+  int64_t sb = 0, sn = 0;
+  int64_t ignore = -100;
+};
+
+struct RowsJob {        // one tensor to copy; units = 0 for none
+  const void* x;
+  int64_t sb, sn, sd;
+  int vec;              // rows can be read 16 bytes at a time
+  uint16_t* out;
+  int64_t part;         // elements from one part to the next
+  int N, D, Dp;
+  int64_t units;        // of eight elements
+  Labels y;             // p: ignored rows become zeros
+};
+struct RowsJobs {
+  RowsJob job[2];
+};
+
 template <typename T>
-__global__ void head_rows_kernel(const T* __restrict__ x, int64_t sb, int64_t sn, int64_t sd, int vec,
-                                 uint16_t* __restrict__ out, int64_t part, int N, int D, int Dp,
-                                 int64_t units, const void* labels, int label_dtype, int64_t lb,
-                                 int64_t ln, int64_t ignore_index) {
-  const int per = Dp / 8;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < units;
+__global__ void head_rows_kernel(const RowsJobs jobs) {
+  const RowsJob& j = jobs.job[blockIdx.y];
+  const T* __restrict__ x = static_cast<const T*>(j.x);
+  const int per = j.Dp / 8, D = j.D;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < j.units;
        u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t row = u / per;
     const int d0 = static_cast<int>(u - row * per) * 8;
-    const int64_t b = row / N, n = row - b * N;
+    const int64_t b = row / j.N, n = row - b * j.N;
     T v[8];
-    const bool zero = labels && load_label(labels, b * lb + n * ln, label_dtype) == ignore_index;
-    const T* src = x + b * sb + n * sn;
+    const bool zero = j.y.p && load_label(j.y.p, b * j.y.sb + n * j.y.sn, j.y.dtype) == j.y.ignore;
+    const T* src = x + b * j.sb + n * j.sn;
     if (zero) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = Elem<T>::from_f(0.0f);
-    } else if (vec && d0 + 8 <= D) {
+    } else if (j.vec && d0 + 8 <= D) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
         reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src + d0)[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = d0 + i < D ? src[(d0 + i) * sd] : Elem<T>::from_f(0.0f);
+      for (int i = 0; i < 8; ++i) v[i] = d0 + i < D ? src[(d0 + i) * j.sd] : Elem<T>::from_f(0.0f);
     }
-    uint16_t* dst = out + row * Dp + d0;
+    uint16_t* dst = j.out + row * j.Dp + d0;
     if constexpr (sizeof(T) == 2) {
       *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(v);
     } else {
@@ -97,42 +117,47 @@ __global__ void head_rows_kernel(const T* __restrict__ x, int64_t sb, int64_t sn
         uint32_t* ww = &w.x;
 #pragma unroll
         for (int i = 0; i < 4; ++i) ww[i] = p[2 * i][q] | static_cast<uint32_t>(p[2 * i + 1][q]) << 16;
-        *reinterpret_cast<uint4*>(dst + q * part) = w;
+        *reinterpret_cast<uint4*>(dst + q * j.part) = w;
       }
     }
   }
 }
 
-struct Labels {
-  const void* p = nullptr;
-  int dtype = FK_I32;
-  int64_t sb = 0, sn = 0;
-  int64_t ignore = -100;
-};
-
-template <typename T>
-static int rows_copy_typed(const void* x, int64_t B, int64_t N, int64_t D, const int64_t* xs,
-                           uint16_t* out, int64_t Dp, const Labels& y, bool mask, cudaStream_t s) {
-  const int64_t units = B * N * (Dp / 8);
-  const int vec = (xs[2] == 1 || D == 1) && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
-                  (N == 1 || xs[1] * sizeof(T) % 16 == 0) && (B == 1 || xs[0] * sizeof(T) % 16 == 0);
-  const int sms = sm_count_current();
-  const int64_t cap = (sms > 0 ? sms : 148) * 16ll;
-  const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(units, 256), cap));
-  head_rows_kernel<T><<<blocks, 256, 0, s>>>(static_cast<const T*>(x), xs[0], xs[1], xs[2], vec, out,
-                                             B * N * Dp, static_cast<int>(N), static_cast<int>(D),
-                                             static_cast<int>(Dp), units, mask ? y.p : nullptr,
-                                             y.dtype, y.sb, y.sn, y.ignore);
-  return check_launch("head_rows_kernel");
+static RowsJob rows_job(const void* x, int dtype, int64_t B, int64_t N, int64_t D, const int64_t* xs,
+                        uint16_t* out, int64_t Dp, const Labels* y) {
+  RowsJob j = {};
+  if (!out) return j;
+  const int64_t eb = dtype_bytes(dtype);
+  j.x = x;
+  j.sb = xs[0];
+  j.sn = xs[1];
+  j.sd = xs[2];
+  j.vec = (xs[2] == 1 || D == 1) && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+          (N == 1 || xs[1] * eb % 16 == 0) && (B == 1 || xs[0] * eb % 16 == 0);
+  j.out = out;
+  j.part = B * N * Dp;
+  j.N = static_cast<int>(N);
+  j.D = static_cast<int>(D);
+  j.Dp = static_cast<int>(Dp);
+  j.units = B * N * (Dp / 8);
+  if (y) j.y = *y;
+  return j;
 }
 
-static int rows_copy(const void* x, int dtype, int64_t B, int64_t N, int64_t D, const int64_t* xs,
-                     uint16_t* out, int64_t Dp, const Labels& y, bool mask, cudaStream_t s) {
+// Both copies in one launch.
+static int rows_copy(int dtype, const RowsJob& a, const RowsJob& b, cudaStream_t s) {
+  RowsJobs jobs = {{a.units ? a : b, b}};
+  const int n = (a.units ? 1 : 0) + (b.units ? 1 : 0);
+  if (n == 0) return FK_OK;
+  const int sms = sm_count_current();
+  const int64_t cap = (sms > 0 ? sms : 148) * 16ll;
+  const dim3 grid(static_cast<unsigned>(std::min(ceil_div(std::max(a.units, b.units), 256), cap)), n);
   switch (dtype) {
-    case FK_F16: return rows_copy_typed<__half>(x, B, N, D, xs, out, Dp, y, mask, s);
-    case FK_BF16: return rows_copy_typed<__nv_bfloat16>(x, B, N, D, xs, out, Dp, y, mask, s);
-    default: return rows_copy_typed<float>(x, B, N, D, xs, out, Dp, y, mask, s);
+    case FK_F16: head_rows_kernel<__half><<<grid, 256, 0, s>>>(jobs); break;
+    case FK_BF16: head_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(jobs); break;
+    default: head_rows_kernel<float><<<grid, 256, 0, s>>>(jobs); break;
   }
+  return check_launch("head_rows_kernel");
 }
 
 // ------------------------------------------------------------------ combine
@@ -345,18 +370,32 @@ __global__ void xent_weight_kernel(const float* __restrict__ g, const RowStat* _
 }
 
 // ---------------------------------------------------- split sums to the output
-__global__ void head_join_kernel(const float* __restrict__ acc, int splits, int64_t split_stride,
-                                 int64_t acc_batch, int64_t acc_ld, void* out, int dtype, int64_t ob,
-                                 int64_t orow, int rows, int cols, int64_t total) {
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+struct JoinJob {        // total = 0 for none
+  const float* acc;
+  int splits;
+  int64_t split_stride, acc_batch, acc_ld;
+  void* out;
+  int dtype;
+  int64_t ob, orow;
+  int rows, cols;
+  int64_t total;
+};
+struct JoinJobs {
+  JoinJob job[2];
+};
+
+__global__ void head_join_kernel(const JoinJobs jobs) {
+  const JoinJob& j = jobs.job[blockIdx.y];
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < j.total;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / cols;
-    const int c = static_cast<int>(i - r * cols);
-    const int64_t b = r / rows, n = r - b * rows;
-    const float* a = acc + b * acc_batch + n * acc_ld + c;
+    const int64_t r = i / j.cols;
+    const int c = static_cast<int>(i - r * j.cols);
+    const int64_t b = r / j.rows, n = r - b * j.rows;
+    const float* a = j.acc + b * j.acc_batch + n * j.acc_ld + c;
     float v = 0.0f;
-    for (int s = 0; s < splits; ++s) v += a[s * split_stride];
-    store_f(out, b * ob + n * orow + c, dtype, v);
+#pragma unroll 4
+    for (int s = 0; s < j.splits; ++s) v += a[s * j.split_stride];
+    store_f(j.out, b * j.ob + n * j.orow + c, j.dtype, v);
   }
 }
 
@@ -480,13 +519,12 @@ static ForwardPlan plan_forward(const Xent& q, void* ws) {
 static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, void* ws, int* status,
                    cudaStream_t s) {
   const ForwardPlan f = plan_forward(q, ws);
-  int st;
-  if (f.xc && (st = rows_copy(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), q.y, false, s)) != FK_OK)
-    return st;
-  if (f.cc && (st = rows_copy(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), q.y, false, s)) != FK_OK)
-    return st;
-  Params prm = {};
-  Problem& p = prm.p;
+  int st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), nullptr),
+                     rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  if (st != FK_OK) return st;
+  Params<1> prm = {};
+  prm.count = 1;
+  Problem& p = prm.p[0];
   p.M = static_cast<int>(q.N);
   p.N = static_cast<int>(q.K);
   p.batches = static_cast<int>(q.B);
@@ -502,8 +540,9 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   p.zero = f.ticket;
   p.zero_n = 1;
   p.status = status;
-  st = launch<kEpiLse>(prm, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, 0),
-                       operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, 0), q.D, f.sh, s);
+  st = set_problem<kEpiLse>(prm, 0, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, 0),
+                            operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, 0), q.D, f.sh);
+  if (st == FK_OK) st = launch<kEpiLse>(prm, f.sh, s);
   if (st != FK_OK) return st;
   CombineParams cp = {};
   cp.partial = f.partial;
@@ -547,7 +586,7 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
 struct BackwardPlan {
   int64_t R, Kp;               // rows and centroids of a piece
   int64_t n_chunks, n_pieces;
-  ShapeChoice sh_p, sh_x, sh_c;
+  ShapeChoice sh_p, sh;          // of P, of the two gradient products
   int split_x, split_c;
   int64_t ld;                  // of the float32 accumulators
   uint16_t *xc, *cc, *P;
@@ -556,6 +595,51 @@ struct BackwardPlan {
   float* gmax;                 // (largest |g|, the factor it gives)
   size_t bytes;
 };
+
+// Tile shape and splits of the two gradient products: dx is Mx x D over steps_x
+// steps, dc Mc x D over steps_c (0: not wanted).  A product with few tiles and a
+// long contraction is split along it; each split costs a pass over float32
+// partial sums, counted in steps of a tile's contraction (0.27 us each).
+static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc, int64_t steps_c,
+                          BackwardPlan* f) {
+  const bool exact = q.parts() > 1;
+  const int wide = exact || q.D <= 128 ? 128 : 256;
+  auto tiles = [&](int64_t M, int64_t steps, int64_t bm, int64_t bn) {
+    return steps ? q.B * ceil_div(M, bm) * ceil_div(q.D, bn) : 0;
+  };
+  // work in shares of 16 steps, the least that is worth a worker
+  auto shares = [&](int64_t bm, int64_t bn) {
+    return tiles(Mx, steps_x, bm, bn) * std::max<int64_t>(1, steps_x / 16) +
+           tiles(Mc, steps_c, bm, bn) * std::max<int64_t>(1, steps_c / 16);
+  };
+  if (std::max(Mx, Mc) > 128 && shares(256, wide) >= 74) f->sh = {2, wide};
+  else if (q.D > 64 && shares(128, 128) >= 100) f->sh = {1, 128};
+  else f->sh = {1, 64};
+  f->split_x = f->split_c = 1;
+  const int64_t slots = slots_of(f->sh);
+  const int64_t tx = tiles(Mx, steps_x, f->sh.bm(), f->sh.bn), tc = tiles(Mc, steps_c, f->sh.bm(), f->sh.bn);
+  if (tx + tc >= 8 * slots) return;
+  static const int tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+  const double us = 0.27 * f->sh.cg * f->sh.bn / 512.0;   // a step of this shape
+  double best = 1e300;
+  for (int sx : tries) {
+    if (sx > 1 && (sx > steps_x || tx * sx > 4 * slots)) break;
+    for (int sc : tries) {
+      if (sc > 1 && (sc > steps_c || tc * sc > 4 * slots)) break;
+      const double cx = tile_cost(ceil_div(steps_x, sx)), cc = tile_cost(ceil_div(steps_c, sc));
+      const int64_t n = tx * sx + tc * sc, workers = std::min(n, slots);
+      const double span = cx >= cc ? fill(tx * sx, cx, tc * sc, cc, workers).span
+                                   : fill(tc * sc, cc, tx * sx, cx, workers).span;
+      const double bytes = (sx > 1 ? 4.0 * q.B * Mx * q.D * (2 * sx) : 0.0) + (sc > 1 ? 4.0 * q.B * Mc * q.D * (2 * sc) : 0.0);
+      const double join = sx > 1 || sc > 1 ? (3.0 + bytes / 4e6) / us : 0.0;
+      if (span + join < best * 0.999) {
+        best = span + join;
+        f->split_x = sx;
+        f->split_c = sc;
+      }
+    }
+  }
+}
 
 static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void* ws) {
   BackwardPlan f;
@@ -575,13 +659,7 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   const int pairs = q.parts() == 3 ? 6 : 1;
   f.sh_p = choose_shape(f.R, kw, q.B, 1, q.parts() > 1);
   const int64_t steps_x = pairs * ceil_div(kw, 64), steps_c = pairs * ceil_div(f.R, 64);
-  auto pick = [&](int64_t M, int64_t steps, ShapeChoice* sh) {
-    *sh = choose_shape(M, q.D, q.B, std::max<int64_t>(1, steps / 16), q.parts() > 1);
-    const int64_t items = q.B * ceil_div(M, sh->bm()) * ceil_div(q.D, sh->bn);
-    return items >= 4 * slots_of(*sh) ? 1 : choose_chunks(items, steps, slots_of(*sh), 16, 3.0);
-  };
-  f.split_x = pick(f.R, steps_x, &f.sh_x);
-  f.split_c = pick(kw, steps_c, &f.sh_c);
+  plan_products(q, f.R, want_x ? steps_x : 0, kw, want_c ? steps_c : 0, &f);
   f.ld = ceil_div(q.D, 4) * 4;
   f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
   f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
@@ -602,13 +680,13 @@ struct Grad {
   int64_t sb, sr;
 };
 
-// One gradient product over a piece, into the accumulator or the output.
-static int grad_product(const Xent& q, Problem base, const Operand& a, const Operand& b, int64_t M,
-                        int64_t kdim, ShapeChoice sh, int splits, float* acc, int64_t acc_rows,
-                        int64_t acc_row0, int64_t ld, bool first, bool last, const Grad& g,
-                        int64_t out_row0, cudaStream_t s) {
-  Params prm = {};
-  Problem& p = prm.p;
+// One gradient product over a piece, into the accumulator or the output; `join`
+// is what its splits leave to add up.
+static int grad_problem(const Xent& q, Params<2>& prm, JoinJob* join, const Problem& base, const Operand& a,
+                        const Operand& b, int64_t M, int64_t kdim, ShapeChoice sh, int splits, float* acc,
+                        int64_t acc_rows, int64_t acc_row0, int64_t ld, bool first, bool last, const Grad& g,
+                        int64_t out_row0) {
+  Problem& p = prm.p[prm.count];
   p = base;
   p.M = static_cast<int>(M);
   p.N = static_cast<int>(q.D);
@@ -628,20 +706,13 @@ static int grad_product(const Xent& q, Problem base, const Operand& a, const Ope
     p.acc_read = !first;
     p.acc_write = splits > 1 || !last;
   }
-  int st = launch<kEpiOut>(prm, a, b, kdim, sh, s);
-  if (st != FK_OK) return st;
   if (splits > 1 && last) {
-    const int64_t total = q.B * M * q.D;
-    const int sms = sm_count_current();
-    const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(total, 256), (sms > 0 ? sms : 148) * 16ll));
     // a short last piece may have fewer steps than splits: the others hold
     // earlier pieces' sums, or were never written if this is the only piece
-    head_join_kernel<<<blocks, 256, 0, s>>>(p.acc, first ? p.chunks : splits, p.acc_split, p.acc_batch,
-                                            ld, p.out, q.dtype, g.sb, g.sr, static_cast<int>(M),
-                                            static_cast<int>(q.D), total);
-    st = check_launch("head_join_kernel");
+    *join = {p.acc, first ? p.chunks : splits, p.acc_split, p.acc_batch, ld, p.out, q.dtype, g.sb, g.sr,
+             static_cast<int>(M), static_cast<int>(q.D), q.B * M * q.D};
   }
-  return st;
+  return set_problem<kEpiOut>(prm, prm.count++, a, b, kdim, sh);
 }
 
 static int backward(const Xent& q, const RowStat* stat, const int32_t* count, const float* g,
@@ -652,10 +723,9 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
   // float16 P is kept times 2^14: a softmax over 2^20 centroids then still has
   // ten bits above float16's smallest subnormal, and 1 * 2^14 is in range
   const float p_scale = f16 ? 16384.0f : 1.0f;
-  int st;
-  if ((st = rows_copy(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), q.y, true, s)) != FK_OK) return st;
-  if (f.cc && (st = rows_copy(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), q.y, false, s)) != FK_OK)
-    return st;
+  int st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), &q.y),
+                     rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  if (st != FK_OK) return st;
   const float* factor = q.reduction == 0 ? nullptr : g;
   if (q.reduction == 0) {
     const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(rows, 256), 1024));
@@ -677,8 +747,9 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
     for (int64_t chunk = 0; chunk < f.n_chunks; ++chunk) {
       const int64_t r0 = chunk * f.R, rw = std::min(f.R, q.N - r0);
       // dz of the piece
-      Params prm = {};
-      Problem& p = prm.p;
+      Params<1> prm = {};
+      prm.count = 1;
+      Problem& p = prm.p[0];
       p.M = static_cast<int>(rw);
       p.N = static_cast<int>(kw);
       p.batches = static_cast<int>(q.B);
@@ -696,8 +767,9 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       p.p_batch = f.R * f.Kp;
       p.p_part = q.B * f.R * f.Kp;
       p.p_bf16 = !f16;
-      st = launch<kEpiGrad>(prm, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, r0),
-                            operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, k0), q.D, f.sh_p, s);
+      st = set_problem<kEpiGrad>(prm, 0, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, r0),
+                                 operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, k0), q.D, f.sh_p);
+      if (st == FK_OK) st = launch<kEpiGrad>(prm, f.sh_p, s);
       if (st != FK_OK) return st;
 
       Operand po;  // P by rows (for dx); its valid width and height bound the products
@@ -719,19 +791,40 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       base.fscale = q.scale / p_scale;
       base.f_num = factor;
       base.f_den = q.reduction == 1 ? count : nullptr;
-      if (gx.p) {
-        Operand co = operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, true, k0);
-        st = grad_product(q, base, po, co, rw, kw, f.sh_x, f.split_x, f.acc_x, q.N, r0, f.ld, piece == 0,
-                          piece + 1 == f.n_pieces, gx, r0, s);
-        if (st != FK_OK) return st;
-      }
-      if (gc.p) {
+      Params<2> pair = {};
+      JoinJobs joins = {};
+      int n_joins = 0;
+      auto add_x = [&]() {
+        const Operand co = operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, true, k0);
+        const int r = grad_problem(q, pair, &joins.job[n_joins], base, po, co, rw, kw, f.sh, f.split_x, f.acc_x,
+                                   q.N, r0, f.ld, piece == 0, piece + 1 == f.n_pieces, gx, r0);
+        n_joins += joins.job[n_joins].total > 0;
+        return r;
+      };
+      auto add_c = [&]() {
         Operand pt = po;
         pt.mn = true;
-        Operand xo = operand(q, q.x, f.xc, q.B, q.N, q.xs, true, r0);
-        st = grad_product(q, base, pt, xo, kw, rw, f.sh_c, f.split_c, f.acc_c, f.Kp, 0, f.ld, chunk == 0,
-                          chunk + 1 == f.n_chunks, gc, k0, s);
-        if (st != FK_OK) return st;
+        const Operand xo = operand(q, q.x, f.xc, q.B, q.N, q.xs, true, r0);
+        const int r = grad_problem(q, pair, &joins.job[n_joins], base, pt, xo, kw, rw, f.sh, f.split_c, f.acc_c,
+                                   f.Kp, 0, f.ld, chunk == 0, chunk + 1 == f.n_chunks, gc, k0);
+        n_joins += joins.job[n_joins].total > 0;
+        return r;
+      };
+      // the product with the longer tiles first
+      const bool x_first = ceil_div(kw, 64) / f.split_x >= ceil_div(rw, 64) / f.split_c;
+      st = FK_OK;
+      if (gx.p && x_first) st = add_x();
+      if (st == FK_OK && gc.p) st = add_c();
+      if (st == FK_OK && gx.p && !x_first) st = add_x();
+      if (st == FK_OK) st = launch<kEpiOut>(pair, f.sh, s);
+      if (st != FK_OK) return st;
+      if (n_joins) {
+        const int sms = sm_count_current();
+        const int64_t most = std::max(joins.job[0].total, joins.job[1].total);
+        const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ceil_div(most, 256), (sms > 0 ? sms : 148) * 16ll)),
+                        n_joins);
+        head_join_kernel<<<grid, 256, 0, s>>>(joins);
+        if ((st = check_launch("head_join_kernel")) != FK_OK) return st;
       }
     }
   }

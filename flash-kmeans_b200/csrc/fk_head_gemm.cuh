@@ -29,7 +29,6 @@
 namespace fk {
 namespace head {
 
-constexpr int kMaxPairs = 6;
 constexpr int kCtlWarps = 4;
 constexpr int kStageRowBytes = 128;            // one swizzle row: 64 16-bit or 128 8-bit elements
 constexpr int kTableFloats = 2 * 64;           // column scales and biases of an epilogue warp
@@ -59,9 +58,7 @@ struct Problem {
   int m_tiles, n_tiles;     // tiles of this instance's shape
   int batches;
   int chunks;               // running epilogues: column chunks of a row block; else splits of the contraction
-  int kblocks;              // 128-byte steps of the contraction, for each operand pair
-  int npairs;               // operand parts multiplied: 1, or 6 for float32 split into three bf16 parts
-  int pa[kMaxPairs], pb[kMaxPairs];
+  int kblocks;              // 128-byte steps of the contraction
   int a_mn, b_mn;           // MN-major operands
   int a_batch, b_batch;     // z coordinate = batch * this + part * a_part
   int a_part, b_part;
@@ -122,14 +119,16 @@ struct Params {
   int all, short_from, more, rest;
 };
 
-template <int CG, int BN, int EPI>
+template <int CG, int BN, int EPI, bool EXACT>
 struct Shape {
   static constexpr int kBM = 128 * CG;
   static constexpr int kARows = 128;             // of one CTA
   static constexpr int kBRows = BN / CG;         // of one CTA
   static constexpr int kABytes = kARows * kStageRowBytes;
   static constexpr int kBBytes = kBRows * kStageRowBytes;
-  static constexpr int kStageBytes = kABytes + kBBytes;
+  // EXACT: a step brings the three parts of both operands, used by six products
+  static constexpr int kOps = EXACT ? 3 : 1;
+  static constexpr int kStageBytes = kOps * (kABytes + kBBytes);
   // Epilogue warps: four TMEM lane quarters x column parts.  Four parts give
   // each scheduler four warps, which is what hides the exponentials' and the
   // accumulator loads' latency (two left 70 % of the issue slots empty).
@@ -146,11 +145,11 @@ struct Shape {
   static constexpr int kBufs = BN >= 256 ? 2 : 4;
   static constexpr int kTmemCols = kBufs * BN;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kStagingBytes + kExtra + 512;
-  static_assert(kStages >= 4 && kSmem <= 232448, "shared memory");
+  static_assert(kStages >= (EXACT ? 2 : 4) && kSmem <= 232448, "shared memory");
 };
 
-template <int CG, int BN, int EPI>
-constexpr int threads_of() { return Shape<CG, BN, EPI>::kThreads; }
+template <int CG, int BN, int EPI, bool EXACT>
+constexpr int threads_of() { return Shape<CG, BN, EPI, EXACT>::kThreads; }
 // column parts that write partial results of a row
 inline int parts_of(int bn) { return bn >= 128 ? 4 : 2; }
 
@@ -207,7 +206,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 struct Tile {
   int q;               // which problem
   int b, m, n, chunk;
-  int it0, it1;        // steps of the flattened (pair, kblock) contraction
+  int it0, it1;        // steps of the contraction
   bool first, last;    // of the item
 };
 
@@ -262,7 +261,7 @@ struct Walk {
   __device__ void decode() {
     if (item >= total) return;
     const Problem& p = prm.p[NP > 1 ? t.q : 0];
-    const int steps = p.npairs * p.kblocks;
+    const int steps = p.kblocks;
     if constexpr (running(EPI)) {
       uint32_t r = item;
       uint32_t c = 0;
@@ -382,18 +381,24 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
 }
 
 // ------------------------------------------------------------------- kernel
-// EXACT: the tensor core adds to its float32 accumulator with truncation, a
-// bias of up to 2^-24 of the partial sum for every 16 elements.  16-bit inputs
-// leave it at that (the label's score, which the loss hangs on most, is summed
-// in ordinary float32 by the combine kernel); float32 inputs move the
-// accumulator to registers every kSegment steps and add there, rounded.  Their
-// tiles are 128 columns wide: 64 sums a thread leave the epilogue its registers.
-constexpr int kSegment = 4;       // of 64 elements: 16 truncated additions
+// EXACT: float32 operands as three bf16 parts each.  A step loads the six part
+// tiles once and issues the six products that reach above 2^-24 of the leading
+// one, smallest first; loading a pair of parts per product instead fetched twice
+// the bytes and was bound by the L2 (86 -> see fk_xent.cu).  The tensor core
+// adds to its float32 accumulator with truncation, a bias of up to 2^-24 of the
+// partial sum for every 16 elements.  16-bit inputs leave it at that (the
+// label's score, which the loss hangs on most, is summed in ordinary float32 by
+// the combine kernel); here the accumulator moves to registers after every step
+// and is added there, rounded.  The tiles are 128 columns wide: 32 sums a thread
+// leave the epilogue its registers.
+constexpr int kSegment = 1;       // steps of 64 elements: 24 truncated additions
+__device__ constexpr int kPairA[6] = {2, 0, 1, 1, 0, 0};
+__device__ constexpr int kPairB[6] = {0, 2, 1, 0, 1, 0};
 
 template <int CG, int BN, int EPI, bool EXACT>
-__global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const __grid_constant__ Params<problems_of(EPI)> prm) {
+__global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm(const __grid_constant__ Params<problems_of(EPI)> prm) {
   constexpr int NP = problems_of(EPI);
-  using S = Shape<CG, BN, EPI>;
+  using S = Shape<CG, BN, EPI, EXACT>;
   const Problem& p0 = prm.p[0];
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -463,57 +468,47 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
         const CUtensorMap *ma = &prm.a[NP > 1 ? t.q : 0], *mb = &prm.b[NP > 1 ? t.q : 0];
-        const int kblocks = p.kblocks;
-        int pair = 0, kb = t.it0;
-        if (kb >= kblocks) {
-          pair = kb / kblocks;
-          kb -= pair * kblocks;
-        }
         const int am = t.m * S::kBM + static_cast<int>(rank) * S::kARows;
         const int bn = t.n * BN + static_cast<int>(rank) * S::kBRows;
-        int left = t.it1 - t.it0;
         auto load = [&](auto a_mn, auto b_mn) {
           constexpr bool kA = decltype(a_mn)::value, kB = decltype(b_mn)::value;
-          const uint32_t tx =
-              static_cast<uint32_t>((kA ? S::kABytes : p.a_rows * kStageRowBytes) + S::kBBytes) * CG;
+          const uint32_t tx = static_cast<uint32_t>(
+              (kA ? S::kABytes : p.a_rows * kStageRowBytes) + S::kBBytes) * CG * S::kOps;
           const int a_at = kA ? am : p.a_off + am, b_at = kB ? bn : p.b_off + bn;
           const int a_k = kA ? p.a_off : 0, b_k = kB ? p.b_off : 0;
-          while (left > 0) {
-            const int az = t.b * p.a_batch + p.pa[pair] * p.a_part;
-            const int bz = t.b * p.b_batch + p.pb[pair] * p.b_part;
-            const int n = min(left, kblocks - kb);
-            int c = kb * kstep;
-            for (int i = 0; i < n; ++i, c += kstep) {
-              if (!mbar_wait_at<false>(empty0 + stage * 8, phase ^ 1, abort_flag, p0.status,
-                                       FK_DEV_WAIT_TIMEOUT)) {
-                ok = false;
-                return;
-              }
-              const uint32_t sa = smem0 + stage * S::kStageBytes, sb = sa + S::kABytes;
-              if (leader) mbar_expect_at(full0 + stage * 8, tx);
-              const uint32_t bar = bar0 + stage * 8;
+          const int az = t.b * p.a_batch, bz = t.b * p.b_batch;
+          const int ap = p.a_part, bp = p.b_part;
+          int c = t.it0 * kstep;
+          for (int i = t.it0; i < t.it1; ++i, c += kstep) {
+            if (!mbar_wait_at<false>(empty0 + stage * 8, phase ^ 1, abort_flag, p0.status,
+                                     FK_DEV_WAIT_TIMEOUT)) {
+              ok = false;
+              return;
+            }
+            const uint32_t sa = smem0 + stage * S::kStageBytes, sb = sa + S::kOps * S::kABytes;
+            if (leader) mbar_expect_at(full0 + stage * 8, tx);
+            const uint32_t bar = bar0 + stage * 8;
+#pragma unroll
+            for (int o = 0; o < S::kOps; ++o) {
               if constexpr (kA) {
 #pragma unroll
                 for (int g = 0; g < S::kARows / 64; ++g)
-                  tma_load_3d_cg<CG>(sa + g * 8192, ma, bar, a_at + g * 64, a_k + c, az);
+                  tma_load_3d_cg<CG>(sa + o * S::kABytes + g * 8192, ma, bar, a_at + g * 64, a_k + c, az + o * ap);
               } else {
-                tma_load_3d_cg<CG>(sa, ma, bar, c, a_at, az);
+                tma_load_3d_cg<CG>(sa + o * S::kABytes, ma, bar, c, a_at, az + o * ap);
               }
               if constexpr (kB) {
 #pragma unroll
                 for (int g = 0; g < S::kBRows / 64; ++g)
-                  tma_load_3d_cg<CG>(sb + g * 8192, mb, bar, b_at + g * 64, b_k + c, bz);
+                  tma_load_3d_cg<CG>(sb + o * S::kBBytes + g * 8192, mb, bar, b_at + g * 64, b_k + c, bz + o * bp);
               } else {
-                tma_load_3d_cg<CG>(sb, mb, bar, c, b_at, bz);
-              }
-              if (++stage == S::kStages) {
-                stage = 0;
-                phase ^= 1;
+                tma_load_3d_cg<CG>(sb + o * S::kBBytes, mb, bar, c, b_at, bz + o * bp);
               }
             }
-            left -= n;
-            kb = 0;
-            ++pair;
+            if (++stage == S::kStages) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
         };
         if constexpr (EPI == kEpiOut) {
@@ -550,8 +545,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
         const bool a_mn = EPI == kEpiOut && p.a_mn;
         constexpr bool b_mn = EPI == kEpiOut;
         const uint64_t ad0 = a_mn ? smem_desc_sw128_mn(smem0, 8192, 1024) : smem_desc_sw128(smem0);
-        const uint64_t bd0 = b_mn ? smem_desc_sw128_mn(smem0 + S::kABytes, 8192, 1024)
-                                  : smem_desc_sw128(smem0 + S::kABytes);
+        const uint64_t bd0 = b_mn ? smem_desc_sw128_mn(smem0 + S::kOps * S::kABytes, 8192, 1024)
+                                  : smem_desc_sw128(smem0 + S::kOps * S::kABytes);
         const uint32_t a_step = (a_mn ? 2048 : 32) >> 4;
         constexpr uint32_t b_step = (b_mn ? 2048 : 32) >> 4;
         int left = t.it1 - t.it0;
@@ -574,14 +569,21 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI>(), 1) head_gemm(const 
             }
             tc_fence_after();
             const uint32_t at = stage * (S::kStageBytes >> 4);
-            uint64_t ad = ad0 + at, bd = bd0 + at;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t accumulate = k > 0 || i > 0;
-              if constexpr (integer(EPI)) mma_i8_cg<CG>(d, ad, bd, idesc, accumulate);
-              else mma_f16_cg<CG>(d, ad, bd, idesc, accumulate);
-              ad += a_step;
-              bd += b_step;
+            for (int o = 0; o < (EXACT ? 6 : 1); ++o) {
+              uint64_t ad = ad0 + at, bd = bd0 + at;
+              if constexpr (EXACT) {
+                ad += kPairA[o] * (S::kABytes >> 4);
+                bd += kPairB[o] * (S::kBBytes >> 4);
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t accumulate = o > 0 || k > 0 || i > 0;
+                if constexpr (integer(EPI)) mma_i8_cg<CG>(d, ad, bd, idesc, accumulate);
+                else mma_f16_cg<CG>(d, ad, bd, idesc, accumulate);
+                ad += a_step;
+                bd += b_step;
+              }
             }
             mma_commit_cg<CG>(empty0 + stage * 8);
             if (++stage == S::kStages) {

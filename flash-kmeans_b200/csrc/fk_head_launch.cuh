@@ -26,7 +26,11 @@ struct Operand {
 
 struct ShapeChoice {
   int cg, bn;
+  bool exact;          // float32 operands in three parts: 256 x 128 or 128 x 64
   int bm() const { return 128 * cg; }
+  // microseconds of a step: its bytes at what the L2 gives an SM (78 KB a
+  // microsecond with all of them reading), and no less than the issue takes
+  double step_us() const { return std::max(0.2, (16.0 + bn / cg / 8.0) * (exact ? 3 : 1) / 78.0); }
 };
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -34,11 +38,11 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // 256 x 256 tiles on CTA pairs once they give half of the 74 pairs a tile;
 // below that 128 x 128 tiles, and 128 x 64 ones when even those leave most SMs
 // idle.  Measured in profiles/cluster_head.md.
-inline ShapeChoice choose_shape(int64_t M, int64_t N, int64_t batches, int64_t splittable, bool exact) {
+inline ShapeChoice choose_shape(int64_t M, int64_t N, int64_t batches, bool exact) {
   const int wide = exact ? 128 : 256;
-  if (M > 128 && ceil_div(M, 256) * ceil_div(N, wide) * batches * splittable >= 37) return {2, wide};
-  if (ceil_div(M, 128) * ceil_div(N, 128) * batches * splittable >= 100) return {1, 128};
-  return {1, 64};
+  if (M > 128 && ceil_div(M, 256) * ceil_div(N, wide) * batches >= 37) return {2, wide, exact};
+  if (!exact && ceil_div(M, 128) * ceil_div(N, 128) * batches >= 100) return {1, 128, exact};
+  return {1, 64, exact};
 }
 
 // Number of equal chunks of `units` for which `slots` workers finish `items`
@@ -66,7 +70,7 @@ struct Fill {
 };
 inline double tile_cost(int64_t steps) { return static_cast<double>(steps) + 3.0; }
 inline double tile_cost(const Problem& p) {
-  return tile_cost(ceil_div(static_cast<int64_t>(p.npairs) * p.kblocks, p.chunks));
+  return tile_cost(ceil_div(p.kblocks, p.chunks));
 }
 inline Fill fill(int64_t n0, double c0, int64_t n1, double c1, int64_t workers) {
   Fill f = {};
@@ -91,7 +95,7 @@ int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows);
 
 template <int CG, int BN, int EPI, bool EXACT>
 int launch_shape(Params<problems_of(EPI)>& prm, cudaStream_t s) {
-  using S = Shape<CG, BN, EPI>;
+  using S = Shape<CG, BN, EPI, EXACT>;
   auto kern = head_gemm<CG, BN, EPI, EXACT>;
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return fail(FK_ERR_CUDA, "bad current device %d", dev);
@@ -111,7 +115,7 @@ int launch_shape(Params<problems_of(EPI)>& prm, cudaStream_t s) {
     items += n;
     if (i == 0) first = n;
     if (items >= (1ll << 31) || static_cast<int64_t>(p.n_tiles) * p.chunks >= (1ll << 31) ||
-        static_cast<int64_t>(p.npairs) * p.kblocks * p.chunks >= (1ll << 31))
+        static_cast<int64_t>(p.kblocks) * p.chunks >= (1ll << 31))
       return fail(FK_ERR_UNSUPPORTED, "head_gemm: %lld tiles exceed 32-bit", static_cast<long long>(items));
   }
   const int64_t workers = items < slots ? items : slots;
@@ -180,9 +184,8 @@ int set_problem(Params<problems_of(EPI)>& prm, int i, const Operand& a, const Op
 template <int EPI>
 int launch(Params<problems_of(EPI)>& prm, ShapeChoice sh, cudaStream_t s) {
   if constexpr (!integer(EPI)) {
-    if (prm.p[0].npairs > 1) {
+    if (sh.exact) {
       if (sh.cg == 2) return launch_shape<2, 128, EPI, true>(prm, s);
-      if (sh.bn == 128) return launch_shape<1, 128, EPI, true>(prm, s);
       return launch_shape<1, 64, EPI, true>(prm, s);
     }
   }

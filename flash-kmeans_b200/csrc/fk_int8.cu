@@ -266,7 +266,7 @@ static ScoresPlan plan_scores(const Scores& q, bool argmax, void* ws) {
     used += align_up(static_cast<size_t>(bytes), 256);
     return p;
   };
-  f.sh = choose_shape(q.N, q.K, q.B, 1, false);
+  f.sh = choose_shape(q.N, q.K, q.B, false);
   f.chunks = argmax ? choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                                     2 * slots_of(f.sh), 0.25)
                     : 1;
@@ -333,7 +333,6 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   p.N = static_cast<int>(q.K);
   p.batches = static_cast<int>(q.B);
   p.chunks = f.chunks;
-  p.npairs = 1;
   p.a_scale = f.sx ? f.sx : sc.x;
   p.as_sb = f.sx ? q.N : sc.xs[0];
   p.as_sn = f.sx ? 1 : sc.xs[1];

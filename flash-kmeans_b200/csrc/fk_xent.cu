@@ -460,16 +460,6 @@ static Operand operand(const Xent& q, const void* p, const uint16_t* copy, int64
   return o;
 }
 
-static void set_pairs(Problem& p, int parts) {
-  // (A part, B part), smallest products first
-  static const int pa[6] = {2, 0, 1, 1, 0, 0}, pb[6] = {0, 2, 1, 0, 1, 0};
-  p.npairs = parts == 3 ? 6 : 1;
-  for (int i = 0; i < kMaxPairs; ++i) {
-    p.pa[i] = parts == 3 ? pa[i] : 0;
-    p.pb[i] = parts == 3 ? pb[i] : 0;
-  }
-}
-
 static int check_args(const Xent& q, const char* who) {
   if (q.B < 0 || q.N < 0 || q.K <= 0 || q.D <= 0) return fail(FK_ERR_INVALID_ARG, "%s: bad sizes", who);
   if (q.dtype != FK_F16 && q.dtype != FK_BF16 && q.dtype != FK_F32)
@@ -499,7 +489,7 @@ struct ForwardPlan {
 static ForwardPlan plan_forward(const Xent& q, void* ws) {
   ForwardPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
-  f.sh = choose_shape(q.N, q.K, q.B, 1, q.parts() > 1);
+  f.sh = choose_shape(q.N, q.K, q.B, q.parts() > 1);
   f.chunks = choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                            2 * slots_of(f.sh), 0.25);
   f.row_blocks = ceil_div(q.N, 32);
@@ -529,7 +519,6 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   p.N = static_cast<int>(q.K);
   p.batches = static_cast<int>(q.B);
   p.chunks = f.chunks;
-  set_pairs(p, q.parts());
   p.scale2 = q.scale * 1.44269504f;
   p.labels = q.y.p;
   p.label_dtype = q.y.dtype;
@@ -599,7 +588,7 @@ struct BackwardPlan {
 // Tile shape and splits of the two gradient products: dx is Mx x D over steps_x
 // steps, dc Mc x D over steps_c (0: not wanted).  A product with few tiles and a
 // long contraction is split along it; each split costs a pass over float32
-// partial sums, counted in steps of a tile's contraction (0.27 us each).
+// partial sums, counted in steps of a tile's contraction.
 static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc, int64_t steps_c,
                           BackwardPlan* f) {
   const bool exact = q.parts() > 1;
@@ -607,20 +596,21 @@ static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc
   auto tiles = [&](int64_t M, int64_t steps, int64_t bm, int64_t bn) {
     return steps ? q.B * ceil_div(M, bm) * ceil_div(q.D, bn) : 0;
   };
-  // work in shares of 16 steps, the least that is worth a worker
+  // work in shares of a megabyte of operands, the least that is worth a worker
+  const int64_t share = exact ? 3 : 8;
   auto shares = [&](int64_t bm, int64_t bn) {
-    return tiles(Mx, steps_x, bm, bn) * std::max<int64_t>(1, steps_x / 16) +
-           tiles(Mc, steps_c, bm, bn) * std::max<int64_t>(1, steps_c / 16);
+    return tiles(Mx, steps_x, bm, bn) * std::max<int64_t>(1, steps_x / share) +
+           tiles(Mc, steps_c, bm, bn) * std::max<int64_t>(1, steps_c / share);
   };
-  if (std::max(Mx, Mc) > 128 && shares(256, wide) >= 74) f->sh = {2, wide};
-  else if (q.D > 64 && shares(128, 128) >= 100) f->sh = {1, 128};
-  else f->sh = {1, 64};
+  if (std::max(Mx, Mc) > 128 && shares(256, wide) >= 74) f->sh = {2, wide, exact};
+  else if (!exact && q.D > 64 && shares(128, 128) >= 100) f->sh = {1, 128, exact};
+  else f->sh = {1, 64, exact};
   f->split_x = f->split_c = 1;
   const int64_t slots = slots_of(f->sh);
   const int64_t tx = tiles(Mx, steps_x, f->sh.bm(), f->sh.bn), tc = tiles(Mc, steps_c, f->sh.bm(), f->sh.bn);
   if (tx + tc >= 8 * slots) return;
   static const int tries[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-  const double us = 0.27 * f->sh.cg * f->sh.bn / 512.0;   // a step of this shape
+  const double us = f->sh.step_us();
   double best = 1e300;
   for (int sx : tries) {
     if (sx > 1 && (sx > steps_x || tx * sx > 4 * slots)) break;
@@ -656,9 +646,8 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   f.R = std::min(q.N, ceil_div(ceil_div(q.N, f.n_chunks), 128) * 128);
   f.n_chunks = ceil_div(q.N, f.R);
   const int64_t kw = std::min(f.Kp, q.K);
-  const int pairs = q.parts() == 3 ? 6 : 1;
-  f.sh_p = choose_shape(f.R, kw, q.B, 1, q.parts() > 1);
-  const int64_t steps_x = pairs * ceil_div(kw, 64), steps_c = pairs * ceil_div(f.R, 64);
+  f.sh_p = choose_shape(f.R, kw, q.B, q.parts() > 1);
+  const int64_t steps_x = ceil_div(kw, 64), steps_c = ceil_div(f.R, 64);
   plan_products(q, f.R, want_x ? steps_x : 0, kw, want_c ? steps_c : 0, &f);
   f.ld = ceil_div(q.D, 4) * 4;
   f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
@@ -690,7 +679,7 @@ static int grad_problem(const Xent& q, Params<2>& prm, JoinJob* join, const Prob
   p = base;
   p.M = static_cast<int>(M);
   p.N = static_cast<int>(q.D);
-  const int64_t steps = p.npairs * ceil_div(kdim, 64);
+  const int64_t steps = ceil_div(kdim, 64);
   p.chunks = static_cast<int>(std::min<int64_t>(splits, steps));
   const int eb = dtype_bytes(q.dtype);
   p.out = static_cast<uint8_t*>(g.p) + out_row0 * g.sr * eb;
@@ -754,8 +743,7 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       p.N = static_cast<int>(kw);
       p.batches = static_cast<int>(q.B);
       p.chunks = 1;
-      set_pairs(p, q.parts());
-      p.status = status;
+          p.status = status;
       p.scale2 = q.scale * 1.44269504f;
       p.stat = stat;
       p.stat_rows = q.N;
@@ -787,7 +775,6 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       Problem base = {};
       base.batches = static_cast<int>(q.B);
       base.status = status;
-      set_pairs(base, q.parts());
       base.fscale = q.scale / p_scale;
       base.f_num = factor;
       base.f_den = q.reduction == 1 ? count : nullptr;

@@ -51,13 +51,16 @@ inline int choose_chunks(int64_t items, int64_t units, int64_t slots, int64_t mo
   int best = 1;
   double best_cost = 1e300;
   if (most > units) most = units;
-  for (int64_t c = 1; c <= most; ++c) {
+  for (int64_t c = 1; c <= most;) {
+    const int64_t per = ceil_div(units, c);
     const double cost =
-        static_cast<double>(ceil_div(items * c, slots)) * (ceil_div(units, c) + extra) + (c > 1 ? extra : 0.0);
+        static_cast<double>(ceil_div(items * c, slots)) * (per + extra) + (c > 1 ? extra : 0.0);
     if (cost < best_cost * 0.999) {
       best_cost = cost;
       best = static_cast<int>(c);
     }
+    if (per == 1) break;
+    c = ceil_div(units, per - 1);    // the next count with shorter chunks
   }
   return best;
 }

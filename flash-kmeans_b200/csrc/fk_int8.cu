@@ -8,6 +8,7 @@
 // argmax agree to the bit with the formula.  fk_int8_scores stores z rounded
 // once to its output type; fk_int8_assign keeps only each row's argmax.
 #include <algorithm>
+#include <type_traits>
 
 #include "fk_head_launch.cuh"
 
@@ -23,7 +24,52 @@ constexpr int64_t kMaxD8 = 65536;   // 127^2 * D stays below 2^30
 // One group of threads per row: the largest magnitude, then
 // round-to-nearest-even of x * (127 / most) and the scale most / 127.  The
 // second pass finds the row in the caches.
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// Magnitudes compare as their bits do, NaN and infinity above the rest, so the
+// largest one is taken on the bits, two 16-bit values at a time; rounding adds
+// 1.5 * 2^23, whose mantissa then ends in the integer's low byte.  (With a
+// conversion each way the kernel was bound by the instructions: 60 us for
+// 65537 x 1024 bfloat16, which 31 us would read and write.)
+template <typename T>
+__device__ __forceinline__ uint32_t most_bits(uint4 u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    else m = max(m, w[i] & 0x7fffffffu);
+  }
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t join_bits(uint32_t a, uint32_t b) {
+  if constexpr (sizeof(T) == 2) return __vmaxu2(a, b);
+  else return max(a, b);
+}
+// the two halves of a 16-bit pair, as float32 bits
+template <typename T>
+__device__ __forceinline__ uint32_t float_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  const uint32_t h = max(m & 0xffffu, m >> 16);
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) return h << 16;
+  else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+}
+template <typename T>
+__device__ __forceinline__ void floats_of(uint4 u, float (&f)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
+  }
+}
 
 // STEPS: 16-byte loads of a thread that hold its whole share of the row in
 // registers, all in flight at once; 0 for longer rows, which are read twice.
@@ -53,23 +99,17 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(
     }
     return u;
   };
-  auto most_of = [&](uint4 u) {
-    const T* v = reinterpret_cast<const T*>(&u);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) m = max(m, abs_bits(Elem<T>::to_f(v[i])));
-    return m;
-  };
   uint32_t most = 0;
   uint4 held[kHeld];
   if constexpr (STEPS > 0) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) held[s] = ok ? load((s * lanes + sub) * E) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) most = max(most, most_of(held[s]));
+    for (int s = 0; s < STEPS; ++s) most = join_bits<T>(most, most_bits<T>(held[s]));
   } else if (ok) {
-    for (int d = sub * E; d < D; d += lanes * E) most = max(most, most_of(load(d)));
+    for (int d = sub * E; d < D; d += lanes * E) most = join_bits<T>(most, most_bits<T>(load(d)));
   }
+  most = float_bits<T>(most);
   for (int o = min(lanes, 32) >> 1; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
   if (lanes > 32) {
     if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = most;
@@ -87,17 +127,17 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(
   int8_t* dst = q + b * qb + n * qn;
   auto store = [&](int d, uint4 u) {
     if (d >= Dq) return;
-    const T* v = reinterpret_cast<const T*>(&u);
+    float f[E];
+    floats_of<T>(u, f);
     uint32_t w[E / 4];
 #pragma unroll
     for (int j = 0; j < E / 4; ++j) {
-      w[j] = 0;
+      uint32_t r[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // |x * inv| is at most 127 and a rounding
-        const int r = bad ? 0 : __float2int_rn(__fmul_rn(Elem<T>::to_f(v[j * 4 + i]), inv));
-        w[j] |= (static_cast<uint32_t>(r) & 0xffu) << (8 * i);
-      }
+      for (int i = 0; i < 4; ++i)   // |x * inv| is at most 127 and a rounding
+        r[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[j * 4 + i], inv), 12582912.0f));
+      w[j] = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+      if (bad) w[j] = 0;
     }
     if (qvec && d + E <= Dq) {
       if constexpr (E == 8) *reinterpret_cast<uint2*>(dst + d) = make_uint2(w[0], w[1]);
@@ -313,11 +353,10 @@ template <int EPI>
 static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_t ws_bytes,
                 int32_t* label_out, const int64_t* ls, int* status, cudaStream_t s, const char* who) {
   const bool argmax = EPI == kEpiArgmax;
-  const ScoresPlan need = plan_scores(q, argmax, nullptr);
-  if (need.bytes && (!ws || ws_bytes < need.bytes || reinterpret_cast<uintptr_t>(ws) % 256))
-    return fail(FK_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who,
-                need.bytes, ws_bytes);
   const ScoresPlan f = plan_scores(q, argmax, ws);
+  if (f.bytes && (!ws || ws_bytes < f.bytes || reinterpret_cast<uintptr_t>(ws) % 256))
+    return fail(FK_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who,
+                f.bytes, ws_bytes);
   int st;
   if (q.x_dtype != FK_I8)
     st = quantize(q.x, q.x_dtype, q.B, q.N, q.D, q.xs, f.xq, q.N * q.Dp(), q.Dp(), q.Dp(), f.sx, q.N, 1, s);

@@ -475,6 +475,14 @@ static int check_args(const Xent& q, const char* who) {
   return FK_OK;
 }
 
+static int check_workspace(const void* ws, size_t have, size_t need, const char* who) {
+  if (need == 0) return FK_OK;
+  if (!ws || have < need || reinterpret_cast<uintptr_t>(ws) % 256)
+    return fail(FK_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who,
+                need, have);
+  return FK_OK;
+}
+
 struct ForwardPlan {
   ShapeChoice sh;
   int chunks;
@@ -506,9 +514,10 @@ static ForwardPlan plan_forward(const Xent& q, void* ws) {
   return f;
 }
 
-static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, void* ws, int* status,
-                   cudaStream_t s) {
+static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, void* ws, size_t ws_bytes,
+                   int* status, cudaStream_t s) {
   const ForwardPlan f = plan_forward(q, ws);
+  if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_forward")) return bad;
   int st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), nullptr),
                      rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
   if (st != FK_OK) return st;
@@ -705,8 +714,10 @@ static int grad_problem(const Xent& q, Params<2>& prm, JoinJob* join, const Prob
 }
 
 static int backward(const Xent& q, const RowStat* stat, const int32_t* count, const float* g,
-                    const Grad& gx, const Grad& gc, void* ws, int* status, cudaStream_t s) {
+                    const Grad& gx, const Grad& gc, void* ws, size_t ws_bytes, int* status,
+                    cudaStream_t s) {
   const BackwardPlan f = plan_backward(q, gx.p != nullptr, gc.p != nullptr, ws);
+  if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_backward")) return bad;
   const int64_t rows = q.B * q.N;
   const bool f16 = q.dtype == FK_F16;
   // float16 P is kept times 2^14: a softmax over 2^20 centroids then still has
@@ -843,14 +854,6 @@ static int make(Xent& q, const void* x, const void* c, const void* labels, int d
   return check_args(q, who);
 }
 
-static int check_workspace(const void* ws, size_t have, size_t need, const char* who) {
-  if (need == 0) return FK_OK;
-  if (!ws || have < need || reinterpret_cast<uintptr_t>(ws) % 256)
-    return fail(FK_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who,
-                need, have);
-  return FK_OK;
-}
-
 }  // namespace head
 }  // namespace fk
 
@@ -895,9 +898,8 @@ extern "C" int fk_xent_forward(const void* x, const void* centroids, const void*
   if (!x || !centroids || !labels) return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: null pointer");
   if (reinterpret_cast<uintptr_t>(row_stats) % 16)
     return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: row_stats must be 16-byte aligned");
-  st = check_workspace(workspace, workspace_bytes, plan_forward(q, nullptr).bytes, "fk_xent_forward");
-  if (st != FK_OK) return st;
-  return forward(q, loss, reinterpret_cast<RowStat*>(row_stats), count, workspace, dev_status, s);
+  return forward(q, loss, reinterpret_cast<RowStat*>(row_stats), count, workspace, workspace_bytes,
+                 dev_status, s);
 }
 
 extern "C" int fk_xent_backward(const void* x, const void* centroids, const void* labels, int dtype,
@@ -934,12 +936,8 @@ extern "C" int fk_xent_backward(const void* x, const void* centroids, const void
     return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: null pointer");
   if (reinterpret_cast<uintptr_t>(row_stats) % 16)
     return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: row_stats must be 16-byte aligned");
-  st = check_workspace(workspace, workspace_bytes,
-                       plan_backward(q, grad_x != nullptr, grad_centroids != nullptr, nullptr).bytes,
-                       "fk_xent_backward");
-  if (st != FK_OK) return st;
   Grad gx{grad_x, grad_x ? gx_strides3[0] : 0, grad_x ? gx_strides3[1] : 0};
   Grad gc{grad_centroids, grad_centroids ? gc_strides3[0] : 0, grad_centroids ? gc_strides3[1] : 0};
   return backward(q, reinterpret_cast<const RowStat*>(row_stats), count, grad_loss, gx, gc, workspace,
-                  dev_status, s);
+                  workspace_bytes, dev_status, s);
 }

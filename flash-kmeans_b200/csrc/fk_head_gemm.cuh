@@ -89,6 +89,8 @@ struct Problem {
   float* acc;               // kEpiOut: float32 accumulator [split][batch][row][acc_ld]
   int64_t acc_ld, acc_batch, acc_split;
   int acc_read, acc_write;
+  uint32_t* join;           // kEpiOut, splits that are added up here: an arrival counter for each
+  int join_splits;          // warp of a tile, zero on entry and on exit; null otherwise
   void* out;                // kEpiOut final / kEpiScores: [batch][row][col]
   int out_dtype, out_vec;   // out_vec: 4 elements of a row can be stored at once
   int64_t out_sb, out_sr;
@@ -443,8 +445,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       tmem_relinquish();
     }
   }
-  if (warp == 3 && blockIdx.x == 0)
-    for (int i = lane; i < p0.zero_n; i += 32) p0.zero[i] = 0;
+  if (warp == 3)
+    for (int i = blockIdx.x * 32 + lane; i < p0.zero_n; i += gridDim.x * 32) p0.zero[i] = 0;
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
@@ -716,6 +718,26 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           }
       }
 
+      // four columns of an output row, rounded
+      auto emit = [&](const int64_t grow, const int col, const float4 f) {
+        const int64_t o = t.b * p.out_sb + grow * p.out_sr + col;
+        if (p.out_vec && col + 4 <= p.N) {
+          if (p.out_dtype == FK_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = f;
+          } else {
+            uint2 w;
+            w.x = p.out_dtype == FK_BF16 ? pack_bf16(f.x, f.y) : pack_f16(f.x, f.y);
+            w.y = p.out_dtype == FK_BF16 ? pack_bf16(f.z, f.w) : pack_f16(f.z, f.w);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = w;
+          }
+        } else {
+          const float* ff = &f.x;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (col + k < p.N) store_f(p.out, o + k, p.out_dtype, ff[k]);
+        }
+      };
+
       // one chunk of 32 columns, accumulators in v
       auto chunk = [&](const int c, uint32_t (&v)[32]) {
         const int cc = col0 + c * 32;
@@ -857,22 +879,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
                 continue;
               }
             }
-            const int64_t o = t.b * p.out_sb + grow * p.out_sr + col;
-            if (p.out_vec && col + 4 <= p.N) {
-              if (p.out_dtype == FK_F32) {
-                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = f;
-              } else {
-                uint2 w;
-                w.x = p.out_dtype == FK_BF16 ? pack_bf16(f.x, f.y) : pack_f16(f.x, f.y);
-                w.y = p.out_dtype == FK_BF16 ? pack_bf16(f.z, f.w) : pack_f16(f.z, f.w);
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + o) = w;
-              }
-            } else {
-              const float* ff = &f.x;
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (col + k < p.N) store_f(p.out, o + k, p.out_dtype, ff[k]);
-            }
+            emit(grow, col, f);
           }
         } else {  // kEpiArgmax
           const float* tsc = table + c * 32;
@@ -1002,6 +1009,40 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         }
       }
 
+      if constexpr (EPI == kEpiOut) {
+        if (p.join) {
+          // Partial sums of a split contraction: whichever split's warp arrives
+          // last adds all of them up, in the order of the splits, so the result
+          // does not depend on which one that is.
+          __threadfence();
+          __syncwarp();
+          const int64_t tile = (static_cast<int64_t>(t.b) * p.m_tiles + t.m) * p.n_tiles + t.n;
+          uint32_t* arrived = p.join + (tile * CG + rank) * S::kEpiWarps + ew;
+          uint32_t n = 0;
+          if (lane == 0) n = atomicAdd(arrived, 1u) + 1;
+          n = __shfl_sync(0xffffffffu, n, 0);
+          if (n == static_cast<uint32_t>(p.chunks)) {
+            __threadfence();
+            if (lane == 0) *arrived = 0;
+            constexpr int kQuads = kCols / 4;
+            for (int i = lane; i < 32 * kQuads; i += 32) {
+              const int64_t grow = row0 + i / kQuads;
+              const int col = col0 + i % kQuads * 4;
+              if (grow >= p.M || col >= p.N) continue;
+              const float* a = p.acc + t.b * p.acc_batch + grow * p.acc_ld + col;
+              float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              for (int k = 0; k < p.join_splits; ++k) {
+                const float4 o = __ldcg(reinterpret_cast<const float4*>(a + k * p.acc_split));
+                f.x += o.x;
+                f.y += o.y;
+                f.z += o.z;
+                f.w += o.w;
+              }
+              emit(grow, col, f);
+            }
+          }
+        }
+      }
       if constexpr (EPI == kEpiLse) {
         if (t.last && row_ok)
           p.partial[((static_cast<int64_t>(t.b) * p.chunks + t.chunk) * S::kParts + part) * p.M + row] =

@@ -183,6 +183,8 @@ struct CombineParams {
   int32_t* count;          // rows that are not ignored
   double2* block_part;     // (sum, count) of each block
   uint32_t* ticket;        // zero before the launch
+  uint16_t* copy;          // optional: x's rows, 16-bit, Dp apart, ignored ones as zeros
+  int Dp;
   int* status;
 };
 
@@ -231,6 +233,25 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
     const int64_t n = (blockIdx.x % p.row_blocks) * 32 + i;
     if (n >= p.N) break;
     const int64_t y = load_label(p.labels, b * p.lb + n * p.ln, p.label_dtype);
+    if (p.copy) {
+      // the backward pass's copy of x (see head_rows_kernel), while the row is at hand
+      const uint16_t* src = static_cast<const uint16_t*>(p.x) + b * p.xs[0] + n * p.xs[1];
+      uint16_t* dst = p.copy + (static_cast<int64_t>(b) * p.N + n) * p.Dp;
+      for (int d = lane * 8; d < p.Dp; d += 256) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (y != p.ignore) {
+          if (d + 8 <= p.D) {
+            u = *reinterpret_cast<const uint4*>(src + d);
+          } else {
+            uint16_t* v = reinterpret_cast<uint16_t*>(&u);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (d + k < p.D) v[k] = src[d + k];
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + d) = u;
+      }
+    }
     float z = 0.0f;
     if (y != p.ignore && y >= 0 && y < p.K) {
       const int64_t xo = b * p.xs[0] + n * p.xs[1], co = b * p.cs[0] + y * p.cs[1];
@@ -369,36 +390,6 @@ __global__ void xent_weight_kernel(const float* __restrict__ g, const RowStat* _
   }
 }
 
-// ---------------------------------------------------- split sums to the output
-struct JoinJob {        // total = 0 for none
-  const float* acc;
-  int splits;
-  int64_t split_stride, acc_batch, acc_ld;
-  void* out;
-  int dtype;
-  int64_t ob, orow;
-  int rows, cols;
-  int64_t total;
-};
-struct JoinJobs {
-  JoinJob job[2];
-};
-
-__global__ void head_join_kernel(const JoinJobs jobs) {
-  const JoinJob& j = jobs.job[blockIdx.y];
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < j.total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t r = i / j.cols;
-    const int c = static_cast<int>(i - r * j.cols);
-    const int64_t b = r / j.rows, n = r - b * j.rows;
-    const float* a = j.acc + b * j.acc_batch + n * j.acc_ld + c;
-    float v = 0.0f;
-#pragma unroll 4
-    for (int s = 0; s < j.splits; ++s) v += a[s * j.split_stride];
-    store_f(j.out, b * j.ob + n * j.orow + c, j.dtype, v);
-  }
-}
-
 // -------------------------------------------------------------------- plans
 struct Bump {  // workspace layout: the same walk sizes it and hands it out
   uint8_t* base;
@@ -483,6 +474,11 @@ static int check_workspace(const void* ws, size_t have, size_t need, const char*
   return FK_OK;
 }
 
+// Copies of the operands made by the caller of a pass; see fk_xent_loss_grad.
+struct Copies {
+  uint16_t *x_forward, *x_backward, *c;   // null: used in place (x_forward, c)
+};
+
 struct ForwardPlan {
   ShapeChoice sh;
   int chunks;
@@ -494,19 +490,24 @@ struct ForwardPlan {
   size_t bytes;
 };
 
-static ForwardPlan plan_forward(const Xent& q, void* ws) {
+static ForwardPlan plan_forward(const Xent& q, void* ws, const Copies* given = nullptr) {
   ForwardPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
   f.sh = choose_shape(q.N, q.K, q.B, q.parts() > 1);
   f.chunks = choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                            2 * slots_of(f.sh), 0.25);
   f.row_blocks = ceil_div(q.N, 32);
-  f.xc = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
-             ? nullptr
-             : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
-  f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
-             ? nullptr
-             : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  if (given) {
+    f.xc = given->x_forward;
+    f.cc = given->c;
+  } else {
+    f.xc = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
+               ? nullptr
+               : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+    f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
+               ? nullptr
+               : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  }
   f.partial = b.take<float2>(q.B * f.chunks * parts_of(f.sh.bn) * q.N);
   f.block_part = b.take<double2>(q.B * f.row_blocks);
   f.ticket = b.take<uint32_t>(1);
@@ -515,11 +516,13 @@ static ForwardPlan plan_forward(const Xent& q, void* ws) {
 }
 
 static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, void* ws, size_t ws_bytes,
-                   int* status, cudaStream_t s) {
-  const ForwardPlan f = plan_forward(q, ws);
+                   int* status, cudaStream_t s, const Copies* given = nullptr) {
+  const ForwardPlan f = plan_forward(q, ws, given);
   if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_forward")) return bad;
-  int st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), nullptr),
-                     rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  int st = FK_OK;
+  if (!given)
+    st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), nullptr),
+                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
   if (st != FK_OK) return st;
   Params<1> prm = {};
   prm.count = 1;
@@ -576,6 +579,10 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   cp.count = count;
   cp.block_part = f.block_part;
   cp.ticket = f.ticket;
+  if (given && !given->x_forward) {
+    cp.copy = given->x_backward;
+    cp.Dp = static_cast<int>(q.Dp());
+  }
   cp.status = status;
   xent_combine_kernel<<<static_cast<unsigned>(q.B * f.row_blocks), kCombineWarps * 32, 0, s>>>(cp);
   return check_launch("xent_combine_kernel");
@@ -589,6 +596,8 @@ struct BackwardPlan {
   int64_t ld;                  // of the float32 accumulators
   uint16_t *xc, *cc, *P;
   float *acc_x, *acc_c;        // null: the product writes the output itself
+  uint32_t *join_x, *join_c;   // arrival counters of split products
+  int64_t joins;               // of both, from join_x on
   RowStat* weighted;
   float* gmax;                 // (largest |g|, the factor it gives)
   size_t bytes;
@@ -596,8 +605,8 @@ struct BackwardPlan {
 
 // Tile shape and splits of the two gradient products: dx is Mx x D over steps_x
 // steps, dc Mc x D over steps_c (0: not wanted).  A product with few tiles and a
-// long contraction is split along it; each split costs a pass over float32
-// partial sums, counted in steps of a tile's contraction.
+// long contraction is split along it; each split costs a write and a read of
+// float32 partial sums, counted in steps of a tile's contraction.
 static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc, int64_t steps_c,
                           BackwardPlan* f) {
   const bool exact = q.parts() > 1;
@@ -630,7 +639,7 @@ static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc
       const double span = cx >= cc ? fill(tx * sx, cx, tc * sc, cc, workers).span
                                    : fill(tc * sc, cc, tx * sx, cx, workers).span;
       const double bytes = (sx > 1 ? 4.0 * q.B * Mx * q.D * (2 * sx) : 0.0) + (sc > 1 ? 4.0 * q.B * Mc * q.D * (2 * sc) : 0.0);
-      const double join = sx > 1 || sc > 1 ? (3.0 + bytes / 4e6) / us : 0.0;
+      const double join = sx > 1 || sc > 1 ? (1.0 + bytes / 4e6) / us : 0.0;
       if (span + join < best * 0.999) {
         best = span + join;
         f->split_x = sx;
@@ -640,7 +649,8 @@ static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc
   }
 }
 
-static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void* ws) {
+static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void* ws,
+                                  const Copies* given = nullptr) {
   BackwardPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
   const int64_t budget = std::max<int64_t>(kPieceElems / q.parts() / q.B, 256 * 128);
@@ -659,14 +669,27 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   const int64_t steps_x = ceil_div(kw, 64), steps_c = ceil_div(f.R, 64);
   plan_products(q, f.R, want_x ? steps_x : 0, kw, want_c ? steps_c : 0, &f);
   f.ld = ceil_div(q.D, 4) * 4;
-  f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
-  f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
-             ? nullptr
-             : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  if (given) {
+    f.xc = given->x_backward;
+    f.cc = given->c;
+  } else {
+    f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+    f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
+               ? nullptr
+               : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  }
   f.P = b.take<uint16_t>(q.parts() * q.B * f.R * f.Kp);
   f.acc_x = f.acc_c = nullptr;
   if (want_x && (f.n_pieces > 1 || f.split_x > 1)) f.acc_x = b.take<float>(f.split_x * q.B * q.N * f.ld);
   if (want_c && (f.n_chunks > 1 || f.split_c > 1)) f.acc_c = b.take<float>(f.split_c * q.B * f.Kp * f.ld);
+  // 32 warps a tile at most
+  auto counters = [&](int64_t M, int splits) {
+    return splits > 1 ? q.B * ceil_div(M, f.sh.bm()) * ceil_div(q.D, f.sh.bn) * 32 : 0;
+  };
+  const int64_t jx = want_x ? counters(f.R, f.split_x) : 0, jc = want_c ? counters(kw, f.split_c) : 0;
+  f.joins = jx + jc;
+  f.join_x = f.joins ? b.take<uint32_t>(f.joins) : nullptr;
+  f.join_c = f.join_x ? f.join_x + jx : nullptr;
   f.weighted = q.reduction == 0 ? b.take<RowStat>(q.B * q.N) : nullptr;
   f.gmax = q.reduction == 0 ? b.take<float>(2) : nullptr;
   f.bytes = b.used;
@@ -678,9 +701,8 @@ struct Grad {
   int64_t sb, sr;
 };
 
-// One gradient product over a piece, into the accumulator or the output; `join`
-// is what its splits leave to add up.
-static int grad_problem(const Xent& q, Params<2>& prm, JoinJob* join, const Problem& base, const Operand& a,
+// One gradient product over a piece, into the accumulator or the output.
+static int grad_problem(const Xent& q, Params<2>& prm, uint32_t* join, const Problem& base, const Operand& a,
                         const Operand& b, int64_t M, int64_t kdim, ShapeChoice sh, int splits, float* acc,
                         int64_t acc_rows, int64_t acc_row0, int64_t ld, bool first, bool last, const Grad& g,
                         int64_t out_row0) {
@@ -707,24 +729,26 @@ static int grad_problem(const Xent& q, Params<2>& prm, JoinJob* join, const Prob
   if (splits > 1 && last) {
     // a short last piece may have fewer steps than splits: the others hold
     // earlier pieces' sums, or were never written if this is the only piece
-    *join = {p.acc, first ? p.chunks : splits, p.acc_split, p.acc_batch, ld, p.out, q.dtype, g.sb, g.sr,
-             static_cast<int>(M), static_cast<int>(q.D), q.B * M * q.D};
+    p.join = join;
+    p.join_splits = first ? p.chunks : splits;
   }
   return set_problem<kEpiOut>(prm, prm.count++, a, b, kdim, sh);
 }
 
 static int backward(const Xent& q, const RowStat* stat, const int32_t* count, const float* g,
                     const Grad& gx, const Grad& gc, void* ws, size_t ws_bytes, int* status,
-                    cudaStream_t s) {
-  const BackwardPlan f = plan_backward(q, gx.p != nullptr, gc.p != nullptr, ws);
+                    cudaStream_t s, const Copies* given = nullptr) {
+  const BackwardPlan f = plan_backward(q, gx.p != nullptr, gc.p != nullptr, ws, given);
   if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_backward")) return bad;
   const int64_t rows = q.B * q.N;
   const bool f16 = q.dtype == FK_F16;
   // float16 P is kept times 2^14: a softmax over 2^20 centroids then still has
   // ten bits above float16's smallest subnormal, and 1 * 2^14 is in range
   const float p_scale = f16 ? 16384.0f : 1.0f;
-  int st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), &q.y),
-                     rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  int st = FK_OK;
+  if (!given)
+    st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), &q.y),
+                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
   if (st != FK_OK) return st;
   const float* factor = q.reduction == 0 ? nullptr : g;
   if (q.reduction == 0) {
@@ -766,6 +790,10 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       p.p_batch = f.R * f.Kp;
       p.p_part = q.B * f.R * f.Kp;
       p.p_bf16 = !f16;
+      if (piece == 0 && chunk == 0) {
+        p.zero = f.join_x;
+        p.zero_n = static_cast<int>(f.joins);
+      }
       st = set_problem<kEpiGrad>(prm, 0, operand(q, q.x, f.xc, q.B, q.N, q.xs, false, r0),
                                  operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, false, k0), q.D, f.sh_p);
       if (st == FK_OK) st = launch<kEpiGrad>(prm, f.sh_p, s);
@@ -790,23 +818,17 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       base.f_num = factor;
       base.f_den = q.reduction == 1 ? count : nullptr;
       Params<2> pair = {};
-      JoinJobs joins = {};
-      int n_joins = 0;
       auto add_x = [&]() {
         const Operand co = operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, true, k0);
-        const int r = grad_problem(q, pair, &joins.job[n_joins], base, po, co, rw, kw, f.sh, f.split_x, f.acc_x,
-                                   q.N, r0, f.ld, piece == 0, piece + 1 == f.n_pieces, gx, r0);
-        n_joins += joins.job[n_joins].total > 0;
-        return r;
+        return grad_problem(q, pair, f.join_x, base, po, co, rw, kw, f.sh, f.split_x, f.acc_x, q.N, r0, f.ld,
+                            piece == 0, piece + 1 == f.n_pieces, gx, r0);
       };
       auto add_c = [&]() {
         Operand pt = po;
         pt.mn = true;
         const Operand xo = operand(q, q.x, f.xc, q.B, q.N, q.xs, true, r0);
-        const int r = grad_problem(q, pair, &joins.job[n_joins], base, pt, xo, kw, rw, f.sh, f.split_c, f.acc_c,
-                                   f.Kp, 0, f.ld, chunk == 0, chunk + 1 == f.n_chunks, gc, k0);
-        n_joins += joins.job[n_joins].total > 0;
-        return r;
+        return grad_problem(q, pair, f.join_c, base, pt, xo, kw, rw, f.sh, f.split_c, f.acc_c, f.Kp, 0, f.ld,
+                            chunk == 0, chunk + 1 == f.n_chunks, gc, k0);
       };
       // the product with the longer tiles first
       const bool x_first = ceil_div(kw, 64) / f.split_x >= ceil_div(rw, 64) / f.split_c;
@@ -816,17 +838,49 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       if (st == FK_OK && gx.p && !x_first) st = add_x();
       if (st == FK_OK) st = launch<kEpiOut>(pair, f.sh, s);
       if (st != FK_OK) return st;
-      if (n_joins) {
-        const int sms = sm_count_current();
-        const int64_t most = std::max(joins.job[0].total, joins.job[1].total);
-        const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ceil_div(most, 256), (sms > 0 ? sms : 148) * 16ll)),
-                        n_joins);
-        head_join_kernel<<<grid, 256, 0, s>>>(joins);
-        if ((st = check_launch("head_join_kernel")) != FK_OK) return st;
-      }
     }
   }
   return FK_OK;
+}
+
+// Loss and gradients in one call: the operands' copies serve both passes, and a
+// 16-bit x that the forward pass reads in place is copied by its combine kernel.
+struct LossGradPlan {
+  Copies copies;
+  RowStat* stat;
+  int32_t* count;
+  uint8_t* rest;               // scratch of the passes, one after the other
+  size_t rest_bytes, bytes;
+};
+
+static LossGradPlan plan_loss_grad(const Xent& q, bool want_x, bool want_c, void* ws) {
+  LossGradPlan f;
+  Bump b{static_cast<uint8_t*>(ws)};
+  f.copies.x_backward = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+  f.copies.c = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
+                   ? nullptr
+                   : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
+  f.copies.x_forward = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs) ? nullptr : f.copies.x_backward;
+  f.stat = b.take<RowStat>(q.B * q.N);
+  f.count = b.take<int32_t>(1);
+  f.rest = b.base ? b.base + b.used : nullptr;
+  f.rest_bytes = std::max(plan_forward(q, nullptr, &f.copies).bytes,
+                          plan_backward(q, want_x, want_c, nullptr, &f.copies).bytes);
+  f.bytes = b.used + f.rest_bytes;
+  return f;
+}
+
+static int loss_grad(const Xent& q, float* loss, const float* g, const Grad& gx, const Grad& gc, void* ws,
+                     size_t ws_bytes, int* status, cudaStream_t s) {
+  const LossGradPlan f = plan_loss_grad(q, gx.p != nullptr, gc.p != nullptr, ws);
+  if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_loss_grad")) return bad;
+  int st = rows_copy(
+      q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.copies.x_forward, q.Dp(), &q.y),
+      rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.copies.c, q.Dp(), nullptr), s);
+  if (st == FK_OK) st = forward(q, loss, f.stat, f.count, f.rest, f.rest_bytes, status, s, &f.copies);
+  if (st == FK_OK)
+    st = backward(q, f.stat, f.count, g, gx, gc, f.rest, f.rest_bytes, status, s, &f.copies);
+  return st;
 }
 
 static int make(Xent& q, const void* x, const void* c, const void* labels, int dtype, int labels_dtype,
@@ -860,6 +914,34 @@ static int make(Xent& q, const void* x, const void* c, const void* labels, int d
 using namespace fk;
 using namespace fk::head;
 
+static int check_grads(int64_t D, const void* gx, const void* gc, const int64_t* gxs, const int64_t* gcs,
+                       const char* who) {
+  if ((gx && !gxs) || (gc && !gcs)) return fail(FK_ERR_INVALID_ARG, "%s: null strides", who);
+  if ((gx && D > 1 && gxs[2] != 1) || (gc && D > 1 && gcs[2] != 1))
+    return fail(FK_ERR_UNSUPPORTED, "%s: gradient rows must have unit stride", who);
+  return FK_OK;
+}
+
+static int no_rows_grad(int64_t B, int64_t K, int64_t D, int dtype, void* gc, const int64_t* gcs,
+                        cudaStream_t s) {
+  if (!gc) return FK_OK;
+  const int64_t eb = dtype_bytes(dtype);
+  for (int64_t b = 0; b < B; ++b) {
+    const cudaError_t e = cudaMemset2DAsync(static_cast<uint8_t*>(gc) + b * gcs[0] * eb,
+                                            static_cast<size_t>(std::max(gcs[1], D) * eb), 0,
+                                            static_cast<size_t>(D * eb), static_cast<size_t>(K), s);
+    if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaMemset2DAsync: %s", cudaGetErrorString(e));
+  }
+  return FK_OK;
+}
+
+static int no_rows_loss(int reduction, float* loss, int32_t* count, cudaStream_t s) {
+  // a sum of 0, a mean of 0 / 0 (all bits set is a NaN)
+  cudaError_t e = count ? cudaMemsetAsync(count, 0, sizeof(int32_t), s) : cudaSuccess;
+  if (e == cudaSuccess && reduction != 0) e = cudaMemsetAsync(loss, reduction == 1 ? 0xff : 0, sizeof(float), s);
+  return e == cudaSuccess ? FK_OK : fail(FK_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+}
+
 extern "C" size_t fk_xent_workspace_size(const void* x, const void* centroids, int dtype, int64_t B,
                                          int64_t N, int64_t K, int64_t D, const int64_t* x_strides3,
                                          const int64_t* c_strides3, int reduction, int backward_x,
@@ -888,18 +970,53 @@ extern "C" int fk_xent_forward(const void* x, const void* centroids, const void*
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (!count || (!loss && (B * N > 0 || reduction != 0)))
     return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: null pointer");
-  if (B == 0 || N == 0) {
-    // no rows: a sum of 0, a mean of 0 / 0 (all bits set is a NaN)
-    cudaError_t e = cudaMemsetAsync(count, 0, sizeof(int32_t), s);
-    if (e == cudaSuccess && reduction != 0)
-      e = cudaMemsetAsync(loss, reduction == 1 ? 0xff : 0, sizeof(float), s);
-    return e == cudaSuccess ? FK_OK : fail(FK_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
-  }
+  if (B == 0 || N == 0) return no_rows_loss(reduction, loss, count, s);
   if (!x || !centroids || !labels) return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: null pointer");
   if (reinterpret_cast<uintptr_t>(row_stats) % 16)
     return fail(FK_ERR_INVALID_ARG, "fk_xent_forward: row_stats must be 16-byte aligned");
   return forward(q, loss, reinterpret_cast<RowStat*>(row_stats), count, workspace, workspace_bytes,
                  dev_status, s);
+}
+
+extern "C" size_t fk_xent_loss_grad_workspace_size(const void* x, const void* centroids, int dtype,
+                                                   int64_t B, int64_t N, int64_t K, int64_t D,
+                                                   const int64_t* x_strides3, const int64_t* c_strides3,
+                                                   int reduction, int want_x, int want_c) {
+  Xent q;
+  const int64_t ls[2] = {0, 0};
+  if (make(q, x, centroids, nullptr, dtype, FK_I32, B, N, K, D, x_strides3, c_strides3, ls, 1.0f, 0,
+           reduction, "fk_xent_loss_grad_workspace_size") != FK_OK ||
+      B == 0 || N == 0)
+    return 0;
+  return plan_loss_grad(q, want_x != 0, want_c != 0, nullptr).bytes;
+}
+
+extern "C" int fk_xent_loss_grad(const void* x, const void* centroids, const void* labels, int dtype,
+                                 int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
+                                 const int64_t* x_strides3, const int64_t* c_strides3,
+                                 const int64_t* l_strides2, float scale, int64_t ignore_index,
+                                 int reduction, float* loss, const float* grad_loss, void* grad_x,
+                                 void* grad_centroids, const int64_t* gx_strides3,
+                                 const int64_t* gc_strides3, void* workspace, size_t workspace_bytes,
+                                 int32_t* dev_status, void* stream) {
+  Xent q;
+  int st = make(q, x, centroids, labels, dtype, labels_dtype, B, N, K, D, x_strides3, c_strides3,
+                l_strides2, scale, ignore_index, reduction, "fk_xent_loss_grad");
+  if (st != FK_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  st = check_grads(D, grad_x, grad_centroids, gx_strides3, gc_strides3, "fk_xent_loss_grad");
+  if (st != FK_OK) return st;
+  if (!loss && (B * N > 0 || reduction != 0))
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_loss_grad: null pointer");
+  if (B == 0 || N == 0) {
+    st = no_rows_loss(reduction, loss, nullptr, s);
+    return st == FK_OK ? no_rows_grad(B, K, D, dtype, grad_centroids, gc_strides3, s) : st;
+  }
+  if (!x || !centroids || !labels || (!grad_x && !grad_centroids) || (reduction == 0 && !grad_loss))
+    return fail(FK_ERR_INVALID_ARG, "fk_xent_loss_grad: null pointer");
+  Grad gx{grad_x, grad_x ? gx_strides3[0] : 0, grad_x ? gx_strides3[1] : 0};
+  Grad gc{grad_centroids, grad_centroids ? gc_strides3[0] : 0, grad_centroids ? gc_strides3[1] : 0};
+  return loss_grad(q, loss, grad_loss, gx, gc, workspace, workspace_bytes, dev_status, s);
 }
 
 extern "C" int fk_xent_backward(const void* x, const void* centroids, const void* labels, int dtype,
@@ -916,22 +1033,9 @@ extern "C" int fk_xent_backward(const void* x, const void* centroids, const void
                 l_strides2, scale, ignore_index, reduction, "fk_xent_backward");
   if (st != FK_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if ((grad_x && !gx_strides3) || (grad_centroids && !gc_strides3))
-    return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: null strides");
-  if ((grad_x && D > 1 && gx_strides3[2] != 1) || (grad_centroids && D > 1 && gc_strides3[2] != 1))
-    return fail(FK_ERR_UNSUPPORTED, "fk_xent_backward: gradient rows must have unit stride");
-  if (!grad_x && !grad_centroids) return FK_OK;
-  if (B == 0 || N == 0) {
-    if (!grad_centroids || B == 0) return FK_OK;
-    const int64_t eb = dtype_bytes(dtype);
-    for (int64_t b = 0; b < B; ++b) {
-      const cudaError_t e = cudaMemset2DAsync(static_cast<uint8_t*>(grad_centroids) + b * gc_strides3[0] * eb,
-                                              static_cast<size_t>(std::max(gc_strides3[1], D) * eb), 0,
-                                              static_cast<size_t>(D * eb), static_cast<size_t>(K), s);
-      if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaMemset2DAsync: %s", cudaGetErrorString(e));
-    }
-    return FK_OK;
-  }
+  st = check_grads(D, grad_x, grad_centroids, gx_strides3, gc_strides3, "fk_xent_backward");
+  if (st != FK_OK || (!grad_x && !grad_centroids)) return st;
+  if (B == 0 || N == 0) return no_rows_grad(B, K, D, dtype, grad_centroids, gc_strides3, s);
   if (!x || !centroids || !labels || !row_stats || !count || (reduction == 0 && !grad_loss))
     return fail(FK_ERR_INVALID_ARG, "fk_xent_backward: null pointer");
   if (reinterpret_cast<uintptr_t>(row_stats) % 16)

@@ -90,6 +90,9 @@ SIGNATURES = {
                              _P, _P, _S, _P, _P]),
     "fk_xent_backward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P,
                               _P, _P, _P, _P, _PL, _PL, _P, _S, _P, _P]),
+    "fk_xent_loss_grad_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I, _I, _I]),
+    "fk_xent_loss_grad": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P,
+                               _P, _P, _P, _PL, _PL, _P, _S, _P, _P]),
     "fk_quantize_rows": (_I, [_P, _I, _L, _L, _L, _PL, _P, _PL, _P, _PL, _P]),
     "fk_int8_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I]),
     "fk_int8_scores": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _PL,

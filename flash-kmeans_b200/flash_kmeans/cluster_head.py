@@ -137,6 +137,8 @@ class _XentLayout:
         self.bytes = {w: self.lib.fk_xent_workspace_size(x.data_ptr(), centroids.data_ptr(), dtype,
                                                          *sizes, xs, cs, code, *w)
                       for w in ((0, 0), (0, 1), (1, 0), (1, 1))}
+        self.both = self.lib.fk_xent_loss_grad_workspace_size(
+            x.data_ptr(), centroids.data_ptr(), dtype, *sizes, xs, cs, code, 1, 1)
         self.device = x.device
 
 
@@ -200,6 +202,19 @@ class _Xent:
         _call(at.lib.fk_xent_forward, "fk_xent_forward", self.dev, self.x.data_ptr(), self.c.data_ptr(),
               self.labels.data_ptr(), *at.middle, loss.data_ptr(), stats, count, ws.data_ptr(), nbytes)
         return loss, kept
+
+    def loss_grad(self, grad_loss):
+        """(loss, gradient by x, by the centroids)"""
+        at = self.at
+        xshape, cshape = self.shapes
+        loss = torch.empty(xshape[:-1] if self.none else (), dtype=torch.float32, device=at.device)
+        gx, gc = self.x.new_empty(xshape), self.x.new_empty(cshape)
+        ws = torch.empty(at.both, dtype=torch.uint8, device=at.device)
+        _call(at.lib.fk_xent_loss_grad, "fk_xent_loss_grad", self.dev, self.x.data_ptr(),
+              self.c.data_ptr(), self.labels.data_ptr(), *at.middle, loss.data_ptr(),
+              None if grad_loss is None else grad_loss.data_ptr(), gx.data_ptr(), gc.data_ptr(),
+              *at.grad_strides, ws.data_ptr(), at.both)
+        return loss, gx, gc
 
     def backward(self, kept, grad_loss, want_x, want_c):
         """(gradient by x or None, by the centroids or None)"""
@@ -294,8 +309,7 @@ def cluster_cross_entropy_grad(x: torch.Tensor, centroids: torch.Tensor, labels:
             grad_loss = grad_loss.contiguous()
         elif call.none:
             grad_loss = torch.ones(shape, dtype=torch.float32, device=x.device)
-        loss, kept = call.forward(True)
-        return loss, *call.backward(kept, grad_loss, True, True)
+        return call.loss_grad(grad_loss)
 
 
 # ------------------------------------------------------------- 8-bit scores

@@ -307,6 +307,21 @@ int fk_xent_backward(const void* x, const void* centroids, const void* labels, i
                      const int64_t* gc_strides3, void* workspace, size_t workspace_bytes,
                      int32_t* dev_status, void* stream);
 
+/* Both in one call, for a step whose upstream gradient is known (grad_loss as
+ * for fk_xent_backward): operands are copied once, and what the backward pass
+ * needs of the forward pass stays in the workspace.  At least one gradient. */
+size_t fk_xent_loss_grad_workspace_size(const void* x, const void* centroids, int dtype, int64_t B,
+                                        int64_t N, int64_t K, int64_t D, const int64_t* x_strides3,
+                                        const int64_t* c_strides3, int reduction, int want_x,
+                                        int want_c);
+int fk_xent_loss_grad(const void* x, const void* centroids, const void* labels, int dtype,
+                      int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
+                      const int64_t* x_strides3, const int64_t* c_strides3,
+                      const int64_t* l_strides2, float scale, int64_t ignore_index, int reduction,
+                      float* loss, const float* grad_loss, void* grad_x, void* grad_centroids,
+                      const int64_t* gx_strides3, const int64_t* gc_strides3, void* workspace,
+                      size_t workspace_bytes, int32_t* dev_status, void* stream);
+
 /* Rows of x as 8-bit integers with one scale each: scale = most / 127 and
  * q = rint(x * (127 / most)) for the row's largest magnitude `most`, in
  * float32.  A row with most < 1e-36 becomes zeros with scale 0; one that holds

@@ -1024,21 +1024,34 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           if (n == static_cast<uint32_t>(p.chunks)) {
             __threadfence();
             if (lane == 0) *arrived = 0;
-            constexpr int kQuads = kCols / 4;
-            for (int i = lane; i < 32 * kQuads; i += 32) {
-              const int64_t grow = row0 + i / kQuads;
-              const int col = col0 + i % kQuads * 4;
+            // eight loads in flight a lane: the sums are a chain of `splits` of them
+            constexpr int kQuads = kCols / 4, kRows = 32 / kQuads;
+#pragma unroll 1
+            for (int r = 0; r < 32; r += 8 * kRows) {
+              const int grow = row0 + r + lane / kQuads;
+              const int col = col0 + lane % kQuads * 4;
               if (grow >= p.M || col >= p.N) continue;
-              const float* a = p.acc + t.b * p.acc_batch + grow * p.acc_ld + col;
-              float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              for (int k = 0; k < p.join_splits; ++k) {
-                const float4 o = __ldcg(reinterpret_cast<const float4*>(a + k * p.acc_split));
-                f.x += o.x;
-                f.y += o.y;
-                f.z += o.z;
-                f.w += o.w;
+              // rows past the last one load it again: no branch between the loads
+              const float* a = p.acc + t.b * p.acc_batch + col;
+              int64_t at[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) at[i] = min(grow + i * kRows, p.M - 1) * p.acc_ld;
+              float4 f[8] = {};
+              for (int k = 0; k < p.join_splits; ++k, a += p.acc_split) {
+                float4 o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = __ldcg(reinterpret_cast<const float4*>(a + at[i]));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  f[i].x += o[i].x;
+                  f[i].y += o[i].y;
+                  f[i].z += o[i].z;
+                  f[i].w += o[i].w;
+                }
               }
-              emit(grow, col, f);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (grow + i * kRows < p.M) emit(grow + i * kRows, col, f[i]);
             }
           }
         }

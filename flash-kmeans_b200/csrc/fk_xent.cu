@@ -639,7 +639,9 @@ static void plan_products(const Xent& q, int64_t Mx, int64_t steps_x, int64_t Mc
       const double span = cx >= cc ? fill(tx * sx, cx, tc * sc, cc, workers).span
                                    : fill(tc * sc, cc, tx * sx, cx, workers).span;
       const double bytes = (sx > 1 ? 4.0 * q.B * Mx * q.D * (2 * sx) : 0.0) + (sc > 1 ? 4.0 * q.B * Mc * q.D * (2 * sc) : 0.0);
-      const double join = sx > 1 || sc > 1 ? (1.0 + bytes / 4e6) / us : 0.0;
+      // the last split's warp reads the others' sums one after another
+      const double chain = 0.7 * (sx > 1 || sc > 1 ? std::max(sx, sc) : 0) * (f->sh.bn == 256 ? 2 : 1);
+      const double join = (chain + bytes / 4e6) / us;
       if (span + join < best * 0.999) {
         best = span + join;
         f->split_x = sx;

@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       tmem_relinquish();
     }
   }
+  pdl_wait_then_release();
   if (warp == 3)
     for (int i = blockIdx.x * 32 + lane; i < p0.zero_n; i += gridDim.x * 32) p0.zero[i] = 0;
   tc_fence_before();
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       if constexpr (EPI == kEpiGrad) {
         st_next = {0.0f, 0.0f, 0.0f, -1};
         if (row < p.M) {
-          const float4 f = __ldg(reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + p.stat_off + row));
+          const float4 f = *reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + p.stat_off + row);
           st_next = {f.x, f.y, f.z, __float_as_int(f.w)};
         }
       }

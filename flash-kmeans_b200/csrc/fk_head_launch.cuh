@@ -3,7 +3,7 @@
 #pragma once
 #include <algorithm>
 #include <atomic>
-#include <mutex>
+#include <type_traits>
 
 #include "fk_head_gemm.cuh"
 
@@ -94,6 +94,27 @@ inline Fill fill(int64_t n0, double c0, int64_t n1, double c1, int64_t workers) 
   return f;
 }
 
+// Launch of a kernel that begins with pdl_wait_then_release().
+template <typename... Args>
+int launch_plain(const char* what, void (*kern)(Args...), dim3 grid, int threads, cudaStream_t s,
+                 std::common_type_t<Args>... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(FK_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+  }
+  return FK_OK;
+}
+
 int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows);
 
 template <int CG, int BN, int EPI, bool EXACT>
@@ -135,12 +156,14 @@ int launch_shape(Params<problems_of(EPI)>& prm, cudaStream_t s) {
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = CG;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
+  cfg.numAttrs = CG > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, prm);
   if (e != cudaSuccess) {
     cudaGetLastError();

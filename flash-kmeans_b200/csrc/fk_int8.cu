@@ -75,11 +75,12 @@ __device__ __forceinline__ void floats_of(uint4 u, float (&f)[16 / sizeof(T)]) {
 // registers, all in flight at once; 0 for longer rows, which are read twice.
 template <typename T, int STEPS>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(
-    const T* __restrict__ x, int64_t sb, int64_t sn, int64_t sd, int vec, int8_t* __restrict__ q,
-    int64_t qb, int64_t qn, int Dq, int qvec, float* __restrict__ scale, int64_t scb, int64_t scn, int N,
+    const T* x, int64_t sb, int64_t sn, int64_t sd, int vec, int8_t* q, int64_t qb, int64_t qn, int Dq,
+    int qvec, float* scale, int64_t scb, int64_t scn, int N,
     int D, int64_t rows, int lanes) {
   // `lanes` threads per row: a power of two up to a block
   __shared__ uint32_t sm[8];
+  pdl_wait_then_release();
   constexpr int E = 16 / sizeof(T);
   constexpr int kHeld = STEPS > 0 ? STEPS : 1;
   const int sub = threadIdx.x & (lanes - 1);
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(
   auto load = [&](int d) -> uint4 {
     uint4 u = make_uint4(0, 0, 0, 0);
     if (vec && d + E <= D) {
-      u = __ldg(reinterpret_cast<const uint4*>(src + d));
+      u = *reinterpret_cast<const uint4*>(src + d);
     } else {
       T* v = reinterpret_cast<T*>(&u);
 #pragma unroll
@@ -180,10 +181,9 @@ static int quantize_typed(const void* x, int64_t B, int64_t N, int64_t D, const 
               : steps <= 4 ? quantize_rows_kernel<T, 4>
               : steps <= 8 ? quantize_rows_kernel<T, 8>
                            : quantize_rows_kernel<T, 0>;
-  kern<<<static_cast<unsigned>(blocks), 256, 0, s>>>(
-      static_cast<const T*>(x), xs[0], xs[1], xs[2], vec, q, qb, qn, static_cast<int>(Dq), qvec, scale, scb,
-      scn, static_cast<int>(N), static_cast<int>(D), rows, lanes);
-  return check_launch("quantize_rows_kernel");
+  return launch_plain("quantize_rows_kernel", kern, dim3(static_cast<unsigned>(blocks)), 256, s,
+                      static_cast<const T*>(x), xs[0], xs[1], xs[2], vec, q, qb, qn, static_cast<int>(Dq), qvec,
+                      scale, scb, scn, static_cast<int>(N), static_cast<int>(D), rows, lanes);
 }
 
 static int quantize(const void* x, int dtype, int64_t B, int64_t N, int64_t D, const int64_t* xs,
@@ -196,39 +196,60 @@ static int quantize(const void* x, int dtype, int64_t B, int64_t N, int64_t D, c
   }
 }
 
-// 8-bit rows that are not 16-byte addressable, copied to padded ones.
-__global__ void pack8_kernel(const int8_t* __restrict__ x, int64_t sb, int64_t sn, int64_t sd,
-                             int8_t* __restrict__ out, int N, int D, int Dp, int64_t units) {
-  const int per = Dp / 16;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < units;
+// 8-bit rows that are not 16-byte addressable, copied to padded ones; x's and
+// the centroids' in one launch.
+struct Pack8 {
+  const int8_t* x;
+  int64_t sb, sn, sd;
+  int8_t* out;
+  int N, D, Dp;
+  int64_t units;     // of 16 bytes; 0 for none
+};
+struct Pack8Jobs {
+  Pack8 job[2];
+};
+
+__global__ void pack8_kernel(const Pack8Jobs jobs) {
+  pdl_wait_then_release();
+  const Pack8& j = jobs.job[blockIdx.y];
+  const int per = j.Dp / 16;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < j.units;
        u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t row = u / per;
     const int d0 = static_cast<int>(u - row * per) * 16;
-    const int64_t b = row / N, n = row - b * N;
-    const int8_t* src = x + b * sb + n * sn;
+    const int64_t b = row / j.N, n = row - b * j.N;
+    const int8_t* src = j.x + b * j.sb + n * j.sn;
     int8_t v[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = d0 + i < D ? src[(d0 + i) * sd] : 0;
-    *reinterpret_cast<uint4*>(out + row * Dp + d0) = *reinterpret_cast<const uint4*>(v);
+    for (int i = 0; i < 16; ++i) v[i] = d0 + i < j.D ? src[(d0 + i) * j.sd] : 0;
+    *reinterpret_cast<uint4*>(j.out + row * j.Dp + d0) = *reinterpret_cast<const uint4*>(v);
   }
 }
 
-static int pack8(const void* x, int64_t B, int64_t N, int64_t D, const int64_t* xs, int8_t* out,
-                 int64_t Dp, cudaStream_t s) {
-  const int64_t units = B * N * (Dp / 16);
+static Pack8 pack8_job(const void* x, int64_t B, int64_t N, int64_t D, const int64_t* xs, int8_t* out,
+                       int64_t Dp) {
+  Pack8 j = {};
+  if (out)
+    j = {static_cast<const int8_t*>(x), xs[0], xs[1], xs[2], out, static_cast<int>(N), static_cast<int>(D),
+         static_cast<int>(Dp), B * N * (Dp / 16)};
+  return j;
+}
+
+static int pack8(const Pack8& a, const Pack8& b, cudaStream_t s) {
+  const Pack8Jobs jobs = {{a.units ? a : b, b}};
+  const int n = (a.units ? 1 : 0) + (b.units ? 1 : 0);
+  if (n == 0) return FK_OK;
   const int sms = sm_count_current();
-  const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(units, 256), (sms > 0 ? sms : 148) * 16ll));
-  pack8_kernel<<<blocks, 256, 0, s>>>(static_cast<const int8_t*>(x), xs[0], xs[1], xs[2], out,
-                                      static_cast<int>(N), static_cast<int>(D), static_cast<int>(Dp), units);
-  return check_launch("pack8_kernel");
+  const int64_t blocks = std::min<int64_t>(ceil_div(std::max(a.units, b.units), 256), (sms > 0 ? sms : 148) * 16ll);
+  return launch_plain("pack8_kernel", pack8_kernel, dim3(static_cast<unsigned>(blocks), n), 256, s, jobs);
 }
 
 // Joins the column chunks of a row's argmax.
 constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(kJoinWarps * 32) argmax_join_kernel(const float2* __restrict__ partial,
-                                                                      int pieces, int N, int row_blocks,
-                                                                      int32_t* out, int64_t ob, int64_t on) {
+__global__ void __launch_bounds__(kJoinWarps * 32) argmax_join_kernel(const float2* partial, int pieces, int N,
+                                                                      int row_blocks, int32_t* out, int64_t ob, int64_t on) {
   __shared__ float2 sm[kJoinWarps][33];
+  pdl_wait_then_release();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / row_blocks;
   const int row = (blockIdx.x % row_blocks) * 32 + lane;
@@ -357,13 +378,13 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   if (f.bytes && (!ws || ws_bytes < f.bytes || reinterpret_cast<uintptr_t>(ws) % 256))
     return fail(FK_ERR_WORKSPACE, "%s: workspace of %zu bytes (256-byte aligned) needed, %zu given", who,
                 f.bytes, ws_bytes);
-  int st;
+  int st = FK_OK;
   if (q.x_dtype != FK_I8)
     st = quantize(q.x, q.x_dtype, q.B, q.N, q.D, q.xs, f.xq, q.N * q.Dp(), q.Dp(), q.Dp(), f.sx, q.N, 1, s);
-  else
-    st = f.xq ? pack8(q.x, q.B, q.N, q.D, q.xs, f.xq, q.Dp(), s) : FK_OK;
+  if (st == FK_OK)
+    st = pack8(pack8_job(q.x, q.B, q.N, q.D, q.xs, q.x_dtype == FK_I8 ? f.xq : nullptr, q.Dp()),
+               pack8_job(q.c, q.Bc(), q.K, q.D, q.cs, f.cq, q.Dp()), s);
   if (st != FK_OK) return st;
-  if (f.cq && (st = pack8(q.c, q.Bc(), q.K, q.D, q.cs, f.cq, q.Dp(), s)) != FK_OK) return st;
   Params<1> prm = {};
   prm.count = 1;
   Problem& p = prm.p[0];
@@ -392,9 +413,9 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   if (st == FK_OK) st = launch<EPI>(prm, f.sh, s);
   if (st != FK_OK || !f.partial) return st;
   const int64_t row_blocks = ceil_div(q.N, 32);
-  argmax_join_kernel<<<static_cast<unsigned>(q.B * row_blocks), kJoinWarps * 32, 0, s>>>(
-      f.partial, f.chunks * parts_of(f.sh.bn), static_cast<int>(q.N), static_cast<int>(row_blocks), label_out, ls[0], ls[1]);
-  return check_launch("argmax_join_kernel");
+  return launch_plain("argmax_join_kernel", argmax_join_kernel, dim3(static_cast<unsigned>(q.B * row_blocks)),
+                      kJoinWarps * 32, s, f.partial, f.chunks * parts_of(f.sh.bn), static_cast<int>(q.N),
+                      static_cast<int>(row_blocks), label_out, ls[0], ls[1]);
 }
 
 }  // namespace head

@@ -223,6 +223,15 @@ __device__ __forceinline__ void setmaxnreg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// ------------------------------------------ programmatic dependent launch
+// A kernel launched with programmatic stream serialisation may start while the
+// one before it still runs: it waits here before its first access to global
+// memory, and lets the one after it start likewise.
+__device__ __forceinline__ void pdl_wait_then_release() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // --------------------------------------------- CTA pairs (cta_group::2)
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;

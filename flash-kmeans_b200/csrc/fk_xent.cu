@@ -82,8 +82,9 @@ struct RowsJobs {
 
 template <typename T>
 __global__ void head_rows_kernel(const RowsJobs jobs) {
+  pdl_wait_then_release();
   const RowsJob& j = jobs.job[blockIdx.y];
-  const T* __restrict__ x = static_cast<const T*>(j.x);
+  const T* x = static_cast<const T*>(j.x);
   const int per = j.Dp / 8, D = j.D;
   for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < j.units;
        u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -153,11 +154,10 @@ static int rows_copy(int dtype, const RowsJob& a, const RowsJob& b, cudaStream_t
   const int64_t cap = (sms > 0 ? sms : 148) * 16ll;
   const dim3 grid(static_cast<unsigned>(std::min(ceil_div(std::max(a.units, b.units), 256), cap)), n);
   switch (dtype) {
-    case FK_F16: head_rows_kernel<__half><<<grid, 256, 0, s>>>(jobs); break;
-    case FK_BF16: head_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(jobs); break;
-    default: head_rows_kernel<float><<<grid, 256, 0, s>>>(jobs); break;
+    case FK_F16: return launch_plain("head_rows_kernel", head_rows_kernel<__half>, grid, 256, s, jobs);
+    case FK_BF16: return launch_plain("head_rows_kernel", head_rows_kernel<__nv_bfloat16>, grid, 256, s, jobs);
+    default: return launch_plain("head_rows_kernel", head_rows_kernel<float>, grid, 256, s, jobs);
   }
-  return check_launch("head_rows_kernel");
 }
 
 // ------------------------------------------------------------------ combine
@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
   __shared__ float z_label[32];
   __shared__ double2 red[kCombineWarps];
   __shared__ bool last;
+  pdl_wait_then_release();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.row_blocks;
   const int row = (blockIdx.x % p.row_blocks) * 32 + lane;
@@ -352,8 +353,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
 // largest finite one, so that P stays within float16; it comes back as a factor
 // of the outputs.  The maximum of non-negative floats is the maximum of their
 // bits, whose order of arrival does not matter.
-__global__ void xent_gmax_kernel(const float* __restrict__ g, const RowStat* __restrict__ stat,
-                                 int64_t rows, uint32_t* out) {
+__global__ void xent_gmax_kernel(const float* g, const RowStat* stat, int64_t rows, uint32_t* out) {
+  pdl_wait_then_release();
   uint32_t m = 0;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -364,9 +365,9 @@ __global__ void xent_gmax_kernel(const float* __restrict__ g, const RowStat* __r
   if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
 }
 
-__global__ void xent_weight_kernel(const float* __restrict__ g, const RowStat* __restrict__ stat,
-                                   int64_t rows, const float* __restrict__ gmax, RowStat* out,
-                                   float* factor) {
+__global__ void xent_weight_kernel(const float* g, const RowStat* stat, int64_t rows, const float* gmax,
+                                   RowStat* out, float* factor) {
+  pdl_wait_then_release();
   // a power of two, so that the division is exact
   float inv = 1.0f, f = 1.0f;
   if (gmax && *gmax > 0.0f) {
@@ -584,8 +585,8 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
     cp.Dp = static_cast<int>(q.Dp());
   }
   cp.status = status;
-  xent_combine_kernel<<<static_cast<unsigned>(q.B * f.row_blocks), kCombineWarps * 32, 0, s>>>(cp);
-  return check_launch("xent_combine_kernel");
+  return launch_plain("xent_combine_kernel", xent_combine_kernel,
+                      dim3(static_cast<unsigned>(q.B * f.row_blocks)), kCombineWarps * 32, s, cp);
 }
 
 struct BackwardPlan {
@@ -758,13 +759,14 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
     if (f16) {
       const cudaError_t e = cudaMemsetAsync(f.gmax, 0, 2 * sizeof(float), s);
       if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
-      xent_gmax_kernel<<<blocks, 256, 0, s>>>(g, stat, rows, reinterpret_cast<uint32_t*>(f.gmax));
-      if ((st = check_launch("xent_gmax_kernel")) != FK_OK) return st;
+      st = launch_plain("xent_gmax_kernel", xent_gmax_kernel, dim3(blocks), 256, s, g, stat, rows,
+                        reinterpret_cast<uint32_t*>(f.gmax));
+      if (st != FK_OK) return st;
       factor = f.gmax + 1;
     }
-    xent_weight_kernel<<<blocks, 256, 0, s>>>(g, stat, rows, f16 ? f.gmax : nullptr, f.weighted,
-                                              f16 ? f.gmax + 1 : nullptr);
-    if ((st = check_launch("xent_weight_kernel")) != FK_OK) return st;
+    st = launch_plain("xent_weight_kernel", xent_weight_kernel, dim3(blocks), 256, s, g, stat, rows,
+                      f16 ? f.gmax : nullptr, f.weighted, f16 ? f.gmax + 1 : nullptr);
+    if (st != FK_OK) return st;
     stat = f.weighted;
   }
 

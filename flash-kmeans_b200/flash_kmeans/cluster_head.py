@@ -233,24 +233,31 @@ class _Xent:
         return gx, gc
 
 
+def _backward(ctx, grad_loss):
+    ctx.saved_tensors  # raises if an input was changed in place since
+    if not grad_loss.is_contiguous():
+        grad_loss = grad_loss.contiguous()
+    gx, gc = ctx.call.backward(ctx.kept, grad_loss, *ctx.needs_input_grad[:2])
+    return gx, gc, None, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
+
+
 class _ClusterCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, centroids, labels, scale, ignore_index, reduction):
-        call = _Xent(x, centroids, labels, scale, ignore_index, reduction, "cluster_cross_entropy")
-        loss, kept = call.forward(True)
-        ctx.save_for_backward(x, centroids, labels, kept)
-        ctx.args = (scale, ignore_index, reduction)
+        ctx.call = _Xent(x, centroids, labels, scale, ignore_index, reduction,
+                         "cluster_cross_entropy")
+        loss, ctx.kept = ctx.call.forward(True)
+        ctx.save_for_backward(x, centroids, labels)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        x, centroids, labels, kept = ctx.saved_tensors
-        call = _Xent(x, centroids, labels, *ctx.args, "cluster_cross_entropy")
-        if not grad_loss.is_contiguous():
-            grad_loss = grad_loss.contiguous()
-        gx, gc = call.backward(kept, grad_loss, *ctx.needs_input_grad[:2])
-        return gx, gc, None, None, None, None
+        # the guard against a second derivative is only needed, and paid for,
+        # where a graph of the backward pass is recorded
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_loss)
 
 
 def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torch.Tensor, *,

@@ -98,7 +98,6 @@ struct Problem {
   const float* b_scale;
   const float* bias;
   int64_t as_sb, as_sn, bs_sb, bs_sn, bias_sb, bias_sn;
-  int small_acc;            // |acc| < 2^22: conversion by an integer add
   int32_t* label_out;       // kEpiArgmax with one chunk: labels
   int64_t lo_sb, lo_sn;
   uint32_t* zero;           // words cleared for the kernel that follows
@@ -333,23 +332,10 @@ __device__ __forceinline__ int64_t load_label(const void* p, int64_t i, int dt) 
   return dt == FK_I64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
-// 32 int32 accumulators as floats, in place.  |acc| < 2^22 (`small`): an integer
-// add places it in the mantissa of 1.5 * 2^23 and a float add takes that off
-// again, exact, at an eighth of what the conversion instruction costs.
-__device__ __forceinline__ void acc_to_f(uint32_t (&v)[32], bool small) {
-  if (small) {
-    const uint64_t off = pack2(-12582912.0f, -12582912.0f);
+// 32 int32 accumulators as floats, in place.
+__device__ __forceinline__ void acc_to_f(uint32_t (&v)[32]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      float a, b;
-      unpack2(add2(pack2(__uint_as_float(v[i] + 0x4B400000u), __uint_as_float(v[i + 1] + 0x4B400000u)), off), a, b);
-      v[i] = __float_as_uint(a);
-      v[i + 1] = __float_as_uint(b);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[i])));
-  }
+  for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(static_cast<float>(static_cast<int32_t>(v[i])));
 }
 
 // Maximum that a NaN wins, as argmax counts it.
@@ -842,7 +828,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             put(std::false_type{}, 0);
           }
         } else if constexpr (EPI == kEpiOut || EPI == kEpiScores) {
-          if constexpr (EPI == kEpiScores) acc_to_f(v, p.small_acc != 0);
+          if constexpr (EPI == kEpiScores) acc_to_f(v);
           __syncwarp();
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -885,7 +871,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         } else {  // kEpiArgmax
           const float* tsc = table + c * 32;
           const float* tbi = tsc + 64;
-          acc_to_f(v, p.small_acc != 0);
+          acc_to_f(v);
           const uint64_t x2 = pack2(xs, xs);
           float z[32];
 #pragma unroll

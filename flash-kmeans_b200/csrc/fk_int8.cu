@@ -402,7 +402,6 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   p.bias = sc.bias;
   p.bias_sb = sc.bias ? sc.bs[0] : 0;
   p.bias_sn = sc.bias ? sc.bs[1] : 0;
-  p.small_acc = q.D * 128 * 128 < (1 << 22);
   p.partial = f.partial;
   p.label_out = label_out;
   p.lo_sb = ls ? ls[0] : 0;

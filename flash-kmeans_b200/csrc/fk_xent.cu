@@ -161,10 +161,14 @@ static int rows_copy(int dtype, const RowsJob& a, const RowsJob& b, cudaStream_t
 }
 
 // ------------------------------------------------------------------ combine
-// One warp column of 16 warps joins the column chunks of 32 rows; block sums
-// of the losses go to `block_part`, and the last block adds them up in block
-// order, so the result does not depend on which block came last.
+// Sixteen warps join the column chunks of 32 rows and sum the label's score of
+// two rows each; block sums of the losses go to `block_part`, and the last
+// block adds them up in block order, so the result does not depend on which
+// block came last.  What bounds this kernel is the chain of dependent loads
+// (label, centroid row, partial results), so a warp's rows and chunks are in flight
+// together.
 constexpr int kCombineWarps = 16;
+constexpr int kRowsPerWarp = 32 / kCombineWarps;
 
 struct CombineParams {
   const float2* partial;   // [batch][pieces][N]
@@ -188,24 +192,45 @@ struct CombineParams {
   int* status;
 };
 
-// x[n] . c[y] by one warp, in float32 (each lane's partial sum, then a tree).
+// x[n] . c[y] of a warp's rows, in float32 (each lane's partial sum, then a tree).
 template <typename T>
-__device__ __forceinline__ float row_dot(const T* x, int64_t xd, const T* c, int64_t cd, int D, bool vec,
-                                         int lane) {
+__device__ __forceinline__ void row_dots(const CombineParams& p, int b, const int64_t (&n)[kRowsPerWarp],
+                                         const int64_t (&y)[kRowsPerWarp], const bool (&on)[kRowsPerWarp],
+                                         int lane, float (&z)[kRowsPerWarp]) {
   constexpr int E = 16 / sizeof(T);
-  float s = 0.0f;
-  int d = 0;
-  if (vec) {
-    for (d = lane * E; d + E <= D; d += 32 * E) {
-      const uint4 a = *reinterpret_cast<const uint4*>(x + d), b = *reinterpret_cast<const uint4*>(c + d);
-      const T *pa = reinterpret_cast<const T*>(&a), *pb = reinterpret_cast<const T*>(&b);
+  const T *x[kRowsPerWarp], *c[kRowsPerWarp];
 #pragma unroll
-      for (int i = 0; i < E; ++i) s = fmaf(Elem<T>::to_f(pa[i]), Elem<T>::to_f(pb[i]), s);
-    }
-    d = D / E * E;
+  for (int i = 0; i < kRowsPerWarp; ++i) {
+    x[i] = static_cast<const T*>(p.x) + (on[i] ? b * p.xs[0] + n[i] * p.xs[1] : 0);
+    c[i] = static_cast<const T*>(p.c) + (on[i] ? b * p.cs[0] + y[i] * p.cs[1] : 0);
+    z[i] = 0.0f;
   }
-  for (d += lane; d < D; d += 32) s = fmaf(Elem<T>::to_f(x[d * xd]), Elem<T>::to_f(c[d * cd]), s);
-  return warp_sum(s);
+  int d = 0;
+  if (p.vec) {
+    for (d = lane * E; d + E <= p.D; d += 32 * E) {
+      uint4 a[kRowsPerWarp], w[kRowsPerWarp];
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i)
+        if (on[i]) {
+          a[i] = *reinterpret_cast<const uint4*>(x[i] + d);
+          w[i] = *reinterpret_cast<const uint4*>(c[i] + d);
+        }
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i)
+        if (on[i]) {
+          const T *pa = reinterpret_cast<const T*>(&a[i]), *pb = reinterpret_cast<const T*>(&w[i]);
+#pragma unroll
+          for (int k = 0; k < E; ++k) z[i] = fmaf(Elem<T>::to_f(pa[k]), Elem<T>::to_f(pb[k]), z[i]);
+        }
+    }
+    d = p.D / E * E;
+  }
+  for (d += lane; d < p.D; d += 32)
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i)
+      if (on[i]) z[i] = fmaf(Elem<T>::to_f(x[i][d * p.xs[2]]), Elem<T>::to_f(c[i][d * p.cs[2]]), z[i]);
+#pragma unroll
+  for (int i = 0; i < kRowsPerWarp; ++i) z[i] = warp_sum(z[i]);
 }
 
 __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const CombineParams p) {
@@ -220,53 +245,64 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
   const float2* part = p.partial + static_cast<int64_t>(b) * p.pieces * p.N + row;
   float m = -INFINITY, s = 0.0f;
   if (row < p.N) {
-    for (int i = warp; i < p.pieces; i += kCombineWarps) {
-      const float2 v = part[static_cast<int64_t>(i) * p.N];
-      const float mn = fmaxf(m, v.x);
-      const float mu = mn == -INFINITY ? 0.0f : mn;
-      // a piece whose exponents were NaN has a NaN sum, which stays
-      s = s * ex2((m - mu) * p.scale2) + v.y * ex2((v.x - mu) * p.scale2);
-      m = mn;
+    for (int i0 = warp; i0 < p.pieces; i0 += 4 * kCombineWarps) {
+      float2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = i0 + i * kCombineWarps;
+        v[i] = k < p.pieces ? part[static_cast<int64_t>(k) * p.N] : make_float2(-INFINITY, 0.0f);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float mn = fmaxf(m, v[i].x);
+        const float mu = mn == -INFINITY ? 0.0f : mn;
+        // a piece whose exponents were NaN has a NaN sum, which stays
+        s = s * ex2((m - mu) * p.scale2) + v[i].y * ex2((v[i].x - mu) * p.scale2);
+        m = mn;
+      }
     }
   }
   sm[warp][lane] = make_float2(m, s);
-  for (int i = warp; i < 32; i += kCombineWarps) {
-    const int64_t n = (blockIdx.x % p.row_blocks) * 32 + i;
-    if (n >= p.N) break;
-    const int64_t y = load_label(p.labels, b * p.lb + n * p.ln, p.label_dtype);
-    if (p.copy) {
-      // the backward pass's copy of x (see head_rows_kernel), while the row is at hand
-      const uint16_t* src = static_cast<const uint16_t*>(p.x) + b * p.xs[0] + n * p.xs[1];
-      uint16_t* dst = p.copy + (static_cast<int64_t>(b) * p.N + n) * p.Dp;
-      for (int d = lane * 8; d < p.Dp; d += 256) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (y != p.ignore) {
-          if (d + 8 <= p.D) {
-            u = *reinterpret_cast<const uint4*>(src + d);
-          } else {
-            uint16_t* v = reinterpret_cast<uint16_t*>(&u);
+  {
+    int64_t n[kRowsPerWarp], y[kRowsPerWarp];
+    bool on[kRowsPerWarp];
+    float z[kRowsPerWarp];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (d + k < p.D) v[k] = src[d + k];
+    for (int i = 0; i < kRowsPerWarp; ++i) {
+      n[i] = (blockIdx.x % p.row_blocks) * 32 + warp * kRowsPerWarp + i;
+      y[i] = n[i] < p.N ? load_label(p.labels, b * p.lb + n[i] * p.ln, p.label_dtype) : p.ignore;
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) on[i] = n[i] < p.N && y[i] != p.ignore && y[i] >= 0 && y[i] < p.K;
+    if (p.copy) {
+      // the backward pass's copy of x (see head_rows_kernel), while the rows are at hand
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i) {
+        if (n[i] >= p.N) continue;
+        const uint16_t* src = static_cast<const uint16_t*>(p.x) + b * p.xs[0] + n[i] * p.xs[1];
+        uint16_t* dst = p.copy + (static_cast<int64_t>(b) * p.N + n[i]) * p.Dp;
+        for (int d = lane * 8; d < p.Dp; d += 256) {
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (y[i] != p.ignore) {
+            if (d + 8 <= p.D) {
+              u = *reinterpret_cast<const uint4*>(src + d);
+            } else {
+              uint16_t* v = reinterpret_cast<uint16_t*>(&u);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (d + k < p.D) v[k] = src[d + k];
+            }
           }
+          *reinterpret_cast<uint4*>(dst + d) = u;
         }
-        *reinterpret_cast<uint4*>(dst + d) = u;
       }
     }
-    float z = 0.0f;
-    if (y != p.ignore && y >= 0 && y < p.K) {
-      const int64_t xo = b * p.xs[0] + n * p.xs[1], co = b * p.cs[0] + y * p.cs[1];
-      if (p.dtype == FK_F32)
-        z = row_dot(static_cast<const float*>(p.x) + xo, p.xs[2], static_cast<const float*>(p.c) + co,
-                    p.cs[2], p.D, p.vec, lane);
-      else if (p.dtype == FK_F16)
-        z = row_dot(static_cast<const __half*>(p.x) + xo, p.xs[2], static_cast<const __half*>(p.c) + co,
-                    p.cs[2], p.D, p.vec, lane);
-      else
-        z = row_dot(static_cast<const __nv_bfloat16*>(p.x) + xo, p.xs[2],
-                    static_cast<const __nv_bfloat16*>(p.c) + co, p.cs[2], p.D, p.vec, lane);
-    }
-    if (lane == 0) z_label[i] = z;
+    if (p.dtype == FK_F32) row_dots<float>(p, b, n, y, on, lane, z);
+    else if (p.dtype == FK_F16) row_dots<__half>(p, b, n, y, on, lane, z);
+    else row_dots<__nv_bfloat16>(p, b, n, y, on, lane, z);
+    if (lane == 0)
+#pragma unroll
+      for (int i = 0; i < kRowsPerWarp; ++i) z_label[warp * kRowsPerWarp + i] = z[i];
   }
   __syncthreads();
   double sum = 0.0, cnt = 0.0;

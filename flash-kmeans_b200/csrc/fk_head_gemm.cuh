@@ -67,6 +67,12 @@ struct Problem {
   int group;                // row blocks that share a sweep over the columns
   int window;               // running epilogues: column tiles among which row blocks start apart
   uint32_t idesc;
+  // kEpiGrad, kEpiOut: only the rows that are not ignored take part, gathered;
+  // their number is known on the device alone
+  const int32_t* live;      // that number; null: all rows
+  int live_off, live_cap;   // this chunk's first row, its rows at most
+  int live_steps;           // the rows are the contraction, not the rows of A
+  const int32_t* row_map;   // kEpiOut: where gathered row live_off + r goes in the output
 
   // ---- epilogue
   float scale2;             // scale * log2(e)
@@ -214,41 +220,80 @@ struct Tile {
 // Every role walks the tiles by itself, in one thread: the decoding is kept to
 // 32-bit divisions, once per item (64-bit ones at every tile took 2000 cycles,
 // more than a short tile's products).
-template <int EPI>
+template <int EPI, int BM>
 struct Walk {
   static constexpr int NP = problems_of(EPI);
+  static constexpr bool kLive = EPI == kEpiGrad || EPI == kEpiOut;
   const Params<NP>& prm;
   uint32_t item, total;
   const uint32_t slot, slots;
   Tile t;
   int j_begin, j_end, w_end, wl, w0, j;
+  int m_tiles[NP], steps[NP];
+  int all, short_from, more, rest;
 
   __device__ Walk(const Params<NP>& q, int first, int stride) : prm(q), slot(first), slots(stride) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const Problem& p = prm.p[i];
+      m_tiles[i] = p.m_tiles;
+      steps[i] = p.kblocks;
+      if (kLive && p.live) {
+        const int rows = live_rows(p);
+        if (p.live_steps) steps[i] = (rows + 63) / 64;
+        else m_tiles[i] = (rows + BM - 1) / BM;
+      }
+    }
+    all = prm.all;
+    short_from = prm.short_from;
+    more = prm.more;
+    rest = prm.rest;
+    if constexpr (NP > 1) {
+      if (prm.count > 1 && prm.p[0].live) {
+        // the shares that the host worked out (fill) for the rows that are left
+        const uint32_t n0 = items_of(0), n1 = items_of(1);
+        const uint32_t c0 = steps[0] / prm.p[0].chunks + 3, c1 = steps[1] / prm.p[1].chunks + 3;
+        short_from = n0 % slots;
+        const uint32_t behind = slots - short_from, want = short_from ? c0 / c1 : 0;
+        const uint32_t got = min(want, n1 / behind), left = n1 - got * behind;
+        more = got;
+        all = got < want ? 0 : left / slots;
+        rest = left - all * slots;
+      }
+    }
     t.q = 0;
     item = slot;
-    total = items_of(prm.p[0]);
+    total = items_of(0);
     j = -1;
     if (NP > 1 && item >= total) second();
     decode();
   }
-  __device__ static uint32_t items_of(const Problem& p) {
-    return static_cast<uint32_t>(p.batches) * p.chunks * p.m_tiles * (running(EPI) ? 1 : p.n_tiles);
+  __device__ static int live_rows(const Problem& p) {
+    return min(max(*p.live - p.live_off, 0), p.live_cap);
+  }
+  // rows of A that count, and those of P that are written
+  __device__ static int rows_of(const Problem& p) {
+    return kLive && p.live && !p.live_steps ? live_rows(p) : p.M;
+  }
+  __device__ uint32_t items_of(int i) const {
+    const Problem& p = prm.p[i];
+    return static_cast<uint32_t>(p.batches) * p.chunks * m_tiles[i] * (running(EPI) ? 1 : p.n_tiles);
   }
   // this worker's next tile of the second problem
   __device__ void second() {
     t.q = NP - 1;
-    total = prm.count > 1 ? items_of(prm.p[NP - 1]) : 0;
+    total = prm.count > 1 ? items_of(NP - 1) : 0;
     ++j;
-    const uint32_t behind = prm.short_from, tail = slots - prm.rest;
-    if (j < prm.all) {
+    const uint32_t behind = short_from, tail = slots - rest;
+    if (j < all) {
       item = j * slots + slot;
       return;
     }
-    const int k = j - prm.all;
-    const int mine = slot >= behind ? prm.more : 0;
-    item = prm.all * slots;
+    const int k = j - all;
+    const int mine = slot >= behind ? more : 0;
+    item = all * slots;
     if (k < mine) item += k * (slots - behind) + slot - behind;
-    else if (k == mine && slot >= tail) item += prm.more * (slots - behind) + slot - tail;
+    else if (k == mine && slot >= tail) item += more * (slots - behind) + slot - tail;
     else item = total;
   }
   // Row blocks start at different tiles of a window, so that they do not all
@@ -262,7 +307,7 @@ struct Walk {
   __device__ void decode() {
     if (item >= total) return;
     const Problem& p = prm.p[NP > 1 ? t.q : 0];
-    const int steps = p.kblocks;
+    const int steps = this->steps[NP > 1 ? t.q : 0], m_tiles = this->m_tiles[NP > 1 ? t.q : 0];
     if constexpr (running(EPI)) {
       uint32_t r = item;
       uint32_t c = 0;
@@ -271,8 +316,8 @@ struct Walk {
         c = item - r * p.chunks;
       }
       t.chunk = c;
-      t.b = r / static_cast<uint32_t>(p.m_tiles);
-      t.m = r - t.b * p.m_tiles;
+      t.b = r / static_cast<uint32_t>(m_tiles);
+      t.m = r - t.b * m_tiles;
       j_begin = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * c / static_cast<uint32_t>(p.chunks));
       j_end = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * (c + 1) / static_cast<uint32_t>(p.chunks));
       t.it0 = 0;
@@ -282,7 +327,7 @@ struct Walk {
       window(j_begin);
       j = j_begin;
     } else {
-      const uint32_t per = static_cast<uint32_t>(p.m_tiles) * p.n_tiles;
+      const uint32_t per = static_cast<uint32_t>(m_tiles) * p.n_tiles;
       const uint32_t r = item / per;
       uint32_t i = item - r * per;
       t.b = r;
@@ -297,7 +342,7 @@ struct Walk {
       }
       const uint32_t g = i / static_cast<uint32_t>(p.group * p.n_tiles);
       const int g0 = g * p.group;
-      const uint32_t gl = min(p.group, p.m_tiles - g0);
+      const uint32_t gl = min(p.group, m_tiles - g0);
       i -= static_cast<uint32_t>(g0) * p.n_tiles;
       t.n = i / gl;
       t.m = g0 + i - t.n * gl;
@@ -452,7 +497,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const uint32_t bar0 = CG == 2 ? map_to_rank(full, 0) : full0;        // of the pair's first
       int stage = 0;
       uint32_t phase = 0;
-      Walk<EPI> walk(prm, first, stride);
+      Walk<EPI, S::kBM> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
@@ -526,7 +571,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const uint32_t smem0 = smem_u32(smem);
       int stage = 0, buf = 0;
       uint32_t phase = 0, aphase = 0;
-      Walk<EPI> walk(prm, first, stride);
+      Walk<EPI, S::kBM> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
@@ -609,7 +654,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     const uint32_t save = smem_u32(stg) + lane * 128 + (lane & 7) * 16;
     int buf = 0, tab = 0;
     uint32_t aphase = 0;
-    Walk<EPI> walk(prm, first, stride);
+    Walk<EPI, S::kBM> walk(prm, first, stride);
 
     // running state of a row
     float run_m = -INFINITY, run_s = 0.0f;
@@ -634,8 +679,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const int64_t row = nt.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       if constexpr (EPI == kEpiGrad) {
         st_next = {0.0f, 0.0f, 0.0f, -1};
-        if (row < p.M) {
-          const float4 f = *reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + p.stat_off + row);
+        if (row < Walk<EPI, S::kBM>::rows_of(p)) {
+          const float4 f = *reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + (p.row_map ? p.row_map[p.stat_off + row] : p.stat_off + row));
           st_next = {f.x, f.y, f.z, __float_as_int(f.w)};
         }
       }
@@ -657,7 +702,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const Problem& p = prm.p[NP > 1 ? t.q : 0];
       const int row = t.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       const int row0 = row - lane;
-      const bool row_ok = row < p.M;
+      const int rows = Walk<EPI, S::kBM>::rows_of(p);
+      const bool row_ok = row < rows;
       const int col0 = t.n * BN + part * kCols;
 
       if constexpr (EPI == kEpiLse) {
@@ -707,7 +753,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
 
       // four columns of an output row, rounded
       auto emit = [&](const int64_t grow, const int col, const float4 f) {
-        const int64_t o = t.b * p.out_sb + grow * p.out_sr + col;
+        const int64_t at = EPI == kEpiOut && p.row_map ? p.row_map[p.live_off + grow] : grow;
+        const int64_t o = t.b * p.out_sb + at * p.out_sr + col;
         if (p.out_vec && col + 4 <= p.N) {
           if (p.out_dtype == FK_F32) {
             *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = f;
@@ -794,6 +841,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           const uint32_t wr = smem_u32(stg) + lane * 64, wx = (lane >> 1) & 3;
           const uint32_t rd = smem_u32(stg) + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) * 16);
           const bool in = cc < p.p_ld;
+          // with gathered rows, zeros up to the next step of the contraction over them
+          const int rows_p = p.live ? min(p.M, (rows + 63) & ~63) : rows;
           auto put = [&](auto bf16, const int pp) {
             __syncwarp();
 #pragma unroll
@@ -815,7 +864,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint4 u = lds128(rd + i * 512);
-              if (in && row0 + i * 8 + (lane >> 2) < p.M) *reinterpret_cast<uint4*>(d + i * step8) = u;
+              if (in && row0 + i * 8 + (lane >> 2) < rows_p) *reinterpret_cast<uint4*>(d + i * step8) = u;
             }
           };
           if constexpr (EXACT) {
@@ -846,7 +895,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           for (int i = 0; i < 8; ++i) {
             const int rr = i * 4 + (lane >> 3);
             const int64_t grow = row0 + rr;
-            if (grow >= p.M || col >= p.N) continue;
+            if (grow >= rows || col >= p.N) continue;
             float4 f = *reinterpret_cast<const float4*>(stg + rr * 128 + ((q ^ (rr & 7)) * 16));
             if constexpr (EPI == kEpiScores) {
               float* ff = &f.x;
@@ -956,8 +1005,10 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           chunk(c, v);
         }
       } else {
-        got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
-                                                FK_DEV_WAIT_TIMEOUT));
+        // no gathered row in this split of them: nothing comes, nothing is added
+        const bool none = EPI == kEpiOut && t.it0 == t.it1;
+        got = none || __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
+                                                        FK_DEV_WAIT_TIMEOUT));
         if (!got) {
           if constexpr (EPI == kEpiArgmax) {
             // the warps of a row meet at its end: keep to that
@@ -980,9 +1031,15 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           uint32_t v[32];
-          tmem_ld32(taddr + c * 32, v);
-          tmem_ld_wait(v);
-          if (c + 1 == kChunks) {
+          if (none) {
+            keep_branch();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0;
+          } else {
+            tmem_ld32(taddr + c * 32, v);
+            tmem_ld_wait(v);
+          }
+          if (c + 1 == kChunks && !none) {
             // the accumulator is in registers: hand it back
             tc_fence_before();
             __syncwarp();
@@ -990,7 +1047,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           }
           chunk(c, v);
         }
-        if (++buf == S::kBufs) {
+        if (!none && ++buf == S::kBufs) {
           buf = 0;
           aphase ^= 1;
         }
@@ -1017,12 +1074,12 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             for (int r = 0; r < 32; r += 8 * kRows) {
               const int grow = row0 + r + lane / kQuads;
               const int col = col0 + lane % kQuads * 4;
-              if (grow >= p.M || col >= p.N) continue;
+              if (grow >= rows || col >= p.N) continue;
               // rows past the last one load it again: no branch between the loads
               const float* a = p.acc + t.b * p.acc_batch + col;
               int64_t at[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) at[i] = min(grow + i * kRows, p.M - 1) * p.acc_ld;
+              for (int i = 0; i < 8; ++i) at[i] = min(grow + i * kRows, rows - 1) * p.acc_ld;
               float4 f[8] = {};
               for (int k = 0; k < p.join_splits; ++k, a += p.acc_split) {
                 float4 o[8];
@@ -1038,7 +1095,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
               }
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                if (grow + i * kRows < p.M) emit(grow + i * kRows, col, f[i]);
+                if (grow + i * kRows < rows) emit(grow + i * kRows, col, f[i]);
             }
           }
         }

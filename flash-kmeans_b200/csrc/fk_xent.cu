@@ -75,6 +75,8 @@ struct RowsJob {        // one tensor to copy; units = 0 for none
   int N, D, Dp;
   int64_t units;        // of eight elements
   Labels y;             // p: ignored rows become zeros
+  const int32_t* map;   // gathered rows: row r of the copy is row map[r] of x
+  const int32_t* live;  // and there are this many, zeros up to the next 128 behind them
 };
 struct RowsJobs {
   RowsJob job[2];
@@ -90,9 +92,16 @@ __global__ void head_rows_kernel(const RowsJobs jobs) {
        u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t row = u / per;
     const int d0 = static_cast<int>(u - row * per) * 8;
-    const int64_t b = row / j.N, n = row - b * j.N;
+    int64_t b = row / j.N, n = row - b * j.N;
     T v[8];
-    const bool zero = j.y.p && load_label(j.y.p, b * j.y.sb + n * j.y.sn, j.y.dtype) == j.y.ignore;
+    bool zero = j.y.p && load_label(j.y.p, b * j.y.sb + n * j.y.sn, j.y.dtype) == j.y.ignore;
+    if (j.map) {
+      const int live = *j.live;
+      if (row >= (static_cast<int64_t>(live) + 127) / 128 * 128) break;
+      zero = row >= live;
+      b = 0;
+      n = zero ? 0 : j.map[row];
+    }
     const T* src = x + b * j.sb + n * j.sn;
     if (zero) {
 #pragma unroll
@@ -427,6 +436,64 @@ __global__ void xent_weight_kernel(const float* g, const RowStat* stat, int64_t 
   }
 }
 
+// ------------------------------------------------------------ rows that count
+// The rows that are not ignored, in order (map[r] is the r-th of them) and how
+// many there are; the gradients of the others are set to zero here.  A block
+// counts what lies before its segment by itself: segments are few, and reading
+// labels again is cheaper than a second launch.
+constexpr int kLiveThreads = 1024;
+
+__global__ void __launch_bounds__(kLiveThreads) xent_live_kernel(const Labels y, int64_t N, int64_t segment,
+                                                                 int32_t* map, int32_t* live, void* gx,
+                                                                 int64_t gx_row, int64_t gx_bytes, int gx_vec) {
+  __shared__ int sm[32];
+  __shared__ int base;
+  pdl_wait_then_release();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t first = blockIdx.x * segment, last = min(first + segment, N);
+  int before = 0;
+#pragma unroll 4
+  for (int64_t n = tid; n < first; n += kLiveThreads) before += load_label(y.p, n * y.sn, y.dtype) != y.ignore;
+  before = __reduce_add_sync(0xffffffffu, before);
+  if (lane == 0) sm[warp] = before;
+  __syncthreads();
+  if (tid == 0) {
+    int t = 0;
+    for (int w = 0; w < 32; ++w) t += sm[w];
+    base = t;
+  }
+  __syncthreads();
+  for (int64_t n0 = first; n0 < last; n0 += kLiveThreads) {
+    const int64_t n = n0 + tid;
+    const bool on = n < last && load_label(y.p, n * y.sn, y.dtype) != y.ignore;
+    const uint32_t votes = __ballot_sync(0xffffffffu, on);
+    if (lane == 0) sm[warp] = __popc(votes);
+    __syncthreads();
+    int at = base;
+    for (int w = 0; w < warp; ++w) at += sm[w];
+    if (on) map[at + __popc(votes & ((1u << lane) - 1))] = static_cast<int32_t>(n);
+    if (gx) {
+      for (uint32_t off = __ballot_sync(0xffffffffu, n < last && !on); off; off &= off - 1) {
+        uint8_t* row = static_cast<uint8_t*>(gx) + (n0 + warp * 32 + __ffs(off) - 1) * gx_row;
+        if (gx_vec) {
+          for (int64_t k = lane * 16; k < gx_bytes; k += 512)
+            *reinterpret_cast<uint4*>(row + k) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int64_t k = lane * 2; k < gx_bytes; k += 64) *reinterpret_cast<uint16_t*>(row + k) = 0;
+        }
+      }
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int t = base;
+      for (int w = 0; w < 32; ++w) t += sm[w];
+      base = t;
+    }
+    __syncthreads();
+  }
+  if (tid == 0 && last == N) *live = base;
+}
+
 // -------------------------------------------------------------------- plans
 struct Bump {  // workspace layout: the same walk sizes it and hands it out
   uint8_t* base;
@@ -511,9 +578,15 @@ static int check_workspace(const void* ws, size_t have, size_t need, const char*
   return FK_OK;
 }
 
+// Whether the backward pass leaves ignored rows out of its products.  Finding
+// them takes a launch and a gather (8 to 10 us at 16384 rows), which work of this
+// size, 0.1 ms or more, gets back where a tenth of the rows is ignored; separate
+// codebooks keep one block of rows for each batch, and go without.
+static bool gathers(const Xent& q) { return q.B == 1 && q.N >= 1024 && q.N * q.K >= (1ll << 34) / q.D; }
+
 // Copies of the operands made by the caller of a pass; see fk_xent_loss_grad.
 struct Copies {
-  uint16_t *x_forward, *x_backward, *c;   // null: used in place (x_forward, c)
+  uint16_t *x_forward, *x_backward, *c;   // null: used in place (x_forward, c), gathered later (x_backward)
 };
 
 struct ForwardPlan {
@@ -636,6 +709,7 @@ struct BackwardPlan {
   uint32_t *join_x, *join_c;   // arrival counters of split products
   int64_t joins;               // of both, from join_x on
   RowStat* weighted;
+  int32_t* map;                // gathered rows, their number behind it
   float* gmax;                 // (largest |g|, the factor it gives)
   size_t bytes;
 };
@@ -709,7 +783,7 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   plan_products(q, f.R, want_x ? steps_x : 0, kw, want_c ? steps_c : 0, &f);
   f.ld = ceil_div(q.D, 4) * 4;
   if (given) {
-    f.xc = given->x_backward;
+    f.xc = given->x_backward ? given->x_backward : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
     f.cc = given->c;
   } else {
     f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
@@ -717,6 +791,7 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
                ? nullptr
                : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
   }
+  f.map = gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
   f.P = b.take<uint16_t>(q.parts() * q.B * f.R * f.Kp);
   f.acc_x = f.acc_c = nullptr;
   if (want_x && (f.n_pieces > 1 || f.split_x > 1)) f.acc_x = b.take<float>(f.split_x * q.B * q.N * f.ld);
@@ -752,7 +827,8 @@ static int grad_problem(const Xent& q, Params<2>& prm, uint32_t* join, const Pro
   const int64_t steps = ceil_div(kdim, 64);
   p.chunks = static_cast<int>(std::min<int64_t>(splits, steps));
   const int eb = dtype_bytes(q.dtype);
-  p.out = static_cast<uint8_t*>(g.p) + out_row0 * g.sr * eb;
+  // gathered rows go where the map says, counted from the first row
+  p.out = static_cast<uint8_t*>(g.p) + (p.row_map ? 0 : out_row0 * g.sr * eb);
   p.out_dtype = q.dtype;
   p.out_sb = g.sb;
   p.out_sr = g.sr;
@@ -785,9 +861,24 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
   // ten bits above float16's smallest subnormal, and 1 * 2^14 is in range
   const float p_scale = f16 ? 16384.0f : 1.0f;
   int st = FK_OK;
-  if (!given)
-    st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), &q.y),
-                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  const int32_t* live = f.map ? f.map + q.N : nullptr;
+  if (f.map) {
+    // at most 128 segments, as a block reads every label before its own
+    const int64_t segment = ceil_div(ceil_div(q.N, 128), kLiveThreads) * kLiveThreads;
+    const int64_t eb = dtype_bytes(q.dtype);
+    const bool vec = reinterpret_cast<uintptr_t>(gx.p) % 16 == 0 && gx.sr * eb % 16 == 0 && q.D * eb % 16 == 0;
+    st = launch_plain("xent_live_kernel", xent_live_kernel, dim3(static_cast<unsigned>(ceil_div(q.N, segment))),
+                      kLiveThreads, s, q.y, q.N, segment, f.map, f.map + q.N, gx.p, gx.sr * eb, q.D * eb,
+                      vec ? 1 : 0);
+    if (st != FK_OK) return st;
+  }
+  if (!given || !given->x_backward) {
+    RowsJob xj = rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), f.map ? nullptr : &q.y);
+    xj.map = f.map;
+    xj.live = live;
+    st = rows_copy(q.dtype, xj,
+                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, given ? nullptr : f.cc, q.Dp(), nullptr), s);
+  }
   if (st != FK_OK) return st;
   const float* factor = q.reduction == 0 ? nullptr : g;
   if (q.reduction == 0) {
@@ -818,7 +909,11 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       p.N = static_cast<int>(kw);
       p.batches = static_cast<int>(q.B);
       p.chunks = 1;
-          p.status = status;
+      p.status = status;
+      p.live = live;
+      p.live_off = static_cast<int>(r0);
+      p.live_cap = static_cast<int>(rw);
+      p.row_map = f.map;
       p.scale2 = q.scale * 1.44269504f;
       p.stat = stat;
       p.stat_rows = q.N;
@@ -857,9 +952,14 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       base.fscale = q.scale / p_scale;
       base.f_num = factor;
       base.f_den = q.reduction == 1 ? count : nullptr;
+      base.live = live;
+      base.live_off = static_cast<int>(r0);
+      base.live_cap = static_cast<int>(rw);
       Params<2> pair = {};
       auto add_x = [&]() {
         const Operand co = operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, true, k0);
+        base.live_steps = 0;
+        base.row_map = f.map;
         return grad_problem(q, pair, f.join_x, base, po, co, rw, kw, f.sh, f.split_x, f.acc_x, q.N, r0, f.ld,
                             piece == 0, piece + 1 == f.n_pieces, gx, r0);
       };
@@ -867,6 +967,8 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
         Operand pt = po;
         pt.mn = true;
         const Operand xo = operand(q, q.x, f.xc, q.B, q.N, q.xs, true, r0);
+        base.live_steps = 1;
+        base.row_map = nullptr;
         return grad_problem(q, pair, f.join_c, base, pt, xo, kw, rw, f.sh, f.split_c, f.acc_c, f.Kp, 0, f.ld,
                             chunk == 0, chunk + 1 == f.n_chunks, gc, k0);
       };
@@ -896,11 +998,13 @@ struct LossGradPlan {
 static LossGradPlan plan_loss_grad(const Xent& q, bool want_x, bool want_c, void* ws) {
   LossGradPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
-  f.copies.x_backward = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+  const bool in = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs);
+  uint16_t* copy = !in || !gathers(q) ? b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp()) : nullptr;
+  f.copies.x_backward = gathers(q) ? nullptr : copy;
   f.copies.c = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
                    ? nullptr
                    : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
-  f.copies.x_forward = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs) ? nullptr : f.copies.x_backward;
+  f.copies.x_forward = in ? nullptr : copy;
   f.stat = b.take<RowStat>(q.B * q.N);
   f.count = b.take<int32_t>(1);
   f.rest = b.base ? b.base + b.used : nullptr;

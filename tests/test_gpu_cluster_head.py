@@ -241,6 +241,50 @@ def test_several_pieces_and_row_chunks(dtype):
         close(got, w, what)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("live", ["all", "most", "few", "first", "last", "one chunk", "none"])
+def test_only_the_rows_that_count_are_multiplied(live, dtype):
+    """Work large enough that the backward pass gathers the rows that are not
+    ignored, in two chunks of rows, with float rows that ignored ones would spoil."""
+    N, K, D = 20000, 9000, 104
+    x, c, y = make(0, N, K, D, dtype, seed=26, ids=torch.int64)
+    g = torch.Generator(device="cuda").manual_seed(27)
+    keep = torch.ones(N, dtype=torch.bool, device="cuda")
+    if live == "most":
+        keep = torch.rand(N, device="cuda", generator=g) < 0.8
+    elif live != "all":
+        keep[:] = False
+        if live == "few":
+            keep[torch.randint(0, N, (37,), device="cuda", generator=g)] = True
+        elif live == "first":
+            keep[0] = True
+        elif live == "last":
+            keep[-1] = True
+        elif live == "one chunk":
+            keep[: 16384 // 2] = True      # as many as a chunk of rows holds, less than two
+    y = torch.where(keep, y, torch.full_like(y, -100))
+    dirty = x.clone()
+    dirty[~keep] = float("nan")
+    loss, gx, gc = fk.cluster_cross_entropy_grad(dirty, c, y, scale=4.0)
+    if live == "none":
+        assert torch.isnan(loss) and gx.eq(0).all() and gc.eq(0).all()
+        return
+    for got, w, what in zip((loss, gx, gc), reference(x, c, y, 4.0, "mean"), ("loss", "gx", "gc")):
+        close(got, w, what)
+    assert gx[~keep].eq(0).all()
+    # the same through autograd, one gradient at a time, and a gradient per row
+    xr, cr = dirty.clone().requires_grad_(), c.clone().requires_grad_()
+    fk.cluster_cross_entropy(xr, cr, y, scale=4.0).backward()
+    assert torch.equal(xr.grad, gx) and torch.equal(cr.grad, gc)
+    cr = c.clone().requires_grad_()
+    fk.cluster_cross_entropy(dirty, cr, y, scale=4.0).backward()
+    close(cr.grad, reference(x, c, y, 4.0, "mean")[2], "gc alone")   # (split into other sums)
+    up = torch.rand(N, device="cuda", generator=g)
+    got = fk.cluster_cross_entropy_grad(dirty, c, y, scale=4.0, reduction="none", grad_loss=up)
+    for a, w, what in zip(got, reference(x, c, y, 4.0, "none", g=up), ("rows", "gx", "gc")):
+        close(a, w, what)
+
+
 def test_few_rows_many_centroids_split_the_sums():
     """A short product over a long axis is split and joined."""
     for dtype in (BF, FP):

@@ -579,10 +579,11 @@ static int check_workspace(const void* ws, size_t have, size_t need, const char*
 }
 
 // Whether the backward pass leaves ignored rows out of its products.  Finding
-// them takes a launch and a gather (8 to 10 us at 16384 rows), which work of this
-// size, 0.1 ms or more, gets back where a tenth of the rows is ignored; separate
-// codebooks keep one block of rows for each batch, and go without.
-static bool gathers(const Xent& q) { return q.B == 1 && q.N >= 1024 && q.N * q.K >= (1ll << 34) / q.D; }
+// and gathering them takes 20 to 30 us at 16384 rows (25 of 470 us were lost at
+// 32444 x 8192 x 128 with none ignored); from 2^36 products on, 0.4 ms, that is
+// what a twentieth of ignored rows gives back.  Separate codebooks keep one
+// block of rows for each batch, and go without.
+static bool gathers(const Xent& q) { return q.B == 1 && q.N >= 1024 && q.N * q.K >= (1ll << 36) / q.D; }
 
 // Copies of the operands made by the caller of a pass; see fk_xent_loss_grad.
 struct Copies {

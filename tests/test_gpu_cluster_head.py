@@ -246,7 +246,7 @@ def test_several_pieces_and_row_chunks(dtype):
 def test_only_the_rows_that_count_are_multiplied(live, dtype):
     """Work large enough that the backward pass gathers the rows that are not
     ignored, in two chunks of rows, with float rows that ignored ones would spoil."""
-    N, K, D = 20000, 9000, 104
+    N, K, D = 20000, 9000, 392
     x, c, y = make(0, N, K, D, dtype, seed=26, ids=torch.int64)
     g = torch.Generator(device="cuda").manual_seed(27)
     keep = torch.ones(N, dtype=torch.bool, device="cuda")

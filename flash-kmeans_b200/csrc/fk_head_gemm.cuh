@@ -31,8 +31,8 @@ namespace head {
 
 constexpr int kCtlWarps = 4;
 constexpr int kStageRowBytes = 128;            // one swizzle row: 64 16-bit or 128 8-bit elements
-constexpr int kTableFloats = 2 * 64;           // column scales and biases of an epilogue warp
-constexpr int kSlotBytes = 3 * 128 * 8;        // (value, index) of a row from the other column parts
+constexpr int kTableFloats = 2 * 64;           // column scales and biases of an argmax warp
+constexpr int kSlotBytes = 2 * 128 * 8;        // (value, index) of two rows from the other column part
 
 enum Epilogue {
   kEpiLse = 0,     // running maximum and sum of exp2 over the columns
@@ -116,6 +116,9 @@ struct Problem {
 // finish together.  In the second product every worker has `all` tiles, the
 // workers from `short_from` on (one tile of the first product behind) `more`
 // others, and the last `rest` workers one more.
+// Row blocks that share a pass over the columns (an item is so many blocks):
+// two where four accumulators allow for it.
+__host__ __device__ constexpr int subs_of(int epi, int bn) { return epi == kEpiArgmax && bn <= 128 ? 2 : 1; }
 constexpr int problems_of(int epi) { return epi == kEpiOut ? 2 : 1; }
 
 template <int NP>
@@ -139,11 +142,13 @@ struct Shape {
   // Epilogue warps: four TMEM lane quarters x column parts.  Four parts give
   // each scheduler four warps, which is what hides the exponentials' and the
   // accumulator loads' latency (two left 70 % of the issue slots empty).
-  static constexpr int kParts = BN >= 128 ? 4 : 2;
+  // The argmax holds two rows a thread instead: two parts.
+  static constexpr int kParts = BN >= 128 && EPI != kEpiArgmax ? 4 : 2;
   static constexpr int kEpiWarps = 4 * kParts;
   static constexpr int kThreads = (kCtlWarps + kEpiWarps) * 32;
-  // shared memory of an epilogue warp: 32 rows of 128 bytes (64 for P)
-  static constexpr int kStaging = (EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : 4096);
+  // shared memory of an epilogue warp: 32 rows of 128 bytes (64 for P, 64 rows for the argmax)
+  static constexpr int kStaging =
+      EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : EPI == kEpiArgmax ? 8192 : 4096;
   static constexpr int kStagingBytes = kEpiWarps * kStaging;
   static constexpr int kExtra = EPI == kEpiArgmax ? kEpiWarps * 2 * kTableFloats * 4 + kSlotBytes : 0;
   static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes - kExtra;
@@ -158,7 +163,7 @@ struct Shape {
 template <int CG, int BN, int EPI, bool EXACT>
 constexpr int threads_of() { return Shape<CG, BN, EPI, EXACT>::kThreads; }
 // column parts that write partial results of a row
-inline int parts_of(int bn) { return bn >= 128 ? 4 : 2; }
+inline int parts_of(int epi, int bn) { return bn >= 128 && epi != kEpiArgmax ? 4 : 2; }
 
 // ------------------------------------------------------------------ helpers
 __device__ __forceinline__ float ex2(float v) {
@@ -170,6 +175,9 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) { return fmaxf
 
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void sts32(uint32_t at, uint32_t a) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(a) : "memory");
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
   uint4 u;
@@ -212,7 +220,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // (batch, row block, chunk) item in turn; the others one tile per item.
 struct Tile {
   int q;               // which problem
-  int b, m, n, chunk;
+  int b, m, n, chunk;  // m: row block, of subs_of() of an item
+  int sub;
   int it0, it1;        // steps of the contraction
   bool first, last;    // of the item
 };
@@ -220,7 +229,7 @@ struct Tile {
 // Every role walks the tiles by itself, in one thread: the decoding is kept to
 // 32-bit divisions, once per item (64-bit ones at every tile took 2000 cycles,
 // more than a short tile's products).
-template <int EPI, int BM>
+template <int EPI, int BM, int SUBS>
 struct Walk {
   static constexpr int NP = problems_of(EPI);
   static constexpr bool kLive = EPI == kEpiGrad || EPI == kEpiOut;
@@ -228,7 +237,7 @@ struct Walk {
   uint32_t item, total;
   const uint32_t slot, slots;
   Tile t;
-  int j_begin, j_end, w_end, wl, w0, j;
+  int j_begin, j_end, w_end, wl, w0, j, m0, subs;
   int m_tiles[NP], steps[NP];
   int all, short_from, more, rest;
 
@@ -302,7 +311,7 @@ struct Walk {
     w0 = from;
     wl = min(prm.p[0].window, j_end - from);
     w_end = from + wl;
-    t.n = w0 + static_cast<int>(static_cast<uint32_t>(t.m) % static_cast<uint32_t>(wl));
+    t.n = w0 + static_cast<int>(static_cast<uint32_t>(m0) % static_cast<uint32_t>(wl));
   }
   __device__ void decode() {
     if (item >= total) return;
@@ -317,7 +326,10 @@ struct Walk {
       }
       t.chunk = c;
       t.b = r / static_cast<uint32_t>(m_tiles);
-      t.m = r - t.b * m_tiles;
+      m0 = r - t.b * m_tiles;
+      t.sub = 0;
+      t.m = m0 * SUBS;
+      subs = SUBS > 1 && (t.m + 1) * BM < p.M ? 2 : 1;
       j_begin = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * c / static_cast<uint32_t>(p.chunks));
       j_end = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * (c + 1) / static_cast<uint32_t>(p.chunks));
       t.it0 = 0;
@@ -355,6 +367,14 @@ struct Walk {
   }
   __device__ void next() {
     if constexpr (running(EPI)) {
+      if (SUBS > 1) {
+        if (++t.sub < subs) {
+          ++t.m;
+          return;
+        }
+        t.sub = 0;
+        t.m = m0 * SUBS;
+      }
       if (++j < j_end) {
         t.first = false;
         t.last = j + 1 == j_end;
@@ -411,6 +431,206 @@ __device__ __forceinline__ void keep_branch() { asm volatile(""); }
 template <int THREADS>
 __device__ __forceinline__ void quarter_sync(int quarter) {
   asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(THREADS) : "memory");
+}
+
+// ------------------------------------------------------------------- kernel
+// Epilogue of the argmax.  Every score takes its column's scale and bias from
+// shared memory, 16 bytes to each of 32 lanes at a time, which the load path
+// delivers at a quarter of that; with one row a thread it was busy 72 % of the
+// time.  So a thread takes its row of two row blocks, and each scale and bias
+// serves two scores.  A row keeps its best score and the 32 scores of the chunk
+// that it came from, in shared memory; which column of it won is looked up once,
+// at the end of the row.
+template <int CG, int BN>
+__device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* staging, uint32_t tmem,
+                                                uint64_t* acc_full, uint64_t* acc_empty,
+                                                volatile int* abort_flag, int ew, int lane, uint32_t rank,
+                                                int first, int stride) {
+  using S = Shape<CG, BN, kEpiArgmax, false>;
+  const Problem& p = prm.p[0];
+  constexpr int kCols = BN / S::kParts;      // columns of this warp
+  constexpr int kChunks = kCols / 32;
+  const int part = ew >> 2, quarter = ew & 3;
+  const uint32_t save = smem_u32(staging + ew * S::kStaging) + lane * 128 + (lane & 7) * 16;
+  const uint32_t tables = smem_u32(staging + S::kStagingBytes) + ew * (2 * kTableFloats * 4);
+  float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + S::kEpiWarps * 2 * kTableFloats * 4) +
+                 quarter * 32 + lane;
+  int buf = 0, tab = 0;
+  uint32_t aphase = 0;
+  constexpr int U = subs_of(kEpiArgmax, BN);   // rows of a thread
+  Walk<kEpiArgmax, S::kBM, U> walk(prm, first, stride);
+  Tile t;
+  bool more = walk.get(t);
+
+  float run_m[U], xs[U], xs_next[U] = {}, sc_next[kChunks], bi_next[kChunks];
+  int run_i[U];
+  // The next tile's columns, and at an item's start its rows' scales: fetched a
+  // tile ahead, as their latency would stand between the accumulator and its use.
+  auto fetch = [&](const Tile& a, int subs) {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int64_t col = a.n * BN + part * kCols + c * 32 + lane;
+      sc_next[c] = col < p.N ? p.b_scale[a.b * p.bs_sb + col * p.bs_sn] : 0.0f;
+      bi_next[c] = col < p.N && p.bias ? p.bias[a.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+    }
+    if (a.first)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = (a.m + u) * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+        xs_next[u] = u < subs && row < p.M ? p.a_scale[a.b * p.as_sb + row * p.as_sn] : 0.0f;
+      }
+  };
+  if (more) fetch(t, walk.subs);
+  while (more) {
+    // a tile of each row block of the item
+    const Tile now = t;
+    const int subs = walk.subs;
+    for (int u = 0; u < subs; ++u) walk.next();
+    more = walk.get(t);
+    const int row = now.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+    if (now.first)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        run_m[u] = -INFINITY;
+        run_i[u] = INT_MAX;
+        xs[u] = xs_next[u];
+      }
+    const uint32_t table = tables + tab * (kTableFloats * 4);
+    tab ^= 1;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      sts32(table + (c * 32 + lane) * 4, __float_as_uint(sc_next[c]));
+      sts32(table + (64 + c * 32 + lane) * 4, __float_as_uint(bi_next[c]));
+    }
+    __syncwarp();
+    if (more) fetch(t, walk.subs);
+
+    const int buf0 = buf;
+    bool got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
+    if (++buf == S::kBufs) {
+      buf = 0;
+      aphase ^= 1;
+    }
+    const int buf1 = subs > 1 ? buf : buf0;
+    if (subs > 1) {
+      got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT) && got;
+      if (++buf == S::kBufs) {
+        buf = 0;
+        aphase ^= 1;
+      }
+    }
+    if (__all_sync(0xffffffffu, got)) {
+      tc_fence_after();
+      const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int at = part * kCols + c * 32, cc = now.n * BN + at, left = p.N - cc;
+        uint32_t v[U][32];
+        tmem_ld32(tmem + buf0 * BN + at + lanes, v[0]);
+        if constexpr (U > 1) tmem_ld32(tmem + buf1 * BN + at + lanes, v[U - 1]);   // (the same again for one block)
+#pragma unroll
+        for (int u = 0; u < U; ++u) tmem_ld_wait(v[u]);
+        if (c + 1 == kChunks) {
+          // the accumulators are in registers: hand them back
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_cg<CG>(&acc_empty[buf0]);
+            if (subs > 1) mbar_arrive_cg<CG>(&acc_empty[buf1]);
+          }
+        }
+        if (left <= 0) continue;
+#pragma unroll
+        for (int u = 0; u < U; ++u) acc_to_f(v[u]);
+        float z[U][32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          // without a bias the table holds zeros: no branch for every column
+          const uint4 s4 = lds128(table + (c * 32 + i) * 4), b4 = lds128(table + (64 + c * 32 + i) * 4);
+          const uint64_t sa = pack2(__uint_as_float(s4.x), __uint_as_float(s4.y));
+          const uint64_t sb = pack2(__uint_as_float(s4.z), __uint_as_float(s4.w));
+          const uint64_t ba = pack2(__uint_as_float(b4.x), __uint_as_float(b4.y));
+          const uint64_t bb = pack2(__uint_as_float(b4.z), __uint_as_float(b4.w));
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const uint64_t x2 = pack2(xs[u], xs[u]);
+            unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[u][i]), __uint_as_float(v[u][i + 1])), x2), sa), ba),
+                    z[u][i], z[u][i + 1]);
+            unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[u][i + 2]), __uint_as_float(v[u][i + 3])), x2), sb), bb),
+                    z[u][i + 2], z[u][i + 3]);
+          }
+        }
+        if (left < 32) {
+          keep_branch();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i >= left) z[0][i] = z[U - 1][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float mx[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            mx[q] = max_nan3(z[u][q], z[u][q + 4], z[u][q + 8]);
+            mx[q] = max_nan3(mx[q], z[u][q + 12], z[u][q + 16]);
+            mx[q] = max_nan(max_nan3(mx[q], z[u][q + 20], z[u][q + 24]), z[u][q + 28]);
+          }
+          const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
+          if (!(m < run_m[u]) && argmax_better(m, cc, run_m[u], run_i[u])) {
+            run_m[u] = m;
+            run_i[u] = cc;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              sts128((save + u * 4096) ^ (q * 16), __float_as_uint(z[u][q * 4]), __float_as_uint(z[u][q * 4 + 1]),
+                     __float_as_uint(z[u][q * 4 + 2]), __float_as_uint(z[u][q * 4 + 3]));
+          }
+        }
+      }
+    }
+    if (!now.last) continue;
+
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (run_i[u] == INT_MAX) continue;
+      int at = 0;
+#pragma unroll
+      for (int q = 7; q >= 0; --q) {
+        const uint4 f = lds128((save + u * 4096) ^ (q * 16));
+        const uint32_t* fu = &f.x;
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+          const float g = __uint_as_float(fu[i]);
+          if (g == run_m[u] || g != g) at = q * 4 + i;
+        }
+      }
+      run_i[u] += at;
+    }
+    if (p.chunks == 1) {
+      // the column parts of a row meet in shared memory
+      if (part == 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u) slot[u * 128] = make_float2(run_m[u], __int_as_float(run_i[u]));
+      quarter_sync<S::kParts * 32>(quarter);
+      if (part == 0)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float2 o = slot[u * 128];
+          if (argmax_better(o.x, __float_as_int(o.y), run_m[u], run_i[u])) run_i[u] = __float_as_int(o.y);
+          const int r = row + u * S::kBM;
+          if (u < subs && r < p.M) p.label_out[now.b * p.lo_sb + r * p.lo_sn] = run_i[u];
+        }
+      // the slots are read before the next rows write them
+      quarter_sync<S::kParts * 32>(quarter);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = row + u * S::kBM;
+        if (u < subs && r < p.M)
+          p.partial[((static_cast<int64_t>(now.b) * p.chunks + now.chunk) * S::kParts + part) * p.M + r] =
+              make_float2(run_m[u], __int_as_float(run_i[u]));
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------- kernel
@@ -497,7 +717,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const uint32_t bar0 = CG == 2 ? map_to_rank(full, 0) : full0;        // of the pair's first
       int stage = 0;
       uint32_t phase = 0;
-      Walk<EPI, S::kBM> walk(prm, first, stride);
+      Walk<EPI, S::kBM, subs_of(EPI, BN)> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
@@ -571,7 +791,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const uint32_t smem0 = smem_u32(smem);
       int stage = 0, buf = 0;
       uint32_t phase = 0, aphase = 0;
-      Walk<EPI, S::kBM> walk(prm, first, stride);
+      Walk<EPI, S::kBM, subs_of(EPI, BN)> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
@@ -642,6 +862,10 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         }
       }
     }
+  } else if (EPI == kEpiArgmax && warp >= kCtlWarps) {
+    if constexpr (EPI == kEpiArgmax)
+      argmax_epilogue<CG, BN>(prm, staging, tmem, acc_full, acc_empty, abort_flag, warp - kCtlWarps, lane, rank,
+                              first, stride);
   } else if (warp >= kCtlWarps) {
     // ------------------------------------------------------------ epilogue
     const int ew = warp - kCtlWarps;
@@ -650,15 +874,12 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     constexpr int kCols = BN / S::kParts;  // columns of this warp
     constexpr int kChunks = kCols / 32;
     uint8_t* stg = staging + ew * S::kStaging;
-    // kEpiArgmax: this lane's 128 bytes, 16-byte groups in swizzled order
-    const uint32_t save = smem_u32(stg) + lane * 128 + (lane & 7) * 16;
-    int buf = 0, tab = 0;
+    int buf = 0;
     uint32_t aphase = 0;
-    Walk<EPI, S::kBM> walk(prm, first, stride);
+    Walk<EPI, S::kBM, subs_of(EPI, BN)> walk(prm, first, stride);
 
     // running state of a row
     float run_m = -INFINITY, run_s = 0.0f;
-    int run_i = 0;
     int label = -1;
     float xs = 0.0f;
     float fac = 0.0f;
@@ -673,26 +894,18 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     Tile t, nt;
     bool more = walk.get(nt);
     RowStat st_next = {0.0f, 0.0f, 0.0f, -1};
-    float xs_next = 0.0f, sc_next[kChunks] = {}, bi_next[kChunks] = {};
+    float xs_next = 0.0f;
     auto fetch = [&]() {
       const Problem& p = p0;
       const int64_t row = nt.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       if constexpr (EPI == kEpiGrad) {
         st_next = {0.0f, 0.0f, 0.0f, -1};
-        if (row < Walk<EPI, S::kBM>::rows_of(p)) {
+        if (row < Walk<EPI, S::kBM, subs_of(EPI, BN)>::rows_of(p)) {
           const float4 f = *reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + (p.row_map ? p.row_map[p.stat_off + row] : p.stat_off + row));
           st_next = {f.x, f.y, f.z, __float_as_int(f.w)};
         }
       }
       if constexpr (integer(EPI)) xs_next = row < p.M ? p.a_scale[nt.b * p.as_sb + row * p.as_sn] : 0.0f;
-      if constexpr (EPI == kEpiArgmax) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const int64_t col = nt.n * BN + part * kCols + c * 32 + lane;
-          sc_next[c] = col < p.N ? p.b_scale[nt.b * p.bs_sb + col * p.bs_sn] : 0.0f;
-          bi_next[c] = col < p.N && p.bias ? p.bias[nt.b * p.bias_sb + col * p.bias_sn] : 0.0f;
-        }
-      }
     };
     if (more) fetch();
     while (more) {
@@ -702,7 +915,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const Problem& p = prm.p[NP > 1 ? t.q : 0];
       const int row = t.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       const int row0 = row - lane;
-      const int rows = Walk<EPI, S::kBM>::rows_of(p);
+      const int rows = Walk<EPI, S::kBM, subs_of(EPI, BN)>::rows_of(p);
       const bool row_ok = row < rows;
       const int col0 = t.n * BN + part * kCols;
 
@@ -721,22 +934,6 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       st.coef *= p.p_scale;
       st.at_label *= p.p_scale;
       xs = xs_next;
-      float* table = reinterpret_cast<float*>(staging + S::kStagingBytes) + ew * 2 * kTableFloats;
-      if constexpr (EPI == kEpiArgmax) {
-        if (t.first) {
-          run_m = -INFINITY;
-          run_i = INT_MAX;
-        }
-        // this tile's column scales and biases, two tables of the warp in turn
-        table += tab * kTableFloats;
-        tab ^= 1;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          table[c * 32 + lane] = sc_next[c];
-          table[64 + c * 32 + lane] = bi_next[c];
-        }
-        __syncwarp();
-      }
       if (more) fetch();
       // this lane's columns of every chunk
       float sc[kChunks][4], bi[kChunks][4];
@@ -917,49 +1114,6 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             }
             emit(grow, col, f);
           }
-        } else {  // kEpiArgmax
-          const float* tsc = table + c * 32;
-          const float* tbi = tsc + 64;
-          acc_to_f(v);
-          const uint64_t x2 = pack2(xs, xs);
-          float z[32];
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 s4 = *reinterpret_cast<const float4*>(tsc + i);
-            uint64_t z0 = mul2(mul2(pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), x2), pack2(s4.x, s4.y));
-            uint64_t z1 = mul2(mul2(pack2(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), x2), pack2(s4.z, s4.w));
-            // without a bias the table holds zeros: no branch for every column
-            const float4 b4 = *reinterpret_cast<const float4*>(tbi + i);
-            z0 = add2(z0, pack2(b4.x, b4.y));
-            z1 = add2(z1, pack2(b4.z, b4.w));
-            unpack2(z0, z[i], z[i + 1]);
-            unpack2(z1, z[i + 2], z[i + 3]);
-          }
-          const int left = p.N - cc;
-          if (left < 32) {
-            keep_branch();
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i >= left) z[i] = -INFINITY;
-          }
-          float mx[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            mx[q] = max_nan3(z[q], z[q + 4], z[q + 8]);
-            mx[q] = max_nan3(mx[q], z[q + 12], z[q + 16]);
-            mx[q] = max_nan(max_nan3(mx[q], z[q + 20], z[q + 24]), z[q + 28]);
-          }
-          const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
-          if (left > 0 && argmax_better(m, cc, run_m, run_i)) {
-            // keep the chunk: which of its columns won is looked up once, at
-            // the end of the row, instead of at every improvement
-            run_m = m;
-            run_i = cc;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              sts128(save ^ (q * 16), __float_as_uint(z[q * 4]), __float_as_uint(z[q * 4 + 1]),
-                     __float_as_uint(z[q * 4 + 2]), __float_as_uint(z[q * 4 + 3]));
-          }
         }
       };
 
@@ -1009,22 +1163,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         const bool none = EPI == kEpiOut && t.it0 == t.it1;
         got = none || __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
                                                         FK_DEV_WAIT_TIMEOUT));
-        if (!got) {
-          if constexpr (EPI == kEpiArgmax) {
-            // the warps of a row meet at its end: keep to that
-            if (t.last && p.chunks == 1) {
-              quarter_sync<S::kParts * 32>(quarter);
-              quarter_sync<S::kParts * 32>(quarter);
-            }
-            if (++buf == S::kBufs) {
-              buf = 0;
-              aphase ^= 1;
-            }
-            continue;
-          } else {
-            break;
-          }
-        }
+        if (!got) break;
         tc_fence_after();
         const uint32_t taddr =
             tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -1104,48 +1243,6 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         if (t.last && row_ok)
           p.partial[((static_cast<int64_t>(t.b) * p.chunks + t.chunk) * S::kParts + part) * p.M + row] =
               make_float2(run_m, run_s);
-      }
-      if constexpr (EPI == kEpiArgmax) {
-        if (t.last) {
-          if (run_i != INT_MAX) {
-            int at = 0;
-#pragma unroll
-            for (int q = 7; q >= 0; --q) {
-              const uint4 f = lds128(save ^ (q * 16));
-              const uint32_t* fu = &f.x;
-#pragma unroll
-              for (int i = 3; i >= 0; --i) {
-                const float g = __uint_as_float(fu[i]);
-                if (g == run_m || g != g) at = q * 4 + i;
-              }
-            }
-            run_i += at;
-          }
-          if (p.chunks == 1) {
-            // the column parts of a row meet in shared memory
-            float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes +
-                                                      S::kEpiWarps * 2 * kTableFloats * 4) +
-                           (quarter * 32 + lane);
-            if (part > 0) slot[(part - 1) * 128] = make_float2(run_m, __int_as_float(run_i));
-            quarter_sync<S::kParts * 32>(quarter);
-            if (part == 0 && row_ok) {
-#pragma unroll
-              for (int o = 0; o < S::kParts - 1; ++o) {
-                const float2 v = slot[o * 128];
-                if (argmax_better(v.x, __float_as_int(v.y), run_m, run_i)) {
-                  run_m = v.x;
-                  run_i = __float_as_int(v.y);
-                }
-              }
-              p.label_out[t.b * p.lo_sb + row * p.lo_sn] = run_i;
-            }
-            // the slots are read before the next row block writes them
-            quarter_sync<S::kParts * 32>(quarter);
-          } else if (row_ok) {
-            p.partial[((static_cast<int64_t>(t.b) * p.chunks + t.chunk) * S::kParts + part) * p.M + row] =
-                make_float2(run_m, __int_as_float(run_i));
-          }
-        }
       }
     }
   }

@@ -328,14 +328,18 @@ static ScoresPlan plan_scores(const Scores& q, bool argmax, void* ws) {
     return p;
   };
   f.sh = choose_shape(q.N, q.K, q.B, false);
-  f.chunks = argmax ? choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
+  // Up to 512 features the argmax's scores outweigh the products, and two row
+  // blocks share each column's scale (256 x 128 tiles); beyond, the wider tile's
+  // fewer bytes count (assign of 65537 x 500 x 1024: 80 us against 94).
+  if (argmax && f.sh.bn == 256 && q.D <= 512) f.sh.bn = 128;
+  f.chunks = argmax ? choose_chunks(q.B * ceil_div(q.N, subs_of(kEpiArgmax, f.sh.bn) * f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                                     2 * slots_of(f.sh), 0.25)
                     : 1;
   if (q.x_dtype != FK_I8 || !in_place8(q.x, q.B, q.N, q.D, q.xs))
     f.xq = static_cast<int8_t*>(take(q.B * q.N * q.Dp()));
   if (q.x_dtype != FK_I8) f.sx = static_cast<float*>(take(q.B * q.N * 4));
   if (!in_place8(q.c, q.Bc(), q.K, q.D, q.cs)) f.cq = static_cast<int8_t*>(take(q.Bc() * q.K * q.Dp()));
-  if (f.chunks > 1) f.partial = static_cast<float2*>(take(q.B * f.chunks * parts_of(f.sh.bn) * q.N * 8));
+  if (f.chunks > 1) f.partial = static_cast<float2*>(take(q.B * f.chunks * parts_of(kEpiArgmax, f.sh.bn) * q.N * 8));
   f.bytes = used;
   return f;
 }
@@ -413,7 +417,7 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   if (st != FK_OK || !f.partial) return st;
   const int64_t row_blocks = ceil_div(q.N, 32);
   return launch_plain("argmax_join_kernel", argmax_join_kernel, dim3(static_cast<unsigned>(q.B * row_blocks)),
-                      kJoinWarps * 32, s, f.partial, f.chunks * parts_of(f.sh.bn), static_cast<int>(q.N),
+                      kJoinWarps * 32, s, f.partial, f.chunks * parts_of(kEpiArgmax, f.sh.bn), static_cast<int>(q.N),
                       static_cast<int>(row_blocks), label_out, ls[0], ls[1]);
 }
 

@@ -619,7 +619,7 @@ static ForwardPlan plan_forward(const Xent& q, void* ws, const Copies* given = n
                ? nullptr
                : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
   }
-  f.partial = b.take<float2>(q.B * f.chunks * parts_of(f.sh.bn) * q.N);
+  f.partial = b.take<float2>(q.B * f.chunks * parts_of(kEpiLse, f.sh.bn) * q.N);
   f.block_part = b.take<double2>(q.B * f.row_blocks);
   f.ticket = b.take<uint32_t>(1);
   f.bytes = b.used;
@@ -681,7 +681,7 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   cp.ignore = q.y.ignore;
   cp.K = q.K;
   cp.N = static_cast<int>(q.N);
-  cp.pieces = f.chunks * parts_of(f.sh.bn);
+  cp.pieces = f.chunks * parts_of(kEpiLse, f.sh.bn);
   cp.batches = static_cast<int>(q.B);
   cp.row_blocks = static_cast<int>(f.row_blocks);
   cp.reduction = q.reduction;

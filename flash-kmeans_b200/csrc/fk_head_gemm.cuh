@@ -67,12 +67,12 @@ struct Problem {
   int group;                // row blocks that share a sweep over the columns
   int window;               // running epilogues: column tiles among which row blocks start apart
   uint32_t idesc;
-  // kEpiGrad, kEpiOut: only the rows that are not ignored take part, gathered;
-  // their number is known on the device alone
+  // kEpiLse, kEpiGrad, kEpiOut: only the rows that are not ignored take part,
+  // gathered; their number is known on the device alone
   const int32_t* live;      // that number; null: all rows
   int live_off, live_cap;   // this chunk's first row, its rows at most
   int live_steps;           // the rows are the contraction, not the rows of A
-  const int32_t* row_map;   // kEpiOut: where gathered row live_off + r goes in the output
+  const int32_t* row_map;   // gathered row live_off + r is row row_map[live_off + r] of the call
 
   // ---- epilogue
   float scale2;             // scale * log2(e)
@@ -232,7 +232,7 @@ struct Tile {
 template <int EPI, int BM, int SUBS>
 struct Walk {
   static constexpr int NP = problems_of(EPI);
-  static constexpr bool kLive = EPI == kEpiGrad || EPI == kEpiOut;
+  static constexpr bool kLive = EPI == kEpiLse || EPI == kEpiGrad || EPI == kEpiOut;
   const Params<NP>& prm;
   uint32_t item, total;
   const uint32_t slot, slots;
@@ -925,7 +925,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
           run_s = 0.0f;
           label = -1;
           if (row_ok) {
-            const int64_t y = load_label(p.labels, t.b * p.label_sb + row * p.label_sn, p.label_dtype);
+            const int64_t n = p.row_map ? p.row_map[row] : row;
+            const int64_t y = load_label(p.labels, t.b * p.label_sb + n * p.label_sn, p.label_dtype);
             label = y == p.ignore_index || y < 0 || y >= p.N ? -1 : static_cast<int>(y);
           }
         }

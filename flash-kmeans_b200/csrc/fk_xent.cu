@@ -196,6 +196,7 @@ struct CombineParams {
   int32_t* count;          // rows that are not ignored
   double2* block_part;     // (sum, count) of each block
   uint32_t* ticket;        // zero before the launch
+  const int32_t *map, *live;  // gathered rows (see xent_live_kernel), null: all, in order
   uint16_t* copy;          // optional: x's rows, 16-bit, Dp apart, ignored ones as zeros
   int Dp;
   int* status;
@@ -251,9 +252,10 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / p.row_blocks;
   const int row = (blockIdx.x % p.row_blocks) * 32 + lane;
+  const int rows = p.live ? *p.live : p.N;
   const float2* part = p.partial + static_cast<int64_t>(b) * p.pieces * p.N + row;
   float m = -INFINITY, s = 0.0f;
-  if (row < p.N) {
+  if (row < rows) {
     for (int i0 = warp; i0 < p.pieces; i0 += 4 * kCombineWarps) {
       float2 v[4];
 #pragma unroll
@@ -279,10 +281,14 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
 #pragma unroll
     for (int i = 0; i < kRowsPerWarp; ++i) {
       n[i] = (blockIdx.x % p.row_blocks) * 32 + warp * kRowsPerWarp + i;
-      y[i] = n[i] < p.N ? load_label(p.labels, b * p.lb + n[i] * p.ln, p.label_dtype) : p.ignore;
+      on[i] = n[i] < rows;
+      if (on[i] && p.map) n[i] = p.map[n[i]];
     }
 #pragma unroll
-    for (int i = 0; i < kRowsPerWarp; ++i) on[i] = n[i] < p.N && y[i] != p.ignore && y[i] >= 0 && y[i] < p.K;
+    for (int i = 0; i < kRowsPerWarp; ++i)
+      y[i] = on[i] ? load_label(p.labels, b * p.lb + n[i] * p.ln, p.label_dtype) : p.ignore;
+#pragma unroll
+    for (int i = 0; i < kRowsPerWarp; ++i) on[i] = on[i] && y[i] != p.ignore && y[i] >= 0 && y[i] < p.K;
     if (p.copy) {
       // the backward pass's copy of x (see head_rows_kernel), while the rows are at hand
 #pragma unroll
@@ -323,9 +329,10 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
       s = s * ex2((m - mu) * p.scale2) + v.y * ex2((v.x - mu) * p.scale2);
       m = mn;
     }
-    if (row < p.N) {
-      const int64_t r = static_cast<int64_t>(b) * p.N + row;
-      const int64_t y = load_label(p.labels, b * p.lb + row * p.ln, p.label_dtype);
+    if (row < rows) {
+      const int64_t n = p.map ? p.map[row] : row;
+      const int64_t r = static_cast<int64_t>(b) * p.N + n;
+      const int64_t y = load_label(p.labels, b * p.lb + n * p.ln, p.label_dtype);
       const bool ignored = y == p.ignore;
       RowStat st = {0.0f, 0.0f, 0.0f, -1};
       float loss = 0.0f;
@@ -438,14 +445,16 @@ __global__ void xent_weight_kernel(const float* g, const RowStat* stat, int64_t 
 
 // ------------------------------------------------------------ rows that count
 // The rows that are not ignored, in order (map[r] is the r-th of them) and how
-// many there are; the gradients of the others are set to zero here.  A block
+// many there are; the losses, statistics and gradients of the others, where
+// wanted, are set to zero here.  A block
 // counts what lies before its segment by itself: segments are few, and reading
 // labels again is cheaper than a second launch.
 constexpr int kLiveThreads = 1024;
 
 __global__ void __launch_bounds__(kLiveThreads) xent_live_kernel(const Labels y, int64_t N, int64_t segment,
-                                                                 int32_t* map, int32_t* live, void* gx,
-                                                                 int64_t gx_row, int64_t gx_bytes, int gx_vec) {
+                                                                 int32_t* map, int32_t* live, float* loss,
+                                                                 RowStat* stat, void* gx, int64_t gx_row,
+                                                                 int64_t gx_bytes, int gx_vec) {
   __shared__ int sm[32];
   __shared__ int base;
   pdl_wait_then_release();
@@ -472,6 +481,10 @@ __global__ void __launch_bounds__(kLiveThreads) xent_live_kernel(const Labels y,
     int at = base;
     for (int w = 0; w < warp; ++w) at += sm[w];
     if (on) map[at + __popc(votes & ((1u << lane) - 1))] = static_cast<int32_t>(n);
+    if (n < last && !on) {
+      if (loss) loss[n] = 0.0f;
+      if (stat) stat[n] = {0.0f, 0.0f, 0.0f, -1};
+    }
     if (gx) {
       for (uint32_t off = __ballot_sync(0xffffffffu, n < last && !on); off; off &= off - 1) {
         uint8_t* row = static_cast<uint8_t*>(gx) + (n0 + warp * 32 + __ffs(off) - 1) * gx_row;
@@ -578,16 +591,29 @@ static int check_workspace(const void* ws, size_t have, size_t need, const char*
   return FK_OK;
 }
 
-// Whether the backward pass leaves ignored rows out of its products.  Finding
-// and gathering them takes 20 to 30 us at 16384 rows (25 of 470 us were lost at
-// 32444 x 8192 x 128 with none ignored); from 2^36 products on, 0.4 ms, that is
-// what a twentieth of ignored rows gives back.  Separate codebooks keep one
-// block of rows for each batch, and go without.
+// Whether ignored rows are left out of the products.  Finding and gathering them
+// takes 20 to 30 us at 16384 rows (25 of 470 us were lost at 32444 x 8192 x 128
+// with none ignored); from 2^36 products on, 0.1 ms forward and 0.4 ms with the
+// gradients, a tenth or a twentieth of ignored rows gives that back.  Separate
+// codebooks keep one block of rows for each batch, and go without.
 static bool gathers(const Xent& q) { return q.B == 1 && q.N >= 1024 && q.N * q.K >= (1ll << 36) / q.D; }
+
+// Finds the rows that count: map gets N + 1 words, their number the last.
+static int find_live(const Xent& q, int32_t* map, float* loss, RowStat* stat, void* gx, int64_t gx_row,
+                     cudaStream_t s) {
+  // at most 128 segments, as a block reads every label before its own
+  const int64_t segment = ceil_div(ceil_div(q.N, 128), kLiveThreads) * kLiveThreads;
+  const int64_t eb = dtype_bytes(q.dtype);
+  const bool vec = reinterpret_cast<uintptr_t>(gx) % 16 == 0 && gx_row * eb % 16 == 0 && q.D * eb % 16 == 0;
+  return launch_plain("xent_live_kernel", xent_live_kernel, dim3(static_cast<unsigned>(ceil_div(q.N, segment))),
+                      kLiveThreads, s, q.y, q.N, segment, map, map + q.N, loss, stat, gx, gx_row * eb, q.D * eb,
+                      vec ? 1 : 0);
+}
 
 // Copies of the operands made by the caller of a pass; see fk_xent_loss_grad.
 struct Copies {
-  uint16_t *x_forward, *x_backward, *c;   // null: used in place (x_forward, c), gathered later (x_backward)
+  uint16_t *x_forward, *x_backward, *c;   // null: used in place (x_forward, c)
+  int32_t* map;                           // gathered rows, which the copies of x hold then; or null
 };
 
 struct ForwardPlan {
@@ -595,6 +621,7 @@ struct ForwardPlan {
   int chunks;
   int64_t row_blocks;
   uint16_t *xc, *cc;
+  int32_t* map;
   float2* partial;
   double2* block_part;
   uint32_t* ticket;
@@ -608,11 +635,12 @@ static ForwardPlan plan_forward(const Xent& q, void* ws, const Copies* given = n
   f.chunks = choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                            2 * slots_of(f.sh), 0.25);
   f.row_blocks = ceil_div(q.N, 32);
+  f.map = given ? given->map : gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
   if (given) {
     f.xc = given->x_forward;
     f.cc = given->c;
   } else {
-    f.xc = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
+    f.xc = !gathers(q) && in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
                ? nullptr
                : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
     f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
@@ -631,9 +659,15 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   const ForwardPlan f = plan_forward(q, ws, given);
   if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_forward")) return bad;
   int st = FK_OK;
-  if (!given)
-    st = rows_copy(q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), nullptr),
-                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  const int32_t* live = f.map ? f.map + q.N : nullptr;
+  if (!given) {
+    if (f.map) st = find_live(q, f.map, q.reduction == 0 ? loss : nullptr, stat, nullptr, 0, s);
+    RowsJob xj = rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), nullptr);
+    xj.map = f.map;
+    xj.live = live;
+    if (st == FK_OK)
+      st = rows_copy(q.dtype, xj, rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
+  }
   if (st != FK_OK) return st;
   Params<1> prm = {};
   prm.count = 1;
@@ -648,6 +682,9 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   p.label_sb = q.y.sb;
   p.label_sn = q.y.sn;
   p.ignore_index = q.y.ignore;
+  p.live = live;
+  p.live_cap = p.M;
+  p.row_map = f.map;
   p.partial = f.partial;
   p.zero = f.ticket;
   p.zero_n = 1;
@@ -690,6 +727,8 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   cp.count = count;
   cp.block_part = f.block_part;
   cp.ticket = f.ticket;
+  cp.map = f.map;
+  cp.live = live;
   if (given && !given->x_forward) {
     cp.copy = given->x_backward;
     cp.Dp = static_cast<int>(q.Dp());
@@ -784,7 +823,7 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   plan_products(q, f.R, want_x ? steps_x : 0, kw, want_c ? steps_c : 0, &f);
   f.ld = ceil_div(q.D, 4) * 4;
   if (given) {
-    f.xc = given->x_backward ? given->x_backward : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+    f.xc = given->x_backward;
     f.cc = given->c;
   } else {
     f.xc = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
@@ -792,7 +831,7 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
                ? nullptr
                : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
   }
-  f.map = gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
+  f.map = given ? given->map : gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
   f.P = b.take<uint16_t>(q.parts() * q.B * f.R * f.Kp);
   f.acc_x = f.acc_c = nullptr;
   if (want_x && (f.n_pieces > 1 || f.split_x > 1)) f.acc_x = b.take<float>(f.split_x * q.B * q.N * f.ld);
@@ -863,22 +902,13 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
   const float p_scale = f16 ? 16384.0f : 1.0f;
   int st = FK_OK;
   const int32_t* live = f.map ? f.map + q.N : nullptr;
-  if (f.map) {
-    // at most 128 segments, as a block reads every label before its own
-    const int64_t segment = ceil_div(ceil_div(q.N, 128), kLiveThreads) * kLiveThreads;
-    const int64_t eb = dtype_bytes(q.dtype);
-    const bool vec = reinterpret_cast<uintptr_t>(gx.p) % 16 == 0 && gx.sr * eb % 16 == 0 && q.D * eb % 16 == 0;
-    st = launch_plain("xent_live_kernel", xent_live_kernel, dim3(static_cast<unsigned>(ceil_div(q.N, segment))),
-                      kLiveThreads, s, q.y, q.N, segment, f.map, f.map + q.N, gx.p, gx.sr * eb, q.D * eb,
-                      vec ? 1 : 0);
-    if (st != FK_OK) return st;
-  }
-  if (!given || !given->x_backward) {
+  if (!given) {
+    if (f.map) st = find_live(q, f.map, nullptr, nullptr, gx.p, gx.sr, s);
     RowsJob xj = rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.xc, q.Dp(), f.map ? nullptr : &q.y);
     xj.map = f.map;
     xj.live = live;
-    st = rows_copy(q.dtype, xj,
-                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, given ? nullptr : f.cc, q.Dp(), nullptr), s);
+    if (st == FK_OK)
+      st = rows_copy(q.dtype, xj, rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
   }
   if (st != FK_OK) return st;
   const float* factor = q.reduction == 0 ? nullptr : g;
@@ -999,13 +1029,13 @@ struct LossGradPlan {
 static LossGradPlan plan_loss_grad(const Xent& q, bool want_x, bool want_c, void* ws) {
   LossGradPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
-  const bool in = in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs);
-  uint16_t* copy = !in || !gathers(q) ? b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp()) : nullptr;
-  f.copies.x_backward = gathers(q) ? nullptr : copy;
+  f.copies.x_backward = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
+  f.copies.map = gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
   f.copies.c = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
                    ? nullptr
                    : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
-  f.copies.x_forward = in ? nullptr : copy;
+  f.copies.x_forward =
+      !gathers(q) && in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs) ? nullptr : f.copies.x_backward;
   f.stat = b.take<RowStat>(q.B * q.N);
   f.count = b.take<int32_t>(1);
   f.rest = b.base ? b.base + b.used : nullptr;
@@ -1019,9 +1049,15 @@ static int loss_grad(const Xent& q, float* loss, const float* g, const Grad& gx,
                      size_t ws_bytes, int* status, cudaStream_t s) {
   const LossGradPlan f = plan_loss_grad(q, gx.p != nullptr, gc.p != nullptr, ws);
   if (const int bad = check_workspace(ws, ws_bytes, f.bytes, "fk_xent_loss_grad")) return bad;
-  int st = rows_copy(
-      q.dtype, rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.copies.x_forward, q.Dp(), &q.y),
-      rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.copies.c, q.Dp(), nullptr), s);
+  int st = FK_OK;
+  int32_t* map = f.copies.map;
+  if (map) st = find_live(q, map, q.reduction == 0 ? loss : nullptr, f.stat, gx.p, gx.sr, s);
+  RowsJob xj = rows_job(q.x, q.dtype, q.B, q.N, q.D, q.xs, f.copies.x_forward, q.Dp(), map ? nullptr : &q.y);
+  xj.map = map;
+  xj.live = map ? map + q.N : nullptr;
+  if (st == FK_OK)
+    st = rows_copy(q.dtype, xj,
+                   rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.copies.c, q.Dp(), nullptr), s);
   if (st == FK_OK) st = forward(q, loss, f.stat, f.count, f.rest, f.rest_bytes, status, s, &f.copies);
   if (st == FK_OK)
     st = backward(q, f.stat, f.count, g, gx, gc, f.rest, f.rest_bytes, status, s, &f.copies);

@@ -85,20 +85,21 @@ SIGNATURES = {
     "fk_centroid_accumulate": (_I, [_P, _I, _L, _L, _L, _L, _PL, _P, _I, _PL, _P, _P, _P, _P,
                                     _S, _P, _P]),
     "fk_centroid_finalize": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _PL, _PL, _P, _P, _I, _P]),
-    "fk_xent_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I, _I, _I]),
-    "fk_xent_forward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P, _P,
+    # strides of these go in as addresses: converting arrays cost a microsecond a call
+    "fk_xent_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _P, _P, _I, _I, _I]),
+    "fk_xent_forward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _P, _P, _P, _F, _L, _I, _P, _P,
                              _P, _P, _S, _P, _P]),
-    "fk_xent_backward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P,
-                              _P, _P, _P, _P, _PL, _PL, _P, _S, _P, _P]),
-    "fk_xent_loss_grad_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I, _I, _I]),
-    "fk_xent_loss_grad": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _F, _L, _I, _P,
-                               _P, _P, _P, _PL, _PL, _P, _S, _P, _P]),
-    "fk_quantize_rows": (_I, [_P, _I, _L, _L, _L, _PL, _P, _PL, _P, _PL, _P]),
-    "fk_int8_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _PL, _PL, _I]),
-    "fk_int8_scores": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _L, _PL, _PL, _PL, _PL,
-                            _PL, _PL, _P, _S, _P, _P]),
-    "fk_int8_assign": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _PL, _PL, _PL, _PL, _PL,
-                            _PL, _P, _S, _P, _P]),
+    "fk_xent_backward": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _P, _P, _P, _F, _L, _I, _P,
+                              _P, _P, _P, _P, _P, _P, _P, _S, _P, _P]),
+    "fk_xent_loss_grad_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _P, _P, _I, _I, _I]),
+    "fk_xent_loss_grad": (_I, [_P, _P, _P, _I, _I, _L, _L, _L, _L, _P, _P, _P, _F, _L, _I, _P,
+                               _P, _P, _P, _P, _P, _P, _S, _P, _P]),
+    "fk_quantize_rows": (_I, [_P, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P]),
+    "fk_int8_workspace_size": (_S, [_P, _P, _I, _L, _L, _L, _L, _P, _P, _I]),
+    "fk_int8_scores": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _L, _L, _L, _L, _P, _P, _P, _P,
+                            _P, _P, _P, _S, _P, _P]),
+    "fk_int8_assign": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _L, _L, _L, _P, _P, _P, _P, _P,
+                            _P, _P, _S, _P, _P]),
     "fk_centroid_finalize_normalized": (_I, [_P, _P, _P, _P, _I, _L, _L, _L, _PL, _PL, _P, _I,
                                              _P]),
 }

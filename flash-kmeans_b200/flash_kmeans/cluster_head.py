@@ -74,13 +74,20 @@ def _layout(key, make):
     return found
 
 
+# the current stream's handle; torch's public way makes an object of it first,
+# a sixteenth of a small call's time
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(fn, what, dev: _Device, *args):
     """fn(*args, status word, current stream) on device dev."""
-    if torch.cuda.current_device() == dev.index:
-        st = fn(*args, dev.status_ptr(), torch.cuda.current_stream(dev.index).cuda_stream)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        st = fn(*args, dev.status or dev.status_ptr(), _raw_stream(index))
     else:
-        with torch.cuda.device(dev.index):
-            st = fn(*args, dev.status_ptr(), torch.cuda.current_stream(dev.index).cuda_stream)
+        with torch.cuda.device(index):
+            st = fn(*args, dev.status_ptr(), _raw_stream(index))
     if st:
         nat.check(st, what)
 
@@ -113,8 +120,14 @@ def _two(t):
     return st if len(sh) == 2 else (0, *st)
 
 
-def _c(strides):
-    return (nat.ctypes.c_int64 * len(strides))(*strides)
+class _Strides:
+    """Strides for the C side: an array and its address."""
+
+    __slots__ = ("array", "at")
+
+    def __init__(self, strides):
+        self.array = (nat.ctypes.c_int64 * len(strides))(*strides)
+        self.at = nat.ctypes.addressof(self.array)
 
 
 # ------------------------------------------------------------- cross entropy
@@ -129,17 +142,17 @@ class _XentLayout:
         dtype = nat.dtype_code(x.dtype)
         sizes = (B, N, K, D)
         self.rows = B * N
-        xs, cs = _c(xs), _c(cs)
-        self.middle = (dtype, nat.dtype_code(labels.dtype), *sizes, xs, cs, _c(_two(labels)), scale,
-                       ignore_index, code)
-        self.grad_strides = _c((N * D, D, 1)), _c((K * D, D, 1))
+        self.kept = kept = [_Strides(s) for s in (xs, cs, _two(labels), (N * D, D, 1), (K * D, D, 1))]
+        xs, cs, ls, gxs, gcs = (s.at for s in kept)
+        self.middle = (dtype, nat.dtype_code(labels.dtype), *sizes, xs, cs, ls, scale, ignore_index,
+                       code)
+        self.grad_strides = gxs, gcs
         # by which gradients are wanted; (0, 0) is the forward pass
         self.bytes = {w: self.lib.fk_xent_workspace_size(x.data_ptr(), centroids.data_ptr(), dtype,
                                                          *sizes, xs, cs, code, *w)
                       for w in ((0, 0), (0, 1), (1, 0), (1, 1))}
         self.both = self.lib.fk_xent_loss_grad_workspace_size(
             x.data_ptr(), centroids.data_ptr(), dtype, *sizes, xs, cs, code, 1, 1)
-        self.device = x.device
 
 
 def _check_xent(x, centroids, labels, scale, ignore_index, reduction, name):
@@ -191,12 +204,12 @@ class _Xent:
     def forward(self, keep: bool):
         """(loss, row statistics and count for the backward pass, or None)"""
         at = self.at
-        device = at.device
         nbytes = at.bytes[0, 0]
-        loss = torch.empty(self.shapes[0][:-1] if self.none else (), dtype=torch.float32, device=device)
+        new = self.x.new_empty
+        loss = new(self.shapes[0][:-1] if self.none else (), dtype=torch.float32)
         # the count of rows behind the statistics, or behind the workspace
-        ws = torch.empty(nbytes + 16, dtype=torch.uint8, device=device)
-        kept = torch.empty(4 * at.rows + 4, dtype=torch.float32, device=device) if keep else None
+        ws = new(nbytes + 16, dtype=torch.uint8)
+        kept = new(4 * at.rows + 4, dtype=torch.float32) if keep else None
         stats = kept.data_ptr() if keep else None
         count = stats + 16 * at.rows if keep else ws.data_ptr() + nbytes
         _call(at.lib.fk_xent_forward, "fk_xent_forward", self.dev, self.x.data_ptr(), self.c.data_ptr(),
@@ -207,9 +220,10 @@ class _Xent:
         """(loss, gradient by x, by the centroids)"""
         at = self.at
         xshape, cshape = self.shapes
-        loss = torch.empty(xshape[:-1] if self.none else (), dtype=torch.float32, device=at.device)
-        gx, gc = self.x.new_empty(xshape), self.x.new_empty(cshape)
-        ws = torch.empty(at.both, dtype=torch.uint8, device=at.device)
+        new = self.x.new_empty
+        loss = new(xshape[:-1] if self.none else (), dtype=torch.float32)
+        gx, gc = new(xshape), new(cshape)
+        ws = new(at.both, dtype=torch.uint8)
         _call(at.lib.fk_xent_loss_grad, "fk_xent_loss_grad", self.dev, self.x.data_ptr(),
               self.c.data_ptr(), self.labels.data_ptr(), *at.middle, loss.data_ptr(),
               None if grad_loss is None else grad_loss.data_ptr(), gx.data_ptr(), gc.data_ptr(),
@@ -219,12 +233,12 @@ class _Xent:
     def backward(self, kept, grad_loss, want_x, want_c):
         """(gradient by x or None, by the centroids or None)"""
         at = self.at
-        device = at.device
         nbytes = at.bytes[int(want_x), int(want_c)]
         xshape, cshape = self.shapes
-        gx = torch.empty(xshape, dtype=self.x.dtype, device=device) if want_x else None
-        gc = torch.empty(cshape, dtype=self.x.dtype, device=device) if want_c else None
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        new = self.x.new_empty
+        gx = new(xshape) if want_x else None
+        gc = new(cshape) if want_c else None
+        ws = new(nbytes, dtype=torch.uint8)
         stats = kept.data_ptr()
         _call(at.lib.fk_xent_backward, "fk_xent_backward", self.dev, self.x.data_ptr(), self.c.data_ptr(),
               self.labels.data_ptr(), *at.middle, stats, stats + 16 * at.rows,
@@ -345,9 +359,9 @@ def quantize_rows(x: torch.Tensor):
     scale = torch.empty((B, N), dtype=torch.float32, device=x.device)
     lib = nat.load()
     with torch.cuda.device(x.device):
-        nat.check(lib.fk_quantize_rows(nat.ptr(xb), nat.dtype_code(x.dtype), B, N, D,
-                                       nat.strides(xb, 3), nat.ptr(q), nat.strides(q, 3),
-                                       nat.ptr(scale), nat.strides(scale, 2),
+        xs, qs, ss = (_Strides(t.stride()) for t in (xb, q, scale))
+        nat.check(lib.fk_quantize_rows(xb.data_ptr(), nat.dtype_code(x.dtype), B, N, D, xs.at,
+                                       q.data_ptr(), qs.at, scale.data_ptr(), ss.at,
                                        nat.stream_handle(x.device)), "fk_quantize_rows")
     return (q, scale) if x.dim() == 3 else (q[0], scale[0])
 
@@ -385,9 +399,10 @@ class _ScoresLayout:
         self.lib = nat.load()
         self.x_code = nat.dtype_code(x.dtype)
         self.sizes = (B, N, K, D)
-        xs, cs = _c(xs), _c(cs)
-        two = lambda t: None if t is None else _c(_two(t))  # noqa: E731
-        self.strides = (xs, cs, two(x_scale), two(c_scale), two(bias))
+        self.kept = [None if s is None else _Strides(s) for s in (
+            xs, cs, *(None if t is None else _two(t) for t in (x_scale, c_scale, bias)))]
+        self.strides = tuple(None if s is None else s.at for s in self.kept)
+        xs, cs = self.strides[:2]
         self.bytes = self.lib.fk_int8_workspace_size(x.data_ptr(), centroids.data_ptr(), self.x_code,
                                                      *self.sizes, xs, cs, argmax)
 
@@ -408,10 +423,11 @@ class _Scores:
             _check_int8(x, centroids, c_scale, x_scale, bias, name)
             x = x.reshape(-1, x.shape[-1])
             x_scale = None if x_scale is None else x_scale.reshape(-1)
-        sig = lambda t: None if t is None else (t.shape, t.stride(), t.dtype, t.device)  # noqa: E731
         key = (x.shape, x.stride(), x.dtype, x.device, x.data_ptr() & 15, centroids.shape,
                centroids.stride(), centroids.dtype, centroids.device, centroids.data_ptr() & 15,
-               sig(c_scale), sig(x_scale), sig(bias), argmax)
+               c_scale.shape, c_scale.stride(), c_scale.dtype, c_scale.device,
+               x_scale is not None and (x_scale.shape, x_scale.stride(), x_scale.dtype, x_scale.device),
+               bias is not None and (bias.shape, bias.stride(), bias.dtype, bias.device), argmax)
 
         def make():
             _check_int8(x, centroids, c_scale, x_scale, bias, name)
@@ -429,7 +445,7 @@ class _Scores:
         n = self.at.bytes
         if not n:
             return None, None, 0
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+        ws = self.operands[0].new_empty(n, dtype=torch.uint8)
         return ws, ws.data_ptr(), n
 
 
@@ -478,7 +494,7 @@ def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
         raise TypeError(f"{name}: unsupported out_dtype {out_dtype}")
     shape = (*q.lead, centroids.shape[-2])
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=q.device)
+        out = x.new_empty(shape, dtype=out_dtype)
     else:
         _check_out(out, shape, out_dtype, q.device, name)
         if shape[-1] > 1 and out.stride(-1) != 1:
@@ -489,9 +505,10 @@ def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
         strides = out.stride() if B == out.shape[0] else _fold_strides(out, name)
     else:
         strides = (N * out.stride(0), *out.stride())
+    strides = _Strides(strides)
     ws, ws_ptr, nbytes = q.workspace()
     _call(q.at.lib.fk_int8_scores, "fk_int8_scores", q.dev, *q.pointers(), out.data_ptr(), q.at.x_code,
-          nat.dtype_code(out_dtype), *q.at.sizes, *q.at.strides, _c(strides), ws_ptr, nbytes)
+          nat.dtype_code(out_dtype), *q.at.sizes, *q.at.strides, strides.at, ws_ptr, nbytes)
     return out
 
 
@@ -508,7 +525,7 @@ def int8_assign(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
     name = "int8_assign"
     q = _Scores(x, centroids, c_scale, x_scale, bias, True, name)
     if out is None:
-        out = torch.empty(q.lead, dtype=torch.int32, device=q.device)
+        out = x.new_empty(q.lead, dtype=torch.int32)
     else:
         _check_out(out, q.lead, torch.int32, q.device, name)
     B = q.at.sizes[0]
@@ -516,7 +533,8 @@ def int8_assign(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
         strides = out.stride() if B == out.shape[0] else _fold_strides(out, name)
     else:
         strides = (0, *out.stride())
+    strides = _Strides(strides)
     ws, ws_ptr, nbytes = q.workspace()
     _call(q.at.lib.fk_int8_assign, "fk_int8_assign", q.dev, *q.pointers(), out.data_ptr(), q.at.x_code,
-          *q.at.sizes, *q.at.strides, _c(strides), ws_ptr, nbytes)
+          *q.at.sizes, *q.at.strides, strides.at, ws_ptr, nbytes)
     return out

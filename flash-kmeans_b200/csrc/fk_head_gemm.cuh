@@ -13,12 +13,14 @@
 // up epilogue (four TMEM lane quarters x two or four column parts).  With CG = 2 two
 // CTAs of a cluster form one 256 x 256 tile (cta_group::2): each loads its own
 // 128 rows of A and its own half of B, so a CTA moves 32 KB per 64 columns of
-// the contraction instead of the 48 KB of a 128 x 256 tile, which is what
-// keeps the L2 feed below the tensor core's pace.  CG = 1 (128 x 128, 128 x 64
-// tiles) serves problems with too few tiles to fill 74 pairs.
+// the contraction instead of the 48 KB of a 128 x 256 tile.  That matters: with
+// all SMs reading, the L2 delivers 11 to 12 TB/s, and a 256 x 256 pair tile needs
+// 32 KB for 0.38 us of products (16384 x 32768 x 1024 forward: 658 us, 1.67
+// PFLOP/s alone; 128 x 128 tiles took 1.6 times as long).  CG = 1 (128 x 128,
+// 128 x 64 tiles) serves problems with too few tiles to fill 74 pairs.
 //
-// Two accumulators alternate in TMEM, so the epilogue of one tile overlaps the
-// products of the next.  Every wait is bounded (fk_ptx.cuh).
+// Two or four accumulators alternate in TMEM, so the epilogue of one tile
+// overlaps the products of the next.  Every wait is bounded (fk_ptx.cuh).
 #pragma once
 #include <climits>
 #include <type_traits>
@@ -637,7 +639,7 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
 // EXACT: float32 operands as three bf16 parts each.  A step loads the six part
 // tiles once and issues the six products that reach above 2^-24 of the leading
 // one, smallest first; loading a pair of parts per product instead fetched twice
-// the bytes and was bound by the L2 (86 -> see fk_xent.cu).  The tensor core
+// the bytes and was bound by the L2 (8192 x 1024 x 512 forward 71 -> 49 us).  The tensor core
 // adds to its float32 accumulator with truncation, a bias of up to 2^-24 of the
 // partial sum for every 16 elements.  16-bit inputs leave it at that (the
 // label's score, which the loss hangs on most, is summed in ordinary float32 by

@@ -35,9 +35,11 @@ struct ShapeChoice {
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// 256 x 256 tiles on CTA pairs once they give half of the 74 pairs a tile;
-// below that 128 x 128 tiles, and 128 x 64 ones when even those leave most SMs
-// idle.  Measured in profiles/cluster_head.md.
+// 256 x 256 tiles on CTA pairs once they give half of the 74 pairs a tile; below
+// that 128 x 128 tiles, and 128 x 64 ones when even those leave a third of the
+// SMs idle.  Losses of bfloat16 rows in us, as pairs / 128 / 64: 1024 x 4096 x
+// 1024 19.3 / 21.1 / 28.2, 512 x 4096 x 1024 17.5 / 16.0 / 19.1, 512 x 1000 x 128
+// 11.9 / 10.4 / 9.8, 1 x 32768 x 1024 28.2 / 21.1 / 27.3.
 inline ShapeChoice choose_shape(int64_t M, int64_t N, int64_t batches, bool exact) {
   const int wide = exact ? 128 : 256;
   if (M > 128 && ceil_div(M, 256) * ceil_div(N, wide) * batches >= 37) return {2, wide, exact};

@@ -14,14 +14,22 @@
 // The backward pass goes over the centroids in pieces.  For each it recomputes
 // the scores, writes dz of the piece rounded to 16 bits (the operand type of
 // the tensor cores: one rounding of half a step at most, next to the rounding
-// of the 16-bit gradients themselves) and runs the two products that read it;
-// accumulators are float32 throughout.  That is 8 N K D operations instead of
-// the 6 N K D of a pass that keeps N x K scores.
+// of the 16-bit gradients themselves) and runs the two products that read it,
+// in one launch whose workers finish together; accumulators are float32
+// throughout.  That is 8 N K D operations instead of the 6 N K D of a pass that
+// keeps N x K scores.
+//
+// Measured alone at 16384 x 32768 x 1024 bfloat16 with 15 % of the rows ignored:
+// forward product 571 us, combine 19, four pieces of 156 (scores again, dz) and
+// 326 (both gradients), 1.5 PFLOP/s; back to back the power cap stretches the
+// 2.6 ms to 3.1.  With 128 features the exponentials bind: the forward product of
+// 32444 x 8192 keeps the special-function units 74 % busy (103 us).
 //
 // float32 inputs are split exactly into three bf16 parts, and the six products
 // of parts down to 2^-16 of the leading one are accumulated, smallest first:
 // the terms left out are below 2^-24 of |x||c|.  That costs what 3xTF32 costs
-// and keeps one kernel, MN-major operands included.
+// and keeps one kernel, MN-major operands included (8192 x 1024 x 512, loss and
+// gradients: 0.22 ms, errors a fifth of plain float32's).
 #include <algorithm>
 #include <cmath>
 

@@ -33,7 +33,6 @@ namespace head {
 
 constexpr int kCtlWarps = 4;
 constexpr int kStageRowBytes = 128;            // one swizzle row: 64 16-bit or 128 8-bit elements
-constexpr int kTableFloats = 2 * 64;           // column scales and biases of an argmax warp
 constexpr int kSlotBytes = 2 * 128 * 8;        // (value, index) of two rows from the other column part
 
 enum Epilogue {
@@ -152,7 +151,10 @@ struct Shape {
   static constexpr int kStaging =
       EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : EPI == kEpiArgmax ? 8192 : 4096;
   static constexpr int kStagingBytes = kEpiWarps * kStaging;
-  static constexpr int kExtra = EPI == kEpiArgmax ? kEpiWarps * 2 * kTableFloats * 4 + kSlotBytes : 0;
+  // the argmax's column scales and biases, of this tile and of the next, by warp
+  static constexpr int kTable = 2 * (BN / kParts) * 4;
+  static constexpr int kTables = kEpiWarps * 2 * kTable;
+  static constexpr int kExtra = EPI == kEpiArgmax ? kTables + kSlotBytes : 0;
   static constexpr int kRoom = 232448 - 1024 - 512 - kStagingBytes - kExtra;
   static constexpr int kStages = kRoom / kStageBytes > 8 ? 8 : kRoom / kStageBytes;
   // accumulators in turn: the more, the less a tile waits for the one before
@@ -454,8 +456,9 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
   constexpr int kChunks = kCols / 32;
   const int part = ew >> 2, quarter = ew & 3;
   const uint32_t save = smem_u32(staging + ew * S::kStaging) + lane * 128 + (lane & 7) * 16;
-  const uint32_t tables = smem_u32(staging + S::kStagingBytes) + ew * (2 * kTableFloats * 4);
-  float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + S::kEpiWarps * 2 * kTableFloats * 4) +
+  const uint32_t tables = smem_u32(staging + S::kStagingBytes) + ew * 2 * S::kTable;
+  constexpr int kBias = kCols * 4;           // the biases, behind the scales
+  float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + S::kTables) +
                  quarter * 32 + lane;
   int buf = 0, tab = 0;
   uint32_t aphase = 0;
@@ -497,12 +500,12 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
         run_i[u] = INT_MAX;
         xs[u] = xs_next[u];
       }
-    const uint32_t table = tables + tab * (kTableFloats * 4);
+    const uint32_t table = tables + tab * S::kTable;
     tab ^= 1;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       sts32(table + (c * 32 + lane) * 4, __float_as_uint(sc_next[c]));
-      sts32(table + (64 + c * 32 + lane) * 4, __float_as_uint(bi_next[c]));
+      sts32(table + kBias + (c * 32 + lane) * 4, __float_as_uint(bi_next[c]));
     }
     __syncwarp();
     if (more) fetch(t, walk.subs);
@@ -548,7 +551,7 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           // without a bias the table holds zeros: no branch for every column
-          const uint4 s4 = lds128(table + (c * 32 + i) * 4), b4 = lds128(table + (64 + c * 32 + i) * 4);
+          const uint4 s4 = lds128(table + (c * 32 + i) * 4), b4 = lds128(table + kBias + (c * 32 + i) * 4);
           const uint64_t sa = pack2(__uint_as_float(s4.x), __uint_as_float(s4.y));
           const uint64_t sb = pack2(__uint_as_float(s4.z), __uint_as_float(s4.w));
           const uint64_t ba = pack2(__uint_as_float(b4.x), __uint_as_float(b4.y));

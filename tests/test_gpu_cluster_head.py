@@ -200,6 +200,9 @@ INT_SIZES = [
     (3, 50, 300, 256, True), (0, 400, 700, 255, False), (0, 1200, 2100, 160, False),
     (4, 300, 257, 1025, False), (0, 3, 4096, 4096, False),
     (3, 9000, 700, 64, False),    # several row blocks of CTA pairs in turn, one column chunk
+    (0, 300, 9100, 4096, False),  # columns past a window of tiles
+    (2, 2000, 900, 640, True),    # 256 columns wide and one chunk
+    (1, 257, 128, 33, True), (2, 513, 129, 20, False),   # one row more than a block, or two blocks
 ]
 
 

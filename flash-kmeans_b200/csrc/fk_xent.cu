@@ -46,8 +46,9 @@ constexpr int64_t kMaxRowChunk = 16384;
 int encode_operand(CUtensorMap* map, const Operand& o, uint32_t box_rows) {
   const int64_t eb = o.dtype == FK_I8 ? 1 : 2;
   const uint32_t box0 = o.dtype == FK_I8 ? 128 : 64;
+  // (one matrix: its distance to the next is never used, but has to be encodable)
   return encode_tmap_3d(map, o.p, o.dtype, o.inner, o.rows, o.mats, o.ld * eb,
-                        (o.mats > 1 ? o.mat : o.rows * o.ld) * eb, box0, box_rows);
+                        (o.mats > 1 ? o.mat : o.ld) * eb, box0, box_rows);
 }
 
 // ------------------------------------------------------------ operand copies

@@ -20,6 +20,7 @@ and can be captured into a CUDA graph.  The reference has no counterpart.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import Optional
 
@@ -72,6 +73,11 @@ def _layout(key, make):
             _layouts.clear()
         _layouts[key] = found
     return found
+
+
+def _on(device):
+    """Workspaces are sized for the current device."""
+    return torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext()
 
 
 # the current stream's handle; torch's public way makes an object of it first,
@@ -169,6 +175,8 @@ def _check_xent(x, centroids, labels, scale, ignore_index, reduction, name):
         raise ValueError(f"{name}: x is on {x.device}, labels on {labels.device}")
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"{name}: ignore_index does not fit 64 bits: {ignore_index}")
     if reduction not in _REDUCTIONS:
         raise ValueError(f"{name}: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
 
@@ -196,7 +204,8 @@ class _Xent:
 
         def make():
             _check_xent(x, centroids, labels, scale, ignore_index, reduction, name)
-            return _XentLayout(x, centroids, labels, scale, ignore_index, reduction)
+            with _on(x.device):
+                return _XentLayout(x, centroids, labels, scale, ignore_index, reduction)
 
         self.at = _layout(key, make)
         self.dev = _device(x.device)
@@ -248,10 +257,10 @@ class _Xent:
 
 
 def _backward(ctx, grad_loss):
-    ctx.saved_tensors  # raises if an input was changed in place since
+    call = _Xent(*ctx.saved_tensors, *ctx.args, "cluster_cross_entropy")
     if not grad_loss.is_contiguous():
         grad_loss = grad_loss.contiguous()
-    gx, gc = ctx.call.backward(ctx.kept, grad_loss, *ctx.needs_input_grad[:2])
+    gx, gc = call.backward(ctx.kept, grad_loss, *ctx.needs_input_grad[:2])
     return gx, gc, None, None, None, None
 
 
@@ -261,10 +270,10 @@ _backward_once = torch.autograd.function.once_differentiable(_backward)
 class _ClusterCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, centroids, labels, scale, ignore_index, reduction):
-        ctx.call = _Xent(x, centroids, labels, scale, ignore_index, reduction,
-                         "cluster_cross_entropy")
-        loss, ctx.kept = ctx.call.forward(True)
+        call = _Xent(x, centroids, labels, scale, ignore_index, reduction, "cluster_cross_entropy")
+        loss, ctx.kept = call.forward(True)
         ctx.save_for_backward(x, centroids, labels)
+        ctx.args = (scale, ignore_index, reduction)
         return loss
 
     @staticmethod
@@ -431,7 +440,8 @@ class _Scores:
 
         def make():
             _check_int8(x, centroids, c_scale, x_scale, bias, name)
-            return _ScoresLayout(x, centroids, c_scale, x_scale, bias, argmax)
+            with _on(x.device):
+                return _ScoresLayout(x, centroids, c_scale, x_scale, bias, argmax)
 
         self.at = _layout(key, make)
         self.dev = _device(self.device)

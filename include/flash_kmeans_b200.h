@@ -297,7 +297,7 @@ int fk_xent_forward(const void* x, const void* centroids, const void* labels, in
  * memory, one value (reduction 1, 2; NULL for 1.0) or (B,N) contiguous
  * (reduction 0).  Gradient rows have unit stride.  The centroids are gone
  * through in pieces; a piece's softmax is kept in 16 bits in the workspace
- * (at most 256 MB, or 64 KiB * B if that is more). */
+ * (at most 256 MB, or 64 KiB * B if that is more; 192 KiB * B for float32). */
 int fk_xent_backward(const void* x, const void* centroids, const void* labels, int dtype,
                      int labels_dtype, int64_t B, int64_t N, int64_t K, int64_t D,
                      const int64_t* x_strides3, const int64_t* c_strides3,

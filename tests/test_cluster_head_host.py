@@ -48,12 +48,13 @@ def _cuda(t):
     (dict(scale=float("nan")), ValueError, "positive and finite"),
     (dict(scale=float("inf")), ValueError, "positive and finite"),
     (dict(reduction="max"), ValueError, "reduction"),
+    (dict(ignore_index=1 << 63), ValueError, "64 bits"),
 ])
 def test_cross_entropy_argument_checks(kw, err, match):
-    a = dict(x=X, c=C, y=Y, scale=1.0, reduction="mean") | kw
+    a = dict(x=X, c=C, y=Y, scale=1.0, reduction="mean", ignore_index=-100) | kw
     with pytest.raises(err, match=match):
         fk.cluster_cross_entropy_grad(_cuda(a["x"]), _cuda(a["c"]), a["y"], scale=a["scale"],
-                                      reduction=a["reduction"])
+                                      reduction=a["reduction"], ignore_index=a["ignore_index"])
 
 
 @pytest.mark.parametrize("g,err", [(torch.ones(6), ValueError), (torch.ones((), dtype=torch.float16), TypeError),
@@ -61,6 +62,16 @@ def test_cross_entropy_argument_checks(kw, err, match):
 def test_grad_loss_checks(g, err):
     with pytest.raises(err, match="grad_loss"):
         fk.cluster_cross_entropy_grad(_cuda(X), _cuda(C), Y, grad_loss=g)
+
+
+def test_the_layouts_kept_are_bounded(monkeypatch):
+    from flash_kmeans import cluster_head as ch
+    monkeypatch.setattr(ch, "_layouts", {})
+    monkeypatch.setattr(ch, "_MOST_LAYOUTS", 5)
+    for i in range(23):
+        assert ch._layout(("size", i), lambda: i) == i
+        assert ch._layout(("size", i), lambda: -1) == i
+        assert len(ch._layouts) <= 5
 
 
 XQ, CQ = torch.zeros(6, 8, dtype=torch.int8), torch.zeros(4, 8, dtype=torch.int8)

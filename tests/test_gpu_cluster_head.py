@@ -121,6 +121,8 @@ SIZES = [
     (1, 300, 5000, 96, False),
     (0, 1500, 3000, 72, False),   # CTA pairs
     (5, 600, 512, 128, False),
+    (0, 300, 40100, 512, False),  # columns past a window of tiles
+    (1, 257, 256, 64, False), (0, 129, 65, 8, False),   # one row, one column more than a tile
 ]
 
 
@@ -320,6 +322,31 @@ def test_upstream_factor(reduction):
     got = fk.cluster_cross_entropy_grad(x, c, y, reduction=reduction, grad_loss=g)
     for a, w, what in zip(got, reference(x, c, y, 1.0, reduction, g=g), ("loss", "gx", "gc")):
         close(a, w, what)
+
+
+def test_saved_tensors_go_through_hooks():
+    """What autograd keeps can be moved away or computed again."""
+    from torch.utils.checkpoint import checkpoint
+    x, c, y = make(0, 300, 500, 64, BF, seed=28, ignored=0.2)
+    _, gx, gc = fk.cluster_cross_entropy_grad(x, c, y, scale=2.0)
+
+    def step(wrap):
+        xr, cr = x.clone().requires_grad_(), c.clone().requires_grad_()
+        wrap(lambda a, b: fk.cluster_cross_entropy(a, b, y, scale=2.0), xr, cr).backward()
+        assert torch.equal(xr.grad, gx) and torch.equal(cr.grad, gc)
+
+    def on_cpu(f, *args):
+        with torch.autograd.graph.save_on_cpu():
+            return f(*args)
+
+    step(on_cpu)
+    step(lambda f, *args: checkpoint(f, *args, use_reentrant=False))
+    xr = x.clone().requires_grad_()
+    loss = fk.cluster_cross_entropy(xr, c, y)
+    with torch.no_grad():
+        y[0] = 3
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
 
 
 def test_one_gradient_alone():
@@ -631,6 +658,19 @@ def test_int8_strides_and_outputs():
     assert torch.equal(lab[:, 1:101, 1], ids)
     lab[:, 1:101, 1] = -5
     assert lab.eq(-5).all()
+    # one codebook: all rows in one call, into a view whose batches follow each other
+    want1 = fk.int8_scores(xq, cq[0], cs[0], x_scale=xs)
+    rows = torch.full((2, 100, 157), 7.0, device="cuda")
+    assert torch.equal(fk.int8_scores(xq, cq[0], cs[0], x_scale=xs, out=rows[..., 4:154]), want1)
+    rows[..., 4:154] = 7.0
+    assert rows.eq(7.0).all()
+    ids1 = torch.empty(2, 100, 2, dtype=torch.int32, device="cuda")[..., 0]
+    assert torch.equal(fk.int8_assign(xq, cq[0], cs[0], x_scale=xs, out=ids1),
+                       fk.int8_assign(xq, cq[0], cs[0], x_scale=xs))
+    with pytest.raises(ValueError, match="follow each other"):
+        fk.int8_scores(xq, cq[0], cs[0], x_scale=xs, out=frame[:, 1:101, 3:153])
+    with pytest.raises(ValueError, match="follow each other"):
+        fk.int8_assign(xq, cq[0], cs[0], x_scale=xs, out=lab[:, 1:101, 1])
     # a codebook expanded over the batches
     e = fk.int8_scores(xq, cq[0].expand(2, 150, 48), cs[0].expand(2, 150), x_scale=xs)
     assert torch.equal(e, fk.int8_scores(xq, cq[0], cs[0], x_scale=xs))

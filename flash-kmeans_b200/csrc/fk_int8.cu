@@ -361,6 +361,9 @@ static int make8(Scores& q, const void* x, const void* c, int x_dtype, int64_t B
                 static_cast<long long>(kMaxD8));
   if (N >= (1ll << 30) || K >= (1ll << 30) || B >= (1ll << 30) || B * N >= (1ll << 31))
     return fail(FK_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit", who);
+  // (expanded centroids can have any size: no workspace may wrap around)
+  if (static_cast<double>(B) * static_cast<double>(K) * static_cast<double>(D) >= 0x1p58)
+    return fail(FK_ERR_UNSUPPORTED, "%s: sizes exceed 64-bit", who);
   q.x = x;
   q.c = c;
   q.x_dtype = x_dtype;

@@ -589,6 +589,9 @@ static int check_args(const Xent& q, const char* who) {
   if (q.N >= (1ll << 30) || q.K >= (1ll << 30) || q.D >= (1ll << 30) || q.B * 3 >= (1ll << 30) ||
       q.B * q.N >= (1ll << 31))
     return fail(FK_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit", who);
+  // (expanded centroids can have any size: no workspace may wrap around)
+  if (static_cast<double>(q.B) * static_cast<double>(q.K) * static_cast<double>(q.D) >= 0x1p58)
+    return fail(FK_ERR_UNSUPPORTED, "%s: sizes exceed 64-bit", who);
   return FK_OK;
 }
 

@@ -464,6 +464,8 @@ def _check_out(out, shape, dtype, device, name):
         raise ValueError(f"{name}: out must be a {dtype} tensor of shape {tuple(shape)}")
     if out.device != device:
         raise ValueError(f"{name}: x is on {device}, out on {out.device}")
+    if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{name}: out must not be expanded, its elements share memory")
 
 
 def _fold_strides(out, name):

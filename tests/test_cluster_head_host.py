@@ -102,6 +102,10 @@ def test_int8_output_checks():
         fk.int8_scores(_cuda(X), _cuda(CQ), CS, out_dtype=torch.float64)
     with pytest.raises(ValueError, match="unit stride"):
         fk.int8_scores(_cuda(X), _cuda(CQ), CS, out=torch.zeros(4, 6).t())
+    with pytest.raises(ValueError, match="expanded"):
+        fk.int8_scores(_cuda(X), _cuda(CQ), CS, out=torch.zeros(4).expand(6, 4))
+    with pytest.raises(ValueError, match="expanded"):
+        fk.int8_assign(_cuda(X), _cuda(CQ), CS, out=torch.zeros(1, dtype=torch.int32).expand(6))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         fk.int8_scores(X, CQ, CS)
 
@@ -148,6 +152,36 @@ def test_xent_entry_point_checks(lib, kw, code):
     assert lib.fk_last_error()
 
 
+def _bwd(lib, x=P, c=P, y=P, dtype=1, B=1, N=4, K=3, D=8, reduction=1, stats=P, count=P, g=P, gx=P, gc=P,
+         gxs=(32, 8, 1), gcs=(24, 8, 1), ws=None, nbytes=0):
+    return lib.fk_xent_backward(x, c, y, dtype, 3, B, N, K, D, L3(32, 8, 1), L3(24, 8, 1), L2(4, 1), 1.0,
+                                -100, reduction, stats, count, g, gx, gc, gxs and L3(*gxs),
+                                gcs and L3(*gcs), ws, nbytes, None, None)
+
+
+def _both(lib, x=P, c=P, y=P, dtype=1, B=1, N=4, K=3, D=8, reduction=1, loss=P, g=P, gx=P, gc=P,
+          gxs=(32, 8, 1), gcs=(24, 8, 1), ws=None, nbytes=0):
+    return lib.fk_xent_loss_grad(x, c, y, dtype, 3, B, N, K, D, L3(32, 8, 1), L3(24, 8, 1), L2(4, 1), 1.0,
+                                 -100, reduction, loss, g, gx, gc, gxs and L3(*gxs),
+                                 gcs and L3(*gcs), ws, nbytes, None, None)
+
+
+@pytest.mark.parametrize("fn,kw,code", [
+    *((fn, kw, code) for fn in (_bwd, _both) for kw, code in [
+        (dict(K=0), 1), (dict(dtype=6), 1), (dict(x=None), 1), (dict(y=None), 1),
+        (dict(reduction=0, g=None), 1), (dict(gxs=None), 1), (dict(gcs=None), 1),
+        (dict(gxs=(32, 1, 4)), 2), (dict(gcs=(24, 1, 3)), 2), (dict(N=1 << 30), 2),
+        (dict(B=1 << 20, N=1, K=1 << 20, D=1 << 20), 2),
+        (dict(), 3), (dict(ws=ctypes.c_void_p((1 << 20) + 16), nbytes=1 << 30), 3),
+    ]),
+    (_bwd, dict(stats=None), 1), (_bwd, dict(count=None), 1), (_bwd, dict(stats=ctypes.c_void_p(8)), 1),
+    (_bwd, dict(gx=None, gc=None), 0),               # nothing wanted
+    (_both, dict(gx=None, gc=None), 1), (_both, dict(loss=None), 1),
+])
+def test_xent_gradient_entry_point_checks(lib, fn, kw, code):
+    assert fn(lib, **kw) == code
+
+
 def test_xent_workspace_covers_copies_and_the_piece(lib):
     def size(dtype, D, bx, bc, N=1000, K=5000, p=P):
         return lib.fk_xent_workspace_size(p, p, dtype, 1, N, K, D, L3(N * D, D, 1), L3(K * D, D, 1),
@@ -174,6 +208,7 @@ def test_int8_entry_point_checks(lib):
     assert scores(sx=None) == 1 and scores(xdt=1) == 1 and scores(sc=None) == 1 and scores(out=None) == 1
     assert scores(D=65537) == 2 and b"overflow" in lib.fk_last_error()
     assert scores(N=1 << 30) == 2
+    assert scores(B=1 << 22, N=1, K=1 << 22, D=1 << 15) == 2
     assert scores(ostr=(12, 1, 4)) == 2
     assert scores(xdt=1, sx=None) == 3              # float x needs room for its integers
     assert scores(N=0) == 0

@@ -400,6 +400,32 @@ def test_whatever_an_ignored_row_holds(dtype):
     assert rows[drop].eq(0).all() and clean[1][drop].eq(0).all()
 
 
+@pytest.mark.parametrize("N,K,D", [(300, 400, 64), (20000, 9000, 392)])
+def test_an_ignored_id_within_the_vocabulary(N, K, D):
+    x, c, y = make(0, N, K, D, BF, seed=31, ids=torch.int64)
+    y[: N // 2] = 5
+    got = fk.cluster_cross_entropy_grad(x, c, y, scale=2.0, ignore_index=5)
+    for a, w, what in zip(got, reference(x, c, y, 2.0, "mean", ignore_index=5), ("loss", "gx", "gc")):
+        close(a, w, what)
+    want = fk.cluster_cross_entropy_grad(x, c, y.masked_fill(y == 5, -100), scale=2.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_points_that_are_their_own_centroids():
+    """One tensor as both operands, expanded rows and centroids: each use has its gradient."""
+    w = (torch.randn(40, 24, device="cuda") * 0.3).requires_grad_()
+    y = torch.arange(40, device="cuda")
+    fk.cluster_cross_entropy(w, w, y).backward()
+    wd = w.detach().double().requires_grad_()
+    torch.nn.functional.cross_entropy(wd @ wd.T, y).backward()
+    assert torch.allclose(w.grad.double(), wd.grad, rtol=1e-5, atol=1e-6)
+    w.grad = None
+    fk.cluster_cross_entropy(w[:1].expand(3, 50, 24), w.expand(3, 40, 24), y[:1].expand(3, 50)).backward()
+    wd.grad = None
+    torch.nn.functional.cross_entropy(wd[:1] @ wd.T, y[:1]).backward()
+    assert torch.allclose(w.grad.double(), wd.grad, rtol=1e-5, atol=1e-6)
+
+
 def test_no_row_left():
     x, c, y = make(0, 40, 30, 16, BF, seed=13)
     y.fill_(7)
@@ -518,8 +544,15 @@ def test_streams_and_graphs():
     x, c, y = make(0, 500, 700, 96, BF, seed=18, ignored=0.1)
     x2, c2, y2 = make(0, 500, 700, 96, BF, seed=19, ignored=0.1)
     cq, cs = fk.quantize_rows(c)
+    # (row losses of float16: a cleared word and two kernels of their own; the
+    # long one: rows gathered, several pieces)
+    xh, ch = x.half(), c.half()
+    up = torch.rand(500, device="cuda")
+    xl, cl, yl = make(0, 17000, 9000, 456, BF, seed=29, ignored=0.3)
     calls = [lambda: fk.cluster_cross_entropy_grad(x, c, y, scale=2.0), lambda: (fk.int8_assign(x, cq, cs),),
-             lambda: (fk.int8_scores(x, cq, cs),), lambda: fk.quantize_rows(x)]
+             lambda: (fk.int8_scores(x, cq, cs),), lambda: fk.quantize_rows(x),
+             lambda: fk.cluster_cross_entropy_grad(xh, ch, y, reduction="none", grad_loss=up),
+             lambda: fk.cluster_cross_entropy_grad(xl, cl, yl, scale=2.0)]
     want = [call() for call in calls]
     # two streams at once
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -544,6 +577,21 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     for (g, out), w in zip(graphs, want):
         assert all(torch.equal(p, q) for p, q in zip(out, w))
+    # replayed on two streams at once, twice each
+    for _, out in graphs:
+        for t in out:
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for i, (g, _) in enumerate(graphs):
+            with torch.cuda.stream(streams[i % 2]):
+                g.replay()
+    torch.cuda.synchronize()
+    for (g, out), w in zip(graphs, want):
+        assert all(torch.equal(p, q) for p, q in zip(out, w))
+    yl.fill_(-100)
+    yl[1234] = 17
+    xh.copy_(x2)
     x.copy_(x2)
     y.copy_(y2)
     c.copy_(c2)

@@ -33,7 +33,7 @@ namespace head {
 
 constexpr int kCtlWarps = 4;
 constexpr int kStageRowBytes = 128;            // one swizzle row: 64 16-bit or 128 8-bit elements
-constexpr int kSlotBytes = 2 * 128 * 8;        // (value, index) of two rows from the other column part
+constexpr int kSlotBytes = 2 * 128 * 8;        // (value, index) of two items' rows from the other column part
 
 enum Epilogue {
   kEpiLse = 0,     // running maximum and sum of exp2 over the columns
@@ -117,9 +117,6 @@ struct Problem {
 // finish together.  In the second product every worker has `all` tiles, the
 // workers from `short_from` on (one tile of the first product behind) `more`
 // others, and the last `rest` workers one more.
-// Row blocks that share a pass over the columns (an item is so many blocks):
-// two where four accumulators allow for it.
-__host__ __device__ constexpr int subs_of(int epi, int bn) { return epi == kEpiArgmax && bn <= 128 ? 2 : 1; }
 constexpr int problems_of(int epi) { return epi == kEpiOut ? 2 : 1; }
 
 template <int NP>
@@ -143,13 +140,12 @@ struct Shape {
   // Epilogue warps: four TMEM lane quarters x column parts.  Four parts give
   // each scheduler four warps, which is what hides the exponentials' and the
   // accumulator loads' latency (two left 70 % of the issue slots empty).
-  // The argmax holds two rows a thread instead: two parts.
   static constexpr int kParts = BN >= 128 && EPI != kEpiArgmax ? 4 : 2;
   static constexpr int kEpiWarps = 4 * kParts;
   static constexpr int kThreads = (kCtlWarps + kEpiWarps) * 32;
-  // shared memory of an epilogue warp: 32 rows of 128 bytes (64 for P, 64 rows for the argmax)
+  // shared memory of an epilogue warp: 32 rows of 128 bytes (64 for P)
   static constexpr int kStaging =
-      EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : EPI == kEpiArgmax ? 8192 : 4096;
+      EPI == kEpiLse ? 0 : EPI == kEpiGrad ? 2048 : 4096;
   static constexpr int kStagingBytes = kEpiWarps * kStaging;
   // the argmax's column scales and biases, of this tile and of the next, by warp
   static constexpr int kTable = 2 * (BN / kParts) * 4;
@@ -224,8 +220,7 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // (batch, row block, chunk) item in turn; the others one tile per item.
 struct Tile {
   int q;               // which problem
-  int b, m, n, chunk;  // m: row block, of subs_of() of an item
-  int sub;
+  int b, m, n, chunk;
   int it0, it1;        // steps of the contraction
   bool first, last;    // of the item
 };
@@ -233,7 +228,7 @@ struct Tile {
 // Every role walks the tiles by itself, in one thread: the decoding is kept to
 // 32-bit divisions, once per item (64-bit ones at every tile took 2000 cycles,
 // more than a short tile's products).
-template <int EPI, int BM, int SUBS>
+template <int EPI, int BM>
 struct Walk {
   static constexpr int NP = problems_of(EPI);
   static constexpr bool kLive = EPI == kEpiLse || EPI == kEpiGrad || EPI == kEpiOut;
@@ -241,7 +236,7 @@ struct Walk {
   uint32_t item, total;
   const uint32_t slot, slots;
   Tile t;
-  int j_begin, j_end, w_end, wl, w0, j, m0, subs;
+  int j_begin, j_end, w_end, wl, w0, j;
   int m_tiles[NP], steps[NP];
   int all, short_from, more, rest;
 
@@ -315,7 +310,7 @@ struct Walk {
     w0 = from;
     wl = min(prm.p[0].window, j_end - from);
     w_end = from + wl;
-    t.n = w0 + static_cast<int>(static_cast<uint32_t>(m0) % static_cast<uint32_t>(wl));
+    t.n = w0 + static_cast<int>(static_cast<uint32_t>(t.m) % static_cast<uint32_t>(wl));
   }
   __device__ void decode() {
     if (item >= total) return;
@@ -330,10 +325,7 @@ struct Walk {
       }
       t.chunk = c;
       t.b = r / static_cast<uint32_t>(m_tiles);
-      m0 = r - t.b * m_tiles;
-      t.sub = 0;
-      t.m = m0 * SUBS;
-      subs = SUBS > 1 && (t.m + 1) * BM < p.M ? 2 : 1;
+      t.m = r - t.b * m_tiles;
       j_begin = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * c / static_cast<uint32_t>(p.chunks));
       j_end = static_cast<int>(static_cast<uint32_t>(p.n_tiles) * (c + 1) / static_cast<uint32_t>(p.chunks));
       t.it0 = 0;
@@ -371,14 +363,6 @@ struct Walk {
   }
   __device__ void next() {
     if constexpr (running(EPI)) {
-      if (SUBS > 1) {
-        if (++t.sub < subs) {
-          ++t.m;
-          return;
-        }
-        t.sub = 0;
-        t.m = m0 * SUBS;
-      }
       if (++j < j_end) {
         t.first = false;
         t.last = j + 1 == j_end;
@@ -438,19 +422,20 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
 }
 
 // ------------------------------------------------------------------- kernel
-// Epilogue of the argmax.  Every score takes its column's scale and bias from
-// shared memory, 16 bytes to each of 32 lanes at a time, which the load path
-// delivers at a quarter of that; with one row a thread it was busy 72 % of the
-// time.  So a thread takes its row of two row blocks, and each scale and bias
-// serves two scores.  A row keeps its best score and the 32 scores of the chunk
-// that it came from, in shared memory; which column of it won is looked up once,
-// at the end of the row.
+// Epilogue of the argmax.  The scores' scaling and comparing bounds it, so a row
+// keeps only its best score and the 32 scores of the chunk that it came from, in
+// shared memory; which column of it won is looked up once, at the end of the
+// row.  A column's scale and bias come from shared memory, 16 bytes to all lanes
+// at a time.  (Two rows a thread, to load each of those once for both, needs
+// tiles of 128 columns to keep its accumulators in turn: the same time up to 256
+// features, 31 us against 25 for 65537 x 500 x 512.)
 template <int CG, int BN>
 __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* staging, uint32_t tmem,
                                                 uint64_t* acc_full, uint64_t* acc_empty,
                                                 volatile int* abort_flag, int ew, int lane, uint32_t rank,
                                                 int first, int stride) {
   using S = Shape<CG, BN, kEpiArgmax, false>;
+  static_assert(S::kParts == 2, "one slot a row");
   const Problem& p = prm.p[0];
   constexpr int kCols = BN / S::kParts;      // columns of this warp
   constexpr int kChunks = kCols / 32;
@@ -458,48 +443,39 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
   const uint32_t save = smem_u32(staging + ew * S::kStaging) + lane * 128 + (lane & 7) * 16;
   const uint32_t tables = smem_u32(staging + S::kStagingBytes) + ew * 2 * S::kTable;
   constexpr int kBias = kCols * 4;           // the biases, behind the scales
-  float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + S::kTables) +
-                 quarter * 32 + lane;
-  int buf = 0, tab = 0;
+  float2* slot = reinterpret_cast<float2*>(staging + S::kStagingBytes + S::kTables) + quarter * 32 + lane;
+  int buf = 0, tab = 0, turn = 0;
   uint32_t aphase = 0;
-  constexpr int U = subs_of(kEpiArgmax, BN);   // rows of a thread
-  Walk<kEpiArgmax, S::kBM, U> walk(prm, first, stride);
+  Walk<kEpiArgmax, S::kBM> walk(prm, first, stride);
   Tile t;
   bool more = walk.get(t);
 
-  float run_m[U], xs[U], xs_next[U] = {}, sc_next[kChunks], bi_next[kChunks];
-  int run_i[U];
+  float run_m = -INFINITY, xs = 0.0f, xs_next = 0.0f, sc_next[kChunks], bi_next[kChunks];
+  int run_i = INT_MAX;
   // The next tile's columns, and at an item's start its rows' scales: fetched a
   // tile ahead, as their latency would stand between the accumulator and its use.
-  auto fetch = [&](const Tile& a, int subs) {
+  auto fetch = [&]() {
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      const int64_t col = a.n * BN + part * kCols + c * 32 + lane;
-      sc_next[c] = col < p.N ? p.b_scale[a.b * p.bs_sb + col * p.bs_sn] : 0.0f;
-      bi_next[c] = col < p.N && p.bias ? p.bias[a.b * p.bias_sb + col * p.bias_sn] : 0.0f;
+      const int64_t col = t.n * BN + part * kCols + c * 32 + lane;
+      sc_next[c] = col < p.N ? p.b_scale[t.b * p.bs_sb + col * p.bs_sn] : 0.0f;
+      bi_next[c] = col < p.N && p.bias ? p.bias[t.b * p.bias_sb + col * p.bias_sn] : 0.0f;
     }
-    if (a.first)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t row = (a.m + u) * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-        xs_next[u] = u < subs && row < p.M ? p.a_scale[a.b * p.as_sb + row * p.as_sn] : 0.0f;
-      }
+    if (t.first) {
+      const int64_t row = t.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+      xs_next = row < p.M ? p.a_scale[t.b * p.as_sb + row * p.as_sn] : 0.0f;
+    }
   };
-  if (more) fetch(t, walk.subs);
+  if (more) fetch();
   while (more) {
-    // a tile of each row block of the item
     const Tile now = t;
-    const int subs = walk.subs;
-    for (int u = 0; u < subs; ++u) walk.next();
+    walk.next();
     more = walk.get(t);
-    const int row = now.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-    if (now.first)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        run_m[u] = -INFINITY;
-        run_i[u] = INT_MAX;
-        xs[u] = xs_next[u];
-      }
+    if (now.first) {
+      run_m = -INFINITY;
+      run_i = INT_MAX;
+      xs = xs_next;
+    }
     const uint32_t table = tables + tab * S::kTable;
     tab ^= 1;
 #pragma unroll
@@ -508,132 +484,101 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
       sts32(table + kBias + (c * 32 + lane) * 4, __float_as_uint(bi_next[c]));
     }
     __syncwarp();
-    if (more) fetch(t, walk.subs);
+    if (more) fetch();
 
-    const int buf0 = buf;
-    bool got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
-    if (++buf == S::kBufs) {
-      buf = 0;
-      aphase ^= 1;
-    }
-    const int buf1 = subs > 1 ? buf : buf0;
-    if (subs > 1) {
-      got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT) && got;
-      if (++buf == S::kBufs) {
-        buf = 0;
-        aphase ^= 1;
-      }
-    }
+    const bool got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
     if (__all_sync(0xffffffffu, got)) {
       tc_fence_after();
-      const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+      const uint32_t taddr = tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint64_t x2 = pack2(xs, xs);
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        const int at = part * kCols + c * 32, cc = now.n * BN + at, left = p.N - cc;
-        uint32_t v[U][32];
-        tmem_ld32(tmem + buf0 * BN + at + lanes, v[0]);
-        if constexpr (U > 1) tmem_ld32(tmem + buf1 * BN + at + lanes, v[U - 1]);   // (the same again for one block)
-#pragma unroll
-        for (int u = 0; u < U; ++u) tmem_ld_wait(v[u]);
+        const int cc = now.n * BN + part * kCols + c * 32, left = p.N - cc;
+        uint32_t v[32];
+        tmem_ld32(taddr + c * 32, v);
+        tmem_ld_wait(v);
         if (c + 1 == kChunks) {
-          // the accumulators are in registers: hand them back
+          // the accumulator is in registers: hand it back
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive_cg<CG>(&acc_empty[buf0]);
-            if (subs > 1) mbar_arrive_cg<CG>(&acc_empty[buf1]);
-          }
+          if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
         }
         if (left <= 0) continue;
-#pragma unroll
-        for (int u = 0; u < U; ++u) acc_to_f(v[u]);
-        float z[U][32];
+        acc_to_f(v);
+        float z[32];
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           // without a bias the table holds zeros: no branch for every column
           const uint4 s4 = lds128(table + (c * 32 + i) * 4), b4 = lds128(table + kBias + (c * 32 + i) * 4);
-          const uint64_t sa = pack2(__uint_as_float(s4.x), __uint_as_float(s4.y));
-          const uint64_t sb = pack2(__uint_as_float(s4.z), __uint_as_float(s4.w));
-          const uint64_t ba = pack2(__uint_as_float(b4.x), __uint_as_float(b4.y));
-          const uint64_t bb = pack2(__uint_as_float(b4.z), __uint_as_float(b4.w));
+          const uint32_t* su = &s4.x;
+          const uint32_t* bu = &b4.x;
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const uint64_t x2 = pack2(xs[u], xs[u]);
-            unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[u][i]), __uint_as_float(v[u][i + 1])), x2), sa), ba),
-                    z[u][i], z[u][i + 1]);
-            unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[u][i + 2]), __uint_as_float(v[u][i + 3])), x2), sb), bb),
-                    z[u][i + 2], z[u][i + 3]);
-          }
+          for (int k = 0; k < 4; k += 2)
+            unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[i + k]), __uint_as_float(v[i + k + 1])), x2),
+                              pack2(__uint_as_float(su[k]), __uint_as_float(su[k + 1]))),
+                         pack2(__uint_as_float(bu[k]), __uint_as_float(bu[k + 1]))),
+                    z[i + k], z[i + k + 1]);
         }
         if (left < 32) {
           keep_branch();
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (i >= left) z[0][i] = z[U - 1][i] = -INFINITY;
+            if (i >= left) z[i] = -INFINITY;
         }
+        float mx[4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float mx[4];
+        for (int q = 0; q < 4; ++q) {
+          mx[q] = max_nan3(z[q], z[q + 4], z[q + 8]);
+          mx[q] = max_nan3(mx[q], z[q + 12], z[q + 16]);
+          mx[q] = max_nan(max_nan3(mx[q], z[q + 20], z[q + 24]), z[q + 28]);
+        }
+        const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
+        if (!(m < run_m) && argmax_better(m, cc, run_m, run_i)) {
+          run_m = m;
+          run_i = cc;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            mx[q] = max_nan3(z[u][q], z[u][q + 4], z[u][q + 8]);
-            mx[q] = max_nan3(mx[q], z[u][q + 12], z[u][q + 16]);
-            mx[q] = max_nan(max_nan3(mx[q], z[u][q + 20], z[u][q + 24]), z[u][q + 28]);
-          }
-          const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
-          if (!(m < run_m[u]) && argmax_better(m, cc, run_m[u], run_i[u])) {
-            run_m[u] = m;
-            run_i[u] = cc;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              sts128((save + u * 4096) ^ (q * 16), __float_as_uint(z[u][q * 4]), __float_as_uint(z[u][q * 4 + 1]),
-                     __float_as_uint(z[u][q * 4 + 2]), __float_as_uint(z[u][q * 4 + 3]));
-          }
+          for (int q = 0; q < 8; ++q)
+            sts128(save ^ (q * 16), __float_as_uint(z[q * 4]), __float_as_uint(z[q * 4 + 1]),
+                   __float_as_uint(z[q * 4 + 2]), __float_as_uint(z[q * 4 + 3]));
         }
       }
     }
+    if (++buf == S::kBufs) {
+      buf = 0;
+      aphase ^= 1;
+    }
     if (!now.last) continue;
 
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (run_i[u] == INT_MAX) continue;
+    if (run_i != INT_MAX) {
       int at = 0;
 #pragma unroll
       for (int q = 7; q >= 0; --q) {
-        const uint4 f = lds128((save + u * 4096) ^ (q * 16));
+        const uint4 f = lds128(save ^ (q * 16));
         const uint32_t* fu = &f.x;
 #pragma unroll
         for (int i = 3; i >= 0; --i) {
           const float g = __uint_as_float(fu[i]);
-          if (g == run_m[u] || g != g) at = q * 4 + i;
+          if (g == run_m || g != g) at = q * 4 + i;
         }
       }
-      run_i[u] += at;
+      run_i += at;
     }
+    const int row = now.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
     if (p.chunks == 1) {
-      // the column parts of a row meet in shared memory
-      if (part == 1)
-#pragma unroll
-        for (int u = 0; u < U; ++u) slot[u * 128] = make_float2(run_m[u], __int_as_float(run_i[u]));
+      // the two column parts of a row meet in shared memory
+      // (in turn in two slots: the item after the next one writes this one again,
+      // behind the next one's barrier)
+      if (part == 1) slot[turn] = make_float2(run_m, __int_as_float(run_i));
       quarter_sync<S::kParts * 32>(quarter);
-      if (part == 0)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float2 o = slot[u * 128];
-          if (argmax_better(o.x, __float_as_int(o.y), run_m[u], run_i[u])) run_i[u] = __float_as_int(o.y);
-          const int r = row + u * S::kBM;
-          if (u < subs && r < p.M) p.label_out[now.b * p.lo_sb + r * p.lo_sn] = run_i[u];
-        }
-      // the slots are read before the next rows write them
-      quarter_sync<S::kParts * 32>(quarter);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = row + u * S::kBM;
-        if (u < subs && r < p.M)
-          p.partial[((static_cast<int64_t>(now.b) * p.chunks + now.chunk) * S::kParts + part) * p.M + r] =
-              make_float2(run_m[u], __int_as_float(run_i[u]));
+      if (part == 0) {
+        const float2 o = slot[turn];
+        if (argmax_better(o.x, __float_as_int(o.y), run_m, run_i)) run_i = __float_as_int(o.y);
+        if (row < p.M) p.label_out[now.b * p.lo_sb + row * p.lo_sn] = run_i;
       }
+      turn ^= 128;
+    } else if (row < p.M) {
+      p.partial[((static_cast<int64_t>(now.b) * p.chunks + now.chunk) * S::kParts + part) * p.M + row] =
+          make_float2(run_m, __int_as_float(run_i));
     }
   }
 }
@@ -722,7 +667,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const uint32_t bar0 = CG == 2 ? map_to_rank(full, 0) : full0;        // of the pair's first
       int stage = 0;
       uint32_t phase = 0;
-      Walk<EPI, S::kBM, subs_of(EPI, BN)> walk(prm, first, stride);
+      Walk<EPI, S::kBM> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
@@ -796,7 +741,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const uint32_t smem0 = smem_u32(smem);
       int stage = 0, buf = 0;
       uint32_t phase = 0, aphase = 0;
-      Walk<EPI, S::kBM, subs_of(EPI, BN)> walk(prm, first, stride);
+      Walk<EPI, S::kBM> walk(prm, first, stride);
       bool ok = true;
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
@@ -881,7 +826,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     uint8_t* stg = staging + ew * S::kStaging;
     int buf = 0;
     uint32_t aphase = 0;
-    Walk<EPI, S::kBM, subs_of(EPI, BN)> walk(prm, first, stride);
+    Walk<EPI, S::kBM> walk(prm, first, stride);
 
     // running state of a row
     float run_m = -INFINITY, run_s = 0.0f;
@@ -905,7 +850,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const int64_t row = nt.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       if constexpr (EPI == kEpiGrad) {
         st_next = {0.0f, 0.0f, 0.0f, -1};
-        if (row < Walk<EPI, S::kBM, subs_of(EPI, BN)>::rows_of(p)) {
+        if (row < Walk<EPI, S::kBM>::rows_of(p)) {
           const float4 f = *reinterpret_cast<const float4*>(p.stat + nt.b * p.stat_rows + (p.row_map ? p.row_map[p.stat_off + row] : p.stat_off + row));
           st_next = {f.x, f.y, f.z, __float_as_int(f.w)};
         }
@@ -920,7 +865,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const Problem& p = prm.p[NP > 1 ? t.q : 0];
       const int row = t.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
       const int row0 = row - lane;
-      const int rows = Walk<EPI, S::kBM, subs_of(EPI, BN)>::rows_of(p);
+      const int rows = Walk<EPI, S::kBM>::rows_of(p);
       const bool row_ok = row < rows;
       const int col0 = t.n * BN + part * kCols;
 

@@ -181,7 +181,7 @@ int set_problem(Params<problems_of(EPI)>& prm, int i, const Operand& a, const Op
                 ShapeChoice sh) {
   Problem& p = prm.p[i];
   const int step = integer(EPI) ? 128 : 64;
-  p.m_tiles = static_cast<int>(ceil_div(p.M, subs_of(EPI, sh.bn) * sh.bm()));
+  p.m_tiles = static_cast<int>(ceil_div(p.M, sh.bm()));
   p.n_tiles = static_cast<int>(ceil_div(p.N, sh.bn));
   p.kblocks = static_cast<int>(ceil_div(kdim, step));
   p.a_mn = a.mn;
@@ -217,7 +217,7 @@ int launch(Params<problems_of(EPI)>& prm, ShapeChoice sh, cudaStream_t s) {
       return launch_shape<1, 64, EPI, true>(prm, s);
     }
   }
-  if constexpr (EPI == kEpiOut || EPI == kEpiArgmax) {
+  if constexpr (EPI == kEpiOut) {
     if (sh.cg == 2 && sh.bn == 128) return launch_shape<2, 128, EPI, false>(prm, s);
   }
   if (sh.cg == 2) return launch_shape<2, 256, EPI, false>(prm, s);

@@ -334,11 +334,7 @@ static ScoresPlan plan_scores(const Scores& q, bool argmax, void* ws) {
     return p;
   };
   f.sh = choose_shape(q.N, q.K, q.B, false);
-  // Up to 512 features the argmax's scores outweigh the products, and two row
-  // blocks share each column's scale (256 x 128 tiles); beyond, the wider tile's
-  // fewer bytes count (assign of 65537 x 500 x 1024: 80 us against 94).
-  if (argmax && f.sh.bn == 256 && q.D <= 512) f.sh.bn = 128;
-  f.chunks = argmax ? choose_chunks(q.B * ceil_div(q.N, subs_of(kEpiArgmax, f.sh.bn) * f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
+  f.chunks = argmax ? choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                                     2 * slots_of(f.sh), 0.25)
                     : 1;
   if (q.x_dtype != FK_I8 || !in_place8(q.x, q.B, q.N, q.D, q.xs))

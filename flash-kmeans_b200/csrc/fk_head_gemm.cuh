@@ -140,6 +140,8 @@ struct Shape {
   // Epilogue warps: four TMEM lane quarters x column parts.  Four parts give
   // each scheduler four warps, which is what hides the exponentials' and the
   // accumulator loads' latency (two left 70 % of the issue slots empty).
+  // The argmax has work at every row's end that each part adds to: with four, 302400
+  // x 1000 x 128 took 126 us against 129, 604800 x 256 x 64 93 against 83.
   static constexpr int kParts = BN >= 128 && EPI != kEpiArgmax ? 4 : 2;
   static constexpr int kEpiWarps = 4 * kParts;
   static constexpr int kThreads = (kCtlWarps + kEpiWarps) * 32;
@@ -422,7 +424,8 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
 }
 
 // ------------------------------------------------------------------- kernel
-// Epilogue of the argmax.  The scores' scaling and comparing bounds it, so a row
+// Epilogue of the argmax.  The scores' scaling and comparing bounds it (2.4 scores
+// a ns at 604800 x 1000 x 128: 254 us, of which the products need 47), so a row
 // keeps only its best score and the 32 scores of the chunk that it came from, in
 // shared memory; which column of it won is looked up once, at the end of the
 // row.  A column's scale and bias come from shared memory, 16 bytes to all lanes

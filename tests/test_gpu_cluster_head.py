@@ -11,6 +11,7 @@ Tolerances are bounds on rounding, taken before the first run:
 * a gradient is a float32 sum of P times an operand and is rounded once.
 """
 import math
+import random
 
 import pytest
 import torch
@@ -747,6 +748,63 @@ def test_scores_behind_32_bit_offsets():
 
 
 # --------------------------------------------------------------- as it is used
+@pytest.mark.parametrize("K", [16, 64])
+def test_losses_behind_32_bit_offsets(K):
+    """Rows past 2^31 elements, all multiplied (16 centroids) and gathered (64)."""
+    N, D = (1 << 20) + 77, 2056
+    x = torch.zeros(N, D, dtype=BF, device="cuda")
+    ends = torch.cat([torch.arange(200), torch.arange(N - 300, N)]).cuda()
+    xe, c, ye = make(0, 500, K, D, BF, seed=33, ids=torch.int64, ignored=0.1)
+    x[ends] = xe
+    y = torch.full((N,), -100, dtype=torch.int64, device="cuda")
+    y[ends] = ye
+    up = torch.zeros(N, device="cuda")
+    up[ends] = torch.rand(500, device="cuda") + 0.5
+    loss, gx, gc = fk.cluster_cross_entropy_grad(x, c, y, scale=2.0, reduction="none", grad_loss=up)
+    want = reference(xe, c, ye, 2.0, "none", g=up[ends])
+    for a, w, what in zip((loss[ends], gx[ends], gc), want, ("rows", "gx", "gc")):
+        close(a, w, what)
+    assert loss[200:-300].eq(0).all() and gx[200:-300].eq(0).all()
+    q, s = fk.quantize_rows(x)
+    qe, se = fk.quantize_rows(xe)
+    assert torch.equal(q[ends], qe) and torch.equal(s[ends], se) and q[200:-300].eq(0).all()
+
+
+def _drawn(seed, most):
+    """Sizes of any kind up to `most` products, short and long in every direction."""
+    r = random.Random(seed)
+    while True:
+        B = r.choice([0, 0, 1, 3])
+        N, K, D = (round(math.exp(r.uniform(0.0, math.log(n)))) for n in (12000, 12000, 4096))
+        if max(B, 1) * N * K * D < most and max(B, 1) * N * K < 1 << 25:
+            return r, B, N, K, D
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_sizes_of_8_bit_scores(seed):
+    r, B, N, K, D = _drawn(seed, 1 << 36)
+    args = int_case(B, N, K, D, seed=seed, shared=r.random() < 0.3, bias=r.random() < 0.5)
+    xq, cq, xs, cs, b = args
+    acc = (xq.double() @ cq.double().transpose(-1, -2)).float()     # (exact in 53 bits)
+    z = acc * xs[..., None] * cs[..., None, :]
+    z = z if b is None else z + b[..., None, :]
+    k = torch.arange(K, device="cuda", dtype=torch.int32)
+    first = torch.where(z == z.amax(-1, keepdim=True), k, K).amin(-1)
+    assert torch.equal(fk.int8_assign(xq, cq, cs, x_scale=xs, bias=b), first), (B, N, K, D)
+    assert torch.equal(fk.int8_scores(xq, cq, cs, x_scale=xs, bias=b), z), (B, N, K, D)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_drawn_sizes_of_losses(seed):
+    r, B, N, K, D = _drawn(seed + 100, 1 << 34)
+    dtype, reduction = r.choice([BF, HF, FP]), r.choice(["mean", "sum"])
+    x, c, y = make(B, N, K, D, dtype, seed=seed, shared=r.random() < 0.3, ignored=0.2)
+    y[..., 0] = 0                       # (a row that counts)
+    got = fk.cluster_cross_entropy_grad(x, c, y, scale=2.0, reduction=reduction)
+    for a, w, what in zip(got, reference(x, c, y, 2.0, reduction), ("loss", "gx", "gc")):
+        close(a, w, f"{what} of {(B, N, K, D)}")
+
+
 def test_from_clusters_to_an_8_bit_head():
     """k-means gives the ids, the head learns them, answers in 8 bits."""
     g = torch.Generator(device="cuda").manual_seed(25)

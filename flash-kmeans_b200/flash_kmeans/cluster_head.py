@@ -25,6 +25,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from . import _ops
@@ -96,6 +97,16 @@ def _call(fn, what, dev: _Device, *args):
             st = fn(*args, dev.status_ptr(), _raw_stream(index))
     if st:
         nat.check(st, what)
+
+
+def _refuse_tangents(name, *tensors):
+    """A tangent would be dropped without a word: a dual tensor need not require
+    grad.  (The level is looked at first because unpacking costs 0.3 us each.)"""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")
 
 
 def _check_pair(x, centroids, name):
@@ -299,13 +310,15 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
         reduction: 'mean' over the rows that are not ignored (NaN if there are
             none), 'sum', or 'none' for one loss per row.
     Returns:
-        float32 loss, differentiable (once) by x and centroids.
+        float32 loss, differentiable (once, in reverse mode) by x and centroids;
+        forward-mode tangents are refused.
 
     The (N, K) scores are never stored, forward or backward; sums and softmax
     statistics are float32.  Gradients of 16-bit inputs round the softmax to 16
     bits once, piece by piece, as the tensor cores take it.  A label outside
     [0, K) other than ``ignore_index`` makes the loss NaN.
     """
+    _refuse_tangents("cluster_cross_entropy", x, centroids)
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False)
                                     or getattr(centroids, "requires_grad", False)):
         return _ClusterCrossEntropy.apply(x, centroids, labels, scale, ignore_index, reduction)
@@ -325,6 +338,7 @@ def cluster_cross_entropy_grad(x: torch.Tensor, centroids: torch.Tensor, labels:
     inputs a factor such as a loss scale goes in here).
     """
     name = "cluster_cross_entropy_grad"
+    _refuse_tangents(name, x, centroids, grad_loss)
     with torch.no_grad():
         call = _Xent(x, centroids, labels, scale, ignore_index, reduction, name)
         shape = x.shape[:-1] if call.none else ()

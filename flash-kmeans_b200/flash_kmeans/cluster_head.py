@@ -267,15 +267,17 @@ class _Xent:
         return gx, gc
 
 
-def _backward(ctx, grad_loss):
-    call = _Xent(*ctx.saved_tensors, *ctx.args, "cluster_cross_entropy")
-    if not grad_loss.is_contiguous():
-        grad_loss = grad_loss.contiguous()
-    gx, gc = call.backward(ctx.kept, grad_loss, *ctx.needs_input_grad[:2])
-    return gx, gc, None, None, None, None
+class _OnceOnly(torch.autograd.Function):
+    """Hands gradients on as functions of the tensors behind them, whose own
+    derivative raises: without it a second derivative would be left out."""
 
+    @staticmethod
+    def forward(ctx, gx, gc, x, centroids, grad_loss):
+        return gx, gc
 
-_backward_once = torch.autograd.function.once_differentiable(_backward)
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("cluster_cross_entropy is differentiable once; its gradients have no derivative")
 
 
 class _ClusterCrossEntropy(torch.autograd.Function):
@@ -289,9 +291,13 @@ class _ClusterCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_loss):
-        # the guard against a second derivative is only needed, and paid for,
-        # where a graph of the backward pass is recorded
-        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_loss)
+        x, centroids, labels = ctx.saved_tensors
+        with torch.no_grad():
+            call = _Xent(x, centroids, labels, *ctx.args, "cluster_cross_entropy")
+            gx, gc = call.backward(ctx.kept, grad_loss.contiguous(), *ctx.needs_input_grad[:2])
+        if torch.is_grad_enabled():     # a graph of the backward pass is recorded
+            gx, gc = _OnceOnly.apply(gx, gc, x, centroids, grad_loss)
+        return gx, gc, None, None, None, None
 
 
 def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torch.Tensor, *,

@@ -73,3 +73,48 @@ def test_forward_mode_of_the_upstream_gradient_is_refused():
         g = fwAD.make_dual(torch.ones(()), torch.ones(()))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             fk.cluster_cross_entropy_grad(x, c, y, grad_loss=g)
+
+
+# ------------------------------------------------------------- second order
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("which", ["x", "centroids", "both"])
+def test_a_penalty_on_the_gradient_is_refused(which, reduction):
+    """The loss has a graph of its own, so dropping the penalty's would not show."""
+    x, c, y = _case()
+    x.requires_grad_(which != "centroids")
+    c.requires_grad_(which != "x")
+    of = [t for t in (x, c) if t.requires_grad]
+    loss = fk.cluster_cross_entropy(x, c, y, reduction=reduction).sum()
+    grads = torch.autograd.grad(loss, of, create_graph=True)
+    total = loss + sum(g.square().sum() for g in grads)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        total.backward()
+    for g in grads:     # and each of them alone
+        assert g.requires_grad
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.sum(), of, allow_unused=True, retain_graph=True)
+
+
+def test_a_second_derivative_by_the_upstream_gradient_is_refused():
+    x, c, y = _case()
+    x.requires_grad_()
+    w = torch.ones((), dtype=torch.float64, requires_grad=True)
+    g, = torch.autograd.grad(w * fk.cluster_cross_entropy(x, c, y), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(g.sum(), w)
+
+
+def test_gradients_with_a_graph_can_still_be_used_as_values():
+    x, c, y = _case()
+    x.requires_grad_()
+    c.requires_grad_()
+    loss = fk.cluster_cross_entropy(x, c, y)
+    gx, gc = torch.autograd.grad(loss, (x, c), create_graph=True)
+    want = torch.autograd.grad(torch.nn.functional.cross_entropy(x @ c.T, y), (x, c))
+    assert torch.allclose(gx, want[0]) and torch.allclose(gc, want[1])
+    (loss * gx.detach().norm()).backward()      # a weight that is taken as a constant
+    assert torch.allclose(x.grad, want[0] * want[0].norm())
+    # a plain backward pass gives gradients without a graph
+    x.grad = None
+    fk.cluster_cross_entropy(x, c, y).backward()
+    assert not x.grad.requires_grad

@@ -99,14 +99,34 @@ def _call(fn, what, dev: _Device, *args):
         nat.check(st, what)
 
 
+def _has_tangent(t):
+    # (the level is looked at first because unpacking costs 0.3 us)
+    return (getattr(forward_ad, "_current_level", 0) >= 0 and isinstance(t, torch.Tensor)
+            and forward_ad.unpack_dual(t).tangent is not None)
+
+
 def _refuse_tangents(name, *tensors):
-    """A tangent would be dropped without a word: a dual tensor need not require
-    grad.  (The level is looked at first because unpacking costs 0.3 us each.)"""
-    if getattr(forward_ad, "_current_level", 0) < 0:
-        return
-    for t in tensors:
-        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")
+    """A tangent would be dropped without a word: a dual tensor need not require grad."""
+    if any(map(_has_tangent, tensors)):
+        raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")
+
+
+def _numbers(name, scale, ignore_index):
+    """scale and ignore_index as Python's; what would be lost on the way is refused."""
+    if isinstance(scale, torch.Tensor):
+        if scale.is_cuda:
+            raise TypeError(f"{name}: scale must be a number; reading one from a GPU would wait for it "
+                            "(multiply x by it instead)")
+        if scale.requires_grad and torch.is_grad_enabled() or _has_tangent(scale):
+            raise TypeError(f"{name}: scale must be a number; it gets no gradient (multiply a learnable "
+                            "factor into x instead)")
+    if isinstance(ignore_index, torch.Tensor) and ignore_index.is_cuda:
+        raise TypeError(f"{name}: ignore_index must be a number; reading one from a GPU would wait for it")
+    # (a fraction, NaN or an infinity is no id)
+    if ignore_index != ignore_index or ignore_index in (math.inf, -math.inf) or (
+            int(ignore_index) != ignore_index):
+        raise TypeError(f"{name}: ignore_index must be a whole number, got {ignore_index}")
+    return float(scale), int(ignore_index)
 
 
 def _check_pair(x, centroids, name):
@@ -184,8 +204,10 @@ def _check_xent(x, centroids, labels, scale, ignore_index, reduction, name):
         raise ValueError(f"{name}: labels have shape {tuple(labels.shape)}, x {tuple(x.shape)}")
     if labels.device != x.device:
         raise ValueError(f"{name}: x is on {x.device}, labels on {labels.device}")
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"{name}: scale must be positive and finite, got {scale}")
+    # as the kernels hold it: in float32, and times log2(e)
+    s32 = nat.ctypes.c_float(scale).value
+    if not (s32 > 0.0 and s32 * 1.44269504 <= torch.finfo(torch.float32).max):
+        raise ValueError(f"{name}: scale must be positive and finite in float32, got {scale}")
     if not -(1 << 63) <= ignore_index < 1 << 63:
         raise ValueError(f"{name}: ignore_index does not fit 64 bits: {ignore_index}")
     if reduction not in _REDUCTIONS:
@@ -198,7 +220,6 @@ class _Xent:
     __slots__ = ("x", "c", "labels", "shapes", "none", "at", "dev")
 
     def __init__(self, x, centroids, labels, scale, ignore_index, reduction, name):
-        scale, ignore_index = float(scale), int(ignore_index)
         tensors = isinstance(x, torch.Tensor) and isinstance(centroids, torch.Tensor) and isinstance(
             labels, torch.Tensor)
         if not tensors or not x.is_cuda:
@@ -310,7 +331,8 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
         centroids: (K, D) or (B, K, D), x's dtype.
         labels: (N,) or (B, N) int32 / int64 cluster ids, e.g. the ids that
             ``batch_kmeans_Euclid`` returns.
-        scale: positive factor of the scores (an inverse temperature).
+        scale: positive factor of the scores (an inverse temperature), a number:
+            multiply a learnable one into x.
         ignore_index: rows with this label count for nothing, whatever x holds
             there: loss 0, no gradient, not in the mean's denominator.
         reduction: 'mean' over the rows that are not ignored (NaN if there are
@@ -325,6 +347,7 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
     [0, K) other than ``ignore_index`` makes the loss NaN.
     """
     _refuse_tangents("cluster_cross_entropy", x, centroids)
+    scale, ignore_index = _numbers("cluster_cross_entropy", scale, ignore_index)
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False)
                                     or getattr(centroids, "requires_grad", False)):
         return _ClusterCrossEntropy.apply(x, centroids, labels, scale, ignore_index, reduction)
@@ -345,6 +368,7 @@ def cluster_cross_entropy_grad(x: torch.Tensor, centroids: torch.Tensor, labels:
     """
     name = "cluster_cross_entropy_grad"
     _refuse_tangents(name, x, centroids, grad_loss)
+    scale, ignore_index = _numbers(name, scale, ignore_index)
     with torch.no_grad():
         call = _Xent(x, centroids, labels, scale, ignore_index, reduction, name)
         shape = x.shape[:-1] if call.none else ()

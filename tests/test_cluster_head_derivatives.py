@@ -118,3 +118,18 @@ def test_gradients_with_a_graph_can_still_be_used_as_values():
     x.grad = None
     fk.cluster_cross_entropy(x, c, y).backward()
     assert not x.grad.requires_grad
+
+
+# ---------------------------------------------------------- scale and ignore_index
+@pytest.mark.parametrize("fn", [fk.cluster_cross_entropy, fk.cluster_cross_entropy_grad])
+def test_a_learnable_scale_is_refused(fn):
+    """Its gradient would be dropped: a temperature multiplies x."""
+    x, c, y = _case()
+    for s in (torch.tensor(2.0, requires_grad=True), torch.nn.Parameter(torch.ones(1))):
+        with pytest.raises(TypeError, match="scale"):
+            fn(x, c, y, scale=s)
+        with pytest.raises(TypeError, match="scale"):
+            fn(x.requires_grad_(), c, y, scale=s)
+        x = x.detach()
+    with fwAD.dual_level(), pytest.raises(TypeError, match="scale"):
+        fn(x, c, y, scale=fwAD.make_dual(torch.tensor(2.0), torch.tensor(1.0)))

@@ -219,3 +219,34 @@ def test_int8_entry_point_checks(lib):
     ok = lib.fk_int8_workspace_size(P, P, 6, 1, 300, 300, 128, L3(0, 128, 1), L3(0, 128, 1), 0)
     odd = lib.fk_int8_workspace_size(P, P, 6, 1, 300, 300, 100, L3(0, 100, 1), L3(0, 100, 1), 0)
     assert ok == 0 and odd >= 600 * 112
+
+
+class _Unread(torch.Tensor):
+    """A scalar whose value may not be fetched, as a GPU's cannot without waiting for it."""
+    is_cuda = property(lambda self: True)
+
+    def __float__(self):
+        raise AssertionError("fetched")
+
+    __int__ = __index__ = item = __float__
+
+
+@pytest.mark.parametrize("fn", [fk.cluster_cross_entropy, fk.cluster_cross_entropy_grad])
+@pytest.mark.parametrize("kw", [dict(scale=torch.tensor(2.0).as_subclass(_Unread)),
+                                dict(ignore_index=torch.tensor(3).as_subclass(_Unread))])
+def test_a_scalar_on_a_gpu_is_not_fetched(fn, kw):
+    with pytest.raises(TypeError, match=next(iter(kw))):
+        fn(_cuda(X), _cuda(C), Y, **kw)
+
+
+@pytest.mark.parametrize("fn", [fk.cluster_cross_entropy, fk.cluster_cross_entropy_grad])
+@pytest.mark.parametrize("kw,err,match", [
+    (dict(scale=3.0e38), ValueError, "positive and finite"),     # times log2(e): past float32
+    (dict(scale=1e39), ValueError, "positive and finite"),
+    (dict(scale=1e-46), ValueError, "positive and finite"),      # 0 in float32
+    (dict(ignore_index=0.5), TypeError, "ignore_index"),
+    (dict(ignore_index=float("nan")), TypeError, "ignore_index"),
+])
+def test_values_that_the_kernels_cannot_hold(fn, kw, err, match):
+    with pytest.raises(err, match=match):
+        fn(_cuda(X), _cuda(C), Y, **kw)

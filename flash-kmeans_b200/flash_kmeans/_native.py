@@ -16,7 +16,7 @@ LIB_NAME = "libflashkmeans_b200.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", LIB_NAME)
 
 FK_F16, FK_BF16, FK_F32, FK_I32, FK_I64 = 0, 1, 2, 3, 4
-FK_I8 = 6
+FK_I8 = 6   # the cluster head's entry points only: not in the table below
 FK_F32_XSPLIT = 5   # float32 x split once into tf32 halves (the *_accumulate entry points)
 # Widest rows for which the drivers use FK_F32_XSPLIT: measured 11 % faster at
 # D = 128 and 256, 4 % at 512, no faster at 2048 (there the stages are fed from
@@ -48,7 +48,6 @@ _DTYPE_CODE = {
     torch.float32: FK_F32,
     torch.int32: FK_I32,
     torch.int64: FK_I64,
-    torch.int8: FK_I8,
 }
 
 _P = ctypes.c_void_p

@@ -450,7 +450,7 @@ class _ScoresLayout:
         (B, N, D), xs = _three(x)
         (_, K, _), cs = _three(centroids)
         self.lib = nat.load()
-        self.x_code = nat.dtype_code(x.dtype)
+        self.x_code = nat.FK_I8 if x.dtype == torch.int8 else nat.dtype_code(x.dtype)
         self.sizes = (B, N, K, D)
         self.kept = [None if s is None else _Strides(s) for s in (
             xs, cs, *(None if t is None else _two(t) for t in (x_scale, c_scale, bias)))]

@@ -250,3 +250,16 @@ def test_a_scalar_on_a_gpu_is_not_fetched(fn, kw):
 def test_values_that_the_kernels_cannot_hold(fn, kw, err, match):
     with pytest.raises(err, match=match):
         fn(_cuda(X), _cuda(C), Y, **kw)
+
+
+def test_int8_points_are_still_a_type_error_in_k_means():
+    """8-bit integers are the cluster head's alone."""
+    from flash_kmeans import _native, _ops
+    from flash_kmeans.assign_euclid_triton import euclid_assign
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        _native.dtype_code(torch.int8)
+    xq, cq = _cuda(XQ[None]), _cuda(CQ[None])
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        euclid_assign(xq, cq, _cuda(torch.ones(1, 6)))
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        _ops.row_sqnorm(xq)

@@ -1,4 +1,5 @@
 """Cluster head: what is refused, and the host-only entry points (CPU only)."""
+import contextlib
 import ctypes
 
 import pytest
@@ -252,12 +253,13 @@ def test_values_that_the_kernels_cannot_hold(fn, kw, err, match):
         fn(_cuda(X), _cuda(C), Y, **kw)
 
 
-def test_int8_points_are_still_a_type_error_in_k_means():
+def test_int8_points_are_still_a_type_error_in_k_means(monkeypatch):
     """8-bit integers are the cluster head's alone."""
     from flash_kmeans import _native, _ops
     from flash_kmeans.assign_euclid_triton import euclid_assign
     with pytest.raises(TypeError, match="unsupported dtype"):
         _native.dtype_code(torch.int8)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
     xq, cq = _cuda(XQ[None]), _cuda(CQ[None])
     with pytest.raises(TypeError, match="unsupported dtype"):
         euclid_assign(xq, cq, _cuda(torch.ones(1, 6)))

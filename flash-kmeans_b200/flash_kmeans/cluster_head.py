@@ -510,6 +510,20 @@ def _check_out(out, shape, dtype, device, name):
         raise ValueError(f"{name}: x is on {device}, out on {out.device}")
     if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
         raise ValueError(f"{name}: out must not be expanded, its elements share memory")
+    reach = 0      # of the dimensions with smaller strides
+    for s, n in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
+        if s <= reach and 0 not in out.shape:
+            raise ValueError(f"{name}: out must not overlap itself, got strides {out.stride()}")
+        reach += s * (n - 1)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: out must not require grad, the results have none")
+
+
+def _written(out):
+    """Kernels wrote it through its pointer: for autograd, it has changed in place."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
 
 
 def _fold_strides(out, name):
@@ -537,12 +551,15 @@ def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
         bias: optional float32 (K,) or (B, K), like ``c_scale``.
         out_dtype: float16, bfloat16 or float32 (default: x's dtype, float32 for
             int8 x).
-        out: optional (N, K) or (B, N, K) output with rows of unit stride.
+        out: optional (N, K) or (B, N, K) output with rows of unit stride, which
+            shares no memory with itself or with the inputs.
     Returns:
         The scores.  The integer sum is exact; scaling is float32 in the order
-        above, rounded once to ``out_dtype``.
+        above, rounded once to ``out_dtype``.  They carry no gradient, whatever
+        the inputs require.
     """
     name = "int8_scores"
+    given = out is not None
     q = _Scores(x, centroids, c_scale, x_scale, bias, False, name)
     if out_dtype is None:
         out_dtype = out.dtype if out is not None else x.dtype if x.dtype in _FLOATS else torch.float32
@@ -565,7 +582,7 @@ def int8_scores(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
     ws, ws_ptr, nbytes = q.workspace()
     _call(q.at.lib.fk_int8_scores, "fk_int8_scores", q.dev, *q.pointers(), out.data_ptr(), q.at.x_code,
           nat.dtype_code(out_dtype), *q.at.sizes, *q.at.strides, strides.at, ws_ptr, nbytes)
-    return out
+    return _written(out) if given else out
 
 
 def int8_assign(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor, *,
@@ -579,6 +596,7 @@ def int8_assign(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
     to the lowest index, a NaN score counts as the largest.
     """
     name = "int8_assign"
+    given = out is not None
     q = _Scores(x, centroids, c_scale, x_scale, bias, True, name)
     if out is None:
         out = x.new_empty(q.lead, dtype=torch.int32)
@@ -593,4 +611,4 @@ def int8_assign(x: torch.Tensor, centroids: torch.Tensor, c_scale: torch.Tensor,
     ws, ws_ptr, nbytes = q.workspace()
     _call(q.at.lib.fk_int8_assign, "fk_int8_assign", q.dev, *q.pointers(), out.data_ptr(), q.at.x_code,
           *q.at.sizes, *q.at.strides, strides.at, ws_ptr, nbytes)
-    return out
+    return _written(out) if given else out

@@ -265,3 +265,57 @@ def test_int8_points_are_still_a_type_error_in_k_means(monkeypatch):
         euclid_assign(xq, cq, _cuda(torch.ones(1, 6)))
     with pytest.raises(TypeError, match="unsupported dtype"):
         _ops.row_sqnorm(xq)
+
+
+@pytest.fixture
+def _no_launch(monkeypatch):
+    from flash_kmeans import cluster_head as ch
+    monkeypatch.setattr(ch, "_call", lambda *args: None)
+
+
+@pytest.mark.parametrize("fn,out", [(fk.int8_scores, torch.zeros(6, 4)),
+                                    (fk.int8_assign, torch.zeros(6, dtype=torch.int32))])
+def test_a_written_out_counts_as_changed(_no_launch, fn, out):
+    """What autograd saved of it is not what it holds any more."""
+    w = torch.ones(out.shape, requires_grad=True)
+    later = (w * out).sum()
+    before = out._version
+    assert fn(_cuda(X), _cuda(CQ), CS, out=out) is out
+    assert out._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        later.backward()
+
+
+@pytest.mark.parametrize("fn,bad,good", [
+    (fk.int8_scores,
+     [torch.zeros(9).as_strided((6, 4), (1, 1)), torch.zeros(24).as_strided((6, 4), (3, 1)),
+      torch.zeros(6, 4, requires_grad=True)],
+     [torch.zeros(6, 4), torch.zeros(12, 9)[::2, 3:7], torch.zeros(1, 4).expand(1, 4),
+      torch.zeros(3, 6, 4)[1]]),
+    (fk.int8_assign,
+     [torch.zeros(1, dtype=torch.int32).expand(6)],
+     [torch.zeros(6, dtype=torch.int32), torch.zeros(12, 3, dtype=torch.int32)[::2, 1],
+      torch.zeros(6, 6, dtype=torch.int32).diagonal()]),
+])
+def test_out_has_elements_of_its_own(_no_launch, fn, bad, good):
+    for out in bad:
+        with pytest.raises(ValueError, match="out must not"):
+            fn(_cuda(X), _cuda(CQ), CS, out=out)
+    for out in good:
+        x = X[: out.shape[0]]
+        assert fn(_cuda(x), _cuda(CQ), CS, out=out) is out
+
+
+def test_batched_outputs_have_elements_of_their_own(_no_launch):
+    xb, cb, sb = torch.randn(3, 6, 8), torch.zeros(3, 4, 8, dtype=torch.int8), torch.ones(3, 4)
+    for out in (torch.zeros(3, 6, 4), torch.zeros(6, 3, 4).transpose(0, 1), torch.zeros(3, 8, 9)[:, 1:7, 2:6]):
+        assert fk.int8_scores(_cuda(xb), _cuda(cb), sb, out=out) is out
+    for out in (torch.zeros(60).as_strided((3, 6, 4), (8, 4, 1)), torch.zeros(90).as_strided((3, 6, 4), (4, 4, 1))):
+        with pytest.raises(ValueError, match="out must not"):
+            fk.int8_scores(_cuda(xb), _cuda(cb), sb, out=out)
+    ids = torch.zeros(40, dtype=torch.int32).as_strided((3, 6), (5, 1))
+    with pytest.raises(ValueError, match="out must not"):
+        fk.int8_assign(_cuda(xb), _cuda(cb), sb, out=ids)
+    with torch.no_grad():       # no graph that the writing could spoil
+        out = torch.zeros(6, 4, requires_grad=True)
+        assert fk.int8_scores(_cuda(X), _cuda(CQ), CS, out=out) is out

@@ -321,6 +321,16 @@ class _ClusterCrossEntropy(torch.autograd.Function):
         return gx, gc, None, None, None, None
 
 
+def _autocast(x, centroids):
+    """Under autocast, operands of two float types meet in its type, as a matrix
+    product's do; equal types stay."""
+    dtypes = [getattr(t, "dtype", None) for t in (x, centroids)]
+    if dtypes[0] != dtypes[1] and all(t in _FLOATS for t in dtypes):
+        low = torch.get_autocast_dtype("cuda")
+        x, centroids = x.to(low), centroids.to(low)
+    return x, centroids
+
+
 def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torch.Tensor, *,
                           scale: float = 1.0, ignore_index: int = -100,
                           reduction: str = "mean") -> torch.Tensor:
@@ -328,7 +338,8 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
 
     Args:
         x: (N, D) or (B, N, D) float16 / bfloat16 / float32 CUDA tensor.
-        centroids: (K, D) or (B, K, D), x's dtype.
+        centroids: (K, D) or (B, K, D), x's dtype; under autocast also another
+            float type (both are then cast to autocast's).
         labels: (N,) or (B, N) int32 / int64 cluster ids, e.g. the ids that
             ``batch_kmeans_Euclid`` returns.
         scale: positive factor of the scores (an inverse temperature), a number:
@@ -348,6 +359,8 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
     """
     _refuse_tangents("cluster_cross_entropy", x, centroids)
     scale, ignore_index = _numbers("cluster_cross_entropy", scale, ignore_index)
+    if torch.is_autocast_enabled("cuda"):
+        x, centroids = _autocast(x, centroids)
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False)
                                     or getattr(centroids, "requires_grad", False)):
         return _ClusterCrossEntropy.apply(x, centroids, labels, scale, ignore_index, reduction)

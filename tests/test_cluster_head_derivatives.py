@@ -133,3 +133,39 @@ def test_a_learnable_scale_is_refused(fn):
         x = x.detach()
     with fwAD.dual_level(), pytest.raises(TypeError, match="scale"):
         fn(x, c, y, scale=fwAD.make_dual(torch.tensor(2.0), torch.tensor(1.0)))
+
+
+# ---------------------------------------------------------------- mixed precision
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16])
+def test_autocast_takes_16_bit_points_with_float32_centroids(low, monkeypatch):
+    """Activations of an autocast layer against a head kept in float32."""
+    seen = []
+
+    class Seen(_Formula):
+        def __init__(self, x, centroids, *rest):
+            seen.append((x.dtype, centroids.dtype))
+            if x.dtype != centroids.dtype:
+                raise TypeError("refused")
+            super().__init__(x, centroids, *rest)
+
+    monkeypatch.setattr(ch, "_Xent", Seen)
+    x, c, y = _case()
+    x, c = x.to(low).requires_grad_(), c.float().requires_grad_()
+    with torch.autocast("cuda", dtype=low), torch.autocast("cpu", enabled=False):
+        loss = fk.cluster_cross_entropy(x, c, y)
+        assert seen[-1] == (low, low)
+        with torch.no_grad():
+            fk.cluster_cross_entropy(x, c, y)
+        assert seen[-1] == (low, low)
+        fk.cluster_cross_entropy(c.detach(), c, torch.tensor([0, 1, 2, 3]))
+        assert seen[-1] == (torch.float32, torch.float32)      # equal types stay
+        with pytest.raises(TypeError):                         # no type of the head's
+            fk.cluster_cross_entropy(x.detach().double(), c, y)
+        with pytest.raises(TypeError):                         # its gradients have their inputs' types
+            fk.cluster_cross_entropy_grad(x, c, y)
+    loss.backward()
+    assert x.grad.dtype == low and c.grad.dtype == torch.float32
+    want = torch.autograd.grad(torch.nn.functional.cross_entropy(x @ c.to(low).T, y), (x, c))
+    assert torch.equal(x.grad, want[0]) and torch.equal(c.grad, want[1])
+    with pytest.raises(TypeError):                             # outside of autocast
+        fk.cluster_cross_entropy(x, c, y)

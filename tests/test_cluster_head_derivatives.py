@@ -151,21 +151,24 @@ def test_autocast_takes_16_bit_points_with_float32_centroids(low, monkeypatch):
     monkeypatch.setattr(ch, "_Xent", Seen)
     x, c, y = _case()
     x, c = x.to(low).requires_grad_(), c.float().requires_grad_()
-    with torch.autocast("cuda", dtype=low), torch.autocast("cpu", enabled=False):
-        loss = fk.cluster_cross_entropy(x, c, y)
-        assert seen[-1] == (low, low)
-        with torch.no_grad():
-            fk.cluster_cross_entropy(x, c, y)
-        assert seen[-1] == (low, low)
-        fk.cluster_cross_entropy(c.detach(), c, torch.tensor([0, 1, 2, 3]))
-        assert seen[-1] == (torch.float32, torch.float32)      # equal types stay
-        with pytest.raises(TypeError):                         # no type of the head's
-            fk.cluster_cross_entropy(x.detach().double(), c, y)
-        with pytest.raises(TypeError):                         # its gradients have their inputs' types
-            fk.cluster_cross_entropy_grad(x, c, y)
+    # (torch.autocast("cuda") turns itself off where there is no GPU)
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device: device == "cuda")
+    monkeypatch.setattr(torch, "get_autocast_dtype", lambda device: low)
+    loss = fk.cluster_cross_entropy(x, c, y)
+    assert seen[-1] == (low, low)
+    with torch.no_grad():
+        fk.cluster_cross_entropy(x, c, y)
+    assert seen[-1] == (low, low)
+    fk.cluster_cross_entropy(c.detach(), c, torch.tensor([0, 1, 2, 3]))
+    assert seen[-1] == (torch.float32, torch.float32)      # equal types stay
+    with pytest.raises(TypeError):                         # no type of the head's
+        fk.cluster_cross_entropy(x.detach().double(), c, y)
+    with pytest.raises(TypeError):                         # its gradients have their inputs' types
+        fk.cluster_cross_entropy_grad(x, c, y)
     loss.backward()
     assert x.grad.dtype == low and c.grad.dtype == torch.float32
     want = torch.autograd.grad(torch.nn.functional.cross_entropy(x @ c.to(low).T, y), (x, c))
     assert torch.equal(x.grad, want[0]) and torch.equal(c.grad, want[1])
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device: False)
     with pytest.raises(TypeError):                             # outside of autocast
         fk.cluster_cross_entropy(x, c, y)

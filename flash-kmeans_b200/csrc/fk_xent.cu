@@ -455,12 +455,36 @@ __global__ void xent_weight_kernel(const float* g, const RowStat* stat, int64_t 
 // ------------------------------------------------------------ rows that count
 // The rows that are not ignored, in order (map[r] is the r-th of them) and how
 // many there are; the losses, statistics and gradients of the others, where
-// wanted, are set to zero here.  A block
-// counts what lies before its segment by itself: segments are few, and reading
-// labels again is cheaper than a second launch.
+// wanted, are set to zero here.  A block has a segment of the rows.  What lies
+// before it is counted by a launch in front (`counts`, one a segment) or, where
+// the labels are few, by the block itself.
 constexpr int kLiveThreads = 1024;
+constexpr int kLiveSegments = 128;
+
+// Sum of all threads' v, in the first warp's lanes.
+__device__ __forceinline__ int block_count(int v, int (&sm)[32]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  v = __reduce_add_sync(0xffffffffu, v);
+  if (lane == 0) sm[warp] = v;
+  __syncthreads();
+  return warp == 0 ? __reduce_add_sync(0xffffffffu, sm[lane]) : 0;
+}
+
+__global__ void __launch_bounds__(kLiveThreads) xent_count_kernel(const Labels y, int64_t N, int64_t segment,
+                                                                  int32_t* counts) {
+  __shared__ int sm[32];
+  pdl_wait_then_release();
+  const int64_t first = blockIdx.x * segment, last = min(first + segment, N);
+  int n = 0;
+#pragma unroll 4
+  for (int64_t i = first + threadIdx.x; i < last; i += kLiveThreads)
+    n += load_label(y.p, i * y.sn, y.dtype) != y.ignore;
+  n = block_count(n, sm);
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
 
 __global__ void __launch_bounds__(kLiveThreads) xent_live_kernel(const Labels y, int64_t N, int64_t segment,
+                                                                 const int32_t* counts,
                                                                  int32_t* map, int32_t* live, float* loss,
                                                                  RowStat* stat, void* gx, int64_t gx_row,
                                                                  int64_t gx_bytes, int gx_vec) {
@@ -470,16 +494,14 @@ __global__ void __launch_bounds__(kLiveThreads) xent_live_kernel(const Labels y,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t first = blockIdx.x * segment, last = min(first + segment, N);
   int before = 0;
+  if (counts) {
+    if (tid < static_cast<int>(blockIdx.x)) before = counts[tid];
+  } else {
 #pragma unroll 4
-  for (int64_t n = tid; n < first; n += kLiveThreads) before += load_label(y.p, n * y.sn, y.dtype) != y.ignore;
-  before = __reduce_add_sync(0xffffffffu, before);
-  if (lane == 0) sm[warp] = before;
-  __syncthreads();
-  if (tid == 0) {
-    int t = 0;
-    for (int w = 0; w < 32; ++w) t += sm[w];
-    base = t;
+    for (int64_t n = tid; n < first; n += kLiveThreads) before += load_label(y.p, n * y.sn, y.dtype) != y.ignore;
   }
+  before = block_count(before, sm);
+  if (tid == 0) base = before;
   __syncthreads();
   for (int64_t n0 = first; n0 < last; n0 += kLiveThreads) {
     const int64_t n = n0 + tid;
@@ -603,23 +625,48 @@ static int check_workspace(const void* ws, size_t have, size_t need, const char*
   return FK_OK;
 }
 
-// Whether ignored rows are left out of the products.  Finding and gathering them
-// takes 20 to 30 us at 16384 rows (25 of 470 us were lost at 32444 x 8192 x 128
-// with none ignored); from 2^36 products on, 0.1 ms forward and 0.4 ms with the
-// gradients, a tenth or a twentieth of ignored rows gives that back.  Separate
-// codebooks keep one block of rows for each batch, and go without.
+// Whether ignored rows are left out of the products.  Finding them takes 10 us;
+// where x is copied in any case (the backward pass, float32) gathering adds
+// nothing to that.  Loss and gradients with none / a tenth / half of the rows
+// ignored, gathered to not: 16384 x 8192 x 512 bfloat16 1.00 / 0.98 / 0.63, 65536
+// x 256 x 4096 1.06 / 1.00 / 0.65; the largest loss seen, 1.10 / 1.02 / 0.67, was at
+// 2^20 x 1024 x 128.  Below 2^36 products a call is too short for the 10 us.
+// Separate codebooks keep one block of rows for each batch, and go without.
 static bool gathers(const Xent& q) { return q.B == 1 && q.N >= 1024 && q.N * q.K >= (1ll << 36) / q.D; }
+
+// The forward pass alone reads 16-bit rows in place, and gathering them costs a
+// copy of x, which does not shrink with the centroids as the products do: with
+// none / a tenth / half of the rows ignored, gathered to not, 65536 x 256 x 4096
+// takes 1.89 / 1.85 / 1.27, 65536 x 1024 x 1024 1.45 / 1.43 / 0.97, 65536 x 4096 x 1024
+// 1.15 / 1.2 / 0.70, 16384 x 8192 x 512 1.13 / 1.12 / 0.73, 16384 x 32768 x 1024 1.04 /
+// 1.0 / 0.58.
+static bool gathers_forward(const Xent& q) {
+  return gathers(q) && (q.K >= 8192 || !in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs));
+}
+
+// The rows' indices, their number, and the segments' counts.
+static int64_t map_words(const Xent& q) { return q.N + 1 + kLiveSegments; }
+
+// Rows up to which a block counts all labels before its own: the last one reads
+// nearly all of them, which takes longer than a launch that counts them from
+// 65536 int64 labels on (5 us longer; 25 at 262144, 125 at 2^20; none at 16384).
+constexpr int64_t kLiveAlone = 32768;
 
 // Finds the rows that count: map gets N + 1 words, their number the last.
 static int find_live(const Xent& q, int32_t* map, float* loss, RowStat* stat, void* gx, int64_t gx_row,
                      cudaStream_t s) {
-  // at most 128 segments, as a block reads every label before its own
-  const int64_t segment = ceil_div(ceil_div(q.N, 128), kLiveThreads) * kLiveThreads;
+  const int64_t segment = ceil_div(ceil_div(q.N, kLiveSegments), kLiveThreads) * kLiveThreads;
+  const dim3 blocks(static_cast<unsigned>(ceil_div(q.N, segment)));
+  int32_t* counts = q.N > kLiveAlone ? map + q.N + 1 : nullptr;
+  if (counts) {
+    const int st = launch_plain("xent_count_kernel", xent_count_kernel, blocks, kLiveThreads, s, q.y, q.N, segment,
+                                counts);
+    if (st != FK_OK) return st;
+  }
   const int64_t eb = dtype_bytes(q.dtype);
   const bool vec = reinterpret_cast<uintptr_t>(gx) % 16 == 0 && gx_row * eb % 16 == 0 && q.D * eb % 16 == 0;
-  return launch_plain("xent_live_kernel", xent_live_kernel, dim3(static_cast<unsigned>(ceil_div(q.N, segment))),
-                      kLiveThreads, s, q.y, q.N, segment, map, map + q.N, loss, stat, gx, gx_row * eb, q.D * eb,
-                      vec ? 1 : 0);
+  return launch_plain("xent_live_kernel", xent_live_kernel, blocks, kLiveThreads, s, q.y, q.N, segment, counts, map,
+                      map + q.N, loss, stat, gx, gx_row * eb, q.D * eb, vec ? 1 : 0);
 }
 
 // Copies of the operands made by the caller of a pass; see fk_xent_loss_grad.
@@ -647,12 +694,13 @@ static ForwardPlan plan_forward(const Xent& q, void* ws, const Copies* given = n
   f.chunks = choose_chunks(q.B * ceil_div(q.N, f.sh.bm()), ceil_div(q.K, f.sh.bn), slots_of(f.sh),
                            2 * slots_of(f.sh), 0.25);
   f.row_blocks = ceil_div(q.N, 32);
-  f.map = given ? given->map : gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
+  const bool gather = given ? given->map != nullptr : gathers_forward(q);
+  f.map = given ? given->map : gather ? b.take<int32_t>(map_words(q)) : nullptr;
   if (given) {
     f.xc = given->x_forward;
     f.cc = given->c;
   } else {
-    f.xc = !gathers(q) && in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
+    f.xc = !gather && in_place(q.x, q.dtype, q.B, q.N, q.D, q.xs)
                ? nullptr
                : b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
     f.cc = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
@@ -843,7 +891,7 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
                ? nullptr
                : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());
   }
-  f.map = given ? given->map : gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
+  f.map = given ? given->map : gathers(q) ? b.take<int32_t>(map_words(q)) : nullptr;
   f.P = b.take<uint16_t>(q.parts() * q.B * f.R * f.Kp);
   f.acc_x = f.acc_c = nullptr;
   if (want_x && (f.n_pieces > 1 || f.split_x > 1)) f.acc_x = b.take<float>(f.split_x * q.B * q.N * f.ld);
@@ -1042,7 +1090,7 @@ static LossGradPlan plan_loss_grad(const Xent& q, bool want_x, bool want_c, void
   LossGradPlan f;
   Bump b{static_cast<uint8_t*>(ws)};
   f.copies.x_backward = b.take<uint16_t>(q.parts() * q.B * q.N * q.Dp());
-  f.copies.map = gathers(q) ? b.take<int32_t>(q.N + 1) : nullptr;
+  f.copies.map = gathers(q) ? b.take<int32_t>(map_words(q)) : nullptr;
   f.copies.c = in_place(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs)
                    ? nullptr
                    : b.take<uint16_t>(q.parts() * q.Bc() * q.K * q.Dp());

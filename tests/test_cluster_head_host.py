@@ -319,3 +319,16 @@ def test_batched_outputs_have_elements_of_their_own(_no_launch):
     with torch.no_grad():       # no graph that the writing could spoil
         out = torch.zeros(6, 4, requires_grad=True)
         assert fk.int8_scores(_cuda(X), _cuda(CQ), CS, out=out) is out
+
+
+def test_a_loss_over_few_centroids_copies_no_points(lib):
+    """Gathering the rows that count costs a copy of x, which few centroids do not
+    give back; the backward pass copies x in any case."""
+    def size(N, K, D, dtype=1, bx=0, bc=0):
+        return lib.fk_xent_workspace_size(P, P, dtype, 1, N, K, D, L3(N * D, D, 1), L3(K * D, D, 1), 1, bx, bc)
+    for N, K, D in ((65536, 256, 4096), (1 << 20, 64, 1024), (65536, 4096, 1024)):
+        assert size(N, K, D) < N * D             # (half a copy)
+        assert size(N, K, D, bx=1, bc=1) >= N * D * 2
+    assert size(16384, 32768, 1024) >= 16384 * 1024 * 2
+    # float32 is copied as its three parts, with or without
+    assert size(65536, 256, 4096, dtype=2) >= 65536 * 4096 * 6

@@ -71,7 +71,7 @@ struct Problem {
   // kEpiLse, kEpiGrad, kEpiOut: only the rows that are not ignored take part,
   // gathered; their number is known on the device alone
   const int32_t* live;      // that number; null: all rows
-  int live_off, live_cap;   // this chunk's first row, its rows at most
+  int live_off, live_cap;   // this chunk's first row (of all rows, with none), its rows at most
   int live_steps;           // the rows are the contraction, not the rows of A
   const int32_t* row_map;   // gathered row live_off + r is row row_map[live_off + r] of the call
 
@@ -93,6 +93,7 @@ struct Problem {
   float fscale;             // kEpiOut: factor, times *f_num, over max(*f_den, 1)
   const float* f_num;
   const int32_t* f_den;
+  const float* row_factor;  // and times that of the row, or null: [batch][stat_rows]
   float* acc;               // kEpiOut: float32 accumulator [split][batch][row][acc_ld]
   int64_t acc_ld, acc_batch, acc_split;
   int acc_read, acc_write;
@@ -836,11 +837,6 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     int label = -1;
     float xs = 0.0f;
     float fac = 0.0f;
-    if constexpr (EPI == kEpiOut) {
-      fac = p0.fscale;
-      if (p0.f_num) fac *= *p0.f_num;
-      if (p0.f_den) fac /= static_cast<float>(max(*p0.f_den, 1));
-    }
 
     // What the epilogue needs from memory besides the accumulator is fetched a
     // tile ahead: its latency would stand between the accumulator and its use.
@@ -871,6 +867,16 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const int rows = Walk<EPI, S::kBM>::rows_of(p);
       const bool row_ok = row < rows;
       const int col0 = t.n * BN + part * kCols;
+      if constexpr (EPI == kEpiOut) {
+        // (read at every tile: held for both problems, they would spill)
+        fac = p.fscale;
+        if (p.f_num) fac *= *p.f_num;
+        if (p.f_den) fac /= static_cast<float>(max(*p.f_den, 1));
+        if (p.row_factor && row_ok) {
+          const int n = p.live_off + row;
+          fac *= p.row_factor[t.b * p.stat_rows + (p.row_map ? p.row_map[n] : n)];
+        }
+      }
 
       if constexpr (EPI == kEpiLse) {
         if (t.first) {

@@ -409,46 +409,111 @@ __global__ void __launch_bounds__(kCombineWarps * 32) xent_combine_kernel(const 
 }
 
 // --------------------------------------------------------- row weights (none)
-// Losses that stay per row arrive with one upstream gradient each, which goes
-// into the row's weight.  For float16 the weights are taken relative to the
-// largest finite one, so that P stays within float16; it comes back as a factor
-// of the outputs.  The maximum of non-negative floats is the maximum of their
-// bits, whose order of arrival does not matter.
-__global__ void xent_gmax_kernel(const float* g, const RowStat* stat, int64_t rows, uint32_t* out) {
+// Losses that stay per row arrive with one upstream gradient g each, which goes
+// into the row's weight.
+__global__ void xent_weight_kernel(const float* g, const RowStat* stat, int64_t rows, RowStat* out) {
   pdl_wait_then_release();
-  uint32_t m = 0;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const uint32_t u = __float_as_uint(g[i]) & 0x7fffffffu;
-    if (u < 0x7f800000u && (stat[i].coef != 0.0f || stat[i].at_label != 0.0f)) m = max(m, u);
-  }
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0 && m) atomicMax(out, m);
-}
-
-__global__ void xent_weight_kernel(const float* g, const RowStat* stat, int64_t rows, const float* gmax,
-                                   RowStat* out, float* factor) {
-  pdl_wait_then_release();
-  // a power of two, so that the division is exact
-  float inv = 1.0f, f = 1.0f;
-  if (gmax && *gmax > 0.0f) {
-    int e;
-    frexpf(*gmax, &e);
-    e = min(max(e, -120), 120);
-    f = ldexpf(1.0f, e);
-    inv = ldexpf(1.0f, -e);
-  }
-  if (factor && blockIdx.x == 0 && threadIdx.x == 0) *factor = f;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < rows;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     RowStat st = stat[i];
     const bool ignored = st.label < 0 && st.coef == 0.0f;
     if (!ignored) {
-      const float w = g[i] * inv;
-      st.coef *= w;
-      st.at_label *= w;
+      st.coef *= g[i];
+      st.at_label *= g[i];
     }
     out[i] = st;
+  }
+}
+
+// float16 has 40 powers of two, which the softmax of one row alone can fill.  So
+// only the part of g within [1, 2) goes into P.  The power of two is a factor of
+// the row in dx; in dc, where the rows are summed, it goes into a copy of x:
+// relative to the largest power of two times |x| of all rows, which sits at the
+// upper end of float16 there (below 2^16; powers of two round nothing but what
+// falls under 2^-14).  Gradients of every size keep their softmax that way: with
+// g itself in P, a row whose gradient was 2^-20 of the largest lost the softmax
+// of 40000 centroids.  The two passes over x take 75 us of 728 at 65536 x 1024 x
+// 1024, 30 of 540 at 16384 x 8192 x 512.
+__device__ __forceinline__ float power_of_two(int e) {   // of a normal number
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// A warp has a row; `reach` is 512 + the largest exponent found, 0 for none.
+__global__ void xent_weight16_kernel(const float* g, const RowStat* stat, int64_t rows, RowStat* out,
+                                     float* power, const uint16_t* x, int Dp, const int32_t* map,
+                                     const int32_t* live, uint32_t* reach) {
+  pdl_wait_then_release();
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+  const int64_t used = live ? *live : rows;
+  uint32_t most = 0;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); r < used; r += warps) {
+    const int64_t i = map ? map[r] : r;
+    RowStat st = stat[i];
+    const bool ignored = st.label < 0 && st.coef == 0.0f;
+    const float w = ignored ? 0.0f : g[i];
+    const uint32_t bits = __float_as_uint(w) & 0x7fffffffu;
+    const bool finite = bits < 0x7f800000u && bits != 0;
+    // (a gradient below the normal numbers is left with 2^-126)
+    const int e = finite ? max(static_cast<int>(bits >> 23), 1) - 127 : 0;
+    if (lane == 0) {
+      if (!ignored) {
+        // (in two steps: 2^-127 is no normal number)
+        const float m = w * power_of_two(-(e / 2)) * power_of_two(e / 2 - e);
+        st.coef *= m;
+        st.at_label *= m;
+      }
+      out[i] = st;
+      power[i] = bits ? power_of_two(e) : 0.0f;
+    }
+    if (!x || !finite) continue;
+    uint32_t top = 0;
+    for (int d = lane * 8; d < Dp; d += 256) {
+      const uint4 u = *reinterpret_cast<const uint4*>(x + r * Dp + d);
+      const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = v[k] & 0x7fffu, hi = (v[k] >> 16) & 0x7fffu;
+        if (lo < 0x7c00u) top = max(top, lo);   // infinities and NaN stay what they are
+        if (hi < 0x7c00u) top = max(top, hi);
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (top == 0) continue;
+    int ex;
+    frexpf(__half2float(__ushort_as_half(static_cast<unsigned short>(top))), &ex);
+    most = max(most, static_cast<uint32_t>(512 + e + ex));
+  }
+  if (lane == 0 && most) atomicMax(reach, most);
+}
+
+__global__ void xent_scale16_kernel(const uint16_t* x, int64_t rows, int Dp, const float* power, const int32_t* map,
+                                    const int32_t* live, const uint32_t* reach, uint16_t* out, float* factor) {
+  pdl_wait_then_release();
+  // |x| 2^e < 2^E: what is written is below 2^16
+  const uint32_t most = *reach;
+  const int E = most ? max(static_cast<int>(most) - 512, -100) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *factor = power_of_two(E - 16);
+  const int per = Dp / 8;
+  const int64_t units = rows * per;
+  const int64_t used = live ? *live : rows;
+  for (int64_t u = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; u < units;
+       u += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = u / per;
+    if (r >= (used + 127) / 128 * 128) break;
+    // (rows of weight 0 are not among those that E bounds; behind the last row
+    // that counts the copy holds zeros)
+    const float w = r < used ? power[map ? map[r] : r] : 0.0f;
+    const int e = static_cast<int>(__float_as_uint(w) >> 23) - 127;
+    const float by = w > 0.0f ? power_of_two(min(max(e - E + 16, -126), 127)) : 0.0f;
+    uint4 v = reinterpret_cast<const uint4*>(x)[u];
+    __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __half22float2(h[k]);
+      h[k] = __floats2half2_rn(f.x * by, f.y * by);
+    }
+    reinterpret_cast<uint4*>(out)[u] = v;
   }
 }
 
@@ -810,7 +875,9 @@ struct BackwardPlan {
   int64_t joins;               // of both, from join_x on
   RowStat* weighted;
   int32_t* map;                // gathered rows, their number behind it
-  float* gmax;                 // (largest |g|, the factor it gives)
+  float* power;                // float16 row losses: each row's power of two,
+  uint32_t* reach;             // the largest with x's and the factor that it gives,
+  uint16_t* xs;                // and the copy of x that holds it
   size_t bytes;
 };
 
@@ -905,7 +972,10 @@ static BackwardPlan plan_backward(const Xent& q, bool want_x, bool want_c, void*
   f.join_x = f.joins ? b.take<uint32_t>(f.joins) : nullptr;
   f.join_c = f.join_x ? f.join_x + jx : nullptr;
   f.weighted = q.reduction == 0 ? b.take<RowStat>(q.B * q.N) : nullptr;
-  f.gmax = q.reduction == 0 ? b.take<float>(2) : nullptr;
+  const bool weigh16 = q.reduction == 0 && q.dtype == FK_F16;
+  f.power = weigh16 ? b.take<float>(q.B * q.N) : nullptr;
+  f.reach = weigh16 ? b.take<uint32_t>(2) : nullptr;
+  f.xs = weigh16 && want_c ? b.take<uint16_t>(q.B * q.N * q.Dp()) : nullptr;
   f.bytes = b.used;
   return f;
 }
@@ -958,7 +1028,8 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
   const int64_t rows = q.B * q.N;
   const bool f16 = q.dtype == FK_F16;
   // float16 P is kept times 2^14: a softmax over 2^20 centroids then still has
-  // ten bits above float16's smallest subnormal, and 1 * 2^14 is in range
+  // ten bits above float16's smallest subnormal, and 2 * 2^14 is in range (see
+  // xent_weight16_kernel)
   const float p_scale = f16 ? 16384.0f : 1.0f;
   int st = FK_OK;
   const int32_t* live = f.map ? f.map + q.N : nullptr;
@@ -971,19 +1042,25 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       st = rows_copy(q.dtype, xj, rows_job(q.c, q.dtype, q.Bc(), q.K, q.D, q.cs, f.cc, q.Dp(), nullptr), s);
   }
   if (st != FK_OK) return st;
-  const float* factor = q.reduction == 0 ? nullptr : g;
+  const float* factor_c = nullptr;
   if (q.reduction == 0) {
     const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(rows, 256), 1024));
-    if (f16) {
-      const cudaError_t e = cudaMemsetAsync(f.gmax, 0, 2 * sizeof(float), s);
+    if (f.power) {
+      const cudaError_t e = cudaMemsetAsync(f.reach, 0, 2 * sizeof(uint32_t), s);
       if (e != cudaSuccess) return fail(FK_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
-      st = launch_plain("xent_gmax_kernel", xent_gmax_kernel, dim3(blocks), 256, s, g, stat, rows,
-                        reinterpret_cast<uint32_t*>(f.gmax));
-      if (st != FK_OK) return st;
-      factor = f.gmax + 1;
+      const int many = static_cast<int>(std::min<int64_t>(ceil_div(rows, 8), 2048));
+      const int Dp = static_cast<int>(q.Dp());
+      st = launch_plain("xent_weight16_kernel", xent_weight16_kernel, dim3(many), 256, s, g, stat, rows, f.weighted,
+                        f.power, f.xs ? f.xc : nullptr, Dp, f.map, live, f.reach);
+      if (st == FK_OK && f.xs) {
+        factor_c = reinterpret_cast<const float*>(f.reach + 1);
+        const int wide = static_cast<int>(std::min<int64_t>(ceil_div(rows * (Dp / 8), 256), 2048));
+        st = launch_plain("xent_scale16_kernel", xent_scale16_kernel, dim3(wide), 256, s, f.xc, rows, Dp, f.power,
+                          f.map, live, f.reach, f.xs, reinterpret_cast<float*>(f.reach + 1));
+      }
+    } else {
+      st = launch_plain("xent_weight_kernel", xent_weight_kernel, dim3(blocks), 256, s, g, stat, rows, f.weighted);
     }
-    st = launch_plain("xent_weight_kernel", xent_weight_kernel, dim3(blocks), 256, s, g, stat, rows,
-                      f16 ? f.gmax : nullptr, f.weighted, f16 ? f.gmax + 1 : nullptr);
     if (st != FK_OK) return st;
     stat = f.weighted;
   }
@@ -1041,7 +1118,7 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       base.batches = static_cast<int>(q.B);
       base.status = status;
       base.fscale = q.scale / p_scale;
-      base.f_num = factor;
+      base.stat_rows = q.N;
       base.f_den = q.reduction == 1 ? count : nullptr;
       base.live = live;
       base.live_off = static_cast<int>(r0);
@@ -1051,15 +1128,19 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
         const Operand co = operand(q, q.c, f.cc, q.Bc(), q.K, q.cs, true, k0);
         base.live_steps = 0;
         base.row_map = f.map;
+        base.f_num = q.reduction == 0 ? nullptr : g;
+        base.row_factor = f.power;
         return grad_problem(q, pair, f.join_x, base, po, co, rw, kw, f.sh, f.split_x, f.acc_x, q.N, r0, f.ld,
                             piece == 0, piece + 1 == f.n_pieces, gx, r0);
       };
       auto add_c = [&]() {
         Operand pt = po;
         pt.mn = true;
-        const Operand xo = operand(q, q.x, f.xc, q.B, q.N, q.xs, true, r0);
+        const Operand xo = operand(q, q.x, f.xs ? f.xs : f.xc, q.B, q.N, q.xs, true, r0);
         base.live_steps = 1;
         base.row_map = nullptr;
+        base.f_num = q.reduction == 0 ? factor_c : g;
+        base.row_factor = nullptr;
         return grad_problem(q, pair, f.join_c, base, pt, xo, kw, rw, f.sh, f.split_c, f.acc_c, f.Kp, 0, f.ld,
                             chunk == 0, chunk + 1 == f.n_chunks, gc, k0);
       };

@@ -40,3 +40,109 @@ def test_rows_gathered_in_the_backward_pass_alone(live, N, K, D, dtype):
     rows = fk.cluster_cross_entropy(x, c, y, scale=4.0, reduction="none")
     assert rows[~keep].eq(0).all()
     close(rows[keep], reference(x[keep], c, y[keep], 4.0, "none")[0], "rows")
+
+
+def _row_gradients(x, c, y, scale, g):
+    """Gradients of float16 row losses in float64, with bounds that follow each row's
+    own weight.  P = w (softmax - one-hot) / 2^e with 1 <= |w| / 2^e < 2 is held in float16 times
+    2^14: half a step, or half the smallest subnormal (2^-25, hence 2^-39 |w| of the
+    gradient).  x in the centroids' gradient is held in float16 relative to the
+    largest |w| |x| of all rows, which lies between 2^14 and 2^16 there: off by
+    half the smallest subnormal, 2^-39 of that largest, times the softmax's 2."""
+    xd, cd, w = x.double(), c.double(), g.double()[:, None]
+    z = scale * xd @ cd.T
+    p = torch.softmax(z, -1)
+    own = torch.arange(len(y), device="cuda")
+    # 1 - p at the label as the sum of the others: exact where it is small
+    others = p.scatter(-1, y.long()[:, None], 0.0).sum(-1)
+    p[own, y.long()] = -others
+    ez = (scale * (xd.abs() @ cd.abs().T) * 2.0 ** -21).amax(-1, keepdim=True) + z.abs().amax(-1, keepdim=True) * 2.0 ** -22
+    off = p.abs() * (2 * ez + 2.0 ** -18 + 2.0 ** -11) + 2.0 ** -39
+    gx, gxt = scale * w * (p @ cd), scale * w.abs() * ((off + 2.0 ** -20 * p.abs()) @ cd.abs())
+    top = (w.abs() * xd.abs().amax(-1, keepdim=True)).max()
+    gc = scale * (p * w).T @ xd
+    gct = scale * ((off + 2.0 ** -20 * p.abs()) * w.abs()).T @ xd.abs() + scale * 2.0 ** -38 * top * p.abs().sum(0)[:, None]
+    step = lambda t: t.abs() * 2.0 ** -11 + 2.0 ** -25      # noqa: E731 (the outputs' own rounding)
+    return (gx, gxt + step(gx)), (gc, gct + step(gc))
+
+
+@pytest.mark.parametrize("N,K,D,ignored", [(64, 40000, 64, 0.0), (300, 131072, 24, 0.3), (1100, 60000, 1200, 0.2),
+                                           (65, 3, 8, 0.0)])
+@pytest.mark.parametrize("span", [20, 30])
+def test_float16_rows_of_small_weight_keep_their_softmax(N, K, D, ignored, span):
+    """One upstream gradient a row, over `span` powers of two; flat softmaxes of many
+    centroids, whose entries are small against the label's."""
+    gen = torch.Generator(device="cuda").manual_seed(43)
+    c = (torch.randn(K, D, device="cuda", generator=gen) * 0.1 + 0.3).half()
+    x = (torch.randn(N, D, device="cuda", generator=gen) * 0.02).half()
+    y = torch.randint(0, K, (N,), device="cuda", generator=gen)
+    g = torch.exp2(12.0 - span * torch.linspace(0, 1, N, device="cuda")) * (1 + torch.rand(N, device="cuda", generator=gen))
+    g[1::3] *= -1
+    keep = torch.rand(N, device="cuda", generator=gen) >= ignored
+    keep[[0, -1]] = True
+    y = y.masked_fill(~keep, -100)
+    g[~keep] = 3e38                          # (an ignored row's counts for nothing)
+    x[~keep] = float("nan")
+    _, gx, gc = fk.cluster_cross_entropy_grad(x, c, y, scale=0.5, reduction="none", grad_loss=g)
+    wx, wc = _row_gradients(x[keep], c, y[keep], 0.5, g[keep])
+    close(gx[keep], wx, "gx")
+    assert gx[~keep].eq(0).all()
+    close(gc, wc, "gc")
+    xr, cr = x.clone().requires_grad_(), c.clone().requires_grad_()
+    fk.cluster_cross_entropy(xr, cr, y, scale=0.5, reduction="none").backward(g)
+    close(xr.grad[keep], wx, "gx of autograd")
+    close(cr.grad, wc, "gc of autograd")
+    for t in (x, c):                         # one alone
+        a = t.clone().requires_grad_()
+        fk.cluster_cross_entropy(a if t is x else x, a if t is c else c, y, scale=0.5, reduction="none").backward(g)
+        close(a.grad[keep] if t is x else a.grad, wx if t is x else wc, "alone")
+
+
+def test_float16_row_weights_of_every_kind():
+    """Zero, infinite and NaN upstream gradients, the largest and the smallest."""
+    gen = torch.Generator(device="cuda").manual_seed(44)
+    c = torch.randn(90, 40, device="cuda", generator=gen).half()
+    x = torch.randn(2, 50, 40, device="cuda", generator=gen).half()
+    y = torch.randint(0, 90, (2, 50), device="cuda", generator=gen)
+    zero = torch.zeros(2, 50, device="cuda")
+    _, gx, gc = fk.cluster_cross_entropy_grad(x, c.expand(2, 90, 40), y, reduction="none", grad_loss=zero)
+    assert gx.eq(0).all() and gc.eq(0).all()
+    for big, tiny in ((1.0, 1e-45), (2.0 ** 127, 2.0 ** -126), (1e-30, 1e-40)):
+        g = zero.clone()
+        g[0, 3], g[1, 7] = big, tiny
+        _, gx, gc = fk.cluster_cross_entropy_grad(x, c.expand(2, 90, 40), y, scale=1 / big, reduction="none",
+                                                  grad_loss=g)
+        _, ex, ec = fk.cluster_cross_entropy_grad(x, c.expand(2, 90, 40), y, scale=1 / big, reduction="none",
+                                                  grad_loss=torch.where(g == tiny, 0.0, g))
+        assert torch.isfinite(gx).all() and torch.isfinite(gc).all()
+        assert gx[0, 3].abs().sum() > 0 and torch.equal(gx, ex)      # (the tiny one's underflows)
+        assert torch.equal(gc, ec)
+    for bad in (float("inf"), float("nan")):
+        g = torch.ones(2, 50, device="cuda")
+        g[1, 9] = bad
+        _, gx, gc = fk.cluster_cross_entropy_grad(x, c.expand(2, 90, 40), y, reduction="none", grad_loss=g)
+        _, ex, ec = fk.cluster_cross_entropy_grad(x, c.expand(2, 90, 40), y, reduction="none",
+                                                  grad_loss=torch.ones_like(g))
+        keep = torch.ones(2, 50, dtype=torch.bool, device="cuda")
+        keep[1, 9] = False
+        assert not torch.isfinite(gx[1, 9]).any() and torch.equal(gx[keep], ex[keep])
+        assert not torch.isfinite(gc[1]).all() and torch.equal(gc[0], ec[0])
+
+
+def test_float16_rows_of_no_weight_beside_small_ones():
+    """Rows of weight 0 take no part in the scale of the others', however large they are."""
+    gen = torch.Generator(device="cuda").manual_seed(45)
+    c = torch.randn(500, 72, device="cuda", generator=gen).half()
+    x = torch.randn(400, 72, device="cuda", generator=gen).half()
+    y = torch.randint(0, 500, (400,), device="cuda", generator=gen, dtype=torch.int32)
+    g = torch.full((400,), 2.0 ** -40, device="cuda")
+    g[::2] = 0.0
+    x[::2] *= 1000.0
+    _, gx, gc = fk.cluster_cross_entropy_grad(x, c, y, scale=2.0 ** 20, reduction="none", grad_loss=g)
+    one = torch.ones_like(g)
+    _, ex, ec = fk.cluster_cross_entropy_grad(x[1::2], c, y[1::2], scale=2.0 ** 20, reduction="none",
+                                              grad_loss=one[1::2] * 2.0 ** -40)
+    assert gx[::2].eq(0).all() and torch.isfinite(gx).all() and torch.isfinite(gc).all()
+    assert gx[1::2].abs().max() > 0 and gc.abs().max() > 0
+    # the same sums of the same values; a scale this large makes softmaxes one-hot
+    assert torch.equal(gx[1::2], ex) and torch.equal(gc, ec)

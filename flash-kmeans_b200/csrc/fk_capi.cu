@@ -109,7 +109,7 @@ extern "C" const char* fk_status_string(int status) {
     case FK_ERR_CUDA: return "CUDA error";
     case FK_ERR_TMA: return "tensor map encoding failed";
     case FK_DEV_BAD_LABEL: return "cluster id outside [0, K)";
-    case FK_DEV_WAIT_TIMEOUT: return "assignment pipeline wait timed out";
+    case FK_DEV_WAIT_TIMEOUT: return "a kernel's pipeline wait timed out: what that call wrote is not valid";
     default: return "unknown status";
   }
 }

@@ -88,7 +88,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
     if (*abort_flag) return false;
     if (globaltimer_ns() - t0 > FK_WAIT_LIMIT_NS) {
       *abort_flag = code;
-      if (dev_status) atomicCAS(dev_status, 0, code);
+      if (dev_status) atomicMax(dev_status, code);  // (the gravest stays)
       return false;
     }
   }
@@ -296,7 +296,7 @@ __device__ __forceinline__ bool mbar_wait_at(uint32_t bar, uint32_t parity, vola
     if (*abort_flag) return false;
     if (globaltimer_ns() - t0 > FK_WAIT_LIMIT_NS) {
       *abort_flag = code;
-      if (dev_status) atomicCAS(dev_status, 0, code);
+      if (dev_status) atomicMax(dev_status, code);  // (the gravest stays)
       return false;
     }
   }

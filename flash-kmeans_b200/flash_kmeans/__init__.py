@@ -14,6 +14,7 @@ from .centroid_update_triton import (
     triton_centroid_update_sorted_euclid,
 )
 from .kmeans_large import kmeans_largeN, kmeans_largeN_assign
+from ._ops import DeviceStatus
 from .cluster_head import (
     cluster_cross_entropy,
     cluster_cross_entropy_grad,

@@ -97,7 +97,8 @@ def row_normalize(x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Ten
 
 
 class DeviceStatus:
-    """Per-device int32 word that kernels set on asynchronous errors."""
+    """Per-device int32 word that kernels set on asynchronous errors; the gravest
+    stays.  Nothing reads it by itself: that would wait for the device."""
 
     _words: dict = {}
 
@@ -113,6 +114,8 @@ class DeviceStatus:
 
     @classmethod
     def raise_if_set(cls, device) -> None:
+        """Wait for the device; raise RuntimeError and clear the word if a call since the
+        last time met a cluster id out of range or a pipeline wait that ran out."""
         w = cls.word(device)
         code = int(w[0].item())
         if code:

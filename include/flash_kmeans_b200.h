@@ -78,11 +78,12 @@ enum fk_status {
   FK_ERR_TMA = 5          /* tensor-map encoding failed */
 };
 
-/* device-side codes written to *dev_status (first error wins) */
+/* device-side codes written to *dev_status; the gravest (largest) stays until
+ * the caller clears the word */
 enum fk_device_status {
   FK_DEV_OK = 0,
-  FK_DEV_BAD_LABEL = 101,      /* a cluster id outside [0, K) was fed to the update */
-  FK_DEV_WAIT_TIMEOUT = 102    /* a pipeline wait in the assign kernel exceeded its limit */
+  FK_DEV_BAD_LABEL = 101,      /* a cluster id outside [0, K) was fed to a kernel */
+  FK_DEV_WAIT_TIMEOUT = 102    /* a pipeline wait in a kernel exceeded its limit */
 };
 
 int fk_abi_version(void);

@@ -332,3 +332,25 @@ def test_a_loss_over_few_centroids_copies_no_points(lib):
     assert size(16384, 32768, 1024) >= 16384 * 1024 * 2
     # float32 is copied as its three parts, with or without
     assert size(65536, 256, 4096, dtype=2) >= 65536 * 4096 * 6
+
+
+def test_the_error_word_is_public_and_names_every_kernel(monkeypatch, lib):
+    word = torch.zeros(4, dtype=torch.int32)
+    monkeypatch.setattr(fk.DeviceStatus, "_words", {0: word})
+    fk.DeviceStatus.raise_if_set("cuda:0")
+    for code, text in ((101, "outside"), (102, "pipeline wait")):
+        word[0] = code
+        with pytest.raises(RuntimeError, match=text) as e:
+            fk.DeviceStatus.raise_if_set("cuda:0")
+        assert "assignment" not in str(e.value)      # (other kernels wait too)
+        assert word[0] == 0
+        fk.DeviceStatus.raise_if_set("cuda:0")
+
+
+def test_a_wait_that_ran_out_is_not_hidden_by_a_bad_label():
+    """The word keeps the largest code: waits raise it, labels only set it while it is 0."""
+    import pathlib
+    csrc = pathlib.Path(fk.__file__).parent.parent / "csrc"
+    assert fk._native.FK_DEV_WAIT_TIMEOUT > fk._native.FK_DEV_BAD_LABEL
+    waits = (csrc / "fk_ptx.cuh").read_text()
+    assert "atomicCAS(dev_status" not in waits and waits.count("atomicMax(dev_status, code)") == 2

@@ -470,6 +470,26 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
       xs_next = row < p.M ? p.a_scale[t.b * p.as_sb + row * p.as_sn] : 0.0f;
     }
   };
+  // A row's end: its label, or what its chunk of the columns found.
+  auto finish = [&](const Tile& now) {
+    const int row = now.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
+    if (p.chunks == 1) {
+      // the two column parts of a row meet in shared memory
+      // (in turn in two slots: the item after the next one writes this one again,
+      // behind the next one's barrier)
+      if (part == 1) slot[turn] = make_float2(run_m, __int_as_float(run_i));
+      quarter_sync<S::kParts * 32>(quarter);
+      if (part == 0) {
+        const float2 o = slot[turn];
+        if (argmax_better(o.x, __float_as_int(o.y), run_m, run_i)) run_i = __float_as_int(o.y);
+        if (row < p.M) p.label_out[now.b * p.lo_sb + row * p.lo_sn] = run_i;
+      }
+      turn ^= 128;
+    } else if (row < p.M) {
+      p.partial[((static_cast<int64_t>(now.b) * p.chunks + now.chunk) * S::kParts + part) * p.M + row] =
+          make_float2(run_m, __int_as_float(run_i));
+    }
+  };
   if (more) fetch();
   while (more) {
     const Tile now = t;
@@ -491,60 +511,68 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
     if (more) fetch();
 
     const bool got = mbar_wait(&acc_full[buf], aphase, abort_flag, p.status, FK_DEV_WAIT_TIMEOUT);
-    if (__all_sync(0xffffffffu, got)) {
-      tc_fence_after();
-      const uint32_t taddr = tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
-      const uint64_t x2 = pack2(xs, xs);
+    if (!__all_sync(0xffffffffu, got)) {
+      // The labels from here on are -1, in a loop of its own: a flag looked at in
+      // this one cost 2 %.  (NaN comes first, and of NaNs the lowest index.)
+      for (Tile left = now;; left = t, walk.next(), more = walk.get(t)) {
+        run_m = __uint_as_float(0x7fc00000u);
+        run_i = -1;
+        if (left.last) finish(left);
+        if (!more) return;
+      }
+    }
+    tc_fence_after();
+    const uint32_t taddr = tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint64_t x2 = pack2(xs, xs);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int cc = now.n * BN + part * kCols + c * 32, left = p.N - cc;
-        uint32_t v[32];
-        tmem_ld32(taddr + c * 32, v);
-        tmem_ld_wait(v);
-        if (c + 1 == kChunks) {
-          // the accumulator is in registers: hand it back
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
-        }
-        if (left <= 0) continue;
-        acc_to_f(v);
-        float z[32];
+    for (int c = 0; c < kChunks; ++c) {
+      const int cc = now.n * BN + part * kCols + c * 32, left = p.N - cc;
+      uint32_t v[32];
+      tmem_ld32(taddr + c * 32, v);
+      tmem_ld_wait(v);
+      if (c + 1 == kChunks) {
+        // the accumulator is in registers: hand it back
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cg<CG>(&acc_empty[buf]);
+      }
+      if (left <= 0) continue;
+      acc_to_f(v);
+      float z[32];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          // without a bias the table holds zeros: no branch for every column
-          const uint4 s4 = lds128(table + (c * 32 + i) * 4), b4 = lds128(table + kBias + (c * 32 + i) * 4);
-          const uint32_t* su = &s4.x;
-          const uint32_t* bu = &b4.x;
+      for (int i = 0; i < 32; i += 4) {
+        // without a bias the table holds zeros: no branch for every column
+        const uint4 s4 = lds128(table + (c * 32 + i) * 4), b4 = lds128(table + kBias + (c * 32 + i) * 4);
+        const uint32_t* su = &s4.x;
+        const uint32_t* bu = &b4.x;
 #pragma unroll
-          for (int k = 0; k < 4; k += 2)
-            unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[i + k]), __uint_as_float(v[i + k + 1])), x2),
-                              pack2(__uint_as_float(su[k]), __uint_as_float(su[k + 1]))),
-                         pack2(__uint_as_float(bu[k]), __uint_as_float(bu[k + 1]))),
-                    z[i + k], z[i + k + 1]);
-        }
-        if (left < 32) {
-          keep_branch();
+        for (int k = 0; k < 4; k += 2)
+          unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[i + k]), __uint_as_float(v[i + k + 1])), x2),
+                            pack2(__uint_as_float(su[k]), __uint_as_float(su[k + 1]))),
+                       pack2(__uint_as_float(bu[k]), __uint_as_float(bu[k + 1]))),
+                  z[i + k], z[i + k + 1]);
+      }
+      if (left < 32) {
+        keep_branch();
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i >= left) z[i] = -INFINITY;
-        }
-        float mx[4];
+        for (int i = 0; i < 32; ++i)
+          if (i >= left) z[i] = -INFINITY;
+      }
+      float mx[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          mx[q] = max_nan3(z[q], z[q + 4], z[q + 8]);
-          mx[q] = max_nan3(mx[q], z[q + 12], z[q + 16]);
-          mx[q] = max_nan(max_nan3(mx[q], z[q + 20], z[q + 24]), z[q + 28]);
-        }
-        const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
-        if (!(m < run_m) && argmax_better(m, cc, run_m, run_i)) {
-          run_m = m;
-          run_i = cc;
+      for (int q = 0; q < 4; ++q) {
+        mx[q] = max_nan3(z[q], z[q + 4], z[q + 8]);
+        mx[q] = max_nan3(mx[q], z[q + 12], z[q + 16]);
+        mx[q] = max_nan(max_nan3(mx[q], z[q + 20], z[q + 24]), z[q + 28]);
+      }
+      const float m = max_nan(max_nan3(mx[0], mx[1], mx[2]), mx[3]);
+      if (!(m < run_m) && argmax_better(m, cc, run_m, run_i)) {
+        run_m = m;
+        run_i = cc;
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            sts128(save ^ (q * 16), __float_as_uint(z[q * 4]), __float_as_uint(z[q * 4 + 1]),
-                   __float_as_uint(z[q * 4 + 2]), __float_as_uint(z[q * 4 + 3]));
-        }
+        for (int q = 0; q < 8; ++q)
+          sts128(save ^ (q * 16), __float_as_uint(z[q * 4]), __float_as_uint(z[q * 4 + 1]),
+                 __float_as_uint(z[q * 4 + 2]), __float_as_uint(z[q * 4 + 3]));
       }
     }
     if (++buf == S::kBufs) {
@@ -567,23 +595,7 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
       }
       run_i += at;
     }
-    const int row = now.m * S::kBM + static_cast<int>(rank) * 128 + quarter * 32 + lane;
-    if (p.chunks == 1) {
-      // the two column parts of a row meet in shared memory
-      // (in turn in two slots: the item after the next one writes this one again,
-      // behind the next one's barrier)
-      if (part == 1) slot[turn] = make_float2(run_m, __int_as_float(run_i));
-      quarter_sync<S::kParts * 32>(quarter);
-      if (part == 0) {
-        const float2 o = slot[turn];
-        if (argmax_better(o.x, __float_as_int(o.y), run_m, run_i)) run_i = __float_as_int(o.y);
-        if (row < p.M) p.label_out[now.b * p.lo_sb + row * p.lo_sn] = run_i;
-      }
-      turn ^= 128;
-    } else if (row < p.M) {
-      p.partial[((static_cast<int64_t>(now.b) * p.chunks + now.chunk) * S::kParts + part) * p.M + row] =
-          make_float2(run_m, __int_as_float(run_i));
-    }
+    finish(now);
   }
 }
 
@@ -838,6 +850,11 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     float xs = 0.0f;
     float fac = 0.0f;
 
+    // Once a wait has run out, what this warp still has to write becomes NaN: left
+    // as it is, memory that nobody wrote would pass for a loss or a gradient.
+    bool dead = false;
+    constexpr uint32_t kNan = 0x7fc00000u;
+
     // What the epilogue needs from memory besides the accumulator is fetched a
     // tile ahead: its latency would stand between the accumulator and its use.
     Tile t, nt;
@@ -1077,7 +1094,6 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         }
       };
 
-      bool got = true;
       if constexpr (EXACT) {
         float sum[kChunks][32];
 #pragma unroll
@@ -1085,9 +1101,9 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[c][i] = 0.0f;
         for (int it = t.it0; it < t.it1; it += kSegment) {
-          got = __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
-                                                  FK_DEV_WAIT_TIMEOUT));
-          if (!got) break;
+          dead = dead || !__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
+                                                            FK_DEV_WAIT_TIMEOUT));
+          if (dead) break;
           tc_fence_after();
           const uint32_t taddr =
               tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -1110,35 +1126,40 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             aphase ^= 1;
           }
         }
-        if (!got) break;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           uint32_t v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(sum[c][i]);
+          for (int i = 0; i < 32; ++i) v[i] = dead ? kNan : __float_as_uint(sum[c][i]);
           chunk(c, v);
         }
       } else {
         // no gathered row in this split of them: nothing comes, nothing is added
         const bool none = EPI == kEpiOut && t.it0 == t.it1;
-        got = none || __all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
-                                                        FK_DEV_WAIT_TIMEOUT));
-        if (!got) break;
+        if (!none)
+          dead = dead || !__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
+                                                            FK_DEV_WAIT_TIMEOUT));
+        if constexpr (EPI == kEpiScores) {
+          if (dead) {   // (the accumulators are integers)
+            keep_branch();
+            xs = __uint_as_float(kNan);
+          }
+        }
         tc_fence_after();
         const uint32_t taddr =
             tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           uint32_t v[32];
-          if (none) {
+          if (none || (EPI != kEpiScores && dead)) {
             keep_branch();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0;
+            for (int i = 0; i < 32; ++i) v[i] = dead ? kNan : 0;
           } else {
             tmem_ld32(taddr + c * 32, v);
             tmem_ld_wait(v);
           }
-          if (c + 1 == kChunks && !none) {
+          if (c + 1 == kChunks && !none && !dead) {
             // the accumulator is in registers: hand it back
             tc_fence_before();
             __syncwarp();

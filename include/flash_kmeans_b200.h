@@ -266,7 +266,9 @@ int fk_centroid_finalize_normalized(float* sums, int32_t* counts, const void* ol
  * element strides: rows that TMA cannot address, and float32 ones, are copied
  * into the workspace (256-byte aligned; its size depends on that, hence on the
  * pointers and strides).  centroids with batch stride 0 are shared by all
- * batches and read once.  Requires B*N < 2^31, and N, K, D < 2^30. */
+ * batches and read once.  Requires B*N < 2^31, and N, K, D < 2^30.  Where a
+ * kernel's wait runs out (FK_DEV_WAIT_TIMEOUT), what it still had to write
+ * becomes NaN, labels -1. */
 
 /* Softmax cross entropy of scale * x.c^T (scale positive and finite) against
  * cluster ids, without keeping the scores:

@@ -146,6 +146,12 @@ def _check_pair(x, centroids, name):
         raise ValueError(f"{name}: x is on {x.device}, centroids on {centroids.device}")
 
 
+def _valued(t):
+    """t in memory of its own where that holds t's negatives (such a view is
+    what the imaginary part of a conjugate is): kernels read memory."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
 def _three(t):
     """Shape and strides of (M, D) or (B, M, D) as three."""
     sh, st = t.shape, t.stride()
@@ -224,6 +230,7 @@ class _Xent:
             labels, torch.Tensor)
         if not tensors or not x.is_cuda:
             _check_xent(x, centroids, labels, scale, ignore_index, reduction, name)
+        x, centroids = _valued(x), _valued(centroids)
         self.shapes = x.shape, centroids.shape
         self.none = reduction == "none"
         if x.dim() == 3 and centroids.dim() == 2:
@@ -315,7 +322,7 @@ class _ClusterCrossEntropy(torch.autograd.Function):
         x, centroids, labels = ctx.saved_tensors
         with torch.no_grad():
             call = _Xent(x, centroids, labels, *ctx.args, "cluster_cross_entropy")
-            gx, gc = call.backward(ctx.kept, grad_loss.contiguous(), *ctx.needs_input_grad[:2])
+            gx, gc = call.backward(ctx.kept, _valued(grad_loss).contiguous(), *ctx.needs_input_grad[:2])
         if torch.is_grad_enabled():     # a graph of the backward pass is recorded
             gx, gc = _OnceOnly.apply(gx, gc, x, centroids, grad_loss)
         return gx, gc, None, None, None, None
@@ -393,7 +400,7 @@ def cluster_cross_entropy_grad(x: torch.Tensor, centroids: torch.Tensor, labels:
                                  f"the loss {tuple(shape)}")
             if grad_loss.device != x.device:
                 raise ValueError(f"{name}: x is on {x.device}, grad_loss on {grad_loss.device}")
-            grad_loss = grad_loss.contiguous()
+            grad_loss = _valued(grad_loss).contiguous()
         elif call.none:
             grad_loss = torch.ones(shape, dtype=torch.float32, device=x.device)
         return call.loss_grad(grad_loss)
@@ -417,7 +424,7 @@ def quantize_rows(x: torch.Tensor):
     if x.shape[-1] < 1:
         raise ValueError("quantize_rows: at least one feature is needed")
     _ops._require_cuda(x)
-    x = x.detach()
+    x = _valued(x.detach())
     xb = x if x.dim() == 3 else x.unsqueeze(0)
     B, N, D = xb.shape
     Dp = -(-D // 16) * 16
@@ -484,6 +491,7 @@ class _Scores:
                 and (x_scale is None or isinstance(x_scale, torch.Tensor))
                 and (bias is None or isinstance(bias, torch.Tensor))):
             _check_int8(x, centroids, c_scale, x_scale, bias, name)
+        x, c_scale, x_scale, bias = _valued(x), _valued(c_scale), _valued(x_scale), _valued(bias)
         self.lead, self.device = x.shape[:-1], x.device
         if x.dim() == 3 and centroids.dim() == 2:
             _check_int8(x, centroids, c_scale, x_scale, bias, name)
@@ -523,6 +531,8 @@ def _check_out(out, shape, dtype, device, name):
         raise ValueError(f"{name}: x is on {device}, out on {out.device}")
     if any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
         raise ValueError(f"{name}: out must not be expanded, its elements share memory")
+    if out.is_neg():
+        raise ValueError(f"{name}: out must not be a negated view")
     reach = 0      # of the dimensions with smaller strides
     for s, n in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
         if s <= reach and 0 not in out.shape:

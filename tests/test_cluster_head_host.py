@@ -354,3 +354,65 @@ def test_a_wait_that_ran_out_is_not_hidden_by_a_bad_label():
     assert fk._native.FK_DEV_WAIT_TIMEOUT > fk._native.FK_DEV_BAD_LABEL
     waits = (csrc / "fk_ptx.cuh").read_text()
     assert "atomicCAS(dev_status" not in waits and waits.count("atomicMax(dev_status, code)") == 2
+
+
+def _negated(t):
+    """The same values through memory that holds their negatives (as the imaginary
+    part of a conjugate, and gradients that pass one, do)."""
+    v = torch._neg_view(t.neg())
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def _floats(p, n):
+    return [ctypes.cast(p, ctypes.POINTER(ctypes.c_float))[k] for k in range(n)]
+
+
+def test_negated_views_are_read_by_their_values(monkeypatch):
+    """By the pointers that a call hands to the library."""
+    from flash_kmeans import cluster_head as ch
+    sizes, got = {}, []
+    monkeypatch.setattr(ch, "_call", lambda fn, what, dev, *args: got.append(
+        [_floats(args[i], n) for i, n in sizes.items()]))
+    x, c, g = X.abs(), C.abs(), torch.ones(6)
+    sizes |= {0: 48, 1: 32}
+    fk.cluster_cross_entropy(_cuda(_negated(x)), _cuda(_negated(c)), Y)
+    assert got.pop() == [x.flatten().tolist(), c.flatten().tolist()]
+    sizes.clear()
+    sizes[16] = 6
+    fk.cluster_cross_entropy_grad(_cuda(x), _cuda(c), Y, reduction="none", grad_loss=_negated(g))
+    assert got.pop() == [g.tolist()]
+    sizes.clear()
+    xr = _cuda(x).requires_grad_()
+    loss = fk.cluster_cross_entropy(xr, _cuda(c), Y, reduction="none")
+    sizes[17] = 6
+    loss.backward(_negated(g))
+    assert got.pop() == [g.tolist()]
+    sizes.clear()
+    s, b = torch.ones(4), torch.ones(4) * 2
+    sizes |= {2: 6, 3: 4, 4: 4}
+    fk.int8_scores(_cuda(XQ), _cuda(CQ), _negated(s), x_scale=_negated(XS), bias=_negated(b))
+    assert got.pop() == [XS.tolist(), s.tolist(), b.tolist()]
+    sizes.clear()
+    sizes[0] = 48
+    fk.int8_scores(_cuda(_negated(x)), _cuda(CQ), s)
+    assert got.pop() == [x.flatten().tolist()]
+    sizes.clear()
+    with pytest.raises(ValueError, match="out must not"):
+        fk.int8_scores(_cuda(XQ), _cuda(CQ), s, x_scale=XS, out=_negated(torch.zeros(6, 4)))
+
+
+def test_negated_views_are_quantised_by_their_values(monkeypatch):
+    from flash_kmeans import _native
+    seen = []
+
+    class Lib:
+        def fk_quantize_rows(self, x, *args):
+            seen.extend(_floats(x, 48))
+            return 0
+
+    monkeypatch.setattr(_native, "load", Lib)
+    monkeypatch.setattr(_native, "stream_handle", lambda device: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    fk.quantize_rows(_cuda(_negated(X)))
+    assert seen == X.flatten().tolist()

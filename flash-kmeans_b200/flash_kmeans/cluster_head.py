@@ -100,19 +100,19 @@ def _call(fn, what, dev: _Device, *args):
 
 
 def _has_tangent(t):
-    # (the level is looked at first because unpacking costs 0.3 us)
-    return (getattr(forward_ad, "_current_level", 0) >= 0 and isinstance(t, torch.Tensor)
-            and forward_ad.unpack_dual(t).tangent is not None)
+    return isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
 
 
 def _refuse_tangents(name, *tensors):
     """A tangent would be dropped without a word: a dual tensor need not require grad."""
-    if any(map(_has_tangent, tensors)):
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(map(_has_tangent, tensors)):
         raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")
 
 
 def _numbers(name, scale, ignore_index):
     """scale and ignore_index as Python's; what would be lost on the way is refused."""
+    if type(scale) is float and type(ignore_index) is int:
+        return scale, ignore_index
     if isinstance(scale, torch.Tensor):
         if scale.is_cuda:
             raise TypeError(f"{name}: scale must be a number; reading one from a GPU would wait for it "
@@ -295,6 +295,11 @@ class _Xent:
         return gx, gc
 
 
+def _gradients(ctx, grad_loss):
+    call = _Xent(*ctx.saved_tensors, *ctx.args, "cluster_cross_entropy")
+    return call.backward(ctx.kept, _valued(grad_loss).contiguous(), *ctx.needs_input_grad[:2])
+
+
 class _OnceOnly(torch.autograd.Function):
     """Hands gradients on as functions of the tensors behind them, whose own
     derivative raises: without it a second derivative would be left out."""
@@ -319,13 +324,12 @@ class _ClusterCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_loss):
-        x, centroids, labels = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return *_gradients(ctx, grad_loss), None, None, None, None
+        # a graph of the backward pass is recorded
         with torch.no_grad():
-            call = _Xent(x, centroids, labels, *ctx.args, "cluster_cross_entropy")
-            gx, gc = call.backward(ctx.kept, _valued(grad_loss).contiguous(), *ctx.needs_input_grad[:2])
-        if torch.is_grad_enabled():     # a graph of the backward pass is recorded
-            gx, gc = _OnceOnly.apply(gx, gc, x, centroids, grad_loss)
-        return gx, gc, None, None, None, None
+            gx, gc = _gradients(ctx, grad_loss)
+        return *_OnceOnly.apply(gx, gc, *ctx.saved_tensors[:2], grad_loss), None, None, None, None
 
 
 def _autocast(x, centroids):

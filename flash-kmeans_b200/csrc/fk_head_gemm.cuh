@@ -60,7 +60,7 @@ struct Problem {
   int batches;
   int chunks;               // running epilogues: column chunks of a row block; else splits of the contraction
   int kblocks;              // 128-byte steps of the contraction
-  int a_mn, b_mn;           // MN-major operands
+  int a_mn;                 // MN-major A (B is MN-major in kEpiOut alone)
   int a_batch, b_batch;     // z coordinate = batch * this + part * a_part
   int a_part, b_part;
   int a_off, b_off;         // first row (K-major) or first contraction index (MN-major)

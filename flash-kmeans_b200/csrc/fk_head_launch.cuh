@@ -185,7 +185,6 @@ int set_problem(Params<problems_of(EPI)>& prm, int i, const Operand& a, const Op
   p.n_tiles = static_cast<int>(ceil_div(p.N, sh.bn));
   p.kblocks = static_cast<int>(ceil_div(kdim, step));
   p.a_mn = a.mn;
-  p.b_mn = b.mn;
   p.a_batch = a.batch_step;
   p.b_batch = b.batch_step;
   p.a_part = a.part_step;

@@ -198,7 +198,7 @@ struct CombineParams {
   int label_dtype;
   int64_t lb, ln, ignore;
   int64_t K;
-  int N, pieces, batches, row_blocks;
+  int N, pieces, row_blocks;
   int reduction;           // 0 none, 1 mean, 2 sum
   float* loss;             // rows [batch][N], or one value
   RowStat* stat;           // optional
@@ -844,7 +844,6 @@ static int forward(const Xent& q, float* loss, RowStat* stat, int32_t* count, vo
   cp.K = q.K;
   cp.N = static_cast<int>(q.N);
   cp.pieces = f.chunks * parts_of(kEpiLse, f.sh.bn);
-  cp.batches = static_cast<int>(q.B);
   cp.row_blocks = static_cast<int>(f.row_blocks);
   cp.reduction = q.reduction;
   cp.loss = loss;

@@ -146,3 +146,52 @@ def test_float16_rows_of_no_weight_beside_small_ones():
     assert gx[1::2].abs().max() > 0 and gc.abs().max() > 0
     # the same sums of the same values; a scale this large makes softmaxes one-hot
     assert torch.equal(gx[1::2], ex) and torch.equal(gc, ec)
+
+
+@pytest.mark.parametrize("low", [BF, HF], ids=["bf16", "fp16"])
+def test_autocast_step(low):
+    """A linear layer under autocast in front of a head kept in float32."""
+    x, c, y = make(0, 200, 300, 64, FP, seed=46, ignored=0.1)
+    lin = torch.nn.Linear(64, 64, device="cuda")
+    head = c.clone().requires_grad_()
+    with torch.autocast("cuda", dtype=low):
+        h = lin(x)
+        assert h.dtype == low
+        h.retain_grad()
+        loss = fk.cluster_cross_entropy(h, head, y, scale=3.0, reduction="sum")
+    loss.backward()
+    want = reference(h, head.to(low), y, 3.0, "sum")
+    close(loss, want[0], "loss")
+    close(h.grad, want[1], "h")
+    assert head.grad.dtype == FP and lin.weight.grad is not None
+    close(head.grad, want[2], "head")
+
+
+def test_negated_views():
+    x, c, y = make(0, 100, 200, 48, FP, seed=47)
+    g = torch.rand(100, device="cuda")
+    want = fk.cluster_cross_entropy_grad(x, c, y, reduction="none", grad_loss=g)
+    neg = lambda t: torch._neg_view(t.neg())        # noqa: E731
+    got = fk.cluster_cross_entropy_grad(neg(x), neg(c), y, reduction="none", grad_loss=neg(g))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    xr = neg(x).requires_grad_()
+    fk.cluster_cross_entropy(xr, c, y, reduction="none").backward(neg(g))
+    assert torch.equal(xr.grad, want[1])
+    # as one arises: the imaginary part of a conjugate
+    z = torch.complex(x, x)
+    assert torch.equal(fk.cluster_cross_entropy(z.conj().imag, c, y), fk.cluster_cross_entropy(-x, c, y))
+    cq, cs = fk.quantize_rows(c)
+    assert torch.equal(fk.int8_scores(neg(x), cq, neg(cs)), fk.int8_scores(x, cq, cs))
+    assert all(torch.equal(a, b) for a, b in zip(fk.quantize_rows(neg(x)), fk.quantize_rows(x)))
+
+
+def test_a_recorded_backward_pass():
+    """Gradients with a graph are the same values; their derivative raises."""
+    x, c, y = make(0, 300, 400, 64, BF, seed=48, ignored=0.1)
+    _, gx, gc = fk.cluster_cross_entropy_grad(x, c, y, scale=2.0)
+    xr, cr = x.clone().requires_grad_(), c.clone().requires_grad_()
+    loss = fk.cluster_cross_entropy(xr, cr, y, scale=2.0)
+    got = torch.autograd.grad(loss, (xr, cr), create_graph=True)
+    assert torch.equal(got[0], gx) and torch.equal(got[1], gc)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (loss + got[0].float().square().sum()).backward()

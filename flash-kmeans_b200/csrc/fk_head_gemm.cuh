@@ -40,8 +40,10 @@ enum Epilogue {
   kEpiGrad = 1,    // (softmax - one-hot) * weight, rounded to 16 bits, into a piece
   kEpiOut = 2,     // scaled accumulator, kept in float32 or cast to the output
   kEpiScores = 3,  // int32 -> scaled scores
-  kEpiArgmax = 4   // int32 -> index of the largest scaled score
+  kEpiArgmax = 4,  // int32 -> index of the largest scaled score
+  kEpiOutRows = 5  // kEpiOut with factors of the rows (the test for them would cost kEpiOut 0.9 %)
 };
+__host__ __device__ constexpr bool output(int epi) { return epi == kEpiOut || epi == kEpiOutRows; }
 __host__ __device__ constexpr bool running(int epi) { return epi == kEpiLse || epi == kEpiArgmax; }
 __host__ __device__ constexpr bool integer(int epi) { return epi == kEpiScores || epi == kEpiArgmax; }
 
@@ -60,7 +62,7 @@ struct Problem {
   int batches;
   int chunks;               // running epilogues: column chunks of a row block; else splits of the contraction
   int kblocks;              // 128-byte steps of the contraction
-  int a_mn;                 // MN-major A (B is MN-major in kEpiOut alone)
+  int a_mn;                 // MN-major A (B is MN-major in the output epilogues alone)
   int a_batch, b_batch;     // z coordinate = batch * this + part * a_part
   int a_part, b_part;
   int a_off, b_off;         // first row (K-major) or first contraction index (MN-major)
@@ -93,7 +95,7 @@ struct Problem {
   float fscale;             // kEpiOut: factor, times *f_num, over max(*f_den, 1)
   const float* f_num;
   const int32_t* f_den;
-  const float* row_factor;  // and times that of the row, or null: [batch][stat_rows]
+  const float* row_factor;  // kEpiOutRows: and times that of the row, or null: [batch][stat_rows]
   float* acc;               // kEpiOut: float32 accumulator [split][batch][row][acc_ld]
   int64_t acc_ld, acc_batch, acc_split;
   int acc_read, acc_write;
@@ -118,7 +120,7 @@ struct Problem {
 // finish together.  In the second product every worker has `all` tiles, the
 // workers from `short_from` on (one tile of the first product behind) `more`
 // others, and the last `rest` workers one more.
-constexpr int problems_of(int epi) { return epi == kEpiOut ? 2 : 1; }
+constexpr int problems_of(int epi) { return output(epi) ? 2 : 1; }
 
 template <int NP>
 struct Params {
@@ -234,7 +236,7 @@ struct Tile {
 template <int EPI, int BM>
 struct Walk {
   static constexpr int NP = problems_of(EPI);
-  static constexpr bool kLive = EPI == kEpiLse || EPI == kEpiGrad || EPI == kEpiOut;
+  static constexpr bool kLive = EPI == kEpiLse || EPI == kEpiGrad || output(EPI);
   const Params<NP>& prm;
   uint32_t item, total;
   const uint32_t slot, slots;
@@ -731,7 +733,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             }
           }
         };
-        if constexpr (EPI == kEpiOut) {
+        if constexpr (output(EPI)) {
           // dx: P by rows, centroids by columns; dc: both by columns
           if (p.a_mn) load(std::true_type{}, std::true_type{});
           else load(std::false_type{}, std::true_type{});
@@ -762,8 +764,8 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       for (Tile t; ok && walk.get(t); walk.next()) {
         const Problem& p = prm.p[NP > 1 ? t.q : 0];
         const uint32_t idesc = p.idesc;
-        const bool a_mn = EPI == kEpiOut && p.a_mn;
-        constexpr bool b_mn = EPI == kEpiOut;
+        const bool a_mn = output(EPI) && p.a_mn;
+        constexpr bool b_mn = output(EPI);
         const uint64_t ad0 = a_mn ? smem_desc_sw128_mn(smem0, 8192, 1024) : smem_desc_sw128(smem0);
         const uint64_t bd0 = b_mn ? smem_desc_sw128_mn(smem0 + S::kOps * S::kABytes, 8192, 1024)
                                   : smem_desc_sw128(smem0 + S::kOps * S::kABytes);
@@ -849,11 +851,24 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
     int label = -1;
     float xs = 0.0f;
     float fac = 0.0f;
+    if constexpr (EPI == kEpiOut) {   // (the same for both problems)
+      fac = p0.fscale;
+      if (p0.f_num) fac *= *p0.f_num;
+      if (p0.f_den) fac /= static_cast<float>(max(*p0.f_den, 1));
+    }
 
     // Once a wait has run out, what this warp still has to write becomes NaN: left
-    // as it is, memory that nobody wrote would pass for a loss or a gradient.
+    // as it is, memory that nobody wrote would pass for a loss or a gradient.  (By
+    // a factor of each value, and only that of this epilogue: choosing the values
+    // cost narrow losses 4 %, all factors the gradients' products 1 %.)
     bool dead = false;
-    constexpr uint32_t kNan = 0x7fc00000u;
+    auto spoil = [&](RowStat& st) {
+      if (!dead) return;
+      keep_branch();
+      const float nan = __uint_as_float(0x7fc00000u);
+      if constexpr (output(EPI)) fac = nan;
+      else run_s = xs = st.coef = st.at_label = nan;
+    };
 
     // What the epilogue needs from memory besides the accumulator is fetched a
     // tile ahead: its latency would stand between the accumulator and its use.
@@ -884,11 +899,9 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
       const int rows = Walk<EPI, S::kBM>::rows_of(p);
       const bool row_ok = row < rows;
       const int col0 = t.n * BN + part * kCols;
-      if constexpr (EPI == kEpiOut) {
-        // (read at every tile: held for both problems, they would spill)
+      if constexpr (EPI == kEpiOutRows) {
         fac = p.fscale;
         if (p.f_num) fac *= *p.f_num;
-        if (p.f_den) fac /= static_cast<float>(max(*p.f_den, 1));
         if (p.row_factor && row_ok) {
           const int n = p.live_off + row;
           fac *= p.row_factor[t.b * p.stat_rows + (p.row_map ? p.row_map[n] : n)];
@@ -927,7 +940,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
 
       // four columns of an output row, rounded
       auto emit = [&](const int64_t grow, const int col, const float4 f) {
-        const int64_t at = EPI == kEpiOut && p.row_map ? p.row_map[p.live_off + grow] : grow;
+        const int64_t at = output(EPI) && p.row_map ? p.row_map[p.live_off + grow] : grow;
         const int64_t o = t.b * p.out_sb + at * p.out_sr + col;
         if (p.out_vec && col + 4 <= p.N) {
           if (p.out_dtype == FK_F32) {
@@ -1050,7 +1063,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             keep_branch();
             put(std::false_type{}, 0);
           }
-        } else if constexpr (EPI == kEpiOut || EPI == kEpiScores) {
+        } else if constexpr (output(EPI) || EPI == kEpiScores) {
           if constexpr (EPI == kEpiScores) acc_to_f(v);
           __syncwarp();
 #pragma unroll
@@ -1126,35 +1139,31 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
             aphase ^= 1;
           }
         }
+        spoil(st);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           uint32_t v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = dead ? kNan : __float_as_uint(sum[c][i]);
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(sum[c][i]);
           chunk(c, v);
         }
       } else {
         // no gathered row in this split of them: nothing comes, nothing is added
-        const bool none = EPI == kEpiOut && t.it0 == t.it1;
-        if (!none)
-          dead = dead || !__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status,
-                                                            FK_DEV_WAIT_TIMEOUT));
-        if constexpr (EPI == kEpiScores) {
-          if (dead) {   // (the accumulators are integers)
-            keep_branch();
-            xs = __uint_as_float(kNan);
-          }
-        }
+        const bool none = output(EPI) && t.it0 == t.it1;
+        if (!none && !dead &&
+            !__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], aphase, abort_flag, p0.status, FK_DEV_WAIT_TIMEOUT)))
+          dead = true;
+        spoil(st);
         tc_fence_after();
         const uint32_t taddr =
             tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
           uint32_t v[32];
-          if (none || (EPI != kEpiScores && dead)) {
+          if (none) {
             keep_branch();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = dead ? kNan : 0;
+            for (int i = 0; i < 32; ++i) v[i] = 0;
           } else {
             tmem_ld32(taddr + c * 32, v);
             tmem_ld_wait(v);
@@ -1173,7 +1182,7 @@ __global__ void __launch_bounds__(threads_of<CG, BN, EPI, EXACT>(), 1) head_gemm
         }
       }
 
-      if constexpr (EPI == kEpiOut) {
+      if constexpr (output(EPI)) {
         if (p.join) {
           // Partial sums of a split contraction: whichever split's warp arrives
           // last adds all of them up, in the order of the splits, so the result

@@ -210,13 +210,13 @@ int set_problem(Params<problems_of(EPI)>& prm, int i, const Operand& a, const Op
 
 template <int EPI>
 int launch(Params<problems_of(EPI)>& prm, ShapeChoice sh, cudaStream_t s) {
-  if constexpr (!integer(EPI)) {
+  if constexpr (!integer(EPI) && EPI != kEpiOutRows) {   // (factors of rows are float16's)
     if (sh.exact) {
       if (sh.cg == 2) return launch_shape<2, 128, EPI, true>(prm, s);
       return launch_shape<1, 64, EPI, true>(prm, s);
     }
   }
-  if constexpr (EPI == kEpiOut) {
+  if constexpr (output(EPI)) {
     if (sh.cg == 2 && sh.bn == 128) return launch_shape<2, 128, EPI, false>(prm, s);
   }
   if (sh.cg == 2) return launch_shape<2, 256, EPI, false>(prm, s);

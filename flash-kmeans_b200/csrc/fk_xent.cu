@@ -1149,7 +1149,7 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       if (gx.p && x_first) st = add_x();
       if (st == FK_OK && gc.p) st = add_c();
       if (st == FK_OK && gx.p && !x_first) st = add_x();
-      if (st == FK_OK) st = launch<kEpiOut>(pair, f.sh, s);
+      if (st == FK_OK) st = f.power ? launch<kEpiOutRows>(pair, f.sh, s) : launch<kEpiOut>(pair, f.sh, s);
       if (st != FK_OK) return st;
     }
   }

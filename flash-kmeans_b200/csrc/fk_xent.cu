@@ -20,16 +20,18 @@
 // keeps N x K scores.
 //
 // Measured alone at 16384 x 32768 x 1024 bfloat16 with 15 % of the rows ignored:
-// forward product 571 us, combine 19, four pieces of 156 (scores again, dz) and
-// 326 (both gradients), 1.5 PFLOP/s; back to back the power cap stretches the
-// 2.6 ms to 3.1.  With 128 features the exponentials bind: the forward product of
-// 32444 x 8192 keeps the special-function units 74 % busy (103 us).
+// forward product 580 us, combine 19, four pieces of 158 (scores again, dz) and
+// 324 to 338 (both gradients), 1.5 PFLOP/s; back to back the power cap stretches
+// the 2.7 ms to 3.1.  With 128 features (32444 x 8192) the forward product keeps
+// the special-function units 74 % busy (108 us); each of two backward pieces writes
+// 0.2 GB of dz to memory (80 us) and reads it twice, 0.38 GB of that from memory
+// (94 us).
 //
 // float32 inputs are split exactly into three bf16 parts, and the six products
 // of parts down to 2^-16 of the leading one are accumulated, smallest first:
 // the terms left out are below 2^-24 of |x||c|.  That costs what 3xTF32 costs
 // and keeps one kernel, MN-major operands included (8192 x 1024 x 512, loss and
-// gradients: 0.22 ms, errors a fifth of plain float32's).
+// gradients: 0.23 ms, errors a fifth of plain float32's).
 #include <algorithm>
 #include <cmath>
 

@@ -108,6 +108,7 @@ struct Problem {
   const float* b_scale;
   const float* bias;
   int64_t as_sb, as_sn, bs_sb, bs_sn, bias_sb, bias_sn;
+  float unit;               // kEpiArgmax: 1 (see add2_rounded)
   int32_t* label_out;       // kEpiArgmax with one chunk: labels
   int64_t lo_sb, lo_sn;
   uint32_t* zero;           // words cleared for the kernel that follows
@@ -206,6 +207,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// a + b where a is a product that has to be rounded first: mul2 and add2 in
+// sequence came out as one fused step, for all their .rn.  `one` holds 1 twice,
+// which the compiler must not know.
+__device__ __forceinline__ uint64_t add2_rounded(uint64_t a, uint64_t one, uint64_t b) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(one), "l"(b));
   return r;
 }
 
@@ -428,7 +437,7 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
 
 // ------------------------------------------------------------------- kernel
 // Epilogue of the argmax.  The scores' scaling and comparing bounds it (2400 scores
-// a ns at 604800 x 1000 x 128: 252 us, of which the products need 47), so a row
+// a ns at 604800 x 1000 x 128: 256 us, of which the products need 47), so a row
 // keeps only its best score and the 32 scores of the chunk that it came from, in
 // shared memory; which column of it won is looked up once, at the end of the
 // row.  A column's scale and bias come from shared memory, 16 bytes to all lanes
@@ -525,7 +534,7 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
     }
     tc_fence_after();
     const uint32_t taddr = tmem + buf * BN + part * kCols + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint64_t x2 = pack2(xs, xs);
+    const uint64_t x2 = pack2(xs, xs), one2 = pack2(p.unit, p.unit);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int cc = now.n * BN + part * kCols + c * 32, left = p.N - cc;
@@ -549,9 +558,9 @@ __device__ __forceinline__ void argmax_epilogue(const Params<1>& prm, uint8_t* s
         const uint32_t* bu = &b4.x;
 #pragma unroll
         for (int k = 0; k < 4; k += 2)
-          unpack2(add2(mul2(mul2(pack2(__uint_as_float(v[i + k]), __uint_as_float(v[i + k + 1])), x2),
-                            pack2(__uint_as_float(su[k]), __uint_as_float(su[k + 1]))),
-                       pack2(__uint_as_float(bu[k]), __uint_as_float(bu[k + 1]))),
+          unpack2(add2_rounded(mul2(mul2(pack2(__uint_as_float(v[i + k]), __uint_as_float(v[i + k + 1])), x2),
+                                    pack2(__uint_as_float(su[k]), __uint_as_float(su[k + 1]))),
+                               one2, pack2(__uint_as_float(bu[k]), __uint_as_float(bu[k + 1]))),
                   z[i + k], z[i + k + 1]);
       }
       if (left < 32) {

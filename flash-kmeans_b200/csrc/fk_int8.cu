@@ -12,7 +12,7 @@
 // the time, so long products are bound by the L2: 4096 x 8192 x 4096 takes 95 us
 // (2.9 POP/s, 11 TB/s from the L2).  One token against 32768 x 4096 streams the
 // codebook at 4.8 TB/s (28 us); 604800 points against 1000 centroids of 128
-// features are bound by the argmax's scaling (252 us, see argmax_epilogue).
+// features are bound by the argmax's scaling (256 us, see argmax_epilogue).
 #include <algorithm>
 #include <type_traits>
 
@@ -411,6 +411,7 @@ static int run8(const Scores& q, const Scales& sc, Problem base, void* ws, size_
   p.bias = sc.bias;
   p.bias_sb = sc.bias ? sc.bs[0] : 0;
   p.bias_sn = sc.bias ? sc.bs[1] : 0;
+  p.unit = 1.0f;
   p.partial = f.partial;
   p.label_out = label_out;
   p.lo_sb = ls ? ls[0] : 0;

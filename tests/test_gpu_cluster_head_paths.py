@@ -195,3 +195,41 @@ def test_a_recorded_backward_pass():
     assert torch.equal(got[0], gx) and torch.equal(got[1], gc)
     with pytest.raises(RuntimeError, match="differentiable once"):
         (loss + got[0].float().square().sum()).backward()
+
+
+def _near_ties(N, K, D, seed, B=1, batched=False):
+    """One direction for all centroids, scales and biases a few steps of float32 apart:
+    most rows' best scores are equal or neighbours once they are rounded as documented."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    xq = torch.randint(-127, 128, (B, N, D), device="cuda", generator=g).to(torch.int8)
+    c = torch.randint(-127, 128, (B, 1, D), device="cuda", generator=g).to(torch.int8).repeat(1, K, 1)
+    xs = torch.rand(B, N, device="cuda", generator=g) * 0.02 + 1e-3
+    cs = 0.01 * (1 + torch.randint(-4, 5, (B, K), device="cuda", generator=g) * 2.0 ** -23)
+    size = (xq.double() @ c.double().transpose(-1, -2)).abs().mean() * xs.double().mean() * 0.01
+    b = size.float() * (1 + torch.randint(-2, 3, (B, K), device="cuda", generator=g) * 2.0 ** -23)
+    out = xq, c, xs, cs, b
+    return out if batched else [t[0] for t in out]
+
+
+def _first_of_the_largest(z):
+    k = torch.arange(z.shape[-1], device="cuda", dtype=torch.int32)
+    return torch.where(z == z.amax(-1, keepdim=True), k, z.shape[-1]).amin(-1).int()
+
+
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("N,K,D", [(20000, 60, 40), (3000, 700, 64), (70000, 256, 128), (1, 1000, 16), (200, 5000, 33)])
+def test_labels_of_scores_that_nearly_tie(N, K, D, with_bias):
+    """Labels are those of the scores as documented: the product rounded, then the
+    sum.  One fused step of both ranks neighbours otherwise (a fifth of these rows)."""
+    xq, c, xs, cs, b = _near_ties(N, K, D, seed=N + K)
+    b = b if with_bias else None
+    z = (xq.double() @ c.double().T).float() * xs[:, None] * cs
+    z = z if b is None else z + b
+    assert torch.equal(fk.int8_scores(xq, c, cs, x_scale=xs, bias=b), z)
+    assert torch.equal(fk.int8_assign(xq, c, cs, x_scale=xs, bias=b), _first_of_the_largest(z))
+
+
+def test_labels_of_scores_that_nearly_tie_in_batches():
+    xq, c, xs, cs, b = _near_ties(9000, 700, 64, seed=50, B=3, batched=True)
+    z = (xq.double() @ c.double().transpose(-1, -2)).float() * xs[..., None] * cs[:, None] + b[:, None]
+    assert torch.equal(fk.int8_assign(xq, c, cs, x_scale=xs, bias=b), _first_of_the_largest(z))

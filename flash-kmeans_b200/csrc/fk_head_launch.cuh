@@ -210,7 +210,7 @@ int set_problem(Params<problems_of(EPI)>& prm, int i, const Operand& a, const Op
 
 template <int EPI>
 int launch(Params<problems_of(EPI)>& prm, ShapeChoice sh, cudaStream_t s) {
-  if constexpr (!integer(EPI) && EPI != kEpiOutRows) {   // (factors of rows are float16's)
+  if constexpr (!integer(EPI) && EPI != kEpiOutRows) {   // (16-bit operands only)
     if (sh.exact) {
       if (sh.cg == 2) return launch_shape<2, 128, EPI, true>(prm, s);
       return launch_shape<1, 64, EPI, true>(prm, s);

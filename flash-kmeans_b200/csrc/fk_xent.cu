@@ -14,7 +14,8 @@
 // The backward pass goes over the centroids in pieces.  For each it recomputes
 // the scores, writes dz of the piece rounded to 16 bits (the operand type of
 // the tensor cores: one rounding of half a step at most, next to the rounding
-// of the 16-bit gradients themselves) and runs the two products that read it,
+// of the 16-bit gradients themselves; what it takes from the label's entry is
+// added to dx again) and runs the two products that read it,
 // in one launch whose workers finish together; accumulators are float32
 // throughout.  That is 8 N K D operations instead of the 6 N K D of a pass that
 // keeps N x K scores.
@@ -1119,7 +1120,9 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       base.batches = static_cast<int>(q.B);
       base.status = status;
       base.fscale = q.scale / p_scale;
+      base.stat = stat;
       base.stat_rows = q.N;
+      base.p_scale = p_scale;
       base.f_den = q.reduction == 1 ? count : nullptr;
       base.live = live;
       base.live_off = static_cast<int>(r0);
@@ -1131,6 +1134,12 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
         base.row_map = f.map;
         base.f_num = q.reduction == 0 ? nullptr : g;
         base.row_factor = f.power;
+        base.label_rows = nullptr;
+        if (q.dtype != FK_F32 && piece == 0) {
+          base.label_rows = static_cast<const uint16_t*>(co.p);
+          base.label_ld = co.ld;
+          base.label_batch = co.batch_step ? co.mat : 0;
+        }
         return grad_problem(q, pair, f.join_x, base, po, co, rw, kw, f.sh, f.split_x, f.acc_x, q.N, r0, f.ld,
                             piece == 0, piece + 1 == f.n_pieces, gx, r0);
       };
@@ -1142,6 +1151,7 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
         base.row_map = nullptr;
         base.f_num = q.reduction == 0 ? factor_c : g;
         base.row_factor = nullptr;
+        base.label_rows = nullptr;
         return grad_problem(q, pair, f.join_c, base, pt, xo, kw, rw, f.sh, f.split_c, f.acc_c, f.Kp, 0, f.ld,
                             chunk == 0, chunk + 1 == f.n_chunks, gc, k0);
       };
@@ -1151,7 +1161,8 @@ static int backward(const Xent& q, const RowStat* stat, const int32_t* count, co
       if (gx.p && x_first) st = add_x();
       if (st == FK_OK && gc.p) st = add_c();
       if (st == FK_OK && gx.p && !x_first) st = add_x();
-      if (st == FK_OK) st = f.power ? launch<kEpiOutRows>(pair, f.sh, s) : launch<kEpiOut>(pair, f.sh, s);
+      const bool own = f.power || (gx.p && q.dtype != FK_F32 && piece == 0);
+      if (st == FK_OK) st = own ? launch<kEpiOutRows>(pair, f.sh, s) : launch<kEpiOut>(pair, f.sh, s);
       if (st != FK_OK) return st;
     }
   }

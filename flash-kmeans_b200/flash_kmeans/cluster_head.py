@@ -365,7 +365,8 @@ def cluster_cross_entropy(x: torch.Tensor, centroids: torch.Tensor, labels: torc
 
     The (N, K) scores are never stored, forward or backward; sums and softmax
     statistics are float32.  Gradients of 16-bit inputs round the softmax to 16
-    bits once, piece by piece, as the tensor cores take it.  A label outside
+    bits once, piece by piece, as the tensor cores take it (in the gradient by x,
+    not the label's own entry).  A label outside
     [0, K) other than ``ignore_index`` makes the loss NaN.
     """
     _refuse_tangents("cluster_cross_entropy", x, centroids)

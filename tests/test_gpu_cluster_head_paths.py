@@ -233,3 +233,41 @@ def test_labels_of_scores_that_nearly_tie_in_batches():
     xq, c, xs, cs, b = _near_ties(9000, 700, 64, seed=50, B=3, batched=True)
     z = (xq.double() @ c.double().transpose(-1, -2)).float() * xs[..., None] * cs[:, None] + b[:, None]
     assert torch.equal(fk.int8_assign(xq, c, cs, x_scale=xs, bias=b), _first_of_the_largest(z))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("B,N,K,D,shared,reduction", [
+    (0, 300, 500, 64, False, "sum"), (3, 77, 131, 65, False, "sum"), (2, 130, 300, 100, True, "sum"),
+    (0, 5, 9000, 40, False, "sum"),          # split along the centroids
+    (0, 17001, 9001, 24, False, "sum"),      # pieces of centroids and chunks of rows
+    (0, 20000, 9000, 392, False, "sum"),     # rows gathered
+    (2, 600, 700, 200, False, "none"), (0, 1500, 2000, 257, False, "none")])
+def test_the_label_takes_no_rounding_of_its_own_in_gx(B, N, K, D, shared, reduction, dtype):
+    """softmax - 1 at the label, most of a row's P, is rounded to 16 bits with the
+    rest; what that takes away is added again in float32.  So only the others'
+    entries are off by half a step, which the label's would double at least."""
+    x, c, y = make(B, N, K, D, dtype, seed=51, shared=shared, ignored=0.1, ids=torch.int64, spread=2.0)
+    g = torch.rand(y.shape, device="cuda") + 0.5 if reduction == "none" else None
+    scale = 2.0
+    _, gx, _ = fk.cluster_cross_entropy_grad(x, c, y, scale=scale, reduction=reduction, grad_loss=g)
+    xd, cd = x.double(), c.double()
+    if c.dim() < x.dim():
+        cd = cd.expand(x.shape[0], *c.shape)
+    keep = (y != -100)[..., None]
+    at = y.clamp(min=0)[..., None]
+    z = scale * xd @ cd.transpose(-1, -2)
+    ez = (scale * (xd.abs() @ cd.abs().transpose(-1, -2)) * 2.0 ** -21).amax(-1, keepdim=True) + z.abs().amax(
+        -1, keepdim=True) * 2.0 ** -22
+    p = torch.softmax(z, -1).scatter(-1, at, 0.0)
+    others = p.sum(-1, keepdim=True)
+    w = 1.0 if g is None else g.double()[..., None]
+    u = torch.finfo(dtype).eps / 2
+    own = torch.gather(cd, -2, at.expand(*at.shape[:-1], D))
+    want = torch.where(keep, scale * w * (p @ cd - others * own), 0.0)
+    # (the scores' own error and float32's sums, as elsewhere; no half step for the label)
+    tails, label = u + 2 * ez + 2.0 ** -18, 2 * ez + 2.0 ** -18
+    tol = scale * w * ((p * tails) @ cd.abs() + others * own.abs() * label)
+    if dtype == HF:
+        tol = tol + scale * w * 2.0 ** -39 * cd.abs().sum(-2, keepdim=True)
+    tol = torch.where(keep, tol + want.abs() * u + 2.0 ** -25, 0.0)
+    close(gx, (want, tol), "gx")

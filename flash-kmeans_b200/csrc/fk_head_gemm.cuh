@@ -441,7 +441,7 @@ __device__ __forceinline__ void quarter_sync(int quarter) {
 
 // ------------------------------------------------------------------- kernel
 // Epilogue of the argmax.  The scores' scaling and comparing bounds it (2400 scores
-// a ns at 604800 x 1000 x 128: 256 us, of which the products need 47), so a row
+// a ns at 604800 x 1000 x 128: 255 us, of which the products need 47), so a row
 // keeps only its best score and the 32 scores of the chunk that it came from, in
 // shared memory; which column of it won is looked up once, at the end of the
 // row.  A column's scale and bias come from shared memory, 16 bytes to all lanes

@@ -12,7 +12,7 @@
 // the time, so long products are bound by the L2: 4096 x 8192 x 4096 takes 95 us
 // (2.9 POP/s, 11 TB/s from the L2).  One token against 32768 x 4096 streams the
 // codebook at 4.8 TB/s (28 us); 604800 points against 1000 centroids of 128
-// features are bound by the argmax's scaling (256 us, see argmax_epilogue).
+// features are bound by the argmax's scaling (255 us, see argmax_epilogue).
 #include <algorithm>
 #include <type_traits>
 
